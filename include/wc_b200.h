@@ -377,6 +377,152 @@ int wc_replay_pack_row(const uint8_t* state, size_t len, uint8_t* out);
 int wc_replay_expand(const uint8_t* rows, size_t nrows, const uint8_t* cc, const int64_t* seg, size_t m, float* x,
                      float* phi, void* stream);
 
+/* ---- training operators ---------------------------------------------------- */
+/* The device side of a training step over that batch; they have no
+ * counterpart in the reference, whose trainer runs on torch. Every pointer is
+ * device memory of the current device, nothing is allocated, and a call only
+ * enqueues work on `stream` (a cudaStream_t; NULL is the legacy default
+ * stream). Arguments are checked before anything is enqueued (WC_E_ARG);
+ * what lies in device memory is not read by the host. Sizes of zero are
+ * allowed. Matrices are row-major with unit column stride; a row stride
+ * (ld_*) counts elements and is at least the width. Inputs and outputs of one
+ * call do not overlap. Sums, statistics and gradients accumulate in 32 bits,
+ * in an order fixed by the sizes: equal calls give equal bits. A workspace
+ * (16-byte aligned) may be reused by the next call on the same stream; its
+ * contents are not read. */
+enum { WC_F32 = 0, WC_F16 = 1, WC_BF16 = 2 };
+
+/* The clipped policy loss with a KL term, and its gradient, in one call.
+ * Row t has logits z over `width` entries, of which those with a nonzero
+ * `legal` byte (all, when legal is NULL) and a value above -inf count. With
+ * l = ln softmax(z)[action], ratio = exp(l - old_logp), A the advantage, H
+ * the entropy of softmax(z), and k = exp(r - l) - (r - l) - 1 for the
+ * reference log-probability r (0 when ref_logp is NULL):
+ *   row_loss = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
+ *              + kl_coef k - entropy_coef H
+ *   loss = sum of weight row_loss         (weight 1 when weights is NULL)
+ *   dlogits = upstream dloss/dlogits      (upstream 1 when NULL, else *upstream)
+ * A row is void when its weight is 0, its action lies outside 0 .. width - 1
+ * or is not one of the entries that count (so also when none is left): its
+ * results and its gradient are 0, and its logits need not be finite. Entries
+ * that do not count have gradient 0. NaN and +inf elsewhere give NaN. */
+typedef struct wc_policy_loss_args {
+    const void* logits;      /* rows x width of `type` */
+    const uint8_t* legal;    /* rows x width, or NULL */
+    const void* actions;     /* rows, int32 or int64 (action_bytes) */
+    const float* old_logp;   /* rows */
+    const float* advantages; /* rows */
+    const float* weights;    /* rows, or NULL */
+    const float* ref_logp;   /* rows, or NULL */
+    const float* upstream;   /* 1, or NULL */
+    float* loss;             /* out, 1 */
+    float* row_out;          /* out, 4 x rows: row_loss, l, H, k */
+    void* dlogits;           /* out, rows x width of `type`, or NULL: no gradient */
+    void* workspace;         /* wc_policy_loss_workspace bytes */
+    int64_t rows, width, ld_logits, ld_legal, ld_dlogits;
+    float clip_low, clip_high, kl_coef, entropy_coef;
+    int32_t type, action_bytes;
+} wc_policy_loss_args;
+uint64_t wc_policy_loss_workspace(int64_t rows, int64_t width);
+int wc_policy_loss(const wc_policy_loss_args* a, void* stream);
+
+/* A residual block's norms, gate and residual scale in one pass:
+ *   u = post(h);  y = residual_scale x + gate[t / rows_per_gate] u;  n = pre(y)
+ * post and pre are LayerNorm (WC_NORM_LAYER) or RMSNorm (WC_NORM_RMS) with
+ * 32-bit weight and, for LayerNorm, optional bias; a NULL weight leaves that
+ * norm out (u = h; no n). gate NULL: 1. gate has ceil(rows / rows_per_gate)
+ * rows: rows_per_gate = rows is a gate per channel, 1 one per element, in
+ * between one per sequence or position (a position is 37 rows of the trunk).
+ * n is taken from y before y is rounded. stats receives per row the mean and
+ * reciprocal deviation of post, then of pre (0 and 1 for a norm left out;
+ * mean 0 for RMSNorm). n_q / n_scale, if not NULL, receive n in 8 bits (see
+ * wc_act8_pack). Widths up to 16384. */
+enum { WC_NORM_LAYER = 0, WC_NORM_RMS = 1 };
+typedef struct wc_block_norm_args {
+    const void* x;          /* rows x width of `type`, the residual stream */
+    const void* h;          /* rows x width, the block's output */
+    const void* gate;       /* groups x width (contiguous), or NULL */
+    const float* post_weight;
+    const float* post_bias;
+    const float* pre_weight;
+    const float* pre_bias;
+    void* y;                /* out (forward) */
+    void* n;                /* out (forward), or NULL */
+    int8_t* n_q;            /* out (forward), or NULL */
+    uint8_t* n_scale;       /* out (forward), or NULL */
+    float* stats;           /* 4 x rows as rows x 4: out of the forward, read by the backward */
+    int64_t rows, width, rows_per_gate, ld_x, ld_h, ld_y, ld_n;
+    float residual_scale, eps;
+    int32_t type, kind;
+} wc_block_norm_args;
+int wc_block_norm(const wc_block_norm_args* a, void* stream);
+/* The gradients at x, h, gate and the norms' weights and biases, from those
+ * at y and n and the forward's inputs and stats (y, n, n_q and n_scale of `a`
+ * are not used). dy or dn may be NULL: no gradient from there. Outputs that
+ * are NULL are left out. */
+typedef struct wc_block_norm_grads {
+    const void* dy;
+    const void* dn;
+    void* dx;
+    void* dh;
+    void* dgate;            /* groups x width of `type` */
+    float* dpost_weight;
+    float* dpost_bias;
+    float* dpre_weight;
+    float* dpre_bias;
+    void* workspace;        /* wc_block_norm_workspace bytes */
+    int64_t ld_dy, ld_dn, ld_dx, ld_dh;
+} wc_block_norm_grads;
+uint64_t wc_block_norm_workspace(const wc_block_norm_args* a);
+int wc_block_norm_backward(const wc_block_norm_args* a, const wc_block_norm_grads* g, void* stream);
+
+/* Activations kept in 8 bits between the forward and the backward pass. Rows
+ * are cut into blocks of WC_ACT8_BLOCK values; q holds whole numbers of at
+ * most 127 in rows of whole blocks (the last one padded with zeros), scale
+ * one byte per block: the exponent, plus 127, of the block's unit, the
+ * smallest power of two (at least 2^-126) that its largest value allows. A
+ * value reads back as q 2^(scale - 127), rounded to nearest-even when it was
+ * stored: at most half a unit off, and exact in bf16. A block that holds an
+ * infinity or NaN has scale 255 and reads back as NaN.
+ * wc_act8_pack:   x -> q, scale.            wc_act8_unpack: q, scale -> out.
+ * wc_gelu8:       out = GELU(x + bias) (tanh form), and the 32-bit sum
+ *                 x + bias to q, scale.
+ * wc_gelu8_backward: out = x GELU'(q, scale) with x the gradient at the
+ *                 activation; dbias, if not NULL, the column sums of that
+ *                 (before rounding). */
+enum { WC_ACT8_BLOCK = 32 };
+typedef struct wc_act8_args {
+    const void* x;      /* rows x width of `type` */
+    const float* bias;  /* width, or NULL */
+    int8_t* q;          /* rows x 32 blocks, contiguous, 16-byte aligned */
+    uint8_t* scale;     /* rows x blocks, contiguous */
+    void* out;          /* rows x width of `type` */
+    float* dbias;       /* width, or NULL */
+    void* workspace;    /* wc_gelu8_workspace bytes (wc_gelu8_backward with dbias) */
+    int64_t rows, width, ld_x, ld_out;
+    int32_t type;
+} wc_act8_args;
+int wc_act8_pack(const wc_act8_args* a, void* stream);
+int wc_act8_unpack(const wc_act8_args* a, void* stream);
+int wc_gelu8(const wc_act8_args* a, void* stream);
+uint64_t wc_gelu8_workspace(int64_t rows, int64_t width);
+int wc_gelu8_backward(const wc_act8_args* a, void* stream);
+/* The weight gradient of a linear layer whose input was kept in 8 bits:
+ * dw[k, n] = sum over t of x8[t, k] dy[t, n] (weights as [in, out]), and
+ * db[n] = sum over t of dy[t, n] when db is not NULL. */
+typedef struct wc_act8_wgrad_args {
+    const int8_t* q;        /* rows x 32 blocks of k values */
+    const uint8_t* scale;
+    const void* dy;         /* rows x n of `type` */
+    void* dw;               /* k x n of `out_type`, contiguous */
+    float* db;              /* n, or NULL */
+    void* workspace;        /* wc_act8_wgrad_workspace bytes */
+    int64_t rows, k, n, ld_dy;
+    int32_t type, out_type;
+} wc_act8_wgrad_args;
+uint64_t wc_act8_wgrad_workspace(const wc_act8_wgrad_args* a);
+int wc_act8_wgrad(const wc_act8_wgrad_args* a, void* stream);
+
 /* ---- streaming submit / wait ---------------------------------------------- */
 /* The job stays owned by the caller and must outlive the wc_wait of its
  * ticket; free it (wc_job_free) after that wait returns. */

@@ -1,0 +1,81 @@
+// Shared by the training operators' kernels (policy_loss.cu, block_norm.cu,
+// act8.cu, wgrad8.cu): element types, row reductions, the 8-bit block code.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "train_ops.h"
+
+namespace wctrain {
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Sum over the CTA in a fixed order; every thread gets it. `s` holds one
+// float per warp; the call ends with the array free for the next one.
+__device__ __forceinline__ float cta_sum(float v, float* s) {
+    v = warp_sum(v);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
+    if (lane == 0) s[warp] = v;
+    __syncthreads();
+    float t = lane < nw ? s[lane] : 0.0f;
+    t = warp_sum(t);
+    __syncthreads();
+    return t;
+}
+
+// The unit of an 8-bit block whose largest magnitude is `top`: the smallest
+// power of two 2^e with top <= 127 2^e, as e + 127 (at least 1, so the unit
+// and its reciprocal are normal numbers). top = 1.M 2^(E - 127); 64 (1.M)
+// exceeds 127 just when M > 0x7e0000. 255 (an infinity or NaN in the block)
+// reads back as NaN.
+__device__ __forceinline__ uint32_t act8_code(float top) {
+    const uint32_t b = __float_as_uint(top) & 0x7fffffffu, E = b >> 23;
+    if (E == 255) return 255;
+    const int c = (int)E - 6 + ((b & 0x7fffffu) > 0x7e0000u ? 1 : 0);
+    return c < 1 ? 1u : (uint32_t)c;
+}
+__device__ __forceinline__ float act8_unit(uint32_t code) {
+    return code == 255 ? __uint_as_float(0x7fffffffu) : __uint_as_float(code << 23);
+}
+// 2^-e of a code; the product with a block's value is exact (or too small to round to anything but 0)
+__device__ __forceinline__ float act8_inverse(uint32_t code) { return __uint_as_float((254u - code) << 23); }
+
+// GELU (tanh form) as x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3):
+// no cancellation for negative x. The exponent is held below 126 so that the
+// divisor stays finite.
+__device__ __forceinline__ float gelu(float x) {
+    const float u = x * fmaf(0.044715f * 0.7978845608f, x * x, 0.7978845608f);
+    const float e = exp2f(fminf(-2.8853900817779268f * u, 126.0f));
+    return x / (1.0f + e);
+}
+// Its derivative: s + 2 x s (1 - s) u'(x) with s = 1 / (1 + exp(-2u)); 1 - s
+// is e s, again without cancellation.
+__device__ __forceinline__ float gelu_slope(float x) {
+    const float x2 = x * x;
+    const float u = x * fmaf(0.044715f * 0.7978845608f, x2, 0.7978845608f);
+    const float du = fmaf(3.0f * 0.044715f * 0.7978845608f, x2, 0.7978845608f);
+    const float e = exp2f(fminf(-2.8853900817779268f * u, 60.0f));
+    const float s = 1.0f / (1.0f + e);
+    return s + 2.0f * x * du * (e * s) * s;
+}
+
+}  // namespace wctrain

@@ -116,6 +116,18 @@ def _load() -> C.CDLL:
         "wc_job_from_wcj8": (I, [C.c_char_p, C.c_size_t, P(VP)]),
         "wc_debug_set_wait_limit": (I, [VP, U64]),
         "wc_replay_expand": (I, [VP, C.c_size_t, VP, VP, C.c_size_t, VP, VP, VP]),
+        "wc_policy_loss_workspace": (U64, [C.c_int64, C.c_int64]),
+        "wc_policy_loss": (I, [VP, VP]),
+        "wc_block_norm": (I, [VP, VP]),
+        "wc_block_norm_workspace": (U64, [VP]),
+        "wc_block_norm_backward": (I, [VP, VP, VP]),
+        "wc_act8_pack": (I, [VP, VP]),
+        "wc_act8_unpack": (I, [VP, VP]),
+        "wc_gelu8": (I, [VP, VP]),
+        "wc_gelu8_workspace": (U64, [C.c_int64, C.c_int64]),
+        "wc_gelu8_backward": (I, [VP, VP]),
+        "wc_act8_wgrad_workspace": (U64, [VP]),
+        "wc_act8_wgrad": (I, [VP, VP]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
