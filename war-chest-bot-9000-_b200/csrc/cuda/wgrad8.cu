@@ -1,79 +1,581 @@
-// dw = x8^T dy with x8 kept in 8 bits, and db = the column sums of dy.
+// dw = x8^T dy with x8 kept in 8 bits, and db = the column sums of dy, on the
+// tensor cores (tcgen05, f32 accumulators in TMEM).
 //
-// A CTA owns a 64 x 64 tile of dw and a range of rows; the ranges' partial
-// results are joined by a second kernel in a fixed order.
+// A stored value is a whole number times a power of two, so it is exact in
+// bf16; dy is exact as the sum of `parts` bf16 numbers (1 for bf16, 2 for f16,
+// 3 for f32). The products are therefore those of the 32-bit form, and only
+// the f32 accumulation rounds.
+//
+// Both operands are summed over the rows, their slow axis, so both are MN-major
+// in shared memory: a stage holds 64 rows, 64 columns of a row being one
+// 128-byte swizzled line. Per CTA, `mt` 128-row tiles of dw (channels of x8)
+// by `bn` columns:
+//   converters  (8 warps) bytes and units of x8 from global memory through
+//               registers, one stage ahead, to bf16 in shared memory; dy too
+//               where TMA cannot take it (parts > 1 or an unaligned dy); and
+//               the epilogue out of TMEM
+//   producer    (1 warp) dy by TMA, and x8 prefetched into L2
+//   issuer      (1 warp) the products
+//   column sums (2 warps) db from the dy tiles in shared memory
+// The work is tiles x stages units dealt in equal runs to the CTAs; a tile
+// that falls to several is joined from their partial results by a second
+// kernel, in a fixed order.
+#include <cuda.h>
+
+#include <algorithm>
+#include <stdexcept>
+
 #include "colsum.cuh"
+#include "kernels.h"
+#include "umma.cuh"
 
 namespace wctrain {
 
 namespace {
 
-constexpr int TILE = 64, DEEP = 16, THREADS = 256;
+constexpr int BK = 64;           // rows of a stage
+constexpr int GROUP = BK * 128;  // bytes of 64 columns of a stage
+constexpr int CONVERTERS = 256, THREADS = CONVERTERS + 128;
+constexpr int MAX_STAGES = 8;
+constexpr int RING = 220 * 1024;  // shared memory of the stages
+constexpr uint32_t TMEM_COLS = 512;
+
+struct Plan {
+    int mt, bn, ktiles, ntiles, stages, ctas, joined, limit;
+    int64_t steps, units;  // stages of a tile; tiles x steps
+    __host__ __device__ int stage_bytes() const { return mt * 2 * GROUP + b_bytes; }
+    int b_bytes;
+};
+
+// How dy reaches shared memory: by TMA, or through the converters.
+enum { TMA, BF16, F16, F32 };
+__host__ __device__ constexpr int parts_of(int mode) { return mode == F32 ? 3 : mode == F16 ? 2 : 1; }
+__host__ __device__ constexpr int widest(int mode) { return mode == TMA ? 256 : mode == F32 ? 64 : 128; }
+
+struct Shared {
+    uint64_t full_a[MAX_STAGES], full_b[MAX_STAGES], empty[MAX_STAGES], acc_full, acc_empty;
+    uint32_t tmem;
+    int failed;
+};
+
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
+    // MN-major, 128-byte swizzle: GROUP bytes to the next 64 columns (leading), 1024 to the next 8 rows (stride)
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(GROUP >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1u << 46;
+    d |= (uint64_t)2u << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
+}
+
+// 4 bytes to two pairs of bf16 times `unit` (a bf16 pair). A byte's low seven
+// bits are the mantissa of 128 + them; its sign bit, worth -128, is the
+// exponent step from 128 to 256: (128 + low) - (128 or 256) is the byte.
+__device__ __forceinline__ uint32_t two(uint32_t w, __nv_bfloat162 unit) {
+    const uint32_t a = (w & 0x007f007fu) | 0x43004300u, b = (w & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b)), unit);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint2 four(uint32_t q, __nv_bfloat162 unit) {
+    return make_uint2(two(__byte_perm(q, 0, 0x4140), unit), two(__byte_perm(q, 0, 0x4342), unit));
+}
+
+// Part `p` of v as bf16 and what is left for the next ones. An infinity or NaN goes whole into the first.
+__device__ __forceinline__ float part_of(float& v) {
+    const float hi = __bfloat162float(__float2bfloat16_rn(v));
+    v = isfinite(hi) ? v - hi : 0.0f;
+    return hi;
+}
 
 template <class T>
-__global__ void __launch_bounds__(THREADS) k_wgrad8(wc_act8_wgrad_args a, int64_t chunk_rows, float* part) {
-    __shared__ float sx[DEEP][TILE], sy[DEEP][TILE];
-    const int64_t k0 = (int64_t)blockIdx.x * TILE, n0 = (int64_t)blockIdx.y * TILE;
-    const int64_t blocks = (a.k + 31) / 32, first = blockIdx.z * chunk_rows, last = min(first + chunk_rows, a.rows);
-    const int tk = threadIdx.x / 16 * 4, tn = threadIdx.x % 16 * 4;
-    float acc[4][4] = {}, db[4] = {};
-    for (int64_t t0 = first; t0 < last; t0 += DEEP) {
-        for (int i = threadIdx.x; i < DEEP * TILE; i += THREADS) {
-            const int64_t t = t0 + i / TILE, k = k0 + i % TILE, n = n0 + i % TILE;
-            float x = 0.0f, y = 0.0f;
-            if (t < last && k < a.k) x = (float)a.q[t * blocks * 32 + k] * act8_unit(a.scale[t * blocks + k / 32]);
-            if (t < last && n < a.n) y = to_f(static_cast<const T*>(a.dy)[t * a.ld_dy + n]);
-            sx[i / TILE][i % TILE] = x, sy[i / TILE][i % TILE] = y;
+__device__ __forceinline__ void load_dy(const T* p, int64_t n, int64_t width, bool vec, float* v) {
+    if (vec && n + 8 <= width) {
+        alignas(16) T e[8];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p + n)[i];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = n + i < width ? to_f(p[n + i]) : 0.0f;
+    }
+}
+
+template <class T>
+__device__ __forceinline__ void store_run(T* p, const float* v, int count, bool vec) {
+    if (vec && count == 32) {
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 32 / E; ++i) {
+            alignas(16) T e[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) e[j] = from_f<T>(v[i * E + j]);
+            reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(e);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < count) p[i] = from_f<T>(v[i]);
+    }
+}
+
+__device__ __forceinline__ void add_run(float* v, const float* p, int count, bool vec) {
+    if (vec && count == 32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 w = reinterpret_cast<const float4*>(p)[i];
+            v[4 * i] += w.x, v[4 * i + 1] += w.y, v[4 * i + 2] += w.z, v[4 * i + 3] += w.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < count) v[i] += p[i];
+    }
+}
+
+// A run of stages of one tile that is summed in TMEM. The tensor core's f32
+// accumulation drops the bits below the sum's last place, about 4e-9 of the
+// result for each product of 16 rows, always towards zero; a 32-bit dw
+// therefore takes runs of at most RUN stages (below 8e-7) and adds them up in
+// global memory, each thread the values it wrote itself. For a 16-bit dw a
+// whole segment is one run.
+constexpr int RUN = 40;
+struct Run {
+    int64_t tile;
+    int first, last;       // stages
+    bool whole, head;      // the CTA has the whole tile; its first tile
+    bool begins, ends;     // first and last run of this CTA's share of the tile
+};
+
+// The runs that fall to a CTA, in order
+struct Walk {
+    int64_t u, end, start, steps, tile = 0;
+    int s = 0, s0 = 0, s1 = 0, limit;
+    __device__ Walk(const Plan& p) : steps(p.steps), limit(p.limit) {
+        start = u = p.units * blockIdx.x / p.ctas;
+        end = p.units * (blockIdx.x + 1) / p.ctas;
+    }
+    __device__ bool next(Run& r) {
+        if (s == s1) {
+            if (u >= end) return false;
+            r.head = u == start;
+            tile = u / steps;
+            s = s0 = (int)(u - tile * steps);
+            s1 = (int)min(steps, s0 + (end - u));
+            u += s1 - s0;
+        } else {
+            r.head = tile == start / steps;
+        }
+        r.tile = tile, r.first = s, r.last = min(s1, s + limit);
+        r.whole = s0 == 0 && s1 == steps;
+        r.begins = s == s0, r.ends = r.last == s1;
+        s = r.last;
+        return true;
+    }
+};
+
+template <int MODE, class T>
+__global__ void __launch_bounds__(THREADS, 1)
+    k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
+    constexpr int P = parts_of(MODE);
+    extern __shared__ uint8_t raw[];
+    __shared__ Shared sh;
+    uint8_t* ring = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int stage_bytes = p.stage_bytes(), a_bytes = p.mt * 2 * GROUP;
+    const int groups = (p.bn + 63) / 64;
+    volatile int* failed = &sh.failed;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            umma::mbar_init(&sh.full_a[i], CONVERTERS / 32);
+            umma::mbar_init(&sh.full_b[i], 1);
+            umma::mbar_init(&sh.empty[i], 3);  // the issuer's commit and the two column-sum warps
+        }
+        umma::mbar_init(&sh.acc_full, 1);
+        umma::mbar_init(&sh.acc_empty, CONVERTERS / 32);
+        sh.failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) umma::tmem_alloc(&sh.tmem, TMEM_COLS);
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = sh.tmem;
+    Walk walk(p);
+    Run seg;
+    uint32_t it = 0;  // stages so far
+    // A wait that runs out (umma.cuh) makes every role give up: products and copies in flight are waited for, what
+    // the CTA had still to write becomes NaN, and the tensor memory is released. wait_all: the same for a whole warp.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (!*failed && umma::mbar_wait(bar, parity)) return true;
+        *failed = 1;
+        return false;
+    };
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+    if (warp == 0) {  // ------------------------------------------- issuer
+        const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
+        uint32_t done = 0;
+        bool ok = true;
+        while (ok && walk.next(seg)) {
+            if (done) ok = wait_all(&sh.acc_empty, (done - 1) & 1);
+            umma::fence_after_sync();
+            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
+                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
+                ok = wait_all(&sh.full_a[slot], ph) && (MODE != TMA || wait_all(&sh.full_b[slot], ph));
+                if (!ok) break;
+                umma::fence_after_sync();
+                if (lane == 0) {
+                    const uint32_t A = umma::smem_u32(ring + slot * stage_bytes), B = A + a_bytes;
+                    for (int m = 0; m < p.mt; ++m)
+                        for (int q = 0; q < P; ++q)
+#pragma unroll
+                            for (int k = 0; k < BK / 16; ++k)
+                                umma::mma16(tmem + (m * P + q) * p.bn, desc_mn(A + m * 2 * GROUP + k * 2048),
+                                            desc_mn(B + q * groups * GROUP + k * 2048), idesc, s > seg.first || k);
+                    umma::commit(&sh.empty[slot]);
+                }
+                __syncwarp();
+            }
+            if (ok && lane == 0) umma::commit(&sh.acc_full);
+            __syncwarp();
+            ++done;
+        }
+        // every issued product has finished before TMEM is given back
+        if (!ok) {
+            if (lane == 0) umma::commit(&sh.acc_full);
+            umma::mbar_wait(&sh.acc_full, (done - 1) & 1, umma::DRAIN_NS);
+        }
+    } else if (warp == 1) {  // ------------------------------------ producer
+        if (MODE == TMA && lane == 0) {
+            bool ok = true;
+            while (ok && walk.next(seg)) {
+                const int n0 = (int)(seg.tile / p.ktiles) * p.bn;
+                for (int s = seg.first; s < seg.last; ++s, ++it) {
+                    const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
+                    if (it >= (uint32_t)p.stages && !(ok = wait(&sh.empty[slot], ph ^ 1))) break;
+                    umma::expect_tx(&sh.full_b[slot], groups * GROUP);
+                    const uint32_t B = umma::smem_u32(ring + slot * stage_bytes) + a_bytes;
+                    for (int g = 0; g < groups; ++g) tma_load(B + g * GROUP, &map_dy, n0 + 64 * g, s * BK, &sh.full_b[slot]);
+                }
+            }
+            if (!ok)  // the copies in flight land before the CTA leaves
+                for (uint32_t i = it > (uint32_t)p.stages ? it - p.stages : 0; i < it; ++i)
+                    umma::mbar_wait(&sh.full_b[i % p.stages], (i / p.stages) & 1, umma::DRAIN_NS);
+        }
+    } else if (warp < 4) {  // --------------------------------- column sums
+        const int at = threadIdx.x - 64;
+        bool ok = true;
+        float sum[4] = {};
+        while (walk.next(seg)) {
+            const bool mine = a.db && seg.tile % p.ktiles == 0;
+            if (seg.begins)
+                for (float& v : sum) v = 0.0f;
+            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
+                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
+                ok = MODE == TMA ? wait_all(&sh.full_b[slot], ph) : wait_all(&sh.full_a[slot], ph);
+                if (!ok) break;
+                if (mine) {
+                    const uint8_t* B = ring + slot * stage_bytes + a_bytes;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = 2 * at + 128 * h;  // this thread's pair of columns
+                        if (c >= p.bn) continue;
+                        float x = 0.0f, y = 0.0f;
+                        for (int q = 0; q < P; ++q) {
+                            const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 7) * 2;
+#pragma unroll 8
+                            for (int t = 0; t < BK; ++t) {
+                                const uint32_t w = *reinterpret_cast<const uint32_t*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
+                                x += umma::Op16<false>::lo(w), y += umma::Op16<false>::hi(w);
+                            }
+                        }
+                        sum[2 * h] += x, sum[2 * h + 1] += y;
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) arrive(&sh.empty[slot]);
+            }
+            if (mine && seg.ends) {
+                const int64_t n0 = seg.tile / p.ktiles * p.bn;
+                const float nan = __uint_as_float(0x7fffffffu);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const int c = 2 * at + 128 * (h >> 1) + (h & 1);
+                    if (c >= p.bn) continue;
+                    const float v = ok ? sum[h] : nan;
+                    if (!seg.whole) part_db[(2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)p.bn + c] = v;
+                    else if (n0 + c < a.n) a.db[n0 + c] = v;
+                }
+            }
+        }
+    } else {  // -------------------------------------------------- converters
+        const int tid = threadIdx.x - 128, w = warp - 4;
+        const int64_t blocks = (a.k + 31) / 32;
+        const T* dy = static_cast<const T*>(a.dy);
+        const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
+        // x8: piece i of a stage is 16 channels of one row; a thread has 2 mt of them
+        constexpr int B_PER = BK * widest(MODE) / 8 / CONVERTERS;  // chunks of 8 columns of dy
+        uint4 q[4];
+        uint32_t code[4];
+        float v[MODE == TMA ? 1 : B_PER][8];
+        const int per_row = 8 * p.mt, chunks = groups * 8;
+        auto fetch = [&](const Run& g, int s) {
+            const int64_t k0 = g.tile % p.ktiles * p.mt * 128, n0 = g.tile / p.ktiles * p.bn;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i >= 2 * p.mt) break;
+                const int piece = tid + i * CONVERTERS;
+                const int64_t t = (int64_t)s * BK + piece / per_row, k = k0 + piece % per_row * 16;
+                const bool in = t < a.rows && k < blocks * 32;
+                q[i] = in ? *reinterpret_cast<const uint4*>(a.q + t * blocks * 32 + k) : make_uint4(0, 0, 0, 0);
+                code[i] = in ? a.scale[t * blocks + (k >> 5)] : 127u;
+            }
+            if constexpr (MODE != TMA) {
+#pragma unroll
+                for (int i = 0; i < B_PER; ++i) {
+                    const int piece = tid + i * CONVERTERS;
+                    const int64_t t = (int64_t)s * BK + piece / chunks, n = n0 + piece % chunks * 8;
+                    if (piece < BK * chunks && t < a.rows) load_dy(dy + t * a.ld_dy, n, a.n, vec_dy, v[i]);
+                    else
+                        for (float& x : v[i]) x = 0.0f;
+                }
+            }
+        };
+        bool ok = true, more = walk.next(seg);
+        uint32_t done = 0;
+        if (more) fetch(seg, seg.first);
+        while (more) {
+            Run following;
+            const bool another = walk.next(following);
+            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
+                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
+                if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
+                uint8_t* A = ring + slot * stage_bytes;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i >= 2 * p.mt) break;
+                    const int piece = tid + i * CONVERTERS, t = piece / per_row, g = piece % per_row;
+                    const uint16_t ub = code[i] == 255 ? (uint16_t)0x7fff : (uint16_t)(code[i] << 7);
+                    const uint32_t uu = ub * 0x10001u;
+                    const __nv_bfloat162 unit = *reinterpret_cast<const __nv_bfloat162*>(&uu);
+                    const uint2 c0 = four(q[i].x, unit), c1 = four(q[i].y, unit), c2 = four(q[i].z, unit), c3 = four(q[i].w, unit);
+                    uint8_t* line = A + (g >> 2) * GROUP + t * 128;
+                    const int c = (g & 3) * 2;
+                    // the odd groups store their second chunk first: the 8 threads of a row then fill 8 different chunks
+                    const bool swap = (g >> 2) & 1;
+                    const uint4 lo = make_uint4(c0.x, c0.y, c1.x, c1.y), hi = make_uint4(c2.x, c2.y, c3.x, c3.y);
+                    *reinterpret_cast<uint4*>(line + (((c + swap) ^ (t & 7)) << 4)) = swap ? hi : lo;
+                    *reinterpret_cast<uint4*>(line + (((c + !swap) ^ (t & 7)) << 4)) = swap ? lo : hi;
+                }
+                if constexpr (MODE != TMA) {
+                    uint8_t* B = A + a_bytes;
+#pragma unroll
+                    for (int i = 0; i < B_PER; ++i) {
+                        const int piece = tid + i * CONVERTERS, t = piece / chunks, g = piece % chunks;
+                        if (piece >= BK * chunks) break;
+#pragma unroll
+                        for (int part = 0; part < P; ++part) {
+                            float h[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) h[k] = part_of(v[i][k]);
+                            *reinterpret_cast<uint4*>(B + (part * groups + (g >> 3)) * GROUP + t * 128 + (((g & 7) ^ (t & 7)) << 4)) =
+                                umma::pack_chunk(h);
+                        }
+                    }
+                }
+                umma::fence_async_smem();
+                __syncwarp();
+                if (lane == 0) arrive(&sh.full_a[slot]);
+                if (s + 1 < seg.last) fetch(seg, s + 1);
+                else if (another) fetch(following, following.first);
+            }
+            // the tile out of TMEM: warps w and w + 4 share lanes 32 (w % 4) ...
+            ok = ok && wait_all(&sh.acc_full, done & 1);
+            umma::fence_after_sync();
+            const int64_t k0 = seg.tile % p.ktiles * p.mt * 128, n0 = seg.tile / p.ktiles * p.bn;
+            const int row = (w & 3) * 32 + lane;
+            const int chunks_out = p.bn / 32;
+            for (int i = w >> 2; i < p.mt * chunks_out; i += 2) {
+                const int m = i / chunks_out, c = i % chunks_out * 32;
+                float x[32];
+                const uint32_t from = tmem + ((uint32_t)(w & 3) * 32 << 16) + m * P * p.bn + c;
+                umma::tmem_ld32(from + (P - 1) * p.bn, x);  // the smallest part first
+#pragma unroll
+                for (int part = P - 2; part >= 0; --part) {
+                    float y[32];
+                    umma::tmem_ld32(from + part * p.bn, y);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] += y[e];
+                }
+                if (!ok)
+                    for (float& e : x) e = __uint_as_float(0x7fffffffu);
+                const int64_t k = k0 + m * 128 + row, n = n0 + c;
+                if (!seg.whole) {
+                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)p.mt * 128 + m * 128 + row) * p.bn + c;
+                    if (!seg.begins) add_run(x, to, 32, true);
+                    store_run(to, x, 32, true);
+                } else if (k < a.k && n < a.n) {
+                    const int count = (int)min((int64_t)32, a.n - n);
+                    const int64_t to = k * a.n + n;
+                    const bool vec = ((uintptr_t)a.dw & 15) == 0 && a.n % 8 == 0;
+                    if (a.out_type == WC_F32) {
+                        if (!seg.begins) add_run(x, static_cast<float*>(a.dw) + to, count, vec);
+                        store_run(static_cast<float*>(a.dw) + to, x, count, vec);
+                    } else if (a.out_type == WC_F16) {
+                        store_run(static_cast<__half*>(a.dw) + to, x, count, vec);
+                    } else {
+                        store_run(static_cast<__nv_bfloat16*>(a.dw) + to, x, count, vec);
+                    }
+                }
+            }
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(&sh.acc_empty);
+            ++done;
+            seg = following, more = another;
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == 0) umma::tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// Joins the split tiles: 32 columns of one row a warp row, the CTAs that
+// share the tile dealt to the warps and joined in order. Row mt * 128 is db.
+template <class T>
+__global__ void k_wgrad8_join(wc_act8_wgrad_args a, Plan p, const float* part, const float* part_db) {
+    __shared__ float s[32][33];
+    for (int64_t tile = blockIdx.y; tile < (int64_t)p.ktiles * p.ntiles; tile += gridDim.y) {
+    const int64_t u0 = tile * p.steps, u1 = u0 + p.steps;
+    // the CTA that unit u falls to: the last c with units c / ctas <= u
+    auto owner = [&](int64_t u) { return ((u + 1) * p.ctas - 1) / p.units; };
+    const int64_t c0 = owner(u0), c1 = owner(u1 - 1);
+    if (c0 == c1) continue;
+    const int rows = p.mt * 128, runs = p.bn / 32;
+    const int64_t k0 = tile % p.ktiles * rows, n0 = tile / p.ktiles * p.bn;
+    for (int i = blockIdx.x; i < (rows + 1) * runs; i += gridDim.x) {
+        const int r = i / runs, c = i % runs * 32 + threadIdx.x;
+        const bool bias = r == rows;
+        if (bias ? (!a.db || tile % p.ktiles) : k0 + r >= a.k) continue;
+        float v = 0.0f;
+        for (int64_t j = c0 + threadIdx.y; j <= c1; j += blockDim.y) {
+            const int64_t slot = 2 * j + (p.units * j / p.ctas / p.steps == tile ? 0 : 1);
+            v += bias ? part_db[slot * p.bn + c] : part[(slot * rows + r) * p.bn + c];
+        }
+        s[threadIdx.y][threadIdx.x] = v;
+        __syncthreads();
+        if (threadIdx.y == 0 && n0 + c < a.n) {
+            for (int j = 1; j < (int)blockDim.y; ++j) v += s[j][threadIdx.x];
+            if (bias) a.db[n0 + c] = v;
+            else static_cast<T*>(a.dw)[(k0 + r) * a.n + n0 + c] = from_f<T>(v);
         }
         __syncthreads();
-#pragma unroll
-        for (int d = 0; d < DEEP; ++d)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float y = sy[d][tn + j];
-                db[j] += y;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc[i][j] += sx[d][tk + i] * y;
-            }
-        __syncthreads();
     }
-    float* to = part + (int64_t)blockIdx.z * (a.k + 1) * a.n;
-    for (int j = 0; j < 4; ++j) {
-        if (n0 + tn + j >= a.n) continue;
-        for (int i = 0; i < 4; ++i)
-            if (k0 + tk + i < a.k) to[(k0 + tk + i) * a.n + n0 + tn + j] = acc[i][j];
-        if (blockIdx.x == 0 && tk == 0) to[a.k * a.n + n0 + tn + j] = db[j];
     }
 }
 
-int64_t tiles(int64_t n) { return (n + TILE - 1) / TILE; }
-int64_t splits_of(const wc_act8_wgrad_args& a) {
-    const int64_t t = tiles(a.k) * tiles(a.n), want = t >= 592 ? 1 : 592 / t, most = (a.rows + 255) / 256;
-    return most < 1 ? 1 : most < want ? most : want;
+int mode_of(const wc_act8_wgrad_args& a) {
+    if (a.type == WC_F32) return F32;
+    if (a.type == WC_F16) return F16;
+    return ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0 && a.rows ? TMA : BF16;
+}
+
+Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
+    Plan p{};
+    const int64_t k = std::max<int64_t>(a.k, 1);
+    p.steps = std::max<int64_t>(1, (a.rows + BK - 1) / BK);
+    p.mt = k > 128 ? 2 : 1;
+    int64_t nt = (a.n + widest(mode) - 1) / widest(mode);
+    p.bn = (int)(((a.n + nt - 1) / nt + 31) / 32 * 32);
+    p.ktiles = (int)((k + p.mt * 128 - 1) / (p.mt * 128));
+    p.ntiles = (int)((a.n + p.bn - 1) / p.bn);
+    p.units = (int64_t)p.ktiles * p.ntiles * p.steps;
+    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(148, p.steps == 1 ? p.units : (p.units + 1) / 2));
+    p.joined = p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0;
+    p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
+    p.b_bytes = parts_of(mode) * ((p.bn + 63) / 64) * GROUP;
+    p.stages = std::min(MAX_STAGES, RING / p.stage_bytes());
+    return p;
+}
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                            CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+    static const Encode fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult st;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &st) != cudaSuccess ||
+            st != cudaDriverEntryPointSuccess)
+            throw std::runtime_error("cuTensorMapEncodeTiled is not available");
+        return reinterpret_cast<Encode>(f);
+    }();
+    return fn;
+}
+
+// dy as boxes of 64 columns x 64 rows, 128-byte swizzled, zeros outside
+CUtensorMap dy_map(const wc_act8_wgrad_args& a) {
+    CUtensorMap m;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.n, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.ld_dy * 2};
+    const cuuint32_t box[2] = {64, BK}, step[2] = {1, 1};
+    if (encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.dy), dims, strides, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        throw std::runtime_error("the tensor map of dy was refused");
+    return m;
+}
+
+template <int MODE, class T>
+void launch_mode(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
+    CUtensorMap dy{};
+    if (MODE == TMA) dy = dy_map(a);
+    const size_t smem = (size_t)p.stages * p.stage_bytes() + 1024;
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<MODE, T>), RING + 1024)) return;
+    k_wgrad8<MODE, T><<<p.ctas, THREADS, smem, s>>>(a, p, dy, part, part_db);
 }
 
 template <class T>
-void launch_type(const wc_act8_wgrad_args& a, cudaStream_t s) {
-    const int64_t z = splits_of(a);
-    float* part = static_cast<float*>(a.workspace);
-    k_wgrad8<T><<<dim3((unsigned)tiles(a.k), (unsigned)tiles(a.n), (unsigned)z), THREADS, 0, s>>>(a, (a.rows + z - 1) / z, part);
-    const int64_t ld = (a.k + 1) * a.n;
-    if (a.out_type == WC_F32) launch_colsum<float>(part, z, ld, a.k * a.n, static_cast<float*>(a.dw), s);
-    else if (a.out_type == WC_F16) launch_colsum<__half>(part, z, ld, a.k * a.n, static_cast<__half*>(a.dw), s);
-    else launch_colsum<__nv_bfloat16>(part, z, ld, a.k * a.n, static_cast<__nv_bfloat16*>(a.dw), s);
-    if (a.db) launch_colsum<float>(part + a.k * a.n, z, ld, a.n, a.db, s);
+void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, const float* part_db, cudaStream_t s) {
+    const int64_t shared_by = p.ctas / ((int64_t)p.ktiles * p.ntiles) + 2;
+    const dim3 block(32, shared_by >= 8 ? 32 : 4), grid((p.mt * 128 + 1) * (p.bn / 32), std::min<int64_t>(65535, (int64_t)p.ktiles * p.ntiles));
+    k_wgrad8_join<T><<<grid, block, 0, s>>>(a, p, part, part_db);
 }
 
 }  // namespace
 
 uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
-    return a.k && a.n ? (uint64_t)splits_of(a) * (a.k + 1) * a.n * sizeof(float) : 0;
+    if (!a.n) return 0;
+    uint64_t most = 0;
+    const Plan p = plan_of(a, mode_of(a));
+    if (p.joined) most = (uint64_t)2 * p.ctas * (p.mt * 128 + 1) * p.bn * sizeof(float);
+    return most;
 }
 
 void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
-    if (a.type == WC_F32) launch_type<float>(a, s);
-    else if (a.type == WC_F16) launch_type<__half>(a, s);
-    else launch_type<__nv_bfloat16>(a, s);
+    const int mode = mode_of(a);
+    const Plan p = plan_of(a, mode);
+    float* part = static_cast<float*>(a.workspace);
+    float* part_db = part + (int64_t)2 * p.ctas * p.mt * 128 * p.bn;
+    if (mode == TMA) launch_mode<TMA, __nv_bfloat16>(a, p, part, part_db, s);
+    else if (mode == BF16) launch_mode<BF16, __nv_bfloat16>(a, p, part, part_db, s);
+    else if (mode == F16) launch_mode<F16, __half>(a, p, part, part_db, s);
+    else launch_mode<F32, float>(a, p, part, part_db, s);
+    if (!p.joined) return;
+    if (a.out_type == WC_F32) launch_join<float>(a, p, part, part_db, s);
+    else if (a.out_type == WC_F16) launch_join<__half>(a, p, part, part_db, s);
+    else launch_join<__nv_bfloat16>(a, p, part, part_db, s);
 }
 
 }  // namespace wctrain
