@@ -36,7 +36,7 @@ namespace {
 constexpr int BK = 64;           // rows of a stage
 constexpr int GROUP = BK * 128;  // bytes of 64 columns of a stage
 constexpr int CONVERTERS = 256, THREADS = CONVERTERS + 128;
-constexpr int MAX_STAGES = 8;
+constexpr int MAX_STAGES = 8, MAX_CTAS = 148;
 constexpr int RING = 220 * 1024;  // shared memory of the stages
 constexpr uint32_t TMEM_COLS = 512;
 
@@ -184,7 +184,7 @@ struct Walk {
     }
 };
 
-template <int MODE, class T>
+template <int MODE, int MT, class T>
 __global__ void __launch_bounds__(THREADS, 1)
     k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
     constexpr int P = parts_of(MODE);
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     __shared__ Shared sh;
     uint8_t* ring = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stage_bytes = p.stage_bytes(), a_bytes = p.mt * 2 * GROUP;
+    const int stage_bytes = p.stage_bytes(), a_bytes = MT * 2 * GROUP;
     const int groups = (p.bn + 63) / 64;
     volatile int* failed = &sh.failed;
 
@@ -238,7 +238,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 umma::fence_after_sync();
                 if (lane == 0) {
                     const uint32_t A = umma::smem_u32(ring + slot * stage_bytes), B = A + a_bytes;
-                    for (int m = 0; m < p.mt; ++m)
+                    for (int m = 0; m < MT; ++m)
                         for (int q = 0; q < P; ++q)
 #pragma unroll
                             for (int k = 0; k < BK / 16; ++k)
@@ -288,20 +288,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!ok) break;
                 if (mine) {
                     const uint8_t* B = ring + slot * stage_bytes + a_bytes;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = 2 * at + 128 * h;  // this thread's pair of columns
-                        if (c >= p.bn) continue;
-                        float x = 0.0f, y = 0.0f;
+const int c = 4 * at;  // this thread's four columns
+                    if (c < p.bn) {
+                        float x[4] = {};
                         for (int q = 0; q < P; ++q) {
-                            const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 7) * 2;
-#pragma unroll 8
+                            const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
+#pragma unroll 16
                             for (int t = 0; t < BK; ++t) {
-                                const uint32_t w = *reinterpret_cast<const uint32_t*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
-                                x += umma::Op16<false>::lo(w), y += umma::Op16<false>::hi(w);
+                                const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
+                                x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
+                                x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
                             }
                         }
-                        sum[2 * h] += x, sum[2 * h + 1] += y;
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) sum[h] += x[h];
                     }
                 }
                 __syncwarp();
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    const int c = 2 * at + 128 * (h >> 1) + (h & 1);
+                    const int c = 4 * at + h;
                     if (c >= p.bn) continue;
                     const float v = ok ? sum[h] : nan;
                     if (!seg.whole) part_db[(2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)p.bn + c] = v;
@@ -322,32 +322,39 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else {  // -------------------------------------------------- converters
         const int tid = threadIdx.x - 128, w = warp - 4;
+        // x8: a piece is 16 channels of one row; a thread has 2 MT of a stage, all at the same channels. dy (where it
+        // does not come by TMA): chunks of 8 columns, all of a thread's at the same columns.
+        constexpr int A_PER = 2 * MT, A_ROW = 8 * MT, A_STEP = CONVERTERS / A_ROW;
+        constexpr int B_PER = MODE == TMA ? 1 : BK * widest(MODE) / 8 / CONVERTERS;
         const int64_t blocks = (a.k + 31) / 32;
-        const T* dy = static_cast<const T*>(a.dy);
+        const int at = tid / A_ROW, ag = tid % A_ROW;
+        const int b_bits = groups > 1 ? 4 : 3, bt = tid >> b_bits, bg = tid & ((1 << b_bits) - 1), b_step = CONVERTERS >> b_bits;
         const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
-        // x8: piece i of a stage is 16 channels of one row; a thread has 2 mt of them
-        constexpr int B_PER = BK * widest(MODE) / 8 / CONVERTERS;  // chunks of 8 columns of dy
-        uint4 q[4];
-        uint32_t code[4];
-        float v[MODE == TMA ? 1 : B_PER][8];
-        const int per_row = 8 * p.mt, chunks = groups * 8;
-        auto fetch = [&](const Run& g, int s) {
-            const int64_t k0 = g.tile % p.ktiles * p.mt * 128, n0 = g.tile / p.ktiles * p.bn;
+        uint4 q[A_PER];
+        uint32_t code[A_PER];
+        float v[B_PER][8];
+        int64_t fk = 0, fn = 0;  // first channel and column of this thread in the tile being fetched
+        auto aim = [&](const Run& g) {
+            fk = g.tile % p.ktiles * (MT * 128) + ag * 16;
+            fn = g.tile / p.ktiles * p.bn + bg * 8;
+        };
+        auto fetch = [&](int s) {
+            const int64_t t0 = (int64_t)s * BK;
+            const int rows = (int)min((int64_t)BK, a.rows - t0);
+            const int8_t* from = a.q + (t0 + at) * (blocks * 32) + fk;
+            const uint8_t* unit = a.scale + (t0 + at) * blocks + (fk >> 5);
+            const bool in = fk < blocks * 32;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (i >= 2 * p.mt) break;
-                const int piece = tid + i * CONVERTERS;
-                const int64_t t = (int64_t)s * BK + piece / per_row, k = k0 + piece % per_row * 16;
-                const bool in = t < a.rows && k < blocks * 32;
-                q[i] = in ? *reinterpret_cast<const uint4*>(a.q + t * blocks * 32 + k) : make_uint4(0, 0, 0, 0);
-                code[i] = in ? a.scale[t * blocks + (k >> 5)] : 127u;
+            for (int i = 0; i < A_PER; ++i) {
+                const bool here = in && at + i * A_STEP < rows;
+                q[i] = here ? *reinterpret_cast<const uint4*>(from + i * A_STEP * blocks * 32) : make_uint4(0, 0, 0, 0);
+                code[i] = here ? unit[i * A_STEP * blocks] : 127u;
             }
             if constexpr (MODE != TMA) {
+                const T* dy = static_cast<const T*>(a.dy) + (t0 + bt) * a.ld_dy;
 #pragma unroll
                 for (int i = 0; i < B_PER; ++i) {
-                    const int piece = tid + i * CONVERTERS;
-                    const int64_t t = (int64_t)s * BK + piece / chunks, n = n0 + piece % chunks * 8;
-                    if (piece < BK * chunks && t < a.rows) load_dy(dy + t * a.ld_dy, n, a.n, vec_dy, v[i]);
+                    if (bt + i * b_step < rows) load_dy(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy, v[i]);
                     else
                         for (float& x : v[i]) x = 0.0f;
                 }
@@ -355,7 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         };
         bool ok = true, more = walk.next(seg);
         uint32_t done = 0;
-        if (more) fetch(seg, seg.first);
+        if (more) aim(seg), fetch(seg.first);
         while (more) {
             Run following;
             const bool another = walk.next(following);
@@ -363,59 +370,56 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
                 if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
                 uint8_t* A = ring + slot * stage_bytes;
+                uint8_t* line = A + (ag >> 2) * GROUP + at * 128;
+                const int c = (ag & 3) * 2;
+                // odd groups store their second chunk first: the threads of a row then fill different chunks at a time
+                const int swap = (ag >> 2) & 1;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i >= 2 * p.mt) break;
-                    const int piece = tid + i * CONVERTERS, t = piece / per_row, g = piece % per_row;
-                    const uint16_t ub = code[i] == 255 ? (uint16_t)0x7fff : (uint16_t)(code[i] << 7);
-                    const uint32_t uu = ub * 0x10001u;
+                for (int i = 0; i < A_PER; ++i, line += A_STEP * 128) {
+                    const int t7 = (at + i * A_STEP) & 7;
+                    const uint32_t uu = (code[i] == 255 ? 0x7fffu : code[i] << 7) * 0x10001u;
                     const __nv_bfloat162 unit = *reinterpret_cast<const __nv_bfloat162*>(&uu);
                     const uint2 c0 = four(q[i].x, unit), c1 = four(q[i].y, unit), c2 = four(q[i].z, unit), c3 = four(q[i].w, unit);
-                    uint8_t* line = A + (g >> 2) * GROUP + t * 128;
-                    const int c = (g & 3) * 2;
-                    // the odd groups store their second chunk first: the 8 threads of a row then fill 8 different chunks
-                    const bool swap = (g >> 2) & 1;
                     const uint4 lo = make_uint4(c0.x, c0.y, c1.x, c1.y), hi = make_uint4(c2.x, c2.y, c3.x, c3.y);
-                    *reinterpret_cast<uint4*>(line + (((c + swap) ^ (t & 7)) << 4)) = swap ? hi : lo;
-                    *reinterpret_cast<uint4*>(line + (((c + !swap) ^ (t & 7)) << 4)) = swap ? lo : hi;
+                    *reinterpret_cast<uint4*>(line + (((c + swap) ^ t7) << 4)) = swap ? hi : lo;
+                    *reinterpret_cast<uint4*>(line + (((c + 1 - swap) ^ t7) << 4)) = swap ? lo : hi;
                 }
                 if constexpr (MODE != TMA) {
-                    uint8_t* B = A + a_bytes;
+                    uint8_t* B = A + a_bytes + (bg >> 3) * GROUP;
 #pragma unroll
                     for (int i = 0; i < B_PER; ++i) {
-                        const int piece = tid + i * CONVERTERS, t = piece / chunks, g = piece % chunks;
-                        if (piece >= BK * chunks) break;
+                        const int t = bt + i * b_step;
+                        if (t >= BK) break;
 #pragma unroll
-                        for (int part = 0; part < P; ++part) {
+                        for (int q = 0; q < P; ++q) {
                             float h[8];
 #pragma unroll
                             for (int k = 0; k < 8; ++k) h[k] = part_of(v[i][k]);
-                            *reinterpret_cast<uint4*>(B + (part * groups + (g >> 3)) * GROUP + t * 128 + (((g & 7) ^ (t & 7)) << 4)) =
-                                umma::pack_chunk(h);
+                            *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
                         }
                     }
                 }
                 umma::fence_async_smem();
                 __syncwarp();
                 if (lane == 0) arrive(&sh.full_a[slot]);
-                if (s + 1 < seg.last) fetch(seg, s + 1);
-                else if (another) fetch(following, following.first);
+                if (s + 1 < seg.last) fetch(s + 1);
+                else if (another) aim(following), fetch(following.first);
             }
             // the tile out of TMEM: warps w and w + 4 share lanes 32 (w % 4) ...
             ok = ok && wait_all(&sh.acc_full, done & 1);
             umma::fence_after_sync();
-            const int64_t k0 = seg.tile % p.ktiles * p.mt * 128, n0 = seg.tile / p.ktiles * p.bn;
+            const int64_t k0 = seg.tile % p.ktiles * MT * 128, n0 = seg.tile / p.ktiles * p.bn;
             const int row = (w & 3) * 32 + lane;
             const int chunks_out = p.bn / 32;
-            for (int i = w >> 2; i < p.mt * chunks_out; i += 2) {
+            for (int i = w >> 2; i < MT * chunks_out; i += 2) {
                 const int m = i / chunks_out, c = i % chunks_out * 32;
                 float x[32];
                 const uint32_t from = tmem + ((uint32_t)(w & 3) * 32 << 16) + m * P * p.bn + c;
                 umma::tmem_ld32(from + (P - 1) * p.bn, x);  // the smallest part first
 #pragma unroll
-                for (int part = P - 2; part >= 0; --part) {
+                for (int q = P - 2; q >= 0; --q) {
                     float y[32];
-                    umma::tmem_ld32(from + part * p.bn, y);
+                    umma::tmem_ld32(from + q * p.bn, y);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) x[e] += y[e];
                 }
@@ -423,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (float& e : x) e = __uint_as_float(0x7fffffffu);
                 const int64_t k = k0 + m * 128 + row, n = n0 + c;
                 if (!seg.whole) {
-                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)p.mt * 128 + m * 128 + row) * p.bn + c;
+                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + row) * p.bn + c;
                     if (!seg.begins) add_run(x, to, 32, true);
                     store_run(to, x, 32, true);
                 } else if (k < a.k && n < a.n) {
@@ -452,37 +456,66 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 0) umma::tmem_dealloc(tmem, TMEM_COLS);
 }
 
-// Joins the split tiles: 32 columns of one row a warp row, the CTAs that
-// share the tile dealt to the warps and joined in order. Row mt * 128 is db.
-template <class T>
-__global__ void k_wgrad8_join(wc_act8_wgrad_args a, Plan p, const float* part, const float* part_db) {
-    __shared__ float s[32][33];
-    for (int64_t tile = blockIdx.y; tile < (int64_t)p.ktiles * p.ntiles; tile += gridDim.y) {
-    const int64_t u0 = tile * p.steps, u1 = u0 + p.steps;
-    // the CTA that unit u falls to: the last c with units c / ctas <= u
-    auto owner = [&](int64_t u) { return ((u + 1) * p.ctas - 1) / p.units; };
-    const int64_t c0 = owner(u0), c1 = owner(u1 - 1);
-    if (c0 == c1) continue;
-    const int rows = p.mt * 128, runs = p.bn / 32;
-    const int64_t k0 = tile % p.ktiles * rows, n0 = tile / p.ktiles * p.bn;
-    for (int i = blockIdx.x; i < (rows + 1) * runs; i += gridDim.x) {
-        const int r = i / runs, c = i % runs * 32 + threadIdx.x;
-        const bool bias = r == rows;
-        if (bias ? (!a.db || tile % p.ktiles) : k0 + r >= a.k) continue;
-        float v = 0.0f;
-        for (int64_t j = c0 + threadIdx.y; j <= c1; j += blockDim.y) {
-            const int64_t slot = 2 * j + (p.units * j / p.ctas / p.steps == tile ? 0 : 1);
-            v += bias ? part_db[slot * p.bn + c] : part[(slot * rows + r) * p.bn + c];
+// The tiles that fall to several CTAs, at most one for each boundary between
+// two CTAs: the CTAs' numbers, and the slot of the first one's partial result
+// (the others' is their first, 2 c).
+struct Split {
+    int tile, slot;
+    short c0, c1;
+};
+struct Splits {
+    int n;
+    Split at[MAX_CTAS];
+    Splits(const Plan& p) : n(0) {
+        auto start = [&](int64_t c) { return p.units * c / p.ctas; };
+        for (int c = 0; c + 1 < p.ctas; ++c) {
+            const int64_t cut = start(c + 1), tile = cut / p.steps, u0 = tile * p.steps;
+            if (cut == u0) continue;                                                  // between two tiles
+            if (n && at[n - 1].tile == tile) at[n - 1].c1 = (short)(c + 1);           // one more boundary of the same
+            else at[n++] = Split{(int)tile, 2 * c + (start(c) >= u0 ? 0 : 1), (short)c, (short)(c + 1)};
         }
-        s[threadIdx.y][threadIdx.x] = v;
-        __syncthreads();
-        if (threadIdx.y == 0 && n0 + c < a.n) {
-            for (int j = 1; j < (int)blockDim.y; ++j) v += s[j][threadIdx.x];
-            if (bias) a.db[n0 + c] = v;
-            else static_cast<T*>(a.dw)[(k0 + r) * a.n + n0 + c] = from_f<T>(v);
-        }
-        __syncthreads();
     }
+};
+
+// Joins the split tiles (one a blockIdx.y). A thread has 4 columns of a row
+// (row mt * 128 is db); with many CTAs to a tile they are dealt to blockDim.y
+// threads and those joined in order.
+constexpr int JOINERS = 256;
+template <class T>
+__global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, Plan p, const __grid_constant__ Splits splits,
+                                                         const float* part, const float* part_db) {
+    __shared__ float4 s[JOINERS];
+    const Split& cut = splits.at[blockIdx.y];
+    const int tile = cut.tile, c0 = cut.c0, c1 = cut.c1;
+    const int rows = p.mt * 128, runs = p.bn / 4;
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, r = i / runs, c = i % runs * 4;
+    const int64_t k0 = tile % p.ktiles * rows, n0 = tile / p.ktiles * p.bn, n = n0 + c;
+    const bool bias = r == rows;
+    const bool in = r <= rows && n < a.n && (bias ? a.db && tile % p.ktiles == 0 : k0 + r < a.k);
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (in)
+#pragma unroll 4
+        for (int j = c0 + (int)threadIdx.y; j <= c1; j += blockDim.y) {
+            const int64_t slot = j == c0 ? cut.slot : 2 * j;
+            const float4 w = *reinterpret_cast<const float4*>(bias ? part_db + slot * p.bn + c : part + (slot * rows + r) * p.bn + c);
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+    if (blockDim.y > 1) {
+        s[threadIdx.y * blockDim.x + threadIdx.x] = v;
+        __syncthreads();
+        if (threadIdx.y) return;
+        for (int j = 1; j < (int)blockDim.y; ++j) {
+            const float4 w = s[j * blockDim.x + threadIdx.x];
+            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+    }
+    if (!in) return;
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (n + j >= a.n) break;
+        if (bias) a.db[n + j] = e[j];
+        else static_cast<T*>(a.dw)[(k0 + r) * a.n + n + j] = from_f<T>(e[j]);
     }
 }
 
@@ -502,8 +535,8 @@ Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
     p.ktiles = (int)((k + p.mt * 128 - 1) / (p.mt * 128));
     p.ntiles = (int)((a.n + p.bn - 1) / p.bn);
     p.units = (int64_t)p.ktiles * p.ntiles * p.steps;
-    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(148, p.steps == 1 ? p.units : (p.units + 1) / 2));
-    p.joined = p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0;
+    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
+    p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
     p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
     p.b_bytes = parts_of(mode) * ((p.bn + 63) / 64) * GROUP;
     p.stages = std::min(MAX_STAGES, RING / p.stage_bytes());
@@ -537,20 +570,28 @@ CUtensorMap dy_map(const wc_act8_wgrad_args& a) {
     return m;
 }
 
-template <int MODE, class T>
-void launch_mode(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
+template <int MODE, int MT, class T>
+void launch_tile(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
     CUtensorMap dy{};
     if (MODE == TMA) dy = dy_map(a);
     const size_t smem = (size_t)p.stages * p.stage_bytes() + 1024;
-    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<MODE, T>), RING + 1024)) return;
-    k_wgrad8<MODE, T><<<p.ctas, THREADS, smem, s>>>(a, p, dy, part, part_db);
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<MODE, MT, T>), RING + 1024)) return;
+    k_wgrad8<MODE, MT, T><<<p.ctas, THREADS, smem, s>>>(a, p, dy, part, part_db);
+}
+template <int MODE, class T>
+void launch_mode(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
+    if (p.mt == 2) launch_tile<MODE, 2, T>(a, p, part, part_db, s);
+    else launch_tile<MODE, 1, T>(a, p, part, part_db, s);
 }
 
 template <class T>
 void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, const float* part_db, cudaStream_t s) {
-    const int64_t shared_by = p.ctas / ((int64_t)p.ktiles * p.ntiles) + 2;
-    const dim3 block(32, shared_by >= 8 ? 32 : 4), grid((p.mt * 128 + 1) * (p.bn / 32), std::min<int64_t>(65535, (int64_t)p.ktiles * p.ntiles));
-    k_wgrad8_join<T><<<grid, block, 0, s>>>(a, p, part, part_db);
+    const Splits splits(p);
+    int sharers = 0;
+    for (int i = 0; i < splits.n; ++i) sharers = std::max(sharers, splits.at[i].c1 - splits.at[i].c0 + 1);
+    const int ny = sharers >= 8 ? 32 : 1;
+    const dim3 block(JOINERS / ny, ny), grid(((p.mt * 128 + 1) * (p.bn / 4) + block.x - 1) / block.x, splits.n);
+    k_wgrad8_join<T><<<grid, block, 0, s>>>(a, p, splits, part, part_db);
 }
 
 }  // namespace
