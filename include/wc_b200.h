@@ -483,7 +483,7 @@ int wc_block_norm_backward(const wc_block_norm_args* a, const wc_block_norm_grad
  * smallest power of two (at least 2^-126) that its largest value allows. A
  * value reads back as q 2^(scale - 127), rounded to nearest-even when it was
  * stored: at most half a unit off, and exact in bf16. A block that holds an
- * infinity or NaN has scale 255 and reads back as NaN.
+ * infinity or NaN has scale 255 and q 0, and reads back as NaN.
  * wc_act8_pack:   x -> q, scale.            wc_act8_unpack: q, scale -> out.
  * wc_gelu8:       out = GELU(x + bias) (tanh form), and the 32-bit sum
  *                 x + bias to q, scale.

@@ -34,6 +34,7 @@ namespace wctrain {
 namespace {
 
 constexpr int BK = 64;           // rows of a stage
+constexpr int AHEAD = 6;         // stages by which x8 is prefetched into L2
 constexpr int GROUP = BK * 128;  // bytes of 64 columns of a stage
 constexpr int CONVERTERS = 256, THREADS = CONVERTERS + 128;
 constexpr int MAX_STAGES = 8, MAX_CTAS = 148;
@@ -74,21 +75,24 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                  "l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(bar))
                  : "memory");
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
 }
 
-// 4 bytes to two pairs of bf16 times `unit` (a bf16 pair). A byte's low seven
-// bits are the mantissa of 128 + them; its sign bit, worth -128, is the
-// exponent step from 128 to 256: (128 + low) - (128 or 256) is the byte.
-__device__ __forceinline__ uint32_t two(uint32_t w, __nv_bfloat162 unit) {
+// Bytes 0 and 2 of `w` as a pair of bf16 times `unit` (a bf16 pair). A byte's
+// low seven bits are the mantissa of 128 + them; its sign bit, worth -128, is
+// the exponent step from 128 to 256: (128 + low) - (128 or 256) is the byte.
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w, __nv_bfloat162 unit) {
     const uint32_t a = (w & 0x007f007fu) | 0x43004300u, b = (w & 0x00800080u) | 0x43004300u;
     const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b)), unit);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ uint2 four(uint32_t q, __nv_bfloat162 unit) {
-    return make_uint2(two(__byte_perm(q, 0, 0x4140), unit), two(__byte_perm(q, 0, 0x4342), unit));
+// 8 bytes to 8 bf16; of each four, the middle two change places (the rows of the tile do, see channel())
+__device__ __forceinline__ uint4 eight_bytes(uint32_t x, uint32_t y, __nv_bfloat162 unit) {
+    return make_uint4(even_bytes(x, unit), even_bytes(x >> 8, unit), even_bytes(y, unit), even_bytes(y >> 8, unit));
 }
+__device__ __forceinline__ int channel(int row) { return (row & ~3) | (row & 1) << 1 | (row >> 1 & 1); }
 
 // Part `p` of v as bf16 and what is left for the next ones. An infinity or NaN goes whole into the first.
 __device__ __forceinline__ float part_of(float& v) {
@@ -97,19 +101,30 @@ __device__ __forceinline__ float part_of(float& v) {
     return hi;
 }
 
+// 8 values of a row as they lie in memory; past the width they are 0
 template <class T>
-__device__ __forceinline__ void load_dy(const T* p, int64_t n, int64_t width, bool vec, float* v) {
-    if (vec && n + 8 <= width) {
+struct Eight {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, int64_t n, int64_t width, bool vec) {
+        if (vec && n + 8 <= width) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p + n)[i];
+        } else {
+            alignas(16) T e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) e[i] = n + i < width ? p[n + i] : from_f<T>(0.0f);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+        }
+    }
+    __device__ __forceinline__ void get(float* v) const {
         alignas(16) T e[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p + n)[i];
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(e)[i] = w[i];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = n + i < width ? to_f(p[n + i]) : 0.0f;
     }
-}
+};
 
 template <class T>
 __device__ __forceinline__ void store_run(T* p, const float* v, int count, bool vec) {
@@ -180,6 +195,24 @@ struct Walk {
         r.whole = s0 == 0 && s1 == steps;
         r.begins = s == s0, r.ends = r.last == s1;
         s = r.last;
+        return true;
+    }
+};
+
+// The stages that fall to a CTA, one at a time
+struct Cursor {
+    Walk walk;
+    Run run;
+    int s = 0;
+    bool more;
+    __device__ Cursor(const Plan& p) : walk(p) { enter(); }
+    __device__ void enter() {
+        more = walk.next(run);
+        s = more ? run.first : 0;
+    }
+    __device__ bool step() {  // true: on to another run
+        if (++s < run.last) return false;
+        enter();
         return true;
     }
 };
@@ -258,22 +291,42 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma::mbar_wait(&sh.acc_full, (done - 1) & 1, umma::DRAIN_NS);
         }
     } else if (warp == 1) {  // ------------------------------------ producer
-        if (MODE == TMA && lane == 0) {
-            bool ok = true;
-            while (ok && walk.next(seg)) {
-                const int n0 = (int)(seg.tile / p.ktiles) * p.bn;
-                for (int s = seg.first; s < seg.last; ++s, ++it) {
-                    const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
-                    if (it >= (uint32_t)p.stages && !(ok = wait(&sh.empty[slot], ph ^ 1))) break;
+bool ok = true;
+        const int64_t blocks = (a.k + 31) / 32;
+        Cursor ahead(p);
+        // the lines of x8 and its units of one stage into L2, for the converters' loads of a few stages later
+        auto prefetch = [&] {
+            if (!ahead.more) return;
+            const int64_t k0 = ahead.run.tile % p.ktiles * (MT * 128), t0 = (int64_t)ahead.s * BK;
+#pragma unroll
+            for (int i = 0; i < BK / 32; ++i) {
+                const int64_t t = t0 + i * 32 + lane;
+                if (t >= a.rows) break;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (k0 + m * 128 < blocks * 32) prefetch_l2(a.q + t * blocks * 32 + k0 + m * 128);
+                if (k0 < blocks * 32) prefetch_l2(a.scale + t * blocks + k0 / 32);
+            }
+            ahead.step();
+        };
+        for (int i = 0; i < AHEAD; ++i) prefetch();
+        while (ok && walk.next(seg)) {
+            const int n0 = (int)(seg.tile / p.ktiles) * p.bn;
+            for (int s = seg.first; s < seg.last; ++s, ++it) {
+                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
+                if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
+                if (MODE == TMA && lane == 0) {
                     umma::expect_tx(&sh.full_b[slot], groups * GROUP);
                     const uint32_t B = umma::smem_u32(ring + slot * stage_bytes) + a_bytes;
                     for (int g = 0; g < groups; ++g) tma_load(B + g * GROUP, &map_dy, n0 + 64 * g, s * BK, &sh.full_b[slot]);
                 }
+                __syncwarp();
+                prefetch();
             }
-            if (!ok)  // the copies in flight land before the CTA leaves
-                for (uint32_t i = it > (uint32_t)p.stages ? it - p.stages : 0; i < it; ++i)
-                    umma::mbar_wait(&sh.full_b[i % p.stages], (i / p.stages) & 1, umma::DRAIN_NS);
         }
+        if (MODE == TMA && !ok)  // the copies in flight land before the CTA leaves
+            for (uint32_t i = it > (uint32_t)p.stages ? it - p.stages : 0; i < it; ++i)
+                umma::mbar_wait(&sh.full_b[i % p.stages], (i / p.stages) & 1, umma::DRAIN_NS);
     } else if (warp < 4) {  // --------------------------------- column sums
         const int at = threadIdx.x - 64;
         bool ok = true;
@@ -322,88 +375,97 @@ const int c = 4 * at;  // this thread's four columns
         }
     } else {  // -------------------------------------------------- converters
         const int tid = threadIdx.x - 128, w = warp - 4;
-        // x8: a piece is 16 channels of one row; a thread has 2 MT of a stage, all at the same channels. dy (where it
-        // does not come by TMA): chunks of 8 columns, all of a thread's at the same columns.
-        constexpr int A_PER = 2 * MT, A_ROW = 8 * MT, A_STEP = CONVERTERS / A_ROW;
+        // x8: a thread has one row of a stage and there 16 channels of every group of 64; the 8 threads of two rows then
+        // store to 8 different chunks of a line. dy (where it does not come by TMA): chunks of 8 columns, all of a
+        // thread's at the same columns.
+        constexpr int GROUPS = 2 * MT;
         constexpr int B_PER = MODE == TMA ? 1 : BK * widest(MODE) / 8 / CONVERTERS;
-        const int64_t blocks = (a.k + 31) / 32;
-        const int at = tid / A_ROW, ag = tid % A_ROW;
+        const int64_t pitch = (a.k + 31) / 32 * 32;
+        const int ar = tid >> 2, ac = (tid & 3) * 2;
+        const uint32_t lo_at = ar * 128 + ((ac ^ (ar & 7)) << 4), hi_at = ar * 128 + (((ac + 1) ^ (ar & 7)) << 4);
         const int b_bits = groups > 1 ? 4 : 3, bt = tid >> b_bits, bg = tid & ((1 << b_bits) - 1), b_step = CONVERTERS >> b_bits;
         const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
-        uint4 q[A_PER];
-        uint32_t code[A_PER];
-        float v[B_PER][8];
-        int64_t fk = 0, fn = 0;  // first channel and column of this thread in the tile being fetched
-        auto aim = [&](const Run& g) {
-            fk = g.tile % p.ktiles * (MT * 128) + ag * 16;
-            fn = g.tile / p.ktiles * p.bn + bg * 8;
+        struct Held {  // a thread's share of one stage
+            uint4 q[GROUPS];
+            uint32_t code[GROUPS];
+            Eight<T> dy[MODE == TMA ? 1 : B_PER];
         };
-        auto fetch = [&](int s) {
-            const int64_t t0 = (int64_t)s * BK;
+        Cursor ahead(p);
+        const int8_t* from;      // this thread's channels and units in the row to fetch
+        const uint8_t* unit;
+        int64_t left, fn = 0;    // the channels there are from its first one on; its first column of dy
+        auto aim = [&] {
+            const int64_t k = ahead.run.tile % p.ktiles * (MT * 128) + ac * 8, t = (int64_t)ahead.s * BK + ar;
+            from = a.q + t * pitch + k, unit = a.scale + t * (pitch >> 5) + (k >> 5), left = pitch - k;
+            fn = ahead.run.tile / p.ktiles * p.bn + bg * 8;
+        };
+        if (ahead.more) aim();
+        auto fetch = [&](Held& h) {
+            if (!ahead.more) return;
+            const int64_t t0 = (int64_t)ahead.s * BK;
             const int rows = (int)min((int64_t)BK, a.rows - t0);
-            const int8_t* from = a.q + (t0 + at) * (blocks * 32) + fk;
-            const uint8_t* unit = a.scale + (t0 + at) * blocks + (fk >> 5);
-            const bool in = fk < blocks * 32;
 #pragma unroll
-            for (int i = 0; i < A_PER; ++i) {
-                const bool here = in && at + i * A_STEP < rows;
-                q[i] = here ? *reinterpret_cast<const uint4*>(from + i * A_STEP * blocks * 32) : make_uint4(0, 0, 0, 0);
-                code[i] = here ? unit[i * A_STEP * blocks] : 127u;
+            for (int g = 0; g < GROUPS; ++g) {
+                const bool here = ar < rows && g * 64 < left;
+                h.q[g] = here ? *reinterpret_cast<const uint4*>(from + g * 64) : make_uint4(0, 0, 0, 0);
+                h.code[g] = here ? unit[g * 2] : 127u;
             }
+            from += BK * pitch, unit += BK * (pitch >> 5);
             if constexpr (MODE != TMA) {
                 const T* dy = static_cast<const T*>(a.dy) + (t0 + bt) * a.ld_dy;
 #pragma unroll
                 for (int i = 0; i < B_PER; ++i) {
-                    if (bt + i * b_step < rows) load_dy(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy, v[i]);
-                    else
-                        for (float& x : v[i]) x = 0.0f;
+                    if (bt + i * b_step < rows) h.dy[i].load(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy);
+                    else h.dy[i] = Eight<T>{};
+                }
+            }
+            if (ahead.step() && ahead.more) aim();
+        };
+        auto convert = [&](const Held& held, uint8_t* A) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const uint32_t uu = held.code[g] * 0x00800080u;  // a NaN block (code 255, bytes 0) is 0 times infinity
+                const __nv_bfloat162 unit = *reinterpret_cast<const __nv_bfloat162*>(&uu);
+                *reinterpret_cast<uint4*>(A + g * GROUP + lo_at) = eight_bytes(held.q[g].x, held.q[g].y, unit);
+                *reinterpret_cast<uint4*>(A + g * GROUP + hi_at) = eight_bytes(held.q[g].z, held.q[g].w, unit);
+            }
+            if constexpr (MODE != TMA) {
+                uint8_t* B = A + a_bytes + (bg >> 3) * GROUP;
+#pragma unroll
+                for (int i = 0; i < B_PER; ++i) {
+                    const int t = bt + i * b_step;
+                    if (t >= BK) break;
+                    float left[8];
+                    held.dy[i].get(left);
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        float h[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) h[k] = part_of(left[k]);
+                        *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
+                    }
                 }
             }
         };
-        bool ok = true, more = walk.next(seg);
+        constexpr int HELD = 2;  // stages held in registers ahead of the one being converted
+        Held held[HELD];
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) fetch(held[i]);
+        bool ok = true;
         uint32_t done = 0;
-        if (more) aim(seg), fetch(seg.first);
-        while (more) {
-            Run following;
-            const bool another = walk.next(following);
+        while (walk.next(seg)) {
             for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
                 const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
                 if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
                 uint8_t* A = ring + slot * stage_bytes;
-                uint8_t* line = A + (ag >> 2) * GROUP + at * 128;
-                const int c = (ag & 3) * 2;
-                // odd groups store their second chunk first: the threads of a row then fill different chunks at a time
-                const int swap = (ag >> 2) & 1;
-#pragma unroll
-                for (int i = 0; i < A_PER; ++i, line += A_STEP * 128) {
-                    const int t7 = (at + i * A_STEP) & 7;
-                    const uint32_t uu = (code[i] == 255 ? 0x7fffu : code[i] << 7) * 0x10001u;
-                    const __nv_bfloat162 unit = *reinterpret_cast<const __nv_bfloat162*>(&uu);
-                    const uint2 c0 = four(q[i].x, unit), c1 = four(q[i].y, unit), c2 = four(q[i].z, unit), c3 = four(q[i].w, unit);
-                    const uint4 lo = make_uint4(c0.x, c0.y, c1.x, c1.y), hi = make_uint4(c2.x, c2.y, c3.x, c3.y);
-                    *reinterpret_cast<uint4*>(line + (((c + swap) ^ t7) << 4)) = swap ? hi : lo;
-                    *reinterpret_cast<uint4*>(line + (((c + 1 - swap) ^ t7) << 4)) = swap ? lo : hi;
-                }
-                if constexpr (MODE != TMA) {
-                    uint8_t* B = A + a_bytes + (bg >> 3) * GROUP;
-#pragma unroll
-                    for (int i = 0; i < B_PER; ++i) {
-                        const int t = bt + i * b_step;
-                        if (t >= BK) break;
-#pragma unroll
-                        for (int q = 0; q < P; ++q) {
-                            float h[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) h[k] = part_of(v[i][k]);
-                            *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
-                        }
-                    }
-                }
+                const bool odd = HELD == 2 && (it & 1);
+                if (odd) convert(held[HELD - 1], A);
+                else convert(held[0], A);
                 umma::fence_async_smem();
                 __syncwarp();
                 if (lane == 0) arrive(&sh.full_a[slot]);
-                if (s + 1 < seg.last) fetch(s + 1);
-                else if (another) aim(following), fetch(following.first);
+                if (odd) fetch(held[HELD - 1]);
+                else fetch(held[0]);
             }
             // the tile out of TMEM: warps w and w + 4 share lanes 32 (w % 4) ...
             ok = ok && wait_all(&sh.acc_full, done & 1);
@@ -425,9 +487,9 @@ const int c = 4 * at;  // this thread's four columns
                 }
                 if (!ok)
                     for (float& e : x) e = __uint_as_float(0x7fffffffu);
-                const int64_t k = k0 + m * 128 + row, n = n0 + c;
+                const int64_t k = k0 + m * 128 + channel(row), n = n0 + c;
                 if (!seg.whole) {
-                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + row) * p.bn + c;
+                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
                     if (!seg.begins) add_run(x, to, 32, true);
                     store_run(to, x, 32, true);
                 } else if (k < a.k && n < a.n) {
@@ -448,7 +510,6 @@ const int c = 4 * at;  // this thread's four columns
             __syncwarp();
             if (lane == 0) arrive(&sh.acc_empty);
             ++done;
-            seg = following, more = another;
         }
     }
     umma::fence_before_sync();
