@@ -10,11 +10,10 @@
 // in shared memory: a stage holds 64 rows, 64 columns of a row being one
 // 128-byte swizzled line. Per CTA, `mt` 128-row tiles of dw (channels of x8)
 // by `bn` columns:
-//   converters  (8 warps) bytes and units of x8 from global memory through
-//               registers, one stage ahead, to bf16 in shared memory; dy too
-//               where TMA cannot take it (parts > 1 or an unaligned dy); and
-//               the epilogue out of TMEM
-//   producer    (1 warp) dy by TMA, and x8 prefetched into L2
+//   producer    (1 warp) the bytes of x8, and dy, by TMA
+//   converters  (2 teams of 8 warps, a stage each in turn) x8 to bf16 in shared
+//               memory; dy too where TMA cannot take it (parts > 1 or an
+//               unaligned dy); and the epilogue out of TMEM
 //   issuer      (1 warp) the products
 //   column sums (2 warps) db from the dy tiles in shared memory
 // The work is tiles x stages units dealt in equal runs to the CTAs; a tile
@@ -34,29 +33,41 @@ namespace wctrain {
 namespace {
 
 constexpr int BK = 64;           // rows of a stage
-constexpr int AHEAD = 6;         // stages by which x8 is prefetched into L2
-constexpr int GROUP = BK * 128;  // bytes of 64 columns of a stage
-constexpr int CONVERTERS = 256, THREADS = CONVERTERS + 128;
+constexpr int RAW = BK * 64, GROUP = BK * 128;  // bytes of 64 columns of a stage, as bytes and as bf16
+constexpr int TEAM = 256, CONVERTERS = 2 * TEAM, THREADS = CONVERTERS + 128;
 constexpr int MAX_STAGES = 8, MAX_CTAS = 148;
 constexpr int RING = 220 * 1024;  // shared memory of the stages
 constexpr uint32_t TMEM_COLS = 512;
-
-struct Plan {
-    int mt, bn, ktiles, ntiles, stages, ctas, joined, limit;
-    int64_t steps, units;  // stages of a tile; tiles x steps
-    __host__ __device__ int stage_bytes() const { return mt * 2 * GROUP + b_bytes; }
-    int b_bytes;
-};
 
 // How dy reaches shared memory: by TMA, or through the converters.
 enum { TMA, BF16, F16, F32 };
 __host__ __device__ constexpr int parts_of(int mode) { return mode == F32 ? 3 : mode == F16 ? 2 : 1; }
 __host__ __device__ constexpr int widest(int mode) { return mode == TMA ? 256 : mode == F32 ? 64 : 128; }
 
+struct Plan {
+    int mt, bn, ktiles, ntiles, ctas, joined, limit, mode, operands, inputs;
+    int64_t steps, units;  // stages of a tile; tiles x steps
+    __host__ __device__ int groups() const { return (bn + 63) / 64; }
+    __host__ __device__ int dy_bytes() const { return parts_of(mode) * groups() * GROUP; }
+    // a stage of what TMA brings (x8 as bytes, dy) and of what the converters write (x8 as bf16, dy's parts)
+    __host__ __device__ int input_bytes() const { return mt * 2 * RAW + (mode == TMA ? dy_bytes() : 0); }
+    __host__ __device__ int operand_bytes() const { return mt * 2 * GROUP + (mode == TMA ? 0 : dy_bytes()); }
+};
+
 struct Shared {
-    uint64_t full_a[MAX_STAGES], full_b[MAX_STAGES], empty[MAX_STAGES], acc_full, acc_empty;
+    uint64_t in_full[MAX_STAGES], in_empty[MAX_STAGES], op_full[MAX_STAGES], op_empty[MAX_STAGES], acc_full, acc_empty;
     uint32_t tmem;
     int failed;
+};
+
+// A place in a ring of stages and the parity of its barriers
+struct Place {
+    int count, slot = 0;
+    uint32_t phase = 0;
+    __device__ Place(int n) : count(n) {}
+    __device__ void next() {
+        if (++slot == count) slot = 0, phase ^= 1;
+    }
 };
 
 __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
@@ -75,7 +86,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
                  "l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(bar))
                  : "memory");
 }
-__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
 }
@@ -219,21 +229,25 @@ struct Cursor {
 
 template <int MODE, int MT, class T>
 __global__ void __launch_bounds__(THREADS, 1)
-    k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
-    constexpr int P = parts_of(MODE);
+    k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_q,
+             const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
+    constexpr int P = parts_of(MODE), GROUPS = 2 * MT;
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
-    uint8_t* ring = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
+    uint8_t* operands = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
+    uint8_t* inputs = operands + p.operands * p.operand_bytes();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int stage_bytes = p.stage_bytes(), a_bytes = MT * 2 * GROUP;
-    const int groups = (p.bn + 63) / 64;
+    const int groups = p.groups();
     volatile int* failed = &sh.failed;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.stages; ++i) {
-            umma::mbar_init(&sh.full_a[i], CONVERTERS / 32);
-            umma::mbar_init(&sh.full_b[i], 1);
-            umma::mbar_init(&sh.empty[i], 3);  // the issuer's commit and the two column-sum warps
+        for (int i = 0; i < p.inputs; ++i) {
+            umma::mbar_init(&sh.in_full[i], 1);
+            umma::mbar_init(&sh.in_empty[i], TEAM / 32 + (MODE == TMA ? 3 : 0));
+        }
+        for (int i = 0; i < p.operands; ++i) {
+            umma::mbar_init(&sh.op_full[i], TEAM / 32);
+            umma::mbar_init(&sh.op_empty[i], MODE == TMA ? 1 : 3);
         }
         umma::mbar_init(&sh.acc_full, 1);
         umma::mbar_init(&sh.acc_empty, CONVERTERS / 32);
@@ -246,11 +260,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     umma::fence_after_sync();
     const uint32_t tmem = sh.tmem;
     Walk walk(p);
-    Run seg;
-    uint32_t it = 0;  // stages so far
+    Run run;
+    Place in{p.inputs}, op{p.operands};
     // A wait that runs out (umma.cuh) makes every role give up: products and copies in flight are waited for, what
     // the CTA had still to write becomes NaN, and the tensor memory is released. wait_all: the same for a whole warp.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
+        const uint32_t addr = umma::smem_u32(bar);
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)  // the timer that bounds mbar_wait is slow to read: most waits end before it is needed
+            if (umma::mbar_test(addr, parity)) return true;
         if (!*failed && umma::mbar_wait(bar, parity)) return true;
         *failed = 1;
         return false;
@@ -261,23 +279,25 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
         uint32_t done = 0;
         bool ok = true;
-        while (ok && walk.next(seg)) {
+        while (ok && walk.next(run)) {
             if (done) ok = wait_all(&sh.acc_empty, (done - 1) & 1);
             umma::fence_after_sync();
-            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
-                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
-                ok = wait_all(&sh.full_a[slot], ph) && (MODE != TMA || wait_all(&sh.full_b[slot], ph));
+            for (int s = run.first; ok && s < run.last; ++s, in.next(), op.next()) {
+                ok = wait_all(&sh.op_full[op.slot], op.phase);  // the converters had seen the inputs: dy's copy is complete too
+                if (MODE == TMA) ok = ok && wait_all(&sh.in_full[in.slot], in.phase);
                 if (!ok) break;
                 umma::fence_after_sync();
                 if (lane == 0) {
-                    const uint32_t A = umma::smem_u32(ring + slot * stage_bytes), B = A + a_bytes;
+                    const uint32_t A = umma::smem_u32(operands + op.slot * p.operand_bytes());
+                    const uint32_t B = MODE == TMA ? umma::smem_u32(inputs + in.slot * p.input_bytes()) + GROUPS * RAW : A + GROUPS * GROUP;
                     for (int m = 0; m < MT; ++m)
                         for (int q = 0; q < P; ++q)
 #pragma unroll
                             for (int k = 0; k < BK / 16; ++k)
                                 umma::mma16(tmem + (m * P + q) * p.bn, desc_mn(A + m * 2 * GROUP + k * 2048),
-                                            desc_mn(B + q * groups * GROUP + k * 2048), idesc, s > seg.first || k);
-                    umma::commit(&sh.empty[slot]);
+                                            desc_mn(B + q * groups * GROUP + k * 2048), idesc, s > run.first || k);
+                    umma::commit(&sh.op_empty[op.slot]);
+                    if (MODE == TMA) umma::commit(&sh.in_empty[in.slot]);
                 }
                 __syncwarp();
             }
@@ -291,190 +311,161 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma::mbar_wait(&sh.acc_full, (done - 1) & 1, umma::DRAIN_NS);
         }
     } else if (warp == 1) {  // ------------------------------------ producer
-bool ok = true;
-        const int64_t blocks = (a.k + 31) / 32;
-        Cursor ahead(p);
-        // the lines of x8 and its units of one stage into L2, for the converters' loads of a few stages later
-        auto prefetch = [&] {
-            if (!ahead.more) return;
-            const int64_t k0 = ahead.run.tile % p.ktiles * (MT * 128), t0 = (int64_t)ahead.s * BK;
-#pragma unroll
-            for (int i = 0; i < BK / 32; ++i) {
-                const int64_t t = t0 + i * 32 + lane;
-                if (t >= a.rows) break;
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                    if (k0 + m * 128 < blocks * 32) prefetch_l2(a.q + t * blocks * 32 + k0 + m * 128);
-                if (k0 < blocks * 32) prefetch_l2(a.scale + t * blocks + k0 / 32);
-            }
-            ahead.step();
-        };
-        for (int i = 0; i < AHEAD; ++i) prefetch();
-        while (ok && walk.next(seg)) {
-            const int n0 = (int)(seg.tile / p.ktiles) * p.bn;
-            for (int s = seg.first; s < seg.last; ++s, ++it) {
-                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
-                if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
-                if (MODE == TMA && lane == 0) {
-                    umma::expect_tx(&sh.full_b[slot], groups * GROUP);
-                    const uint32_t B = umma::smem_u32(ring + slot * stage_bytes) + a_bytes;
-                    for (int g = 0; g < groups; ++g) tma_load(B + g * GROUP, &map_dy, n0 + 64 * g, s * BK, &sh.full_b[slot]);
+        if (lane == 0) {
+            bool ok = true;
+            uint32_t it = 0;
+            while (ok && walk.next(run)) {
+                const int k0 = (int)(run.tile % p.ktiles) * MT * 128, n0 = (int)(run.tile / p.ktiles) * p.bn;
+                for (int s = run.first; s < run.last; ++s, ++it, in.next()) {
+                    if (it >= (uint32_t)p.inputs && !(ok = wait(&sh.in_empty[in.slot], in.phase ^ 1))) break;
+                    umma::expect_tx(&sh.in_full[in.slot], p.input_bytes());
+                    const uint32_t to = umma::smem_u32(inputs + in.slot * p.input_bytes());
+                    for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, k0 + 64 * g, s * BK, &sh.in_full[in.slot]);
+                    if (MODE == TMA)
+                        for (int g = 0; g < groups; ++g)
+                            tma_load(to + GROUPS * RAW + g * GROUP, &map_dy, n0 + 64 * g, s * BK, &sh.in_full[in.slot]);
                 }
-                __syncwarp();
-                prefetch();
             }
+            if (!ok)  // the copies in flight land before the CTA leaves
+                for (uint32_t i = it > (uint32_t)p.inputs ? it - p.inputs : 0; i < it; ++i)
+                    umma::mbar_wait(&sh.in_full[i % p.inputs], (i / p.inputs) & 1, umma::DRAIN_NS);
         }
-        if (MODE == TMA && !ok)  // the copies in flight land before the CTA leaves
-            for (uint32_t i = it > (uint32_t)p.stages ? it - p.stages : 0; i < it; ++i)
-                umma::mbar_wait(&sh.full_b[i % p.stages], (i / p.stages) & 1, umma::DRAIN_NS);
     } else if (warp < 4) {  // --------------------------------- column sums
-        const int at = threadIdx.x - 64;
+        const int c = 4 * (threadIdx.x - 64);  // this thread's four columns
         bool ok = true;
         float sum[4] = {};
-        while (walk.next(seg)) {
-            const bool mine = a.db && seg.tile % p.ktiles == 0;
-            if (seg.begins)
+        while (walk.next(run)) {
+            const bool mine = a.db && run.tile % p.ktiles == 0;
+            if (run.begins)
                 for (float& v : sum) v = 0.0f;
-            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
-                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
-                ok = MODE == TMA ? wait_all(&sh.full_b[slot], ph) : wait_all(&sh.full_a[slot], ph);
+            for (int s = run.first; ok && s < run.last; ++s, in.next(), op.next()) {
+                ok = MODE == TMA ? wait_all(&sh.in_full[in.slot], in.phase) : wait_all(&sh.op_full[op.slot], op.phase);
                 if (!ok) break;
-                if (mine) {
-                    const uint8_t* B = ring + slot * stage_bytes + a_bytes;
-const int c = 4 * at;  // this thread's four columns
-                    if (c < p.bn) {
-                        float x[4] = {};
-                        for (int q = 0; q < P; ++q) {
-                            const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
+                if (mine && c < p.bn) {
+                    const uint8_t* B = MODE == TMA ? inputs + in.slot * p.input_bytes() + GROUPS * RAW
+                                                   : operands + op.slot * p.operand_bytes() + GROUPS * GROUP;
+                    float x[4] = {};
+                    for (int q = 0; q < P; ++q) {
+                        const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
 #pragma unroll 16
-                            for (int t = 0; t < BK; ++t) {
-                                const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
-                                x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
-                                x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
-                            }
+                        for (int t = 0; t < BK; ++t) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
+                            x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
+                            x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
                         }
-#pragma unroll
-                        for (int h = 0; h < 4; ++h) sum[h] += x[h];
                     }
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) sum[h] += x[h];
                 }
                 __syncwarp();
-                if (lane == 0) arrive(&sh.empty[slot]);
+                if (lane == 0) arrive(MODE == TMA ? &sh.in_empty[in.slot] : &sh.op_empty[op.slot]);
             }
-            if (mine && seg.ends) {
-                const int64_t n0 = seg.tile / p.ktiles * p.bn;
+            if (mine && run.ends) {
+                const int64_t n0 = run.tile / p.ktiles * p.bn;
                 const float nan = __uint_as_float(0x7fffffffu);
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    const int c = 4 * at + h;
-                    if (c >= p.bn) continue;
+                    if (c + h >= p.bn) continue;
                     const float v = ok ? sum[h] : nan;
-                    if (!seg.whole) part_db[(2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)p.bn + c] = v;
-                    else if (n0 + c < a.n) a.db[n0 + c] = v;
+                    if (!run.whole) part_db[(2 * blockIdx.x + (run.head ? 0 : 1)) * (int64_t)p.bn + c + h] = v;
+                    else if (n0 + c + h < a.n) a.db[n0 + c + h] = v;
                 }
             }
         }
     } else {  // -------------------------------------------------- converters
-        const int tid = threadIdx.x - 128, w = warp - 4;
-        // x8: a thread has one row of a stage and there 16 channels of every group of 64; the 8 threads of two rows then
-        // store to 8 different chunks of a line. dy (where it does not come by TMA): chunks of 8 columns, all of a
-        // thread's at the same columns.
-        constexpr int GROUPS = 2 * MT;
-        constexpr int B_PER = MODE == TMA ? 1 : BK * widest(MODE) / 8 / CONVERTERS;
-        const int64_t pitch = (a.k + 31) / 32 * 32;
+        const int team = (threadIdx.x - 128) / TEAM, tid = (threadIdx.x - 128) % TEAM, w = warp - 4;
+        // x8: a thread has one row of a stage and there 16 channels of every group of 64; 8 threads (two rows) then read
+        // 128 bytes in a row and store to 8 different chunks of a line. dy (where it does not come by TMA): chunks of 8
+        // columns, all of a thread's at the same columns. What comes through registers is fetched one stage ahead.
+        constexpr int B_PER = MODE == TMA ? 1 : BK * widest(MODE) / 8 / TEAM;
+        const int64_t blocks = (a.k + 31) / 32;
         const int ar = tid >> 2, ac = (tid & 3) * 2;
-        const uint32_t lo_at = ar * 128 + ((ac ^ (ar & 7)) << 4), hi_at = ar * 128 + (((ac + 1) ^ (ar & 7)) << 4);
-        const int b_bits = groups > 1 ? 4 : 3, bt = tid >> b_bits, bg = tid & ((1 << b_bits) - 1), b_step = CONVERTERS >> b_bits;
+        const uint32_t raw_at = ar * 64 + ac * 8, lo_at = ar * 128 + ((ac ^ (ar & 7)) << 4), hi_at = ar * 128 + (((ac + 1) ^ (ar & 7)) << 4);
+        const int b_bits = groups > 1 ? 4 : 3, bt = tid >> b_bits, bg = tid & ((1 << b_bits) - 1), b_step = TEAM >> b_bits;
         const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
-        struct Held {  // a thread's share of one stage
-            uint4 q[GROUPS];
-            uint32_t code[GROUPS];
-            Eight<T> dy[MODE == TMA ? 1 : B_PER];
-        };
+        uint32_t code[GROUPS];
+        Eight<T> held[MODE == TMA ? 1 : B_PER];
         Cursor ahead(p);
-        const int8_t* from;      // this thread's channels and units in the row to fetch
-        const uint8_t* unit;
-        int64_t left, fn = 0;    // the channels there are from its first one on; its first column of dy
+        const uint8_t* units = nullptr;  // this thread's units in the tile to fetch from
+        int here = 0;                    // how many of its groups have channels there
+        int64_t fn = 0;                  // its first column of dy
         auto aim = [&] {
-            const int64_t k = ahead.run.tile % p.ktiles * (MT * 128) + ac * 8, t = (int64_t)ahead.s * BK + ar;
-            from = a.q + t * pitch + k, unit = a.scale + t * (pitch >> 5) + (k >> 5), left = pitch - k;
+            const int64_t b = ahead.run.tile % p.ktiles * (MT * 4) + (ac >> 2);
+            units = a.scale + ar * blocks + b;
+            here = (int)min((int64_t)GROUPS, (blocks - b + 1) / 2);
             fn = ahead.run.tile / p.ktiles * p.bn + bg * 8;
         };
+        auto step = [&] {
+            if (ahead.more && ahead.step() && ahead.more) aim();
+        };
         if (ahead.more) aim();
-        auto fetch = [&](Held& h) {
+        if (team) step();
+        auto fetch = [&] {
             if (!ahead.more) return;
             const int64_t t0 = (int64_t)ahead.s * BK;
             const int rows = (int)min((int64_t)BK, a.rows - t0);
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const bool here = ar < rows && g * 64 < left;
-                h.q[g] = here ? *reinterpret_cast<const uint4*>(from + g * 64) : make_uint4(0, 0, 0, 0);
-                h.code[g] = here ? unit[g * 2] : 127u;
-            }
-            from += BK * pitch, unit += BK * (pitch >> 5);
+            for (int g = 0; g < GROUPS; ++g) code[g] = g < here && ar < rows ? units[t0 * blocks + g * 2] : 127u;
             if constexpr (MODE != TMA) {
                 const T* dy = static_cast<const T*>(a.dy) + (t0 + bt) * a.ld_dy;
 #pragma unroll
                 for (int i = 0; i < B_PER; ++i) {
-                    if (bt + i * b_step < rows) h.dy[i].load(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy);
-                    else h.dy[i] = Eight<T>{};
+                    if (bt + i * b_step < rows) held[i].load(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy);
+                    else held[i] = Eight<T>{};
                 }
             }
-            if (ahead.step() && ahead.more) aim();
+            step(), step();
         };
-        auto convert = [&](const Held& held, uint8_t* A) {
+        fetch();
+        bool ok = true;
+        uint32_t done = 0, it = 0;
+        while (walk.next(run)) {
+            for (int s = run.first; ok && s < run.last; ++s, ++it, in.next(), op.next()) {
+                if (op.slot != team) continue;
+                ok = wait_all(&sh.in_full[in.slot], in.phase);
+                if (!ok) break;
+                const uint8_t* X = inputs + in.slot * p.input_bytes() + raw_at;
+                uint4 q[GROUPS];
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const uint32_t uu = held.code[g] * 0x00800080u;  // a NaN block (code 255, bytes 0) is 0 times infinity
-                const __nv_bfloat162 unit = *reinterpret_cast<const __nv_bfloat162*>(&uu);
-                *reinterpret_cast<uint4*>(A + g * GROUP + lo_at) = eight_bytes(held.q[g].x, held.q[g].y, unit);
-                *reinterpret_cast<uint4*>(A + g * GROUP + hi_at) = eight_bytes(held.q[g].z, held.q[g].w, unit);
-            }
-            if constexpr (MODE != TMA) {
-                uint8_t* B = A + a_bytes + (bg >> 3) * GROUP;
+                for (int g = 0; g < GROUPS; ++g) q[g] = *reinterpret_cast<const uint4*>(X + g * RAW);
+                if (it >= (uint32_t)p.operands && !(ok = wait_all(&sh.op_empty[op.slot], op.phase ^ 1))) break;
+                uint8_t* A = operands + op.slot * p.operand_bytes();
 #pragma unroll
-                for (int i = 0; i < B_PER; ++i) {
-                    const int t = bt + i * b_step;
-                    if (t >= BK) break;
-                    float left[8];
-                    held.dy[i].get(left);
+                for (int g = 0; g < GROUPS; ++g) {
+                    const uint32_t uu = code[g] * 0x00800080u;  // a NaN block (code 255, bytes 0) is 0 times infinity
+                    const __nv_bfloat162 unit2 = *reinterpret_cast<const __nv_bfloat162*>(&uu);
+                    *reinterpret_cast<uint4*>(A + g * GROUP + lo_at) = eight_bytes(q[g].x, q[g].y, unit2);
+                    *reinterpret_cast<uint4*>(A + g * GROUP + hi_at) = eight_bytes(q[g].z, q[g].w, unit2);
+                }
+                if constexpr (MODE != TMA) {
+                    uint8_t* B = A + GROUPS * GROUP + (bg >> 3) * GROUP;
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        float h[8];
+                    for (int i = 0; i < B_PER; ++i) {
+                        const int t = bt + i * b_step;
+                        if (t >= BK) break;
+                        float left[8];
+                        held[i].get(left);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) h[k] = part_of(left[k]);
-                        *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
+                        for (int q = 0; q < P; ++q) {
+                            float h[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) h[k] = part_of(left[k]);
+                            *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
+                        }
                     }
                 }
-            }
-        };
-        constexpr int HELD = 2;  // stages held in registers ahead of the one being converted
-        Held held[HELD];
-#pragma unroll
-        for (int i = 0; i < HELD; ++i) fetch(held[i]);
-        bool ok = true;
-        uint32_t done = 0;
-        while (walk.next(seg)) {
-            for (int s = seg.first; ok && s < seg.last; ++s, ++it) {
-                const uint32_t slot = it % p.stages, ph = (it / p.stages) & 1;
-                if (it >= (uint32_t)p.stages && !(ok = wait_all(&sh.empty[slot], ph ^ 1))) break;
-                uint8_t* A = ring + slot * stage_bytes;
-                const bool odd = HELD == 2 && (it & 1);
-                if (odd) convert(held[HELD - 1], A);
-                else convert(held[0], A);
                 umma::fence_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive(&sh.full_a[slot]);
-                if (odd) fetch(held[HELD - 1]);
-                else fetch(held[0]);
+                if (lane == 0) arrive(&sh.op_full[op.slot]), arrive(&sh.in_empty[in.slot]);
+                fetch();
             }
-            // the tile out of TMEM: warps w and w + 4 share lanes 32 (w % 4) ...
+            // the tile out of TMEM: every fourth warp has the lanes of one quarter
             ok = ok && wait_all(&sh.acc_full, done & 1);
             umma::fence_after_sync();
-            const int64_t k0 = seg.tile % p.ktiles * MT * 128, n0 = seg.tile / p.ktiles * p.bn;
-            const int row = (w & 3) * 32 + lane;
-            const int chunks_out = p.bn / 32;
-            for (int i = w >> 2; i < MT * chunks_out; i += 2) {
-                const int m = i / chunks_out, c = i % chunks_out * 32;
+            const int64_t k0 = run.tile % p.ktiles * MT * 128, n0 = run.tile / p.ktiles * p.bn;
+            const int row = (w & 3) * 32 + lane, runs = p.bn / 32;
+            for (int i = w >> 2; i < MT * runs; i += CONVERTERS / 128) {
+                const int m = i / runs, c = i % runs * 32;
                 float x[32];
                 const uint32_t from = tmem + ((uint32_t)(w & 3) * 32 << 16) + m * P * p.bn + c;
                 umma::tmem_ld32(from + (P - 1) * p.bn, x);  // the smallest part first
@@ -488,16 +479,16 @@ const int c = 4 * at;  // this thread's four columns
                 if (!ok)
                     for (float& e : x) e = __uint_as_float(0x7fffffffu);
                 const int64_t k = k0 + m * 128 + channel(row), n = n0 + c;
-                if (!seg.whole) {
-                    float* to = part + ((2 * blockIdx.x + (seg.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
-                    if (!seg.begins) add_run(x, to, 32, true);
+                if (!run.whole) {
+                    float* to = part + ((2 * blockIdx.x + (run.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
+                    if (!run.begins) add_run(x, to, 32, true);
                     store_run(to, x, 32, true);
                 } else if (k < a.k && n < a.n) {
                     const int count = (int)min((int64_t)32, a.n - n);
                     const int64_t to = k * a.n + n;
                     const bool vec = ((uintptr_t)a.dw & 15) == 0 && a.n % 8 == 0;
                     if (a.out_type == WC_F32) {
-                        if (!seg.begins) add_run(x, static_cast<float*>(a.dw) + to, count, vec);
+                        if (!run.begins) add_run(x, static_cast<float*>(a.dw) + to, count, vec);
                         store_run(static_cast<float*>(a.dw) + to, x, count, vec);
                     } else if (a.out_type == WC_F16) {
                         store_run(static_cast<__half*>(a.dw) + to, x, count, vec);
@@ -583,13 +574,13 @@ __global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, P
 int mode_of(const wc_act8_wgrad_args& a) {
     if (a.type == WC_F32) return F32;
     if (a.type == WC_F16) return F16;
-    return ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0 && a.rows ? TMA : BF16;
+    return ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0 ? TMA : BF16;
 }
 
 Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
     Plan p{};
-    const int64_t k = std::max<int64_t>(a.k, 1);
-    p.steps = std::max<int64_t>(1, (a.rows + BK - 1) / BK);
+    const int64_t k = a.k;
+    p.steps = (a.rows + BK - 1) / BK;
     p.mt = k > 128 ? 2 : 1;
     int64_t nt = (a.n + widest(mode) - 1) / widest(mode);
     p.bn = (int)(((a.n + nt - 1) / nt + 31) / 32 * 32);
@@ -599,8 +590,10 @@ Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
     p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
     p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
-    p.b_bytes = parts_of(mode) * ((p.bn + 63) / 64) * GROUP;
-    p.stages = std::min(MAX_STAGES, RING / p.stage_bytes());
+    p.mode = mode;
+    // a stage of operands for each team of converters; the rest of the memory holds inputs in flight
+    p.operands = CONVERTERS / TEAM;
+    p.inputs = std::min(MAX_STAGES, (RING - p.operands * p.operand_bytes()) / p.input_bytes());
     return p;
 }
 
@@ -619,25 +612,27 @@ Encode encoder() {
     return fn;
 }
 
-// dy as boxes of 64 columns x 64 rows, 128-byte swizzled, zeros outside
-CUtensorMap dy_map(const wc_act8_wgrad_args& a) {
+// A row-major matrix as boxes of 64 columns x 64 rows, zeros outside
+CUtensorMap map_of(const void* base, CUtensorMapDataType type, int64_t width, int64_t rows, int64_t row_bytes, CUtensorMapSwizzle swizzle) {
     CUtensorMap m;
-    const cuuint64_t dims[2] = {(cuuint64_t)a.n, (cuuint64_t)a.rows}, strides[1] = {(cuuint64_t)a.ld_dy * 2};
+    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
     const cuuint32_t box[2] = {64, BK}, step[2] = {1, 1};
-    if (encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a.dy), dims, strides, box, step,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-        throw std::runtime_error("the tensor map of dy was refused");
+    if (encoder()(&m, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        throw std::runtime_error("cuTensorMapEncodeTiled refused a tensor map");
     return m;
 }
 
 template <int MODE, int MT, class T>
 void launch_tile(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
+    const int64_t pitch = (a.k + 31) / 32 * 32;
+    const CUtensorMap q = map_of(a.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, a.rows, pitch, CU_TENSOR_MAP_SWIZZLE_NONE);
     CUtensorMap dy{};
-    if (MODE == TMA) dy = dy_map(a);
-    const size_t smem = (size_t)p.stages * p.stage_bytes() + 1024;
+    if (MODE == TMA)
+        dy = map_of(a.dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n, a.rows, a.ld_dy * 2, CU_TENSOR_MAP_SWIZZLE_128B);
+    const size_t smem = (size_t)p.operands * p.operand_bytes() + (size_t)p.inputs * p.input_bytes() + 1024;
     if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<MODE, MT, T>), RING + 1024)) return;
-    k_wgrad8<MODE, MT, T><<<p.ctas, THREADS, smem, s>>>(a, p, dy, part, part_db);
+    k_wgrad8<MODE, MT, T><<<p.ctas, THREADS, smem, s>>>(a, p, q, dy, part, part_db);
 }
 template <int MODE, class T>
 void launch_mode(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
@@ -658,7 +653,7 @@ void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, 
 }  // namespace
 
 uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
-    if (!a.n) return 0;
+    if (!a.n || !a.rows) return 0;
     uint64_t most = 0;
     const Plan p = plan_of(a, mode_of(a));
     if (p.joined) most = (uint64_t)2 * p.ctas * (p.mt * 128 + 1) * p.bn * sizeof(float);
@@ -666,6 +661,11 @@ uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
 }
 
 void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
+    if (!a.rows) {  // empty sums
+        cudaMemsetAsync(a.dw, 0, (size_t)a.k * a.n * (a.out_type == WC_F32 ? 4 : 2), s);
+        if (a.db) cudaMemsetAsync(a.db, 0, (size_t)a.n * 4, s);
+        return;
+    }
     const int mode = mode_of(a);
     const Plan p = plan_of(a, mode);
     float* part = static_cast<float*>(a.workspace);

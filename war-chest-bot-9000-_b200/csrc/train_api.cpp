@@ -162,6 +162,7 @@ static int check_wgrad(const char* me, const wc_act8_wgrad_args* a) {
     if (!type_ok(a->type) || !type_ok(a->out_type)) return bad(me, "unknown element type");
     if (!size_ok(a->rows, a->k) || !size_ok(a->rows, a->n) || a->k > (1 << 20) || a->n > (1 << 20))
         return bad(me, "sizes out of range (k and n up to 2^20)");
+    if (a->k < 1) return bad(me, "k below 1");
     return WC_OK;
 }
 
@@ -172,11 +173,11 @@ uint64_t wc_act8_wgrad_workspace(const wc_act8_wgrad_args* a) {
 int wc_act8_wgrad(const wc_act8_wgrad_args* a, void* stream) {
     const char* me = "act8_wgrad";
     if (const int rc = check_wgrad(me, a)) return rc;
-    if (!a->n || (!a->k && !a->db)) return WC_OK;
-    if (a->k && !a->dw) return bad(me, "null device pointer");
+    if (!a->n) return WC_OK;
+    if (!a->dw) return bad(me, "null device pointer");
     if (!a->workspace || off(a->workspace, 16)) return bad(me, "no 16-byte aligned workspace");
     if (a->rows) {
-        if (!a->dy || (a->k && (!a->q || !a->scale))) return bad(me, "null device pointer");
+        if (!a->dy || !a->q || !a->scale) return bad(me, "null device pointer");
         if (a->ld_dy < a->n) return bad(me, "row stride below the width");
         if (off(a->q, 16)) return bad(me, "q is not 16-byte aligned");
     }
