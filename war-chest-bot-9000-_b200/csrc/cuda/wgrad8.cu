@@ -46,7 +46,8 @@ __host__ __device__ constexpr int widest(int mode) { return mode == TMA ? 256 : 
 
 struct Plan {
     int mt, bn, ktiles, ntiles, ctas, joined, limit, mode, operands, inputs;
-    int64_t steps, units;  // stages of a tile; tiles x steps
+    int steps;              // stages of a tile
+    int64_t units;          // tiles x steps, below 2^31
     __host__ __device__ int groups() const { return (bn + 63) / 64; }
     __host__ __device__ int dy_bytes() const { return parts_of(mode) * groups() * GROUP; }
     // a stage of what TMA brings (x8 as bytes, dy) and of what the converters write (x8 as bf16, dy's parts)
@@ -85,6 +86,19 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
                  "l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(bar))
                  : "memory");
+}
+// One test that may sleep for up to 100 us: a warp that polls instead takes issue slots and shared-memory cycles from
+// the warps it waits for.
+__device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(umma::smem_u32(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    return done != 0;
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
@@ -136,12 +150,13 @@ struct Eight {
     }
 };
 
-template <class T>
+// W columns of one row of dw: stored, or what is there added to them
+template <int W, class T>
 __device__ __forceinline__ void store_run(T* p, const float* v, int count, bool vec) {
-    if (vec && count == 32) {
+    if (vec && count >= W) {
         constexpr int E = 16 / sizeof(T);
 #pragma unroll
-        for (int i = 0; i < 32 / E; ++i) {
+        for (int i = 0; i < W / E; ++i) {
             alignas(16) T e[E];
 #pragma unroll
             for (int j = 0; j < E; ++j) e[j] = from_f<T>(v[i * E + j]);
@@ -149,23 +164,36 @@ __device__ __forceinline__ void store_run(T* p, const float* v, int count, bool 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < W; ++i)
             if (i < count) p[i] = from_f<T>(v[i]);
     }
 }
-
+template <int W>
 __device__ __forceinline__ void add_run(float* v, const float* p, int count, bool vec) {
-    if (vec && count == 32) {
+    if (vec && count >= W) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < W / 4; ++i) {
             const float4 w = reinterpret_cast<const float4*>(p)[i];
             v[4 * i] += w.x, v[4 * i + 1] += w.y, v[4 * i + 2] += w.z, v[4 * i + 3] += w.w;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
+        for (int i = 0; i < W; ++i)
             if (i < count) v[i] += p[i];
     }
+}
+// W consecutive f32 columns of this thread's TMEM lane
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[32]) { umma::tmem_ld32(at, v); }
+__device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at));
+    umma::tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // A run of stages of one tile that is summed in TMEM. The tensor core's f32
@@ -175,55 +203,27 @@ __device__ __forceinline__ void add_run(float* v, const float* p, int count, boo
 // global memory, each thread the values it wrote itself. For a 16-bit dw a
 // whole segment is one run.
 constexpr int RUN = 40;
-struct Run {
-    int64_t tile;
-    int first, last;       // stages
-    bool whole, head;      // the CTA has the whole tile; its first tile
-    bool begins, ends;     // first and last run of this CTA's share of the tile
-};
 
-// The runs that fall to a CTA, in order
+// The units (a stage of a tile each) that fall to a CTA, in order. A share is
+// what it has of one tile, cut into runs.
 struct Walk {
-    int64_t u, end, start, steps, tile = 0;
-    int s = 0, s0 = 0, s1 = 0, limit;
-    __device__ Walk(const Plan& p) : steps(p.steps), limit(p.limit) {
-        start = u = p.units * blockIdx.x / p.ctas;
-        end = p.units * (blockIdx.x + 1) / p.ctas;
+    int u, end, tile, s;      // unit, end of the CTA's, their tile and stage
+    int in_run;               // stages of the run before this one
+    bool whole, head, begins; // the share is the whole tile; the CTA's first share; the share's first run
+    __device__ explicit Walk(const Plan& p) {
+        u = (int)(p.units * blockIdx.x / p.ctas), end = (int)(p.units * (blockIdx.x + 1) / p.ctas);
+        tile = u / p.steps, s = u - tile * p.steps;
+        head = true;
+        share(p);
     }
-    __device__ bool next(Run& r) {
-        if (s == s1) {
-            if (u >= end) return false;
-            r.head = u == start;
-            tile = u / steps;
-            s = s0 = (int)(u - tile * steps);
-            s1 = (int)min(steps, s0 + (end - u));
-            u += s1 - s0;
-        } else {
-            r.head = tile == start / steps;
-        }
-        r.tile = tile, r.first = s, r.last = min(s1, s + limit);
-        r.whole = s0 == 0 && s1 == steps;
-        r.begins = s == s0, r.ends = r.last == s1;
-        s = r.last;
-        return true;
-    }
-};
-
-// The stages that fall to a CTA, one at a time
-struct Cursor {
-    Walk walk;
-    Run run;
-    int s = 0;
-    bool more;
-    __device__ Cursor(const Plan& p) : walk(p) { enter(); }
-    __device__ void enter() {
-        more = walk.next(run);
-        s = more ? run.first : 0;
-    }
-    __device__ bool step() {  // true: on to another run
-        if (++s < run.last) return false;
-        enter();
-        return true;
+    __device__ void share(const Plan& p) { in_run = 0, begins = true, whole = s == 0 && end - u >= p.steps; }
+    __device__ bool more() const { return u < end; }
+    __device__ bool share_ends(const Plan& p) const { return u + 1 == end || s + 1 == p.steps; }
+    __device__ bool run_ends(const Plan& p) const { return share_ends(p) || in_run + 1 == p.limit; }
+    __device__ void next(const Plan& p) {
+        ++u, ++in_run;
+        if (++s == p.steps) s = 0, ++tile, head = false, share(p);
+        else if (in_run == p.limit) in_run = 0, begins = false;
     }
 };
 
@@ -260,15 +260,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     umma::fence_after_sync();
     const uint32_t tmem = sh.tmem;
     Walk walk(p);
-    Run run;
     Place in{p.inputs}, op{p.operands};
     // A wait that runs out (umma.cuh) makes every role give up: products and copies in flight are waited for, what
     // the CTA had still to write becomes NaN, and the tensor memory is released. wait_all: the same for a whole warp.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        const uint32_t addr = umma::smem_u32(bar);
-#pragma unroll 1
-        for (int i = 0; i < 256; ++i)  // the timer that bounds mbar_wait is slow to read: most waits end before it is needed
-            if (umma::mbar_test(addr, parity)) return true;
+        if (mbar_sleep(bar, parity)) return true;
         if (!*failed && umma::mbar_wait(bar, parity)) return true;
         *failed = 1;
         return false;
@@ -276,98 +272,95 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
     if (warp == 0) {  // ------------------------------------------- issuer
-        const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
-        uint32_t done = 0;
-        bool ok = true;
-        while (ok && walk.next(run)) {
-            if (done) ok = wait_all(&sh.acc_empty, (done - 1) & 1);
-            umma::fence_after_sync();
-            for (int s = run.first; ok && s < run.last; ++s, in.next(), op.next()) {
-                ok = wait_all(&sh.op_full[op.slot], op.phase);  // the converters had seen the inputs: dy's copy is complete too
-                if (MODE == TMA) ok = ok && wait_all(&sh.in_full[in.slot], in.phase);
-                if (!ok) break;
+        // One thread, and little for it to compute: its instructions between two products are what keeps the tensor
+        // core waiting when the tiles are small. Descriptors differ from their stage's only in the address field.
+        if (lane == 0) {
+            const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
+            const uint64_t a_first = desc_mn(umma::smem_u32(operands)), b_first = desc_mn(umma::smem_u32(inputs) + GROUPS * RAW);
+            const uint32_t a_step = p.operand_bytes() >> 4, b_step = p.input_bytes() >> 4, q_step = (groups * GROUP) >> 4;
+            uint32_t done = 0;
+            bool ok = true;
+            for (; walk.more(); walk.next(p), in.next(), op.next()) {
+                if (walk.in_run == 0 && done && !(ok = wait(&sh.acc_empty, (done - 1) & 1))) break;
+                if (MODE == TMA && !(ok = wait(&sh.in_full[in.slot], in.phase))) break;
+                if (!(ok = wait(&sh.op_full[op.slot], op.phase))) break;
                 umma::fence_after_sync();
-                if (lane == 0) {
-                    const uint32_t A = umma::smem_u32(operands + op.slot * p.operand_bytes());
-                    const uint32_t B = MODE == TMA ? umma::smem_u32(inputs + in.slot * p.input_bytes()) + GROUPS * RAW : A + GROUPS * GROUP;
-                    for (int m = 0; m < MT; ++m)
-                        for (int q = 0; q < P; ++q)
+                const uint64_t A = a_first + op.slot * a_step;
+                const uint64_t B = MODE == TMA ? b_first + in.slot * b_step : A + (GROUPS * GROUP >> 4);
 #pragma unroll
-                            for (int k = 0; k < BK / 16; ++k)
-                                umma::mma16(tmem + (m * P + q) * p.bn, desc_mn(A + m * 2 * GROUP + k * 2048),
-                                            desc_mn(B + q * groups * GROUP + k * 2048), idesc, s > run.first || k);
-                    umma::commit(&sh.op_empty[op.slot]);
-                    if (MODE == TMA) umma::commit(&sh.in_empty[in.slot]);
-                }
-                __syncwarp();
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int q = 0; q < P; ++q) {
+                        const uint32_t to = tmem + (m * P + q) * p.bn;
+                        const uint64_t Am = A + (m * 2 * GROUP >> 4), Bq = B + q * q_step;
+                        umma::mma16(to, Am, Bq, idesc, walk.in_run);
+#pragma unroll
+                        for (int k = 1; k < BK / 16; ++k) umma::mma16(to, Am + k * 128, Bq + k * 128, idesc, 1);
+                    }
+                umma::commit(&sh.op_empty[op.slot]);
+                if (MODE == TMA) umma::commit(&sh.in_empty[in.slot]);
+                if (walk.run_ends(p)) umma::commit(&sh.acc_full), ++done;
             }
-            if (ok && lane == 0) umma::commit(&sh.acc_full);
-            __syncwarp();
-            ++done;
+            // every issued product has finished before TMEM is given back
+            if (!ok) {
+                umma::commit(&sh.acc_full);
+                umma::mbar_wait(&sh.acc_full, done & 1, umma::DRAIN_NS);
+            }
         }
-        // every issued product has finished before TMEM is given back
-        if (!ok) {
-            if (lane == 0) umma::commit(&sh.acc_full);
-            umma::mbar_wait(&sh.acc_full, (done - 1) & 1, umma::DRAIN_NS);
-        }
+        __syncwarp();
     } else if (warp == 1) {  // ------------------------------------ producer
         if (lane == 0) {
             bool ok = true;
             uint32_t it = 0;
-            while (ok && walk.next(run)) {
-                const int k0 = (int)(run.tile % p.ktiles) * MT * 128, n0 = (int)(run.tile / p.ktiles) * p.bn;
-                for (int s = run.first; s < run.last; ++s, ++it, in.next()) {
-                    if (it >= (uint32_t)p.inputs && !(ok = wait(&sh.in_empty[in.slot], in.phase ^ 1))) break;
-                    umma::expect_tx(&sh.in_full[in.slot], p.input_bytes());
-                    const uint32_t to = umma::smem_u32(inputs + in.slot * p.input_bytes());
-                    for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, k0 + 64 * g, s * BK, &sh.in_full[in.slot]);
-                    if (MODE == TMA)
-                        for (int g = 0; g < groups; ++g)
-                            tma_load(to + GROUPS * RAW + g * GROUP, &map_dy, n0 + 64 * g, s * BK, &sh.in_full[in.slot]);
-                }
+            for (; walk.more(); walk.next(p), in.next(), ++it) {
+                if (it >= (uint32_t)p.inputs && !(ok = wait(&sh.in_empty[in.slot], in.phase ^ 1))) break;
+                const int k0 = walk.tile % p.ktiles * (MT * 128), n0 = walk.tile / p.ktiles * p.bn, t0 = walk.s * BK;
+                umma::expect_tx(&sh.in_full[in.slot], p.input_bytes());
+                const uint32_t to = umma::smem_u32(inputs + in.slot * p.input_bytes());
+                for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, k0 + 64 * g, t0, &sh.in_full[in.slot]);
+                if (MODE == TMA)
+                    for (int g = 0; g < groups; ++g)
+                        tma_load(to + GROUPS * RAW + g * GROUP, &map_dy, n0 + 64 * g, t0, &sh.in_full[in.slot]);
             }
             if (!ok)  // the copies in flight land before the CTA leaves
                 for (uint32_t i = it > (uint32_t)p.inputs ? it - p.inputs : 0; i < it; ++i)
                     umma::mbar_wait(&sh.in_full[i % p.inputs], (i / p.inputs) & 1, umma::DRAIN_NS);
         }
+        __syncwarp();
     } else if (warp < 4) {  // --------------------------------- column sums
         const int c = 4 * (threadIdx.x - 64);  // this thread's four columns
         bool ok = true;
         float sum[4] = {};
-        while (walk.next(run)) {
-            const bool mine = a.db && run.tile % p.ktiles == 0;
-            if (run.begins)
+        for (; walk.more(); walk.next(p), in.next(), op.next()) {
+            const bool mine = a.db && walk.tile % p.ktiles == 0 && c < p.bn;
+            if (walk.begins && walk.in_run == 0)
                 for (float& v : sum) v = 0.0f;
-            for (int s = run.first; ok && s < run.last; ++s, in.next(), op.next()) {
-                ok = MODE == TMA ? wait_all(&sh.in_full[in.slot], in.phase) : wait_all(&sh.op_full[op.slot], op.phase);
-                if (!ok) break;
-                if (mine && c < p.bn) {
-                    const uint8_t* B = MODE == TMA ? inputs + in.slot * p.input_bytes() + GROUPS * RAW
-                                                   : operands + op.slot * p.operand_bytes() + GROUPS * GROUP;
-                    float x[4] = {};
-                    for (int q = 0; q < P; ++q) {
-                        const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
+            ok = ok && (MODE == TMA ? wait_all(&sh.in_full[in.slot], in.phase) : wait_all(&sh.op_full[op.slot], op.phase));
+            if (mine && ok) {
+                const uint8_t* B = MODE == TMA ? inputs + in.slot * p.input_bytes() + GROUPS * RAW
+                                               : operands + op.slot * p.operand_bytes() + GROUPS * GROUP;
+                float x[4] = {};
+                for (int q = 0; q < P; ++q) {
+                    const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
 #pragma unroll 16
-                        for (int t = 0; t < BK; ++t) {
-                            const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
-                            x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
-                            x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
-                        }
+                    for (int t = 0; t < BK; ++t) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
+                        x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
+                        x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
                     }
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) sum[h] += x[h];
                 }
-                __syncwarp();
-                if (lane == 0) arrive(MODE == TMA ? &sh.in_empty[in.slot] : &sh.op_empty[op.slot]);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) sum[h] += x[h];
             }
-            if (mine && run.ends) {
-                const int64_t n0 = run.tile / p.ktiles * p.bn;
-                const float nan = __uint_as_float(0x7fffffffu);
+            __syncwarp();
+            if (ok && lane == 0) arrive(MODE == TMA ? &sh.in_empty[in.slot] : &sh.op_empty[op.slot]);
+            if (mine && walk.share_ends(p)) {
+                const int64_t n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     if (c + h >= p.bn) continue;
-                    const float v = ok ? sum[h] : nan;
-                    if (!run.whole) part_db[(2 * blockIdx.x + (run.head ? 0 : 1)) * (int64_t)p.bn + c + h] = v;
+                    const float v = ok ? sum[h] : __uint_as_float(0x7fffffffu);
+                    if (!walk.whole) part_db[(2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)p.bn + c + h] = v;
                     else if (n0 + c + h < a.n) a.db[n0 + c + h] = v;
                 }
             }
@@ -385,24 +378,29 @@ __global__ void __launch_bounds__(THREADS, 1)
         const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
         uint32_t code[GROUPS];
         Eight<T> held[MODE == TMA ? 1 : B_PER];
-        Cursor ahead(p);
+        // the stage to fetch: this team's next
+        int fetch_u = walk.u, fetch_s = walk.s, fetch_tile = walk.tile;
         const uint8_t* units = nullptr;  // this thread's units in the tile to fetch from
         int here = 0;                    // how many of its groups have channels there
         int64_t fn = 0;                  // its first column of dy
         auto aim = [&] {
-            const int64_t b = ahead.run.tile % p.ktiles * (MT * 4) + (ac >> 2);
+            const int64_t b = (int64_t)(fetch_tile % p.ktiles) * (MT * 4) + (ac >> 2);
             units = a.scale + ar * blocks + b;
             here = (int)min((int64_t)GROUPS, (blocks - b + 1) / 2);
-            fn = ahead.run.tile / p.ktiles * p.bn + bg * 8;
+            fn = (int64_t)(fetch_tile / p.ktiles) * p.bn + bg * 8;
         };
-        auto step = [&] {
-            if (ahead.more && ahead.step() && ahead.more) aim();
+        auto advance = [&](int by) {
+            fetch_u += by, fetch_s += by;
+            if (fetch_s >= p.steps) {
+                while (fetch_s >= p.steps) fetch_s -= p.steps, ++fetch_tile;
+                aim();
+            }
         };
-        if (ahead.more) aim();
-        if (team) step();
+        aim();
+        advance(team);
         auto fetch = [&] {
-            if (!ahead.more) return;
-            const int64_t t0 = (int64_t)ahead.s * BK;
+            if (fetch_u >= walk.end) return;
+            const int64_t t0 = (int64_t)fetch_s * BK;
             const int rows = (int)min((int64_t)BK, a.rows - t0);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) code[g] = g < here && ar < rows ? units[t0 * blocks + g * 2] : 127u;
@@ -414,21 +412,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                     else held[i] = Eight<T>{};
                 }
             }
-            step(), step();
+            advance(2);
         };
         fetch();
         bool ok = true;
         uint32_t done = 0, it = 0;
-        while (walk.next(run)) {
-            for (int s = run.first; ok && s < run.last; ++s, ++it, in.next(), op.next()) {
-                if (op.slot != team) continue;
+        for (; walk.more(); walk.next(p), ++it, in.next(), op.next()) {
+            if (ok && op.slot == team) {
                 ok = wait_all(&sh.in_full[in.slot], in.phase);
-                if (!ok) break;
                 const uint8_t* X = inputs + in.slot * p.input_bytes() + raw_at;
                 uint4 q[GROUPS];
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) q[g] = *reinterpret_cast<const uint4*>(X + g * RAW);
-                if (it >= (uint32_t)p.operands && !(ok = wait_all(&sh.op_empty[op.slot], op.phase ^ 1))) break;
+                if (it >= (uint32_t)p.operands) ok = ok && wait_all(&sh.op_empty[op.slot], op.phase ^ 1);
                 uint8_t* A = operands + op.slot * p.operand_bytes();
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
@@ -456,44 +452,46 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 umma::fence_async_smem();
                 __syncwarp();
-                if (lane == 0) arrive(&sh.op_full[op.slot]), arrive(&sh.in_empty[in.slot]);
+                if (ok && lane == 0) arrive(&sh.op_full[op.slot]), arrive(&sh.in_empty[in.slot]);
                 fetch();
             }
+            if (!walk.run_ends(p)) continue;
             // the tile out of TMEM: every fourth warp has the lanes of one quarter
             ok = ok && wait_all(&sh.acc_full, done & 1);
             umma::fence_after_sync();
-            const int64_t k0 = run.tile % p.ktiles * MT * 128, n0 = run.tile / p.ktiles * p.bn;
-            const int row = (w & 3) * 32 + lane, runs = p.bn / 32;
+            const int64_t k0 = (int64_t)(walk.tile % p.ktiles) * (MT * 128), n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
+            constexpr int W = P == 1 ? 32 : 16;  // columns at a time
+            const int row = (w & 3) * 32 + lane, runs = p.bn / W;
             for (int i = w >> 2; i < MT * runs; i += CONVERTERS / 128) {
-                const int m = i / runs, c = i % runs * 32;
-                float x[32];
+                const int m = i / runs, c = i % runs * W;
+                float x[W];
                 const uint32_t from = tmem + ((uint32_t)(w & 3) * 32 << 16) + m * P * p.bn + c;
-                umma::tmem_ld32(from + (P - 1) * p.bn, x);  // the smallest part first
+                tmem_load(from + (P - 1) * p.bn, x);  // the smallest part first
 #pragma unroll
                 for (int q = P - 2; q >= 0; --q) {
-                    float y[32];
-                    umma::tmem_ld32(from + q * p.bn, y);
+                    float y[W];
+                    tmem_load(from + q * p.bn, y);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] += y[e];
+                    for (int e = 0; e < W; ++e) x[e] += y[e];
                 }
                 if (!ok)
                     for (float& e : x) e = __uint_as_float(0x7fffffffu);
                 const int64_t k = k0 + m * 128 + channel(row), n = n0 + c;
-                if (!run.whole) {
-                    float* to = part + ((2 * blockIdx.x + (run.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
-                    if (!run.begins) add_run(x, to, 32, true);
-                    store_run(to, x, 32, true);
+                if (!walk.whole) {
+                    float* to = part + ((2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
+                    if (!walk.begins) add_run<W>(x, to, W, true);
+                    store_run<W>(to, x, W, true);
                 } else if (k < a.k && n < a.n) {
-                    const int count = (int)min((int64_t)32, a.n - n);
+                    const int count = (int)min((int64_t)W, a.n - n);
                     const int64_t to = k * a.n + n;
                     const bool vec = ((uintptr_t)a.dw & 15) == 0 && a.n % 8 == 0;
                     if (a.out_type == WC_F32) {
-                        if (!run.begins) add_run(x, static_cast<float*>(a.dw) + to, count, vec);
-                        store_run(static_cast<float*>(a.dw) + to, x, count, vec);
+                        if (!walk.begins) add_run<W>(x, static_cast<float*>(a.dw) + to, count, vec);
+                        store_run<W>(static_cast<float*>(a.dw) + to, x, count, vec);
                     } else if (a.out_type == WC_F16) {
-                        store_run(static_cast<__half*>(a.dw) + to, x, count, vec);
+                        store_run<W>(static_cast<__half*>(a.dw) + to, x, count, vec);
                     } else {
-                        store_run(static_cast<__nv_bfloat16*>(a.dw) + to, x, count, vec);
+                        store_run<W>(static_cast<__nv_bfloat16*>(a.dw) + to, x, count, vec);
                     }
                 }
             }
@@ -580,7 +578,7 @@ int mode_of(const wc_act8_wgrad_args& a) {
 Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
     Plan p{};
     const int64_t k = a.k;
-    p.steps = (a.rows + BK - 1) / BK;
+    p.steps = (int)((a.rows + BK - 1) / BK);
     p.mt = k > 128 ? 2 : 1;
     int64_t nt = (a.n + widest(mode) - 1) / widest(mode);
     p.bn = (int)(((a.n + nt - 1) / nt + 31) / 32 * 32);

@@ -163,6 +163,7 @@ static int check_wgrad(const char* me, const wc_act8_wgrad_args* a) {
     if (!size_ok(a->rows, a->k) || !size_ok(a->rows, a->n) || a->k > (1 << 20) || a->n > (1 << 20))
         return bad(me, "sizes out of range (k and n up to 2^20)");
     if (a->k < 1) return bad(me, "k below 1");
+    if ((a->rows / 64 + 1) * (a->k / 128 + 1) * (a->n / 64 + 1) >= 1ll << 31) return bad(me, "sizes out of range");
     return WC_OK;
 }
 
