@@ -2,18 +2,18 @@
 // tensor cores (tcgen05, f32 accumulators in TMEM).
 //
 // A stored value is a whole number times a power of two, so it is exact in
-// bf16; dy is exact as the sum of `parts` bf16 numbers (1 for bf16, 2 for f16,
-// 3 for f32). The products are therefore those of the 32-bit form, and only
-// the f32 accumulation rounds.
+// bf16; dy is exact as the sum of 1 (bf16), 2 (f16) or 3 (f32) bf16 numbers,
+// its parts. The products are therefore those of the 32-bit form, and only the
+// f32 accumulation rounds. Parts of f16 and f32, and a bf16 dy whose rows TMA
+// cannot address, are first laid out in the workspace by a kernel of their own.
 //
 // Both operands are summed over the rows, their slow axis, so both are MN-major
 // in shared memory: a stage holds 64 rows, 64 columns of a row being one
-// 128-byte swizzled line. Per CTA, `mt` 128-row tiles of dw (channels of x8)
-// by `bn` columns:
-//   producer    (1 warp) the bytes of x8, and dy, by TMA
+// 128-byte swizzled line. Per CTA, MT 128-row tiles of dw (channels of x8) by
+// `bn` columns:
+//   producers   (2 warps) x8's bytes and units, and dy, into shared memory
 //   converters  (2 teams of 8 warps, a stage each in turn) x8 to bf16 in shared
-//               memory; dy too where TMA cannot take it (parts > 1 or an
-//               unaligned dy); and the epilogue out of TMEM
+//               memory; and the epilogue out of TMEM
 //   issuer      (1 warp) the products
 //   column sums (2 warps) db from the dy tiles in shared memory
 // The work is tiles x stages units dealt in equal runs to the CTAs; a tile
@@ -34,29 +34,31 @@ namespace {
 
 constexpr int BK = 64;           // rows of a stage
 constexpr int RAW = BK * 64, GROUP = BK * 128;  // bytes of 64 columns of a stage, as bytes and as bf16
-constexpr int TEAM = 256, CONVERTERS = 2 * TEAM, THREADS = CONVERTERS + 128;
+constexpr int UNIT_ROW = 12, UNITS = BK * UNIT_ROW;  // the units of a stage's row (up to 8, in whole words), and of a stage
+constexpr int TEAM = 256, CONVERTERS = 2 * TEAM, THREADS = CONVERTERS + 160;
 constexpr int MAX_STAGES = 8, MAX_CTAS = 148;
-constexpr int RING = 220 * 1024;  // shared memory of the stages
+constexpr int RING = 230912;  // shared memory of the stages: 3 of the widest tile's operands, 3 of its dy, 2 of its x8
 constexpr uint32_t TMEM_COLS = 512;
 
-// How dy reaches shared memory: by TMA, or through the converters.
-enum { TMA, BF16, F16, F32 };
-__host__ __device__ constexpr int parts_of(int mode) { return mode == F32 ? 3 : mode == F16 ? 2 : 1; }
-__host__ __device__ constexpr int widest(int mode) { return mode == TMA ? 256 : mode == F32 ? 64 : 128; }
+// dy's parts, and the widest tile whose sums fit TMEM beside those of the other parts
+__host__ __device__ constexpr int widest(int parts) { return parts == 1 ? 256 : parts == 2 ? 128 : 64; }
 
 struct Plan {
-    int mt, bn, ktiles, ntiles, ctas, joined, limit, mode, operands, inputs;
+    int mt, bn, ktiles, ntiles, ctas, joined, limit, parts, operands, dys, xs;
     int steps;              // stages of a tile
     int64_t units;          // tiles x steps, below 2^31
+    int64_t split_ld;       // elements of a row of dy's parts in the workspace; 0: dy as it is
     __host__ __device__ int groups() const { return (bn + 63) / 64; }
-    __host__ __device__ int dy_bytes() const { return parts_of(mode) * groups() * GROUP; }
-    // a stage of what TMA brings (x8 as bytes, dy) and of what the converters write (x8 as bf16, dy's parts)
-    __host__ __device__ int input_bytes() const { return mt * 2 * RAW + (mode == TMA ? dy_bytes() : 0); }
-    __host__ __device__ int operand_bytes() const { return mt * 2 * GROUP + (mode == TMA ? 0 : dy_bytes()); }
+    // a stage of each ring: x8 as bytes and its units, dy's parts, x8 as bf16
+    __host__ __device__ int x_bytes() const { return mt * 2 * RAW + UNITS; }
+    __host__ __device__ int dy_bytes() const { return parts * groups() * GROUP; }
+    __host__ __device__ int operand_bytes() const { return mt * 2 * GROUP; }
+    __host__ __device__ int ring_bytes() const { return operands * operand_bytes() + dys * dy_bytes() + xs * x_bytes(); }
 };
 
 struct Shared {
-    uint64_t in_full[MAX_STAGES], in_empty[MAX_STAGES], op_full[MAX_STAGES], op_empty[MAX_STAGES], acc_full, acc_empty;
+    uint64_t x_full[MAX_STAGES], x_empty[MAX_STAGES], dy_full[MAX_STAGES], dy_empty[MAX_STAGES];
+    uint64_t op_full[MAX_STAGES], op_empty[MAX_STAGES], acc_full, acc_empty;
     uint32_t tmem;
     int failed;
 };
@@ -82,10 +84,27 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
     return d;
 }
 
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-                 "l"(map), "r"(x), "r"(y), "r"(umma::smem_u32(bar))
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(umma::smem_u32(bar))
                  : "memory");
+}
+// The product and the commit (umma.cuh) by one elected lane of a converged warp.
+__device__ __forceinline__ void mma_one(uint32_t tmem_d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(tmem_d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(umma::smem_u32(bar))
+        : "memory");
 }
 // One test that may sleep for up to 100 us: a warp that polls instead takes issue slots and shared-memory cycles from
 // the warps it waits for.
@@ -125,42 +144,49 @@ __device__ __forceinline__ float part_of(float& v) {
     return hi;
 }
 
-// 8 values of a row as they lie in memory; past the width they are 0
-template <class T>
-struct Eight {
-    uint4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p, int64_t n, int64_t width, bool vec) {
-        if (vec && n + 8 <= width) {
+// dy's parts into the workspace: [parts][rows][ld], columns past the width zero.
+template <class T, int P>
+__global__ void __launch_bounds__(256) k_split(const T* __restrict__ dy, int64_t rows, int64_t n, int64_t ld_dy, bool vec,
+                                               __nv_bfloat16* __restrict__ out, int64_t ld) {
+    const int64_t chunks = ld / 8, total = rows * chunks;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const int64_t t = i / chunks, c = (i - t * chunks) * 8;
+        const T* from = dy + t * ld_dy + c;
+        alignas(16) T e[8];
+        if (vec && c + 8 <= n) {
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p + n)[i];
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(e)[k] = reinterpret_cast<const uint4*>(from)[k];
         } else {
-            alignas(16) T e[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] = n + i < width ? p[n + i] : from_f<T>(0.0f);
+            for (int k = 0; k < 8; ++k) e[k] = c + k < n ? from[k] : from_f<T>(0.0f);
+        }
+        float v[8];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(e)[i];
+        for (int k = 0; k < 8; ++k) v[k] = to_f(e[k]);
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            float h[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) h[k] = part_of(v[k]);
+            *reinterpret_cast<uint4*>(out + (q * rows + t) * ld + c) = umma::pack_chunk(h);
         }
     }
-    __device__ __forceinline__ void get(float* v) const {
-        alignas(16) T e[8];
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(e)[i] = w[i];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
-    }
-};
+}
 
 // W columns of one row of dw: stored, or what is there added to them
 template <int W, class T>
 __device__ __forceinline__ void store_run(T* p, const float* v, int count, bool vec) {
-    if (vec && count >= W) {
-        constexpr int E = 16 / sizeof(T);
+    if (vec && count >= W) {  // whole 32-byte sectors
+        constexpr int E = 32 / sizeof(T);
 #pragma unroll
         for (int i = 0; i < W / E; ++i) {
             alignas(16) T e[E];
 #pragma unroll
             for (int j = 0; j < E; ++j) e[j] = from_f<T>(v[i * E + j]);
-            reinterpret_cast<uint4*>(p)[i] = *reinterpret_cast<const uint4*>(e);
+            const uint32_t* r = reinterpret_cast<const uint32_t*>(e);
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + i * E), "r"(r[0]), "r"(r[1]),
+                         "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                         : "memory");
         }
     } else {
 #pragma unroll
@@ -220,6 +246,12 @@ struct Walk {
     __device__ bool more() const { return u < end; }
     __device__ bool share_ends(const Plan& p) const { return u + 1 == end || s + 1 == p.steps; }
     __device__ bool run_ends(const Plan& p) const { return share_ends(p) || in_run + 1 == p.limit; }
+    // the stages from this one to the end of its run, and past all of them
+    __device__ int run_length(const Plan& p) const { return min(min(end - u, p.steps - s), p.limit - in_run); }
+    __device__ void skip(const Plan& p, int n) {
+        u += n - 1, s += n - 1, in_run += n - 1;
+        next(p);
+    }
     __device__ void next(const Plan& p) {
         ++u, ++in_run;
         if (++s == p.steps) s = 0, ++tile, head = false, share(p);
@@ -227,27 +259,28 @@ struct Walk {
     }
 };
 
-template <int MODE, int MT, class T>
+template <int P, int MT>
 __global__ void __launch_bounds__(THREADS, 1)
     k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_q,
              const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
-    constexpr int P = parts_of(MODE), GROUPS = 2 * MT;
+    constexpr int GROUPS = 2 * MT;
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
     uint8_t* operands = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
-    uint8_t* inputs = operands + p.operands * p.operand_bytes();
+    uint8_t* dys = operands + p.operands * p.operand_bytes();
+    uint8_t* xs = dys + p.dys * p.dy_bytes();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int groups = p.groups();
     volatile int* failed = &sh.failed;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < p.inputs; ++i) {
-            umma::mbar_init(&sh.in_full[i], 1);
-            umma::mbar_init(&sh.in_empty[i], TEAM / 32 + (MODE == TMA ? 3 : 0));
-        }
-        for (int i = 0; i < p.operands; ++i) {
+        for (int i = 0; i < MAX_STAGES; ++i) {
+            umma::mbar_init(&sh.x_full[i], 1 + 32);  // the bytes, and each lane's share of the units
+            umma::mbar_init(&sh.x_empty[i], TEAM / 32);
+            umma::mbar_init(&sh.dy_full[i], 1);
+            umma::mbar_init(&sh.dy_empty[i], 3);  // the issuer's commit, the column sums' two warps
             umma::mbar_init(&sh.op_full[i], TEAM / 32);
-            umma::mbar_init(&sh.op_empty[i], MODE == TMA ? 1 : 3);
+            umma::mbar_init(&sh.op_empty[i], 1);
         }
         umma::mbar_init(&sh.acc_full, 1);
         umma::mbar_init(&sh.acc_empty, CONVERTERS / 32);
@@ -260,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     umma::fence_after_sync();
     const uint32_t tmem = sh.tmem;
     Walk walk(p);
-    Place in{p.inputs}, op{p.operands};
+    Place x{p.xs}, dy{p.dys}, op{p.operands};
     // A wait that runs out (umma.cuh) makes every role give up: products and copies in flight are waited for, what
     // the CTA had still to write becomes NaN, and the tensor memory is released. wait_all: the same for a whole warp.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -272,73 +305,111 @@ __global__ void __launch_bounds__(THREADS, 1)
     auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
     if (warp == 0) {  // ------------------------------------------- issuer
-        // One thread, and little for it to compute: its instructions between two products are what keeps the tensor
-        // core waiting when the tiles are small. Descriptors differ from their stage's only in the address field.
-        if (lane == 0) {
-            const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
-            const uint64_t a_first = desc_mn(umma::smem_u32(operands)), b_first = desc_mn(umma::smem_u32(inputs) + GROUPS * RAW);
-            const uint32_t a_step = p.operand_bytes() >> 4, b_step = p.input_bytes() >> 4, q_step = (groups * GROUP) >> 4;
-            uint32_t done = 0;
-            bool ok = true;
-            for (; walk.more(); walk.next(p), in.next(), op.next()) {
-                if (walk.in_run == 0 && done && !(ok = wait(&sh.acc_empty, (done - 1) & 1))) break;
-                if (MODE == TMA && !(ok = wait(&sh.in_full[in.slot], in.phase))) break;
-                if (!(ok = wait(&sh.op_full[op.slot], op.phase))) break;
+        // Little to compute between two products: that is what keeps the tensor core waiting. The warp stays together
+        // and one lane issues, so that the operands are uniform; a stage's descriptors differ in the address field only.
+        const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
+        const uint64_t a_first = desc_mn(umma::smem_u32(operands)), b_first = desc_mn(umma::smem_u32(dys));
+        const uint32_t a_step = p.operand_bytes() >> 4, b_step = p.dy_bytes() >> 4, q_step = (groups * GROUP) >> 4;
+        uint32_t done = 0;
+        bool ok = true;
+        while (ok && walk.more()) {
+            const int n = walk.run_length(p);
+            if (done) ok = wait_all(&sh.acc_empty, (done - 1) & 1);
+            for (int i = 0; ok && i < n; ++i) {
+                // dy's copy is waited for here, not through the converters: the product reads it with no one between
+                ok = wait_all(&sh.dy_full[dy.slot], dy.phase);
+                ok = ok && wait_all(&sh.op_full[op.slot], op.phase);
                 umma::fence_after_sync();
-                const uint64_t A = a_first + op.slot * a_step;
-                const uint64_t B = MODE == TMA ? b_first + in.slot * b_step : A + (GROUPS * GROUP >> 4);
+                if (ok) {
+                    const uint64_t A = a_first + op.slot * a_step;
+                    const uint64_t B = b_first + dy.slot * b_step;
 #pragma unroll
-                for (int m = 0; m < MT; ++m)
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int q = 0; q < P; ++q) {
-                        const uint32_t to = tmem + (m * P + q) * p.bn;
-                        const uint64_t Am = A + (m * 2 * GROUP >> 4), Bq = B + q * q_step;
-                        umma::mma16(to, Am, Bq, idesc, walk.in_run);
+                        for (int q = 0; q < P; ++q)
 #pragma unroll
-                        for (int k = 1; k < BK / 16; ++k) umma::mma16(to, Am + k * 128, Bq + k * 128, idesc, 1);
-                    }
-                umma::commit(&sh.op_empty[op.slot]);
-                if (MODE == TMA) umma::commit(&sh.in_empty[in.slot]);
-                if (walk.run_ends(p)) umma::commit(&sh.acc_full), ++done;
+                            for (int k = 0; k < BK / 16; ++k)
+                                mma_one(tmem + (m * P + q) * p.bn, A + (m * 2 * GROUP >> 4) + k * 128, B + q * q_step + k * 128,
+                                        idesc, k ? 1 : i);
+                    commit_one(&sh.op_empty[op.slot]);
+                    commit_one(&sh.dy_empty[dy.slot]);
+                }
+                dy.next(), op.next();
             }
-            // every issued product has finished before TMEM is given back
-            if (!ok) {
-                umma::commit(&sh.acc_full);
-                umma::mbar_wait(&sh.acc_full, done & 1, umma::DRAIN_NS);
-            }
+            if (ok) commit_one(&sh.acc_full), ++done;
+            walk.skip(p, n);
         }
-        __syncwarp();
-    } else if (warp == 1) {  // ------------------------------------ producer
+        if (!ok) {  // every issued product has finished before TMEM is given back
+            commit_one(&sh.acc_full);
+            umma::mbar_wait(&sh.acc_full, done & 1, umma::DRAIN_NS);
+        }
+    } else if (warp == 1) {  // ----------------------------- dy's producer
         if (lane == 0) {
+            const uint32_t ring = umma::smem_u32(dys);
+            int it = 0;
             bool ok = true;
-            uint32_t it = 0;
-            for (; walk.more(); walk.next(p), in.next(), ++it) {
-                if (it >= (uint32_t)p.inputs && !(ok = wait(&sh.in_empty[in.slot], in.phase ^ 1))) break;
-                const int k0 = walk.tile % p.ktiles * (MT * 128), n0 = walk.tile / p.ktiles * p.bn, t0 = walk.s * BK;
-                umma::expect_tx(&sh.in_full[in.slot], p.input_bytes());
-                const uint32_t to = umma::smem_u32(inputs + in.slot * p.input_bytes());
-                for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, k0 + 64 * g, t0, &sh.in_full[in.slot]);
-                if (MODE == TMA)
-                    for (int g = 0; g < groups; ++g)
-                        tma_load(to + GROUPS * RAW + g * GROUP, &map_dy, n0 + 64 * g, t0, &sh.in_full[in.slot]);
+            for (; walk.more(); walk.next(p), dy.next(), ++it) {
+                if (it >= p.dys && !(ok = wait(&sh.dy_empty[dy.slot], dy.phase ^ 1))) break;
+                const int n0 = walk.tile / p.ktiles * p.bn;
+                umma::expect_tx(&sh.dy_full[dy.slot], p.dy_bytes());
+                uint32_t to = ring + dy.slot * p.dy_bytes();
+                for (int q = 0; q < P; ++q)
+                    for (int g = 0; g < groups; ++g, to += GROUP)
+                        tma_load(to, &map_dy, n0 + 64 * g, walk.s * BK, q, &sh.dy_full[dy.slot]);
             }
             if (!ok)  // the copies in flight land before the CTA leaves
-                for (uint32_t i = it > (uint32_t)p.inputs ? it - p.inputs : 0; i < it; ++i)
-                    umma::mbar_wait(&sh.in_full[i % p.inputs], (i / p.inputs) & 1, umma::DRAIN_NS);
+                for (int i = it > p.dys ? it - p.dys : 0; i < it; ++i)
+                    umma::mbar_wait(&sh.dy_full[i % p.dys], (i / p.dys) & 1, umma::DRAIN_NS);
         }
+        __syncwarp();
+    } else if (warp == THREADS / 32 - 1) {  // -------------- x8's producer
+        // The units' rows have any alignment: the words that hold a row's are copied, and read at its first one's offset.
+        const int64_t blocks = (a.k + 31) / 32;
+        const uint32_t ring = umma::smem_u32(xs);
+        int it = 0;
+        bool ok = true;
+        for (; walk.more(); walk.next(p), x.next(), ++it) {
+            if (it >= p.xs && !(ok = wait_all(&sh.x_empty[x.slot], x.phase ^ 1))) break;
+            const uint32_t to = ring + x.slot * p.x_bytes();
+            const int tile = walk.tile % p.ktiles, t0 = walk.s * BK;
+            if (lane == 0) {
+                umma::expect_tx(&sh.x_full[x.slot], GROUPS * RAW);
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, tile * (MT * 128) + 64 * g, t0, 0, &sh.x_full[x.slot]);
+            }
+            const int count = (int)min((int64_t)MT * 4, blocks - (int64_t)tile * (MT * 4));
+#pragma unroll
+            for (int i = 0; i < BK / 32; ++i) {
+                const int row = i * 32 + lane;
+                if ((int64_t)t0 + row < a.rows) {
+                    const uintptr_t from = reinterpret_cast<uintptr_t>(a.scale + ((int64_t)t0 + row) * blocks + tile * (MT * 4));
+                    const int words = (int)((from & 3) + count + 3) >> 2;
+#pragma unroll
+                    for (int w = 0; w < UNIT_ROW / 4; ++w)
+                        if (w < words)
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + GROUPS * RAW + row * UNIT_ROW + 4 * w),
+                                         "l"((from & ~(uintptr_t)3) + 4 * w)
+                                         : "memory");
+                }
+            }
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(&sh.x_full[x.slot])) : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (!ok && lane == 0)
+            for (int i = it > p.xs ? it - p.xs : 0; i < it; ++i)
+                umma::mbar_wait(&sh.x_full[i % p.xs], (i / p.xs) & 1, umma::DRAIN_NS);
         __syncwarp();
     } else if (warp < 4) {  // --------------------------------- column sums
         const int c = 4 * (threadIdx.x - 64);  // this thread's four columns
         bool ok = true;
         float sum[4] = {};
-        for (; walk.more(); walk.next(p), in.next(), op.next()) {
+        for (; walk.more(); walk.next(p), dy.next()) {
             const bool mine = a.db && walk.tile % p.ktiles == 0 && c < p.bn;
             if (walk.begins && walk.in_run == 0)
                 for (float& v : sum) v = 0.0f;
-            ok = ok && (MODE == TMA ? wait_all(&sh.in_full[in.slot], in.phase) : wait_all(&sh.op_full[op.slot], op.phase));
+            ok = ok && wait_all(&sh.dy_full[dy.slot], dy.phase);
             if (mine && ok) {
-                const uint8_t* B = MODE == TMA ? inputs + in.slot * p.input_bytes() + GROUPS * RAW
-                                               : operands + op.slot * p.operand_bytes() + GROUPS * GROUP;
+                const uint8_t* B = dys + dy.slot * p.dy_bytes();
                 float x[4] = {};
                 for (int q = 0; q < P; ++q) {
                     const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
@@ -353,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int h = 0; h < 4; ++h) sum[h] += x[h];
             }
             __syncwarp();
-            if (ok && lane == 0) arrive(MODE == TMA ? &sh.in_empty[in.slot] : &sh.op_empty[op.slot]);
+            if (ok && lane == 0) arrive(&sh.dy_empty[dy.slot]);
             if (mine && walk.share_ends(p)) {
                 const int64_t n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
 #pragma unroll
@@ -367,93 +438,43 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else {  // -------------------------------------------------- converters
         const int team = (threadIdx.x - 128) / TEAM, tid = (threadIdx.x - 128) % TEAM, w = warp - 4;
-        // x8: a thread has one row of a stage and there 16 channels of every group of 64; 8 threads (two rows) then read
-        // 128 bytes in a row and store to 8 different chunks of a line. dy (where it does not come by TMA): chunks of 8
-        // columns, all of a thread's at the same columns. What comes through registers is fetched one stage ahead.
-        constexpr int B_PER = MODE == TMA ? 1 : BK * widest(MODE) / 8 / TEAM;
+        // A thread has one row of a stage and there 16 channels of every group of 64; 8 threads (two rows) then read 128
+        // bytes in a row and store to 8 different chunks of a line.
         const int64_t blocks = (a.k + 31) / 32;
         const int ar = tid >> 2, ac = (tid & 3) * 2;
         const uint32_t raw_at = ar * 64 + ac * 8, lo_at = ar * 128 + ((ac ^ (ar & 7)) << 4), hi_at = ar * 128 + (((ac + 1) ^ (ar & 7)) << 4);
-        const int b_bits = groups > 1 ? 4 : 3, bt = tid >> b_bits, bg = tid & ((1 << b_bits) - 1), b_step = TEAM >> b_bits;
-        const bool vec_dy = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
-        uint32_t code[GROUPS];
-        Eight<T> held[MODE == TMA ? 1 : B_PER];
-        // the stage to fetch: this team's next
-        int fetch_u = walk.u, fetch_s = walk.s, fetch_tile = walk.tile;
-        const uint8_t* units = nullptr;  // this thread's units in the tile to fetch from
-        int here = 0;                    // how many of its groups have channels there
-        int64_t fn = 0;                  // its first column of dy
-        auto aim = [&] {
-            const int64_t b = (int64_t)(fetch_tile % p.ktiles) * (MT * 4) + (ac >> 2);
-            units = a.scale + ar * blocks + b;
-            here = (int)min((int64_t)GROUPS, (blocks - b + 1) / 2);
-            fn = (int64_t)(fetch_tile / p.ktiles) * p.bn + bg * 8;
-        };
-        auto advance = [&](int by) {
-            fetch_u += by, fetch_s += by;
-            if (fetch_s >= p.steps) {
-                while (fetch_s >= p.steps) fetch_s -= p.steps, ++fetch_tile;
-                aim();
-            }
-        };
-        aim();
-        advance(team);
-        auto fetch = [&] {
-            if (fetch_u >= walk.end) return;
-            const int64_t t0 = (int64_t)fetch_s * BK;
-            const int rows = (int)min((int64_t)BK, a.rows - t0);
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) code[g] = g < here && ar < rows ? units[t0 * blocks + g * 2] : 127u;
-            if constexpr (MODE != TMA) {
-                const T* dy = static_cast<const T*>(a.dy) + (t0 + bt) * a.ld_dy;
-#pragma unroll
-                for (int i = 0; i < B_PER; ++i) {
-                    if (bt + i * b_step < rows) held[i].load(dy + i * b_step * a.ld_dy, fn, a.n, vec_dy);
-                    else held[i] = Eight<T>{};
-                }
-            }
-            advance(2);
-        };
-        fetch();
+        // where a row's units start in their words, up to the stage's and the tile's share
+        const uint32_t unit_row = (uint32_t)(reinterpret_cast<uintptr_t>(a.scale) + ar * blocks), unit_stage = (uint32_t)(BK * blocks);
         bool ok = true;
         uint32_t done = 0, it = 0;
-        for (; walk.more(); walk.next(p), ++it, in.next(), op.next()) {
-            if (ok && op.slot == team) {
-                ok = wait_all(&sh.in_full[in.slot], in.phase);
-                const uint8_t* X = inputs + in.slot * p.input_bytes() + raw_at;
+        for (; walk.more(); walk.next(p), ++it, x.next(), op.next()) {
+            if (ok && (int)(it & 1) == team) {
+                ok = wait_all(&sh.x_full[x.slot], x.phase);
+                const uint8_t* X = xs + x.slot * p.x_bytes() + raw_at;
+                const uint32_t first = (unit_row + walk.s * unit_stage + walk.tile % p.ktiles * (MT * 4)) & 3;
+                const uint8_t* units = xs + x.slot * p.x_bytes() + GROUPS * RAW + ar * UNIT_ROW + first + (ac >> 2);
                 uint4 q[GROUPS];
+                uint32_t code[GROUPS];
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) q[g] = *reinterpret_cast<const uint4*>(X + g * RAW);
+                for (int g = 0; g < GROUPS; ++g) {
+                    q[g] = *reinterpret_cast<const uint4*>(X + g * RAW);
+                    code[g] = units[2 * g];
+                }
                 if (it >= (uint32_t)p.operands) ok = ok && wait_all(&sh.op_empty[op.slot], op.phase ^ 1);
                 uint8_t* A = operands + op.slot * p.operand_bytes();
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const uint32_t uu = code[g] * 0x00800080u;  // a NaN block (code 255, bytes 0) is 0 times infinity
+                    // Rows and blocks past the end come as bytes 0; their units are whatever the memory held, and have
+                    // to be a number: 0 times a finite one is 0. (A NaN block, code 255, is 0 times infinity.)
+                    const bool there = (int64_t)walk.s * BK + ar < a.rows;
+                    const uint32_t uu = (there ? code[g] : 127u) * 0x00800080u;
                     const __nv_bfloat162 unit2 = *reinterpret_cast<const __nv_bfloat162*>(&uu);
                     *reinterpret_cast<uint4*>(A + g * GROUP + lo_at) = eight_bytes(q[g].x, q[g].y, unit2);
                     *reinterpret_cast<uint4*>(A + g * GROUP + hi_at) = eight_bytes(q[g].z, q[g].w, unit2);
                 }
-                if constexpr (MODE != TMA) {
-                    uint8_t* B = A + GROUPS * GROUP + (bg >> 3) * GROUP;
-#pragma unroll
-                    for (int i = 0; i < B_PER; ++i) {
-                        const int t = bt + i * b_step;
-                        if (t >= BK) break;
-                        float left[8];
-                        held[i].get(left);
-#pragma unroll
-                        for (int q = 0; q < P; ++q) {
-                            float h[8];
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) h[k] = part_of(left[k]);
-                            *reinterpret_cast<uint4*>(B + q * groups * GROUP + t * 128 + (((bg & 7) ^ (t & 7)) << 4)) = umma::pack_chunk(h);
-                        }
-                    }
-                }
                 umma::fence_async_smem();
                 __syncwarp();
-                if (ok && lane == 0) arrive(&sh.op_full[op.slot]), arrive(&sh.in_empty[in.slot]);
-                fetch();
+                if (ok && lane == 0) arrive(&sh.op_full[op.slot]), arrive(&sh.x_empty[x.slot]);
             }
             if (!walk.run_ends(p)) continue;
             // the tile out of TMEM: every fourth warp has the lanes of one quarter
@@ -461,37 +482,46 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma::fence_after_sync();
             const int64_t k0 = (int64_t)(walk.tile % p.ktiles) * (MT * 128), n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
             constexpr int W = P == 1 ? 32 : 16;  // columns at a time
-            const int row = (w & 3) * 32 + lane, runs = p.bn / W;
+            const int row = (warp & 3) * 32 + lane, runs = p.bn / W;
             for (int i = w >> 2; i < MT * runs; i += CONVERTERS / 128) {
                 const int m = i / runs, c = i % runs * W;
-                float x[W];
-                const uint32_t from = tmem + ((uint32_t)(w & 3) * 32 << 16) + m * P * p.bn + c;
-                tmem_load(from + (P - 1) * p.bn, x);  // the smallest part first
+                float v[W];
+                const uint32_t from = tmem + ((uint32_t)(warp & 3) * 32 << 16) + m * P * p.bn + c;
+                tmem_load(from + (P - 1) * p.bn, v);  // the smallest part first
 #pragma unroll
                 for (int q = P - 2; q >= 0; --q) {
                     float y[W];
                     tmem_load(from + q * p.bn, y);
 #pragma unroll
-                    for (int e = 0; e < W; ++e) x[e] += y[e];
+                    for (int e = 0; e < W; ++e) v[e] += y[e];
                 }
                 if (!ok)
-                    for (float& e : x) e = __uint_as_float(0x7fffffffu);
+                    for (float& e : v) e = __uint_as_float(0x7fffffffu);
                 const int64_t k = k0 + m * 128 + channel(row), n = n0 + c;
                 if (!walk.whole) {
-                    float* to = part + ((2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)MT * 128 + m * 128 + channel(row)) * p.bn + c;
-                    if (!walk.begins) add_run<W>(x, to, W, true);
-                    store_run<W>(to, x, W, true);
+                    // four columns at a time, rows next to each other: 512 bytes in a row for the warp
+                    float4* to = reinterpret_cast<float4*>(part) +
+                                 ((2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)MT + m) * (p.bn / 4 * 128) + c / 4 * 128 + row;
+#pragma unroll
+                    for (int e = 0; e < W / 4; ++e) {
+                        float4 w = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        if (!walk.begins) {
+                            const float4 o = to[e * 128];
+                            w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
+                        }
+                        to[e * 128] = w;
+                    }
                 } else if (k < a.k && n < a.n) {
                     const int count = (int)min((int64_t)W, a.n - n);
                     const int64_t to = k * a.n + n;
-                    const bool vec = ((uintptr_t)a.dw & 15) == 0 && a.n % 8 == 0;
+                    const bool vec = ((uintptr_t)a.dw & 31) == 0 && a.n % 16 == 0;
                     if (a.out_type == WC_F32) {
-                        if (!walk.begins) add_run<W>(x, static_cast<float*>(a.dw) + to, count, vec);
-                        store_run<W>(static_cast<float*>(a.dw) + to, x, count, vec);
+                        if (!walk.begins) add_run<W>(v, static_cast<float*>(a.dw) + to, count, vec);
+                        store_run<W>(static_cast<float*>(a.dw) + to, v, count, vec);
                     } else if (a.out_type == WC_F16) {
-                        store_run<W>(static_cast<__half*>(a.dw) + to, x, count, vec);
+                        store_run<W>(static_cast<__half*>(a.dw) + to, v, count, vec);
                     } else {
-                        store_run<W>(static_cast<__nv_bfloat16*>(a.dw) + to, x, count, vec);
+                        store_run<W>(static_cast<__nv_bfloat16*>(a.dw) + to, v, count, vec);
                     }
                 }
             }
@@ -527,8 +557,8 @@ struct Splits {
     }
 };
 
-// Joins the split tiles (one a blockIdx.y). A thread has 4 columns of a row
-// (row mt * 128 is db); with many CTAs to a tile they are dealt to blockDim.y
+// Joins the split tiles (one a blockIdx.y). A thread has 4 columns of a row, or
+// of db; with many CTAs to a tile they are dealt to blockDim.y
 // threads and those joined in order.
 constexpr int JOINERS = 256;
 template <class T>
@@ -538,16 +568,18 @@ __global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, P
     const Split& cut = splits.at[blockIdx.y];
     const int tile = cut.tile, c0 = cut.c0, c1 = cut.c1;
     const int rows = p.mt * 128, runs = p.bn / 4;
-    const int i = blockIdx.x * blockDim.x + threadIdx.x, r = i / runs, c = i % runs * 4;
+    // in the order of the partial results: the rows of four columns, then db's columns
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    const bool bias = i >= rows * runs;
+    const int m = i / (runs * 128), c = bias ? (i - rows * runs) * 4 : i / 128 % runs * 4, r = m * 128 + channel(i & 127);
     const int64_t k0 = tile % p.ktiles * rows, n0 = tile / p.ktiles * p.bn, n = n0 + c;
-    const bool bias = r == rows;
-    const bool in = r <= rows && n < a.n && (bias ? a.db && tile % p.ktiles == 0 : k0 + r < a.k);
+    const bool in = i < (rows + 1) * runs && n < a.n && (bias ? a.db && tile % p.ktiles == 0 : k0 + r < a.k);
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (in)
 #pragma unroll 4
         for (int j = c0 + (int)threadIdx.y; j <= c1; j += blockDim.y) {
             const int64_t slot = j == c0 ? cut.slot : 2 * j;
-            const float4 w = *reinterpret_cast<const float4*>(bias ? part_db + slot * p.bn + c : part + (slot * rows + r) * p.bn + c);
+            const float4 w = *reinterpret_cast<const float4*>(bias ? part_db + slot * p.bn + c : part + (slot * rows * runs + i) * 4);
             v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
         }
     if (blockDim.y > 1) {
@@ -569,30 +601,37 @@ __global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, P
     }
 }
 
-int mode_of(const wc_act8_wgrad_args& a) {
-    if (a.type == WC_F32) return F32;
-    if (a.type == WC_F16) return F16;
-    return ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0 ? TMA : BF16;
-}
-
-Plan plan_of(const wc_act8_wgrad_args& a, int mode) {
+Plan plan_of(const wc_act8_wgrad_args& a) {
     Plan p{};
-    const int64_t k = a.k;
+    p.parts = a.type == WC_F32 ? 3 : a.type == WC_F16 ? 2 : 1;
+    const bool as_is = p.parts == 1 && ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0;
+    p.split_ld = as_is ? 0 : (a.n + 7) / 8 * 8;
     p.steps = (int)((a.rows + BK - 1) / BK);
-    p.mt = k > 128 ? 2 : 1;
-    int64_t nt = (a.n + widest(mode) - 1) / widest(mode);
+    p.mt = a.k > 128 ? 2 : 1;
+    const int64_t nt = (a.n + widest(p.parts) - 1) / widest(p.parts);
     p.bn = (int)(((a.n + nt - 1) / nt + 31) / 32 * 32);
-    p.ktiles = (int)((k + p.mt * 128 - 1) / (p.mt * 128));
+    p.ktiles = (int)((a.k + p.mt * 128 - 1) / (p.mt * 128));
     p.ntiles = (int)((a.n + p.bn - 1) / p.bn);
     p.units = (int64_t)p.ktiles * p.ntiles * p.steps;
     p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
     p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
-    p.mode = mode;
-    // a stage of operands for each team of converters; the rest of the memory holds inputs in flight
-    p.operands = CONVERTERS / TEAM;
-    p.inputs = std::min(MAX_STAGES, (RING - p.operands * p.operand_bytes()) / p.input_bytes());
+    // Converters work a stage or two ahead of the products; what is left holds copies in flight, of dy and x8 in turn
+    p.operands = 3, p.xs = 2, p.dys = 2;
+    for (bool grew = true; grew;) {
+        grew = false;
+        for (int* n : {&p.dys, &p.xs}) {
+            if (*n == MAX_STAGES) continue;
+            ++*n;
+            if (p.ring_bytes() <= RING) grew = true;
+            else --*n;
+        }
+    }
     return p;
+}
+
+uint64_t parts_bytes(const wc_act8_wgrad_args& a, const Plan& p) {
+    return ((uint64_t)p.parts * a.rows * p.split_ld * 2 + 255) / 256 * 256;
 }
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -610,32 +649,37 @@ Encode encoder() {
     return fn;
 }
 
-// A row-major matrix as boxes of 64 columns x 64 rows, zeros outside
-CUtensorMap map_of(const void* base, CUtensorMapDataType type, int64_t width, int64_t rows, int64_t row_bytes, CUtensorMapSwizzle swizzle) {
+// `planes` row-major matrices as boxes of 64 columns x 64 rows, zeros outside
+CUtensorMap map_of(const void* base, CUtensorMapDataType type, int64_t width, int64_t rows, int planes, int64_t row_bytes,
+                   CUtensorMapSwizzle swizzle) {
     CUtensorMap m;
-    const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)row_bytes};
-    const cuuint32_t box[2] = {64, BK}, step[2] = {1, 1};
-    if (encoder()(&m, type, 2, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+    const cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(row_bytes * rows)};
+    const cuuint32_t box[3] = {64, BK, 1}, step[3] = {1, 1, 1};
+    if (encoder()(&m, type, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         throw std::runtime_error("cuTensorMapEncodeTiled refused a tensor map");
     return m;
 }
 
-template <int MODE, int MT, class T>
-void launch_tile(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
-    const int64_t pitch = (a.k + 31) / 32 * 32;
-    const CUtensorMap q = map_of(a.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, a.rows, pitch, CU_TENSOR_MAP_SWIZZLE_NONE);
-    CUtensorMap dy{};
-    if (MODE == TMA)
-        dy = map_of(a.dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n, a.rows, a.ld_dy * 2, CU_TENSOR_MAP_SWIZZLE_128B);
-    const size_t smem = (size_t)p.operands * p.operand_bytes() + (size_t)p.inputs * p.input_bytes() + 1024;
-    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<MODE, MT, T>), RING + 1024)) return;
-    k_wgrad8<MODE, MT, T><<<p.ctas, THREADS, smem, s>>>(a, p, q, dy, part, part_db);
+template <int P, class T>
+void launch_split(const wc_act8_wgrad_args& a, const Plan& p, __nv_bfloat16* to, cudaStream_t s) {
+    const bool vec = ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * sizeof(T)) % 16 == 0;
+    const int64_t blocks = (a.rows * (p.split_ld / 8) + 255) / 256;
+    k_split<T, P><<<(unsigned)std::min<int64_t>(blocks, 148 * 16), 256, 0, s>>>(static_cast<const T*>(a.dy), a.rows, a.n, a.ld_dy,
+                                                                              vec, to, p.split_ld);
 }
-template <int MODE, class T>
-void launch_mode(const wc_act8_wgrad_args& a, const Plan& p, float* part, float* part_db, cudaStream_t s) {
-    if (p.mt == 2) launch_tile<MODE, 2, T>(a, p, part, part_db, s);
-    else launch_tile<MODE, 1, T>(a, p, part, part_db, s);
+
+template <int P, int MT>
+void launch_tile(const wc_act8_wgrad_args& a, const Plan& p, const __nv_bfloat16* split, float* part, float* part_db, cudaStream_t s) {
+    const int64_t pitch = (a.k + 31) / 32 * 32;
+    const CUtensorMap q = map_of(a.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, a.rows, 1, pitch, CU_TENSOR_MAP_SWIZZLE_NONE);
+    const CUtensorMap dy = p.split_ld
+        ? map_of(split, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n, a.rows, P, p.split_ld * 2, CU_TENSOR_MAP_SWIZZLE_128B)
+        : map_of(a.dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n, a.rows, 1, a.ld_dy * 2, CU_TENSOR_MAP_SWIZZLE_128B);
+    const size_t smem = (size_t)p.ring_bytes() + 1024;
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<P, MT>), RING + 1024)) return;
+    k_wgrad8<P, MT><<<p.ctas, THREADS, smem, s>>>(a, p, q, dy, part, part_db);
 }
 
 template <class T>
@@ -652,10 +696,8 @@ void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, 
 
 uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
     if (!a.n || !a.rows) return 0;
-    uint64_t most = 0;
-    const Plan p = plan_of(a, mode_of(a));
-    if (p.joined) most = (uint64_t)2 * p.ctas * (p.mt * 128 + 1) * p.bn * sizeof(float);
-    return most;
+    const Plan p = plan_of(a);
+    return parts_bytes(a, p) + (p.joined ? (uint64_t)2 * p.ctas * (p.mt * 128 + 1) * p.bn * sizeof(float) : 0);
 }
 
 void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
@@ -664,14 +706,17 @@ void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
         if (a.db) cudaMemsetAsync(a.db, 0, (size_t)a.n * 4, s);
         return;
     }
-    const int mode = mode_of(a);
-    const Plan p = plan_of(a, mode);
-    float* part = static_cast<float*>(a.workspace);
+    const Plan p = plan_of(a);
+    __nv_bfloat16* split = static_cast<__nv_bfloat16*>(a.workspace);
+    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + parts_bytes(a, p));
     float* part_db = part + (int64_t)2 * p.ctas * p.mt * 128 * p.bn;
-    if (mode == TMA) launch_mode<TMA, __nv_bfloat16>(a, p, part, part_db, s);
-    else if (mode == BF16) launch_mode<BF16, __nv_bfloat16>(a, p, part, part_db, s);
-    else if (mode == F16) launch_mode<F16, __half>(a, p, part, part_db, s);
-    else launch_mode<F32, float>(a, p, part, part_db, s);
+    if (p.parts == 3) launch_split<3, float>(a, p, split, s);
+    else if (p.parts == 2) launch_split<2, __half>(a, p, split, s);
+    else if (p.split_ld) launch_split<1, __nv_bfloat16>(a, p, split, s);
+    const auto launch = p.parts == 3   ? (p.mt == 2 ? launch_tile<3, 2> : launch_tile<3, 1>)
+                        : p.parts == 2 ? (p.mt == 2 ? launch_tile<2, 2> : launch_tile<2, 1>)
+                                       : (p.mt == 2 ? launch_tile<1, 2> : launch_tile<1, 1>);
+    launch(a, p, split, part, part_db, s);
     if (!p.joined) return;
     if (a.out_type == WC_F32) launch_join<float>(a, p, part, part_db, s);
     else if (a.out_type == WC_F16) launch_join<__half>(a, p, part, part_db, s);
