@@ -9,13 +9,14 @@
 //
 // Both operands are summed over the rows, their slow axis, so both are MN-major
 // in shared memory: a stage holds 64 rows, 64 columns of a row being one
-// 128-byte swizzled line. Per CTA, MT 128-row tiles of dw (channels of x8) by
-// `bn` columns:
+// 128-byte swizzled line. A CTA's tile of dw is MT x 128 columns (of dy, the M
+// of the product) by `bk` channels of x8 (its N, any multiple of 32: little is
+// converted that is not used):
 //   producers   (2 warps) x8's bytes and units, and dy, into shared memory
 //   converters  (2 teams of 8 warps, a stage each in turn) x8 to bf16 in shared
 //               memory; and the epilogue out of TMEM
 //   issuer      (1 warp) the products
-//   column sums (2 warps) db from the dy tiles in shared memory
+//   column sums (1 warp) db from the dy tiles in shared memory
 // The work is tiles x stages units dealt in equal runs to the CTAs; a tile
 // that falls to several is joined from their partial results by a second
 // kernel, in a fixed order.
@@ -34,25 +35,24 @@ namespace {
 
 constexpr int BK = 64;           // rows of a stage
 constexpr int RAW = BK * 64, GROUP = BK * 128;  // bytes of 64 columns of a stage, as bytes and as bf16
-constexpr int UNIT_ROW = 12, UNITS = BK * UNIT_ROW;  // the units of a stage's row (up to 8, in whole words), and of a stage
-constexpr int TEAM = 256, CONVERTERS = 2 * TEAM, THREADS = CONVERTERS + 160;
+constexpr int UNIT_WORDS = 3, UNITS = BK * UNIT_WORDS * 4;  // a stage's units: up to 8 of a row, in whole words
+constexpr int TEAM = 256, CONVERTERS = 2 * TEAM, THREADS = CONVERTERS + 128;
 constexpr int MAX_STAGES = 8, MAX_CTAS = 148;
 constexpr int RING = 230912;  // shared memory of the stages: 3 of the widest tile's operands, 3 of its dy, 2 of its x8
 constexpr uint32_t TMEM_COLS = 512;
 
-// dy's parts, and the widest tile whose sums fit TMEM beside those of the other parts
-__host__ __device__ constexpr int widest(int parts) { return parts == 1 ? 256 : parts == 2 ? 128 : 64; }
-
 struct Plan {
-    int mt, bn, ktiles, ntiles, ctas, joined, limit, parts, operands, dys, xs;
+    int mt, bk, ktiles, ntiles, ctas, joined, limit, parts, operands, dys, xs;
     int steps;              // stages of a tile
     int64_t units;          // tiles x steps, below 2^31
     int64_t split_ld;       // elements of a row of dy's parts in the workspace; 0: dy as it is
-    __host__ __device__ int groups() const { return (bn + 63) / 64; }
+    __host__ __device__ int x_groups() const { return (bk + 63) / 64; }
     // a stage of each ring: x8 as bytes and its units, dy's parts, x8 as bf16
-    __host__ __device__ int x_bytes() const { return mt * 2 * RAW + UNITS; }
-    __host__ __device__ int dy_bytes() const { return parts * groups() * GROUP; }
-    __host__ __device__ int operand_bytes() const { return mt * 2 * GROUP; }
+    __host__ __device__ int x_bytes() const { return x_groups() * RAW + UNITS; }
+    __host__ __device__ int dy_bytes() const { return parts * mt * 2 * GROUP; }
+    __host__ __device__ int operand_bytes() const { return x_groups() * GROUP; }
+    // the CTA that a unit falls to
+    __host__ __device__ int owner(int64_t u) const { return (int)(((u + 1) * ctas - 1) / units); }
     __host__ __device__ int ring_bytes() const { return operands * operand_bytes() + dys * dy_bytes() + xs * x_bytes(); }
 };
 
@@ -131,11 +131,11 @@ __device__ __forceinline__ uint32_t even_bytes(uint32_t w, __nv_bfloat162 unit) 
     const __nv_bfloat162 v = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b)), unit);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
-// 8 bytes to 8 bf16; of each four, the middle two change places (the rows of the tile do, see channel())
+// 8 bytes to 8 bf16; of each four, the middle two change places (so do the tile's channels, see channel())
 __device__ __forceinline__ uint4 eight_bytes(uint32_t x, uint32_t y, __nv_bfloat162 unit) {
     return make_uint4(even_bytes(x, unit), even_bytes(x >> 8, unit), even_bytes(y, unit), even_bytes(y >> 8, unit));
 }
-__device__ __forceinline__ int channel(int row) { return (row & ~3) | (row & 1) << 1 | (row >> 1 & 1); }
+__device__ __forceinline__ constexpr int channel(int i) { return (i & ~3) | (i & 1) << 1 | (i >> 1 & 1); }
 
 // Part `p` of v as bf16 and what is left for the next ones. An infinity or NaN goes whole into the first.
 __device__ __forceinline__ float part_of(float& v) {
@@ -173,39 +173,20 @@ __global__ void __launch_bounds__(256) k_split(const T* __restrict__ dy, int64_t
     }
 }
 
-// W columns of one row of dw: stored, or what is there added to them
+// W channels of one column of dw, `ld` apart, stored or (32-bit results) added to what is there. The operand's
+// channels lie in channel()'s order.
 template <int W, class T>
-__device__ __forceinline__ void store_run(T* p, const float* v, int count, bool vec) {
-    if (vec && count >= W) {  // whole 32-byte sectors
-        constexpr int E = 32 / sizeof(T);
+__device__ __forceinline__ void put(T* p, int64_t ld, const float* v, int count, bool add) {
 #pragma unroll
-        for (int i = 0; i < W / E; ++i) {
-            alignas(16) T e[E];
+    for (int i = 0; i < W; i += 8) {
+        float o[8] = {};
+        if (sizeof(T) == 4 && add)
 #pragma unroll
-            for (int j = 0; j < E; ++j) e[j] = from_f<T>(v[i * E + j]);
-            const uint32_t* r = reinterpret_cast<const uint32_t*>(e);
-            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + i * E), "r"(r[0]), "r"(r[1]),
-                         "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                         : "memory");
-        }
-    } else {
+            for (int j = 0; j < 8; ++j)
+                if (i + j < count) o[j] = to_f(p[j * ld]);
 #pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (i < count) p[i] = from_f<T>(v[i]);
-    }
-}
-template <int W>
-__device__ __forceinline__ void add_run(float* v, const float* p, int count, bool vec) {
-    if (vec && count >= W) {
-#pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const float4 w = reinterpret_cast<const float4*>(p)[i];
-            v[4 * i] += w.x, v[4 * i + 1] += w.y, v[4 * i + 2] += w.z, v[4 * i + 3] += w.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; ++i)
-            if (i < count) v[i] += p[i];
+        for (int j = 0; j < 8; ++j, p += ld)
+            if (i + j < count) *p = from_f<T>(o[j] + v[channel(i + j)]);
     }
 }
 // W consecutive f32 columns of this thread's TMEM lane
@@ -233,12 +214,14 @@ constexpr int RUN = 40;
 // The units (a stage of a tile each) that fall to a CTA, in order. A share is
 // what it has of one tile, cut into runs.
 struct Walk {
-    int u, end, tile, s;      // unit, end of the CTA's, their tile and stage
+    int u, end, s;            // unit, end of the CTA's, its stage
+    int kt, nt;               // its tile: channels fastest
     int in_run;               // stages of the run before this one
     bool whole, head, begins; // the share is the whole tile; the CTA's first share; the share's first run
     __device__ explicit Walk(const Plan& p) {
         u = (int)(p.units * blockIdx.x / p.ctas), end = (int)(p.units * (blockIdx.x + 1) / p.ctas);
-        tile = u / p.steps, s = u - tile * p.steps;
+        const int tile = u / p.steps;
+        s = u - tile * p.steps, nt = tile / p.ktiles, kt = tile - nt * p.ktiles;
         head = true;
         share(p);
     }
@@ -254,8 +237,13 @@ struct Walk {
     }
     __device__ void next(const Plan& p) {
         ++u, ++in_run;
-        if (++s == p.steps) s = 0, ++tile, head = false, share(p);
-        else if (in_run == p.limit) in_run = 0, begins = false;
+        if (++s == p.steps) {
+            s = 0, head = false;
+            if (++kt == p.ktiles) kt = 0, ++nt;
+            share(p);
+        } else if (in_run == p.limit) {
+            in_run = 0, begins = false;
+        }
     }
 };
 
@@ -263,14 +251,14 @@ template <int P, int MT>
 __global__ void __launch_bounds__(THREADS, 1)
     k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_q,
              const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
-    constexpr int GROUPS = 2 * MT;
+    constexpr int GROUPS = 2 * MT;  // of 64 columns of dy
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
     uint8_t* operands = raw + ((1024 - (umma::smem_u32(raw) & 1023)) & 1023);
     uint8_t* dys = operands + p.operands * p.operand_bytes();
     uint8_t* xs = dys + p.dys * p.dy_bytes();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int groups = p.groups();
+    const int x_groups = p.x_groups();
     volatile int* failed = &sh.failed;
 
     if (threadIdx.x == 0) {
@@ -278,7 +266,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             umma::mbar_init(&sh.x_full[i], 1 + 32);  // the bytes, and each lane's share of the units
             umma::mbar_init(&sh.x_empty[i], TEAM / 32);
             umma::mbar_init(&sh.dy_full[i], 1);
-            umma::mbar_init(&sh.dy_empty[i], 3);  // the issuer's commit, the column sums' two warps
+            umma::mbar_init(&sh.dy_empty[i], 2);  // the issuer's commit, the column sums
             umma::mbar_init(&sh.op_full[i], TEAM / 32);
             umma::mbar_init(&sh.op_empty[i], 1);
         }
@@ -307,9 +295,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 0) {  // ------------------------------------------- issuer
         // Little to compute between two products: that is what keeps the tensor core waiting. The warp stays together
         // and one lane issues, so that the operands are uniform; a stage's descriptors differ in the address field only.
-        const uint32_t idesc = umma::idesc_bf16(128, p.bn) | (1u << 15) | (1u << 16);
-        const uint64_t a_first = desc_mn(umma::smem_u32(operands)), b_first = desc_mn(umma::smem_u32(dys));
-        const uint32_t a_step = p.operand_bytes() >> 4, b_step = p.dy_bytes() >> 4, q_step = (groups * GROUP) >> 4;
+        const uint32_t idesc = umma::idesc_bf16(128, p.bk) | (1u << 15) | (1u << 16);
+        const uint64_t a_first = desc_mn(umma::smem_u32(dys)), b_first = desc_mn(umma::smem_u32(operands));
+        const uint32_t a_step = p.dy_bytes() >> 4, b_step = p.operand_bytes() >> 4;
         uint32_t done = 0;
         bool ok = true;
         while (ok && walk.more()) {
@@ -321,15 +309,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                 ok = ok && wait_all(&sh.op_full[op.slot], op.phase);
                 umma::fence_after_sync();
                 if (ok) {
-                    const uint64_t A = a_first + op.slot * a_step;
-                    const uint64_t B = b_first + dy.slot * b_step;
+                    const uint64_t A = a_first + dy.slot * a_step, B = b_first + op.slot * b_step;
 #pragma unroll
                     for (int m = 0; m < MT; ++m)
 #pragma unroll
                         for (int q = 0; q < P; ++q)
 #pragma unroll
                             for (int k = 0; k < BK / 16; ++k)
-                                mma_one(tmem + (m * P + q) * p.bn, A + (m * 2 * GROUP >> 4) + k * 128, B + q * q_step + k * 128,
+                                mma_one(tmem + (m * P + q) * p.bk, A + ((q * GROUPS + m * 2) * GROUP >> 4) + k * 128, B + k * 128,
                                         idesc, k ? 1 : i);
                     commit_one(&sh.op_empty[op.slot]);
                     commit_one(&sh.dy_empty[dy.slot]);
@@ -350,11 +337,13 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool ok = true;
             for (; walk.more(); walk.next(p), dy.next(), ++it) {
                 if (it >= p.dys && !(ok = wait(&sh.dy_empty[dy.slot], dy.phase ^ 1))) break;
-                const int n0 = walk.tile / p.ktiles * p.bn;
+                const int n0 = walk.nt * (MT * 128);
                 umma::expect_tx(&sh.dy_full[dy.slot], p.dy_bytes());
                 uint32_t to = ring + dy.slot * p.dy_bytes();
+#pragma unroll
                 for (int q = 0; q < P; ++q)
-                    for (int g = 0; g < groups; ++g, to += GROUP)
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g, to += GROUP)
                         tma_load(to, &map_dy, n0 + 64 * g, walk.s * BK, q, &sh.dy_full[dy.slot]);
             }
             if (!ok)  // the copies in flight land before the CTA leaves
@@ -362,7 +351,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     umma::mbar_wait(&sh.dy_full[i % p.dys], (i / p.dys) & 1, umma::DRAIN_NS);
         }
         __syncwarp();
-    } else if (warp == THREADS / 32 - 1) {  // -------------- x8's producer
+    } else if (warp == 2) {  // ----------------------------- x8's producer
         // The units' rows have any alignment: the words that hold a row's are copied, and read at its first one's offset.
         const int64_t blocks = (a.k + 31) / 32;
         const uint32_t ring = umma::smem_u32(xs);
@@ -371,23 +360,22 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (; walk.more(); walk.next(p), x.next(), ++it) {
             if (it >= p.xs && !(ok = wait_all(&sh.x_empty[x.slot], x.phase ^ 1))) break;
             const uint32_t to = ring + x.slot * p.x_bytes();
-            const int tile = walk.tile % p.ktiles, t0 = walk.s * BK;
+            const int k0 = walk.kt * p.bk, t0 = walk.s * BK;
             if (lane == 0) {
-                umma::expect_tx(&sh.x_full[x.slot], GROUPS * RAW);
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) tma_load(to + g * RAW, &map_q, tile * (MT * 128) + 64 * g, t0, 0, &sh.x_full[x.slot]);
+                umma::expect_tx(&sh.x_full[x.slot], x_groups * RAW);
+                for (int g = 0; g < x_groups; ++g) tma_load(to + g * RAW, &map_q, k0 + 64 * g, t0, 0, &sh.x_full[x.slot]);
             }
-            const int count = (int)min((int64_t)MT * 4, blocks - (int64_t)tile * (MT * 4));
+            const int count = (int)min((int64_t)(p.bk / 32), blocks - k0 / 32);
 #pragma unroll
             for (int i = 0; i < BK / 32; ++i) {
                 const int row = i * 32 + lane;
                 if ((int64_t)t0 + row < a.rows) {
-                    const uintptr_t from = reinterpret_cast<uintptr_t>(a.scale + ((int64_t)t0 + row) * blocks + tile * (MT * 4));
+                    const uintptr_t from = reinterpret_cast<uintptr_t>(a.scale + ((int64_t)t0 + row) * blocks + k0 / 32);
                     const int words = (int)((from & 3) + count + 3) >> 2;
 #pragma unroll
-                    for (int w = 0; w < UNIT_ROW / 4; ++w)
+                    for (int w = 0; w < UNIT_WORDS; ++w)
                         if (w < words)
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + GROUPS * RAW + row * UNIT_ROW + 4 * w),
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + x_groups * RAW + (w * BK + row) * 4),
                                          "l"((from & ~(uintptr_t)3) + 4 * w)
                                          : "memory");
                 }
@@ -399,41 +387,45 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int i = it > p.xs ? it - p.xs : 0; i < it; ++i)
                 umma::mbar_wait(&sh.x_full[i % p.xs], (i / p.xs) & 1, umma::DRAIN_NS);
         __syncwarp();
-    } else if (warp < 4) {  // --------------------------------- column sums
-        const int c = 4 * (threadIdx.x - 64);  // this thread's four columns
+    } else if (warp == 3) {  // -------------------------------- column sums
+        // A lane has eight columns, and every ROWS-th row of them. The tiles of a column block take the stages in turn,
+        // so that no CTA has more of this than another; a CTA keeps its sums until the column block ends.
+        constexpr int ROWS = 2 / MT;
+        const int c = lane % (32 / ROWS) * 8, first_row = lane / (32 / ROWS);
         bool ok = true;
-        float sum[4] = {};
+        float sum[8] = {};
+        int turn = walk.s % p.ktiles;  // the tile whose stage this is
         for (; walk.more(); walk.next(p), dy.next()) {
-            const bool mine = a.db && walk.tile % p.ktiles == 0 && c < p.bn;
-            if (walk.begins && walk.in_run == 0)
-                for (float& v : sum) v = 0.0f;
+            if (walk.s == 0) turn = 0;
             ok = ok && wait_all(&sh.dy_full[dy.slot], dy.phase);
-            if (mine && ok) {
+            if (a.db && ok && turn == walk.kt) {
                 const uint8_t* B = dys + dy.slot * p.dy_bytes();
-                float x[4] = {};
+                unsigned long long x[4] = {};  // pairs of 32-bit sums
                 for (int q = 0; q < P; ++q) {
-                    const uint8_t* G = B + (q * groups + (c >> 6)) * GROUP + (c & 4) * 2;
-#pragma unroll 16
-                    for (int t = 0; t < BK; ++t) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
-                        x[0] += umma::Op16<false>::lo(w.x), x[1] += umma::Op16<false>::hi(w.x);
-                        x[2] += umma::Op16<false>::lo(w.y), x[3] += umma::Op16<false>::hi(w.y);
+                    const uint8_t* G = B + (q * GROUPS + (c >> 6)) * GROUP;
+#pragma unroll 8
+                    for (int i = 0; i < BK / ROWS; ++i) {
+                        const int t = i * ROWS + first_row;
+                        const uint4 w = *reinterpret_cast<const uint4*>(G + t * 128 + ((((c & 63) >> 3) ^ (t & 7)) << 4));
+                        x[0] = umma::f2_add(x[0], umma::f2(w.x << 16, w.x & 0xffff0000u));
+                        x[1] = umma::f2_add(x[1], umma::f2(w.y << 16, w.y & 0xffff0000u));
+                        x[2] = umma::f2_add(x[2], umma::f2(w.z << 16, w.z & 0xffff0000u));
+                        x[3] = umma::f2_add(x[3], umma::f2(w.w << 16, w.w & 0xffff0000u));
                     }
                 }
 #pragma unroll
-                for (int h = 0; h < 4; ++h) sum[h] += x[h];
+                for (int h = 0; h < 4; ++h) sum[2 * h] += umma::f2_lo(x[h]), sum[2 * h + 1] += umma::f2_hi(x[h]);
             }
             __syncwarp();
             if (ok && lane == 0) arrive(&sh.dy_empty[dy.slot]);
-            if (mine && walk.share_ends(p)) {
-                const int64_t n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    if (c + h >= p.bn) continue;
-                    const float v = ok ? sum[h] : __uint_as_float(0x7fffffffu);
-                    if (!walk.whole) part_db[(2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)p.bn + c + h] = v;
-                    else if (n0 + c + h < a.n) a.db[n0 + c + h] = v;
-                }
+            if (++turn == p.ktiles) turn = 0;
+            if (a.db && (walk.u + 1 == walk.end || (walk.s + 1 == p.steps && walk.kt + 1 == p.ktiles))) {
+                if (!ok)
+                    for (float& v : sum) v = __uint_as_float(0x7fffffffu);
+                // the slot of (column block, CTA): their sum grows along the walk
+                float4* to = reinterpret_cast<float4*>(part_db) + (walk.nt + blockIdx.x) * 64 + lane * 2;
+                to[0] = make_float4(sum[0], sum[1], sum[2], sum[3]), to[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+                for (float& v : sum) v = 0.0f;
             }
         }
     } else {  // -------------------------------------------------- converters
@@ -445,28 +437,31 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t raw_at = ar * 64 + ac * 8, lo_at = ar * 128 + ((ac ^ (ar & 7)) << 4), hi_at = ar * 128 + (((ac + 1) ^ (ar & 7)) << 4);
         // where a row's units start in their words, up to the stage's and the tile's share
         const uint32_t unit_row = (uint32_t)(reinterpret_cast<uintptr_t>(a.scale) + ar * blocks), unit_stage = (uint32_t)(BK * blocks);
+        constexpr int X_GROUPS = 4;  // at most
         bool ok = true;
         uint32_t done = 0, it = 0;
         for (; walk.more(); walk.next(p), ++it, x.next(), op.next()) {
             if (ok && (int)(it & 1) == team) {
                 ok = wait_all(&sh.x_full[x.slot], x.phase);
                 const uint8_t* X = xs + x.slot * p.x_bytes() + raw_at;
-                const uint32_t first = (unit_row + walk.s * unit_stage + walk.tile % p.ktiles * (MT * 4)) & 3;
-                const uint8_t* units = xs + x.slot * p.x_bytes() + GROUPS * RAW + ar * UNIT_ROW + first + (ac >> 2);
-                uint4 q[GROUPS];
-                uint32_t code[GROUPS];
+                const uint32_t first = ((unit_row + walk.s * unit_stage + walk.kt * (p.bk / 32)) & 3) + (ac >> 2);
+                const uint8_t* units = xs + x.slot * p.x_bytes() + x_groups * RAW + ar * 4;
+                // Rows past the end come as bytes 0; their units are whatever the memory held, and have to be a number:
+                // 0 times a finite one is 0. (A NaN block, code 255, is 0 times infinity.)
+                const bool there = (int64_t)walk.s * BK + ar < a.rows;
+                uint4 q[X_GROUPS];
+                uint32_t code[X_GROUPS];
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
+                for (int g = 0; g < X_GROUPS; ++g) {
+                    if (g >= x_groups) break;
                     q[g] = *reinterpret_cast<const uint4*>(X + g * RAW);
-                    code[g] = units[2 * g];
+                    code[g] = units[((first + 2 * g) >> 2) * (BK * 4) + ((first + 2 * g) & 3)];
                 }
                 if (it >= (uint32_t)p.operands) ok = ok && wait_all(&sh.op_empty[op.slot], op.phase ^ 1);
                 uint8_t* A = operands + op.slot * p.operand_bytes();
 #pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    // Rows and blocks past the end come as bytes 0; their units are whatever the memory held, and have
-                    // to be a number: 0 times a finite one is 0. (A NaN block, code 255, is 0 times infinity.)
-                    const bool there = (int64_t)walk.s * BK + ar < a.rows;
+                for (int g = 0; g < X_GROUPS; ++g) {
+                    if (g >= x_groups) break;
                     const uint32_t uu = (there ? code[g] : 127u) * 0x00800080u;
                     const __nv_bfloat162 unit2 = *reinterpret_cast<const __nv_bfloat162*>(&uu);
                     *reinterpret_cast<uint4*>(A + g * GROUP + lo_at) = eight_bytes(q[g].x, q[g].y, unit2);
@@ -480,49 +475,33 @@ __global__ void __launch_bounds__(THREADS, 1)
             // the tile out of TMEM: every fourth warp has the lanes of one quarter
             ok = ok && wait_all(&sh.acc_full, done & 1);
             umma::fence_after_sync();
-            const int64_t k0 = (int64_t)(walk.tile % p.ktiles) * (MT * 128), n0 = (int64_t)(walk.tile / p.ktiles) * p.bn;
-            constexpr int W = P == 1 ? 32 : 16;  // columns at a time
-            const int row = (warp & 3) * 32 + lane, runs = p.bn / W;
+            constexpr int W = P == 1 ? 32 : 16;  // channels at a time; a lane is a column of dw, 32 next to each other
+            const int64_t k0 = (int64_t)walk.kt * p.bk;
+            const int row = (warp & 3) * 32 + lane, runs = p.bk / W;
             for (int i = w >> 2; i < MT * runs; i += CONVERTERS / 128) {
                 const int m = i / runs, c = i % runs * W;
+                const int64_t n = (int64_t)walk.nt * (MT * 128) + m * 128 + row;
                 float v[W];
-                const uint32_t from = tmem + ((uint32_t)(warp & 3) * 32 << 16) + m * P * p.bn + c;
-                tmem_load(from + (P - 1) * p.bn, v);  // the smallest part first
+                const uint32_t from = tmem + ((uint32_t)(warp & 3) * 32 << 16) + m * P * p.bk + c;
+                tmem_load(from + (P - 1) * p.bk, v);  // the smallest part first
 #pragma unroll
                 for (int q = P - 2; q >= 0; --q) {
                     float y[W];
-                    tmem_load(from + q * p.bn, y);
+                    tmem_load(from + q * p.bk, y);
 #pragma unroll
                     for (int e = 0; e < W; ++e) v[e] += y[e];
                 }
                 if (!ok)
                     for (float& e : v) e = __uint_as_float(0x7fffffffu);
-                const int64_t k = k0 + m * 128 + channel(row), n = n0 + c;
                 if (!walk.whole) {
-                    // four columns at a time, rows next to each other: 512 bytes in a row for the warp
-                    float4* to = reinterpret_cast<float4*>(part) +
-                                 ((2 * blockIdx.x + (walk.head ? 0 : 1)) * (int64_t)MT + m) * (p.bn / 4 * 128) + c / 4 * 128 + row;
-#pragma unroll
-                    for (int e = 0; e < W / 4; ++e) {
-                        float4 w = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                        if (!walk.begins) {
-                            const float4 o = to[e * 128];
-                            w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
-                        }
-                        to[e * 128] = w;
-                    }
-                } else if (k < a.k && n < a.n) {
-                    const int count = (int)min((int64_t)W, a.n - n);
-                    const int64_t to = k * a.n + n;
-                    const bool vec = ((uintptr_t)a.dw & 31) == 0 && a.n % 16 == 0;
-                    if (a.out_type == WC_F32) {
-                        if (!walk.begins) add_run<W>(v, static_cast<float*>(a.dw) + to, count, vec);
-                        store_run<W>(static_cast<float*>(a.dw) + to, v, count, vec);
-                    } else if (a.out_type == WC_F16) {
-                        store_run<W>(static_cast<__half*>(a.dw) + to, v, count, vec);
-                    } else {
-                        store_run<W>(static_cast<__nv_bfloat16*>(a.dw) + to, v, count, vec);
-                    }
+                    float* to = part + (((int64_t)(2 * blockIdx.x + (walk.head ? 0 : 1)) * MT + m) * p.bk + c) * 128 + row;
+                    put<W>(to, 128, v, W, !walk.begins);
+                } else if (n < a.n) {
+                    const int count = (int)min((int64_t)W, a.k - k0 - c);
+                    const int64_t to = (k0 + c) * a.n + n;
+                    if (a.out_type == WC_F32) put<W>(static_cast<float*>(a.dw) + to, a.n, v, count, !walk.begins);
+                    else if (a.out_type == WC_F16) put<W>(static_cast<__half*>(a.dw) + to, a.n, v, count, false);
+                    else put<W>(static_cast<__nv_bfloat16*>(a.dw) + to, a.n, v, count, false);
                 }
             }
             umma::fence_before_sync();
@@ -557,31 +536,43 @@ struct Splits {
     }
 };
 
-// Joins the split tiles (one a blockIdx.y). A thread has 4 columns of a row, or
-// of db; with many CTAs to a tile they are dealt to blockDim.y
-// threads and those joined in order.
+// Joins the split tiles (one a blockIdx.y, then a column block of db each). A
+// thread has 4 columns of a channel, or of db; with many CTAs to a tile they
+// are dealt to blockDim.y threads and those joined in order.
 constexpr int JOINERS = 256;
 template <class T>
 __global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, Plan p, const __grid_constant__ Splits splits,
                                                          const float* part, const float* part_db) {
     __shared__ float4 s[JOINERS];
-    const Split& cut = splits.at[blockIdx.y];
-    const int tile = cut.tile, c0 = cut.c0, c1 = cut.c1;
-    const int rows = p.mt * 128, runs = p.bn / 4;
-    // in the order of the partial results: the rows of four columns, then db's columns
-    const int i = blockIdx.x * blockDim.x + threadIdx.x;
-    const bool bias = i >= rows * runs;
-    const int m = i / (runs * 128), c = bias ? (i - rows * runs) * 4 : i / 128 % runs * 4, r = m * 128 + channel(i & 127);
-    const int64_t k0 = tile % p.ktiles * rows, n0 = tile / p.ktiles * p.bn, n = n0 + c;
-    const bool in = i < (rows + 1) * runs && n < a.n && (bias ? a.db && tile % p.ktiles == 0 : k0 + r < a.k);
+    const int i = blockIdx.x * blockDim.x + threadIdx.x, cols = p.mt * 128;
+    const bool bias = (int)blockIdx.y >= splits.n;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (in)
-#pragma unroll 4
-        for (int j = c0 + (int)threadIdx.y; j <= c1; j += blockDim.y) {
-            const int64_t slot = j == c0 ? cut.slot : 2 * j;
-            const float4 w = *reinterpret_cast<const float4*>(bias ? part_db + slot * p.bn + c : part + (slot * rows * runs + i) * 4);
-            v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    auto add = [&](const float* from) {
+        const float4 w = *reinterpret_cast<const float4*>(from);
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+    };
+    int64_t k = 0, n;
+    bool in;
+    if (bias) {
+        const int nt = blockIdx.y - splits.n, rows = 2 / p.mt;
+        const int64_t per = (int64_t)p.ktiles * p.steps;
+        n = (int64_t)nt * cols + i * 4;
+        in = i < cols / 4 && n < a.n;
+        if (in) {
+            const int c0 = p.owner(nt * per), c1 = p.owner((nt + 1) * per - 1);
+            for (int j = c0 + (int)threadIdx.y; j <= c1; j += blockDim.y)
+                for (int r = 0; r < rows; ++r) add(part_db + ((int64_t)(nt + j) * 64 + r * (64 / rows) + i) * 4);
         }
+    } else {
+        const Split& cut = splits.at[blockIdx.y];
+        const int m = i / (p.bk * 32), c = i / 32 % p.bk;
+        k = (int64_t)(cut.tile % p.ktiles) * p.bk + c, n = (int64_t)(cut.tile / p.ktiles) * cols + m * 128 + i % 32 * 4;
+        in = i < p.bk * cols / 4 && n < a.n && k < a.k;
+        if (in)
+#pragma unroll 4
+            for (int j = cut.c0 + (int)threadIdx.y; j <= cut.c1; j += blockDim.y)
+                add(part + ((int64_t)(j == cut.c0 ? cut.slot : 2 * j) * p.bk * cols + i * 4));
+    }
     if (blockDim.y > 1) {
         s[threadIdx.y * blockDim.x + threadIdx.x] = v;
         __syncthreads();
@@ -597,7 +588,7 @@ __global__ void __launch_bounds__(JOINERS) k_wgrad8_join(wc_act8_wgrad_args a, P
     for (int j = 0; j < 4; ++j) {
         if (n + j >= a.n) break;
         if (bias) a.db[n + j] = e[j];
-        else static_cast<T*>(a.dw)[(k0 + r) * a.n + n + j] = from_f<T>(e[j]);
+        else static_cast<T*>(a.dw)[k * a.n + n + j] = from_f<T>(e[j]);
     }
 }
 
@@ -607,11 +598,12 @@ Plan plan_of(const wc_act8_wgrad_args& a) {
     const bool as_is = p.parts == 1 && ((uintptr_t)a.dy & 15) == 0 && (a.ld_dy * 2) % 16 == 0;
     p.split_ld = as_is ? 0 : (a.n + 7) / 8 * 8;
     p.steps = (int)((a.rows + BK - 1) / BK);
-    p.mt = a.k > 128 ? 2 : 1;
-    const int64_t nt = (a.n + widest(p.parts) - 1) / widest(p.parts);
-    p.bn = (int)(((a.n + nt - 1) / nt + 31) / 32 * 32);
-    p.ktiles = (int)((a.k + p.mt * 128 - 1) / (p.mt * 128));
-    p.ntiles = (int)((a.n + p.bn - 1) / p.bn);
+    // TMEM holds 512 columns: MT x parts x bk sums
+    p.mt = p.parts == 1 && a.n > 128 ? 2 : 1;
+    const int64_t widest = p.parts == 3 ? 160 : 256, kt = (a.k + widest - 1) / widest;
+    p.bk = (int)(((a.k + kt - 1) / kt + 31) / 32 * 32);
+    p.ktiles = (int)((a.k + p.bk - 1) / p.bk);
+    p.ntiles = (int)((a.n + p.mt * 128 - 1) / (p.mt * 128));
     p.units = (int64_t)p.ktiles * p.ntiles * p.steps;
     p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
@@ -688,7 +680,9 @@ void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, 
     int sharers = 0;
     for (int i = 0; i < splits.n; ++i) sharers = std::max(sharers, splits.at[i].c1 - splits.at[i].c0 + 1);
     const int ny = sharers >= 8 ? 32 : 1;
-    const dim3 block(JOINERS / ny, ny), grid(((p.mt * 128 + 1) * (p.bn / 4) + block.x - 1) / block.x, splits.n);
+    const dim3 block(JOINERS / ny, ny);
+    const int wide = splits.n ? p.bk * p.mt * 32 : p.mt * 32;  // threads that sum up a tile, or db alone
+    const dim3 grid((wide + block.x - 1) / block.x, splits.n + (a.db ? p.ntiles : 0));
     k_wgrad8_join<T><<<grid, block, 0, s>>>(a, p, splits, part, part_db);
 }
 
@@ -697,7 +691,7 @@ void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, 
 uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
     if (!a.n || !a.rows) return 0;
     const Plan p = plan_of(a);
-    return parts_bytes(a, p) + (p.joined ? (uint64_t)2 * p.ctas * (p.mt * 128 + 1) * p.bn * sizeof(float) : 0);
+    return parts_bytes(a, p) + (uint64_t)(p.ntiles + p.ctas) * 1024 + (p.joined ? (uint64_t)2 * p.ctas * p.mt * 128 * p.bk * sizeof(float) : 0);
 }
 
 void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
@@ -708,8 +702,8 @@ void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
     }
     const Plan p = plan_of(a);
     __nv_bfloat16* split = static_cast<__nv_bfloat16*>(a.workspace);
-    float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + parts_bytes(a, p));
-    float* part_db = part + (int64_t)2 * p.ctas * p.mt * 128 * p.bn;
+    float* part_db = reinterpret_cast<float*>(static_cast<uint8_t*>(a.workspace) + parts_bytes(a, p));
+    float* part = part_db + (int64_t)(p.ntiles + p.ctas) * 256;
     if (p.parts == 3) launch_split<3, float>(a, p, split, s);
     else if (p.parts == 2) launch_split<2, __half>(a, p, split, s);
     else if (p.split_ld) launch_split<1, __nv_bfloat16>(a, p, split, s);
@@ -717,7 +711,7 @@ void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
                         : p.parts == 2 ? (p.mt == 2 ? launch_tile<2, 2> : launch_tile<2, 1>)
                                        : (p.mt == 2 ? launch_tile<1, 2> : launch_tile<1, 1>);
     launch(a, p, split, part, part_db, s);
-    if (!p.joined) return;
+    if (!p.joined && !a.db) return;
     if (a.out_type == WC_F32) launch_join<float>(a, p, part, part_db, s);
     else if (a.out_type == WC_F16) launch_join<__half>(a, p, part, part_db, s);
     else launch_join<__nv_bfloat16>(a, p, part, part_db, s);
