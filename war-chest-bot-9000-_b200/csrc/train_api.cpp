@@ -49,7 +49,8 @@ int wc_policy_loss(const wc_policy_loss_args* a, void* stream) {
     if (!type_ok(a->type)) return bad(me, "unknown element type");
     if (a->action_bytes != 4 && a->action_bytes != 8) return bad(me, "action_bytes is 4 or 8");
     if (!size_ok(a->rows, a->width)) return bad(me, "sizes out of range");
-    if (!a->loss || !a->workspace) return bad(me, "null device pointer");
+    if (!a->loss) return bad(me, "null device pointer");
+    if (!a->workspace || off(a->workspace, 16)) return bad(me, "no 16-byte aligned workspace");
     if (a->rows) {
         if (!a->actions || !a->old_logp || !a->advantages || !a->row_out) return bad(me, "null device pointer");
         if (a->width) {

@@ -175,9 +175,9 @@ def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp
             _fail(me, "legal must have unit column stride and rows that do not overlap")
         ld_legal = _ld(legal)
     device = logits.device
-    space = _policy_workspace(rows, width) // 4
-    flat = torch.empty(4 * rows + 1 + space, dtype=torch.float32, device=device)
-    out, loss, scratch = flat.split((4 * rows, 1, space))
+    space = (_policy_workspace(rows, width) + 15) // 16 * 4
+    flat = torch.empty(space + 4 * rows + 1, dtype=torch.float32, device=device)
+    scratch, out, loss = flat.split((space, 4 * rows, 1))  # the workspace first: it has to be aligned
     grad = torch.empty((rows, width), dtype=logits.dtype, device=device) if want_grad else None
     args = _PolicyLossArgs(
         logits.data_ptr(), legal.data_ptr() if legal is not None else None, actions.data_ptr(), old, adv, wts, ref,
