@@ -6,8 +6,9 @@
 // The row's loss depends on the logits through l and H only, so
 //   dloss/dz_j = g (delta_ja - p_j) + w c p_j (ln p_j + H),
 //   g = w (-ratio A [not clipped] - kl_coef (exp(r - l) - 1)).
-// Powers are taken in base 2, 2^(z_j log2 e - c) with c = m log2 e rounded; the
-// factor that the rounding of c puts on every e_j is taken out of ln S again.
+// A power is 2^x with x = (z - m) log2 e rounded; the sum of what that rounding
+// leaves out, times e, goes into S as a correction, so that l (whose difference
+// with another log-probability is what counts) is good to a few 1e-8.
 //
 // What bounds it is the bytes: each logit is read once and its gradient written
 // once. A row stays in registers as it was loaded (16 bytes of logits and their
@@ -21,6 +22,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "kernels.h"
 #include "train.cuh"
 #include "umma.cuh"
 
@@ -38,49 +40,60 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// What a row needs besides its logits
+// What a row needs besides its logits: loaded a row ahead, since the logits' loads wait for it (a row that is void
+// reads none)
 struct RowIn {
-    float w;
-    int64_t act;
+    float w, old, A, r;
+    int act;  // -1: void
+    __device__ __forceinline__ RowIn(const wc_policy_loss_args& a, int64_t t) : w(0.0f), old(0.0f), A(0.0f), r(0.0f), act(-1) {
+        if (t >= a.rows) return;
+        w = a.weights ? a.weights[t] : 1.0f;
+        const int64_t at = a.action_bytes == 8 ? static_cast<const int64_t*>(a.actions)[t]
+                                               : (int64_t) static_cast<const int32_t*>(a.actions)[t];
+        if (at >= 0 && at < a.width && w != 0.0f) act = (int)at;
+        old = a.old_logp[t], A = a.advantages[t];
+        if (a.ref_logp) r = a.ref_logp[t];
+    }
 };
-__device__ __forceinline__ RowIn row_in(const wc_policy_loss_args& a, int64_t t) {
-    RowIn r;
-    r.w = a.weights ? a.weights[t] : 1.0f;
-    r.act = a.action_bytes == 8 ? static_cast<const int64_t*>(a.actions)[t] : (int64_t) static_cast<const int32_t*>(a.actions)[t];
-    return r;
-}
 
-// A row's loss from its parts (m the maximum of all, S and W sums over all
-// relative to it) and the logit of its action.
+// A row's loss from its parts (m the maximum of all, S and W sums of e and e x)
+// and the logit of its action. l is kept in 64 bits up to its differences with
+// the other log-probabilities: they are small, and what rounding l first would
+// add to them is not.
 struct Row {
     float loss, l, H, kl;   // results
-    float c, inv, g, ce, lH; // gradient: p = 2^(z log2 e - c) inv;  d = p (ce (ln p + H) - g) + [action] g
-    __device__ __forceinline__ Row(const wc_policy_loss_args& a, int64_t t, float w, float m, float S, float W, float za) {
-        c = m * LOG2E;
-        const float off = fmaf(m, LOG2E, -c) * LN2;  // ln S = ln(sum of the rounded powers) - off
-        const float lnS = logf(S) - off;
-        l = (za - m) - lnS;
-        H = lnS - W / S * LN2 + off;  // W counts from c as well
-        const float A = a.advantages[t], lo = 1.0f - a.clip_low, hi = 1.0f + a.clip_high;
-        const float ratio = expf(l - a.old_logp[t]);
+    float m, inv, g, ce, k; // gradient: p = e inv;  d = p (ce ln 2 x + k) + [action] g,  k = ce (H - ln S) - g
+    Row() = default;
+    __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float top, float S, float W, float za) : m(top) {
+        const float mean = W / S;  // of x
+        // ln S from S = 2^n f, f about 1; LOG2E as a float is 1.34e-8 (relative) low, which mean puts right to first order
+        int n;
+        float f = frexpf(S, &n);
+        if (f < 0.75f) f *= 2.0f, --n;
+        const double lnS = (double)n * 0.6931471805599453 + (double)fmaf(mean, 9.25e-9f, logf(f));
+        const double ld = ((double)za - (double)m) - lnS;
+        l = (float)ld;
+        H = (float)lnS - mean * LN2;
+        const float lo = 1.0f - a.clip_low, hi = 1.0f + a.clip_high, A = in.A;
+        const float ratio = expf((float)(ld - (double)in.old));
         const float free = ratio * A, clipped = fminf(fmaxf(ratio, lo), hi) * A;
         const bool held = (A > 0.0f && ratio > hi) || (A < 0.0f && ratio < lo);
-        const float d = a.ref_logp ? a.ref_logp[t] - l : 0.0f, em = a.ref_logp ? expm1f(d) : 0.0f;
+        const float d = a.ref_logp ? (float)((double)in.r - ld) : 0.0f, em = a.ref_logp ? expm1f(d) : 0.0f;
         kl = em - d;
         loss = -(free < clipped || isnan(free) ? free : clipped) + a.kl_coef * kl - a.entropy_coef * H;
-        const float up = (a.upstream ? *a.upstream : 1.0f) * w;
+        const float up = (a.upstream ? *a.upstream : 1.0f) * in.w;
         g = up * ((held ? 0.0f : -free) - a.kl_coef * em);
         ce = up * a.entropy_coef;
         inv = 1.0f / S;
-        lH = H - lnS - off;  // ln p + H = (z log2 e - c) ln 2 + lH
+        k = fmaf(ce, H - (float)lnS, -g);
     }
     __device__ __forceinline__ void put(const wc_policy_loss_args& a, int64_t t) const {
         a.row_out[t] = loss, a.row_out[a.rows + t] = l, a.row_out[2 * a.rows + t] = H, a.row_out[3 * a.rows + t] = kl;
     }
     // the gradient at an entry other than the action
     __device__ __forceinline__ float grad(float z) const {
-        const float x = fmaf(z, LOG2E, -c), p = ex2(x) * inv;
-        return ce != 0.0f ? p * fmaf(ce, fmaf(fmaxf(x, -1000.0f), LN2, lH), -g) : p * -g;
+        const float x = fmaxf((z - m) * LOG2E, -1000.0f);
+        return isnan(z) ? z : ex2(x) * inv * fmaf(ce * LN2, x, k);
     }
 };
 __device__ __forceinline__ void put_void(const wc_policy_loss_args& a, int64_t t) {
@@ -144,61 +157,64 @@ __device__ __forceinline__ float local_max(const Chunk<T>* q) {
         return fmaxf(to_f(m.x), to_f(m.y));
     }
 }
-// One entry's share of the sums from c on. A NaN, and +inf (inf - inf), reach s; an entry that does not count has
-// x = -inf and e = 0.
-__device__ __forceinline__ void add_entry(float v, float c, float& s, float& w) {
-    const float x = fmaf(v, LOG2E, -c), e = ex2(x);
-    s += e;
-    w = fmaf(e, fmaxf(x, -1000.0f), w);
+// z - m, no lower than what makes e 0 in 32 bits: an entry that does not count (-inf) then adds 0 to every sum. NaN, and
+// +inf - inf, stay NaN.
+__device__ __forceinline__ float above(float d) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0fC42C8000;" : "=f"(y) : "f"(d));  // -690
+    return y;
 }
+// One entry's share of the sums
+__device__ __forceinline__ void add_entry(float v, float m, float& s, float& w) {
+    const float d = above(v - m), x = __fmul_rn(d, LOG2E), e = ex2(x);
+    s += fmaf(e * LN2, fmaf(d, LOG2E, -x), e);
+    w = fmaf(e, x, w);
+}
+__device__ __forceinline__ unsigned long long twice(float v) { return f2(v, v); }
+__device__ __forceinline__ unsigned long long distance(float2 z, unsigned long long minus_m) {
+    const unsigned long long d = f2_add(f2(z.x, z.y), minus_m);
+    return f2(above(umma::f2_lo(d)), above(umma::f2_hi(d)));
+}
+__device__ __forceinline__ unsigned long long powers(unsigned long long x) { return f2(ex2(umma::f2_lo(x)), ex2(umma::f2_hi(x))); }
+// ... of NV chunks, two entries at a time
 template <class T, int NV>
 __device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
-    const float c = m * LOG2E;
-    const unsigned long long L = f2(LOG2E, LOG2E), C = f2(-c, -c);
-    unsigned long long s = 0, w = 0;  // pairs of zeros
+    const unsigned long long L = twice(LOG2E), minus_L = twice(-LOG2E), M = twice(-m);
+    unsigned long long s = 0, w = 0, c = 0;  // pairs of zeros; c: what the rounding of x added to s, over ln 2
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int k = 0; k < Chunk<T>::N / 2; ++k) {  // add_entry for two
-            const float2 v = q[i].pair(k);
-            const unsigned long long x = f2_fma(f2(v.x, v.y), L, C);
-            const float x0 = umma::f2_lo(x), x1 = umma::f2_hi(x);
-            const unsigned long long e = f2(ex2(x0), ex2(x1));
-            s = f2_add(s, e);
-            w = f2_fma(e, f2(fmaxf(x0, -1000.0f), fmaxf(x1, -1000.0f)), w);
-        }
-    return make_float2(umma::f2_lo(s) + umma::f2_hi(s), umma::f2_lo(w) + umma::f2_hi(w));
-}
-template <class T, int NV>
-__device__ __forceinline__ void local_grad(const Chunk<T>* q, const Row& r, T* out, int first, int step, int width, int act) {
-    const unsigned long long L = f2(LOG2E, LOG2E), C = f2(-r.c, -r.c);
-    const bool entropy = r.ce != 0.0f;
-    const float f = -r.g * r.inv;  // p times -g
-    const unsigned long long F = f2(f, f), E = f2(r.ce * LN2 * r.inv, r.ce * LN2 * r.inv), K = f2(fmaf(r.ce, r.lH, -r.g) * r.inv, fmaf(r.ce, r.lH, -r.g) * r.inv);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = first + i * step;
-        if (at >= width) break;
-        float v[Chunk<T>::N];
-#pragma unroll
         for (int k = 0; k < Chunk<T>::N / 2; ++k) {
-            const float2 z = q[i].pair(k);
-            const unsigned long long x = f2_fma(f2(z.x, z.y), L, C);
-            const float x0 = umma::f2_lo(x), x1 = umma::f2_hi(x);
-            const unsigned long long e = f2(ex2(x0), ex2(x1));
-            // e inv (ce (x ln 2 + lH) - g)
-            const unsigned long long d = f2_mul(e, entropy ? f2_fma(f2(fmaxf(x0, -1000.0f), fmaxf(x1, -1000.0f)), E, K) : F);
-            v[2 * k] = umma::f2_lo(d), v[2 * k + 1] = umma::f2_hi(d);
+            const unsigned long long d = distance(q[i].pair(k), M), x = f2_mul(d, L), e = powers(x);
+            s = f2_add(s, e);
+            c = f2_fma(e, f2_fma(d, minus_L, x), c);
+            w = f2_fma(e, x, w);
         }
-        if ((unsigned)(act - at) < (unsigned)Chunk<T>::N)
+    const float S = umma::f2_lo(s) + umma::f2_hi(s);
+    return make_float2(fmaf(umma::f2_lo(c) + umma::f2_hi(c), -LN2, S), umma::f2_lo(w) + umma::f2_hi(w));
+}
+// The gradient of a chunk whose first entry is `at`
+template <class T, bool ENTROPY>
+__device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, T* out, int at, int act) {
+    const unsigned long long L = twice(LOG2E), M = twice(-r.m);
+    const unsigned long long E = twice(r.ce * LN2 * r.inv), K = twice(r.k * r.inv);
+    float v[Chunk<T>::N];
 #pragma unroll
-            for (int k = 0; k < Chunk<T>::N; ++k)
-                if (at + k == act) v[k] += r.g;
-        alignas(16) T e[Chunk<T>::N];
-#pragma unroll
-        for (int k = 0; k < Chunk<T>::N; ++k) e[k] = from_f<T>(v[k]);
-        __stcs(reinterpret_cast<uint4*>(out + at), *reinterpret_cast<const uint4*>(e));
+    for (int k = 0; k < Chunk<T>::N / 2; ++k) {
+        const float2 z = q.pair(k);
+        // (an entry that does not count has e = 0 with or without a bound on its x, where no product needs x)
+        const unsigned long long x = f2_mul(ENTROPY ? distance(z, M) : f2_add(f2(z.x, z.y), M), L);
+        const unsigned long long d = f2_mul(powers(x), ENTROPY ? f2_fma(x, E, K) : K);
+        v[2 * k] = umma::f2_lo(d), v[2 * k + 1] = umma::f2_hi(d);
     }
+    if ((unsigned)(act - at) < (unsigned)Chunk<T>::N)
+#pragma unroll
+        for (int k = 0; k < Chunk<T>::N; ++k)
+            if (at + k == act) v[k] += r.g;
+    alignas(16) T e[Chunk<T>::N];
+#pragma unroll
+    for (int k = 0; k < Chunk<T>::N; ++k) e[k] = from_f<T>(v[k]);
+    __stcs(reinterpret_cast<uint4*>(out + at), *reinterpret_cast<const uint4*>(e));
 }
 // A row's logits in registers: NV chunks, `step` entries apart
 template <class T, bool MASK, int NV>
@@ -233,37 +249,37 @@ __device__ __forceinline__ void join(const float4* parts, int n, float& M, float
 #pragma unroll
     for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(~0u, M, o));
     S = W = 0.0f;
-    const float C = M * LOG2E;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const bool none = p[i].x == -INFINITY;
-        const float d = none ? 0.0f : p[i].x * LOG2E - C, f = none ? 0.0f : ex2(d);
+        const float d = none ? 0.0f : p[i].x - M, f = none ? 0.0f : expf(d);
         S = fmaf(p[i].y, f, S);
-        W = fmaf(fmaf(p[i].y, d, p[i].z), f, W);
+        W = fmaf(fmaf(p[i].y, d * LOG2E, p[i].z), f, W);
     }
     S = warp_sum(S), W = warp_sum(W);
 }
 
 // Rows of up to 32 NV chunks: `lanes` threads of a warp a row (a power of two).
-template <class T, bool MASK, int NV>
-__global__ void __launch_bounds__(256) k_policy_warp(wc_policy_loss_args a, int lanes, double* part) {
+template <class T, bool MASK, bool ENTROPY, int NV>
+__global__ void __launch_bounds__(256, NV <= 4 ? 4 : 2) k_policy_warp(wc_policy_loss_args a, int lanes, double* part) {
     constexpr int N = Chunk<T>::N;
     __shared__ double s[8];
     const int lane = threadIdx.x & 31, at = lane & (lanes - 1), per = 256 / lanes, width = (int)a.width;
+    const int64_t stride = (int64_t)gridDim.x * per;
     double total = 0.0;
-    for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < a.rows; t0 += (int64_t)gridDim.x * per) {
+    RowIn next(a, (int64_t)blockIdx.x * per + threadIdx.x / lanes);
+    for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < a.rows; t0 += stride) {
         const int64_t t = t0 + threadIdx.x / lanes;
         const bool in = t < a.rows;
         const T* z = static_cast<const T*>(a.logits) + (in ? t : 0) * a.ld_logits;
         const uint8_t* legal = MASK ? a.legal + (in ? t : 0) * a.ld_legal : nullptr;
-        RowIn r{0.0f, -1};
-        if (in) r = row_in(a, t);
-        bool live = r.w != 0.0f && r.act >= 0 && r.act < width;
+        const RowIn r = next;
         Chunk<T> q[NV];
-        load_row<T, MASK, NV>(q, z, legal, live, at * N, lanes * N, width);
         float za = -INFINITY;
-        if (live && (!MASK || legal[r.act])) za = to_f(z[r.act]);
-        live = live && za != -INFINITY;
+        if (r.act >= 0 && (!MASK || legal[r.act])) za = to_f(z[r.act]);
+        load_row<T, MASK, NV>(q, z, legal, r.act >= 0, at * N, lanes * N, width);
+        next = RowIn(a, t + stride);
+        const bool live = za != -INFINITY;
         float m = local_max<T, NV>(q);
         for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
         float2 sw = local_sums<T, NV>(q, live ? m : 0.0f);
@@ -271,9 +287,15 @@ __global__ void __launch_bounds__(256) k_policy_warp(wc_policy_loss_args a, int 
         if (!in) continue;
         T* out = a.dlogits ? static_cast<T*>(a.dlogits) + t * a.ld_dlogits : nullptr;
         if (live) {
-            const Row row(a, t, r.w, m, sw.x, sw.y, za);
+            const Row row(a, r, m, sw.x, sw.y, za);
             if (at == 0) row.put(a, t), total += (double)(r.w * row.loss);
-            if (out) local_grad<T, NV>(q, row, out, at * N, lanes * N, width, (int)r.act);
+            if (out)
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int c = (i * lanes + at) * N;
+                    if (c >= width) break;
+                    chunk_grad<T, ENTROPY>(q[i], row, out, c, r.act);
+                }
         } else {
             if (at == 0) put_void(a, t);
             if (out)
@@ -294,58 +316,144 @@ __global__ void __launch_bounds__(256) k_policy_warp(wc_policy_loss_args a, int 
     }
 }
 
-// Longer rows: one CTA, or the CTAs of a cluster, a row. Warps, then the CTAs
-// of the cluster, join their parts through shared memory; every thread joins
-// them in the same order.
+// Longer rows: one CTA, or the CTAs of a cluster, a row, each with a slice of
+// it. Slices come into shared memory by bulk copies, and stay until the
+// gradient is written: while a row's parts go round the cluster and its first
+// warp forms the loss, the other warps write the gradient of the row before and
+// sum up the row after. In the order of a CTA's rows, step by step:
+//   sums of row i + 1;  its parts sent, the cluster's barrier entered
+//   gradient of row i
+//   the barrier left; the first warp joins the parts of row i + 1
+constexpr int SLICES = 3;
+template <int CTAS>
+__device__ __forceinline__ void cluster_arrive() {
+    if (CTAS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+template <int CTAS>
+__device__ __forceinline__ void cluster_wait() {
+    if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    else __syncthreads();
+}
 template <class T, bool MASK, int NV, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_policy_loss_args a, double* part) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_policy_loss_args a, int slice, double* part) {
     constexpr int N = Chunk<T>::N, WARPS = THREADS / 32;
-    __shared__ float4 parts[2][CTAS * WARPS];  // of every warp of the cluster, two rows in turn
+    extern __shared__ __align__(128) uint8_t ring[];  // SLICES of the logits, then of the legal bytes
+    __shared__ float4 parts[2][CTAS * WARPS];         // of every warp of the cluster, two rows in turn
+    __shared__ Row rows[2];                           // what the first warp made of them, too
+    __shared__ uint64_t full[SLICES];
     cg::cluster_group cluster = cg::this_cluster();
-    const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0, width = (int)a.width;
+    const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int step = CTAS * THREADS * N, first = (rank * THREADS + (int)threadIdx.x) * N;
-    double total = 0.0;
-    int turn = 0;
-    for (int64_t t = blockIdx.x / CTAS; t < a.rows; t += gridDim.x / CTAS) {
-        const T* z = static_cast<const T*>(a.logits) + t * a.ld_logits;
-        const uint8_t* legal = MASK ? a.legal + t * a.ld_legal : nullptr;
-        T* out = a.dlogits ? static_cast<T*>(a.dlogits) + t * a.ld_dlogits : nullptr;
-        const RowIn r = row_in(a, t);
-        Chunk<T> q[NV];
-        const bool read = r.w != 0.0f && r.act >= 0 && r.act < width;
-        load_row<T, MASK, NV>(q, z, legal, read, first, step, width);
-        float za = -INFINITY;
-        if (read && (!MASK || legal[r.act])) za = to_f(z[r.act]);
-        if (za == -INFINITY) {  // void, for every thread of the cluster
-            if (out)
-#pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    if (first + i * step < width) __stcs(reinterpret_cast<uint4*>(out + first + i * step), make_uint4(0, 0, 0, 0));
-            if (rank == 0 && threadIdx.x == 0) put_void(a, t);
-            continue;
-        }
-        float m = local_max<T, NV>(q);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        float2 v = local_sums<T, NV>(q, m == -INFINITY ? 0.0f : m);
-        v.x = warp_sum(v.x), v.y = warp_sum(v.y);
-        // to every CTA of the cluster; what they read of the row before last they have read before the last barrier
-        if (lane < CTAS) {
-            float4* to = CTAS > 1 ? cluster.map_shared_rank(parts[turn], lane) : parts[turn];
-            to[rank * WARPS + warp] = make_float4(m, v.x, v.y, 0.0f);
-        }
-        if (CTAS > 1) cluster.sync();
-        else __syncthreads();
-        float M, S, W;
-        join<(CTAS * WARPS + 31) / 32>(parts[turn], CTAS * WARPS, M, S, W);
-        turn ^= 1;
-        const Row row(a, t, r.w, M, S, W, za);
-        if (rank == 0 && threadIdx.x == 0) row.put(a, t), total += (double)(r.w * row.loss);
-        if (out) local_grad<T, NV>(q, row, out, first, step, width, (int)r.act);
+    const int first = rank * slice, width = min(slice, max(0, (int)a.width - first));  // this CTA's entries
+    const int64_t t0 = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+    uint8_t* masks = ring + SLICES * slice * sizeof(T);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SLICES; ++i) umma::mbar_init(&full[i], 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    cluster_arrive<CTAS>();
+    cluster_wait<CTAS>();
+    // thread 0: the slice of the CTA's row i
+    auto copy = [&](int64_t i, int act) {
+        const int64_t t = t0 + i * step;
+        if (t >= a.rows) return;
+        const int slot = (int)(i % SLICES);
+        if (act < 0 || !width) {
+            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(&full[slot])) : "memory");
+            return;
+        }
+        umma::expect_tx(&full[slot], width * (sizeof(T) + (MASK ? 1 : 0)));
+        umma::bulk_g2s(ring + slot * slice * sizeof(T), static_cast<const T*>(a.logits) + t * a.ld_logits + first, width * sizeof(T), &full[slot]);
+        if (MASK) umma::bulk_g2s(masks + slot * slice, a.legal + t * a.ld_legal + first, width, &full[slot]);
+    };
+    auto chunk = [&](int slot, int at) {
+        Chunk<T> q;
+        *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(ring + (slot * slice + at) * sizeof(T));
+        if constexpr (MASK) {
+            const uint8_t* on = masks + slot * slice + at;
+            if constexpr (N == 8) q.mask(*reinterpret_cast<const uint2*>(on));
+            else q.mask(make_uint2(*reinterpret_cast<const uint32_t*>(on), 0));
+        }
+        return q;
+    };
+    auto logit = [&](int64_t t, int act) {
+        if (act < 0 || (MASK && !a.legal[t * a.ld_legal + act])) return -INFINITY;
+        return to_f(static_cast<const T*>(a.logits)[t * a.ld_logits + act]);
+    };
+    // The scalars of rows i + 1, i + 2 and i + 3: a load's result is asked for a row later, so that nothing waits for it.
+    RowIn in1(a, t0), in2(a, t0 + step), in3(a, t0 + 2 * step);
+    float za1 = logit(t0, in1.act), za2 = logit(t0 + step, in2.act);
+    if (threadIdx.x == 0) copy(0, in1.act), copy(1, in2.act);
+    double total = 0.0;
+    bool bad = false, live0 = false;
+    int act0 = -1;
+    for (int64_t i = -1, t = t0 - step; t < a.rows; ++i, t += step) {
+        const int64_t t1 = t + step;
+        const int slot1 = (int)((i + 1) % SLICES), turn1 = (int)(i + 1) & 1;
+        const bool live1 = za1 != -INFINITY;
+        // a copy that does not come (umma.cuh) leaves NaN in the rows from here on, after those in flight have landed
+        if (t1 < a.rows && !bad && !umma::mbar_wait(&full[slot1], (uint32_t)((i + 1) / SLICES) & 1)) bad = true;
+        if (live1) {
+            Chunk<T> q[NV];
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int at = (k * THREADS + (int)threadIdx.x) * N;
+                if (at < width) q[k] = chunk(slot1, at);
+                else q[k].none();
+            }
+            float m = local_max<T, NV>(q);
+#pragma unroll
+            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+            if (m == -INFINITY) m = 0.0f;  // nothing here counts (or is a number): its sums are 0 (or NaN)
+            float2 v = local_sums<T, NV>(q, m);
+            v.x = warp_sum(v.x), v.y = warp_sum(v.y);
+            if (bad) v.x = __uint_as_float(0x7fffffffu);
+            if (lane < CTAS) {
+                float4* to = CTAS > 1 ? cluster.map_shared_rank(parts[turn1], lane) : parts[turn1];
+                to[rank * WARPS + warp] = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
+            }
+        }
+        cluster_arrive<CTAS>();
+        __syncthreads();  // rows[] of row i is there, and the slice of row i - 1 has been read by all
+        if (threadIdx.x == 0 && i >= 0 && !bad) copy(i + 2, in2.act);
+        if (t >= 0 && i >= 0 && a.dlogits) {
+            T* out = static_cast<T*>(a.dlogits) + t * a.ld_dlogits + first;
+            const Row& r = rows[turn1 ^ 1];
+            const int slot = (int)(i % SLICES), act = act0 - first;
+            if (live0 && r.ce != 0.0f) {
+                for (int at = threadIdx.x * N; at < width; at += THREADS * N) chunk_grad<T, true>(chunk(slot, at), r, out, at, act);
+            } else if (live0) {
+#pragma unroll
+                for (int k = 0; k < NV; ++k) {
+                    const int at = (k * THREADS + (int)threadIdx.x) * N;
+                    if (at < width) chunk_grad<T, false>(chunk(slot, at), r, out, at, act);
+                }
+            } else {
+                for (int at = threadIdx.x * N; at < width; at += THREADS * N) __stcs(reinterpret_cast<uint4*>(out + at), make_uint4(0, 0, 0, 0));
+            }
+        }
+        cluster_wait<CTAS>();
+        if (warp == 0 && t1 < a.rows) {
+            if (live1) {
+                float M, S, W;
+                join<(CTAS * WARPS + 31) / 32>(parts[turn1], CTAS * WARPS, M, S, W);
+                const Row row(a, in1, M, S, W, za1);
+                if (lane == 0) rows[turn1] = row;
+                if (rank == 0 && lane == 0) row.put(a, t1), total += (double)(in1.w * row.loss);
+            } else if (rank == 0 && lane == 0) {
+                put_void(a, t1);
+            }
+        }
+        live0 = live1, act0 = in1.act;
+        in1 = in2, in2 = in3, za1 = za2;
+        za2 = logit(t1 + 2 * step, in2.act);
+        in3 = RowIn(a, t1 + 3 * step);
+    }
+    if (bad && threadIdx.x == 0)
+        for (int k = 0; k < SLICES; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
     if (rank == 0 && threadIdx.x == 0) part[blockIdx.x / CTAS] = total;
-    if (CTAS > 1) cluster.sync();  // no CTA leaves while another may still write to it
+    cluster_arrive<CTAS>();  // no CTA leaves while another may still write to it
+    cluster_wait<CTAS>();
 }
 
 // Any row: one CTA reads it twice, an entry at a time.
@@ -359,9 +467,9 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
         const T* z = static_cast<const T*>(a.logits) + t * a.ld_logits;
         const uint8_t* legal = a.legal ? a.legal + t * a.ld_legal : nullptr;
         T* out = a.dlogits ? static_cast<T*>(a.dlogits) + t * a.ld_dlogits : nullptr;
-        const RowIn r = row_in(a, t);
+        const RowIn r(a, t);
         float za = -INFINITY;
-        if (r.w != 0.0f && r.act >= 0 && r.act < V && (!legal || legal[r.act])) za = to_f(z[r.act]);
+        if (r.act >= 0 && (!legal || legal[r.act])) za = to_f(z[r.act]);
         if (za == -INFINITY) {
             if (out)
                 for (int64_t j = threadIdx.x; j < V; j += 512) out[j] = from_f<T>(0.0f);
@@ -378,22 +486,22 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
                 v[k] = i < V && (!legal || legal[i]) ? to_f(z[i]) : -INFINITY;
                 top = fmaxf(top, v[k]);
             }
-            const float c = top == -INFINITY ? 0.0f : top * LOG2E, d = m == -INFINITY ? 0.0f : m * LOG2E - c, f = ex2(d);
-            w = fmaf(s, d, w) * f, s *= f, m = top;
+            const float from = top == -INFINITY ? 0.0f : top, d = m == -INFINITY ? 0.0f : m - top, f = expf(d);
+            w = fmaf(s, d * LOG2E, w) * f, s *= f, m = top;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) add_entry(v[k], c, s, w);
+            for (int k = 0; k < 8; ++k) add_entry(v[k], from, s, w);
         }
         float top = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        const float d = m == -INFINITY ? 0.0f : m * LOG2E - top * LOG2E, f = m == -INFINITY ? 0.0f : ex2(d);
-        w = warp_sum(fmaf(s, d, w) * f), s = warp_sum(s * f);
+        const float d = m == -INFINITY ? 0.0f : m - top, f = expf(d);
+        w = warp_sum(fmaf(s, d * LOG2E, w) * f), s = warp_sum(s * f);
         __syncthreads();  // the last row's parts have been read
         if (lane == 0) parts[warp] = make_float4(top, s, w, 0.0f);
         __syncthreads();
         float M, S, W;
         join<1>(parts, 16, M, S, W);
-        const Row row(a, t, r.w, M, S, W, za);
+        const Row row(a, r, M, S, W, za);
         if (threadIdx.x == 0) row.put(a, t), total += (double)(r.w * row.loss);
         if (out)
             for (int64_t j = threadIdx.x; j < V; j += 512) {
@@ -419,13 +527,40 @@ constexpr int MOST_CTAS = 148 * 8;
 
 template <class T, bool MASK, int THREADS, int CTAS>
 int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    const int n = (int)std::min<int64_t>(148 * 1024 / THREADS / CTAS, a.rows);  // what is resident
+    // slices of whole chunks, and of 16 entries so that the legal bytes' are of 16 bytes
+    const int slice = (int)(((a.width + CTAS - 1) / CTAS + 15) / 16 * 16);
+    const size_t smem = SLICES * slice * (sizeof(T) + (MASK ? 1 : 0));
+    const auto kernel = k_policy_cluster<T, MASK, 4, THREADS, CTAS>;
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(kernel), SLICES * THREADS * 4 * Chunk<T>::N * (sizeof(T) + 1))) return 0;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {CTAS, 1, 1};
-    cfg.gridDim = n * CTAS, cfg.blockDim = THREADS, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, k_policy_cluster<T, MASK, 4, THREADS, CTAS>, a, part);
+    cfg.blockDim = THREADS, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1, cfg.dynamicSmemBytes = smem;
+    // As many clusters as are resident at a time: they do not fill the SMs of every GPC, and the ones left over would
+    // start only when the others have ended (37 of 8 CTAs, of which 32 fit, took 2.1 times as long).
+    cfg.gridDim = CTAS * 1024 / THREADS;
+    int most = 0;
+    if (CTAS == 1) most = 148 * 1024 / THREADS;
+    else if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) most = 1;
+    const int n = (int)std::min<int64_t>(most, a.rows);
+    cfg.gridDim = n * CTAS;
+    cudaLaunchKernelEx(&cfg, kernel, a, slice, part);
+    return n;
+}
+
+template <class T, bool MASK, bool ENTROPY>
+int launch_warp(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
+    const int64_t chunks = a.width / Chunk<T>::N;
+    int lanes = 1;
+    while (lanes < 32 && lanes * 4 < chunks) lanes *= 2;
+    const int64_t per = 256 / lanes;
+    const int n = (int)std::min<int64_t>(MOST_CTAS, (a.rows + per - 1) / per);
+    const int nv = (int)((chunks + lanes - 1) / lanes);
+    if (nv <= 1) k_policy_warp<T, MASK, ENTROPY, 1><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv == 2) k_policy_warp<T, MASK, ENTROPY, 2><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv == 3) k_policy_warp<T, MASK, ENTROPY, 3><<<n, 256, 0, s>>>(a, lanes, part);
+    else k_policy_warp<T, MASK, ENTROPY, 4><<<n, 256, 0, s>>>(a, lanes, part);
     return n;
 }
 
@@ -433,18 +568,7 @@ template <class T, bool MASK>
 int launch_vec(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     constexpr int N = Chunk<T>::N;
     const int64_t chunks = a.width / N;
-    if (chunks <= 32 * 4) {
-        int lanes = 1;
-        while (lanes < 32 && lanes * 4 < chunks) lanes *= 2;
-        const int64_t per = 256 / lanes;
-        const int n = (int)std::min<int64_t>(MOST_CTAS, (a.rows + per - 1) / per);
-        const int nv = (int)((chunks + lanes - 1) / lanes);
-        if (nv <= 1) k_policy_warp<T, MASK, 1><<<n, 256, 0, s>>>(a, lanes, part);
-        else if (nv == 2) k_policy_warp<T, MASK, 2><<<n, 256, 0, s>>>(a, lanes, part);
-        else if (nv == 3) k_policy_warp<T, MASK, 3><<<n, 256, 0, s>>>(a, lanes, part);
-        else k_policy_warp<T, MASK, 4><<<n, 256, 0, s>>>(a, lanes, part);
-        return n;
-    }
+    if (chunks <= 32 * 4) return a.entropy_coef != 0.0f ? launch_warp<T, MASK, true>(a, part, s) : launch_warp<T, MASK, false>(a, part, s);
     // 4 chunks a thread, up to 8 CTAs a row
     if (chunks <= 128 * 4) return launch_cluster<T, MASK, 128, 1>(a, part, s);
     if (chunks <= 512 * 4) return launch_cluster<T, MASK, 512, 1>(a, part, s);
@@ -458,9 +582,13 @@ int launch_type(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     constexpr int N = 16 / sizeof(T);
     const auto fits = [&](const void* p, int64_t ld, size_t e) { return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0; };
     const bool vec = a.width % N == 0 && fits(a.logits, a.ld_logits, sizeof(T)) &&
-                     (!a.dlogits || fits(a.dlogits, a.ld_dlogits, sizeof(T))) &&
-                     (!a.legal || (((uintptr_t)a.legal & 7) == 0 && a.ld_legal % 8 == 0));
-    if (vec && a.width / N <= 8 * 512 * 4) return a.legal ? launch_vec<T, true>(a, part, s) : launch_vec<T, false>(a, part, s);
+                     (!a.dlogits || fits(a.dlogits, a.ld_dlogits, sizeof(T)));
+    // short rows load 4 or 8 legal bytes at a time, slices of longer ones come in 16s
+    const bool is_short = a.width / N <= 32 * 4;
+    const bool mask = !a.legal || (is_short ? ((uintptr_t)a.legal & 7) == 0 && a.ld_legal % 8 == 0
+                                            : a.width % 16 == 0 && fits(a.legal, a.ld_legal, 1));
+    if (vec && mask && a.width / N <= 8 * 512 * 4)
+        return a.legal ? launch_vec<T, true>(a, part, s) : launch_vec<T, false>(a, part, s);
     const int n = (int)std::min<int64_t>(148 * 4, a.rows);
     k_policy_long<T><<<n, 512, 0, s>>>(a, part);
     return n;
