@@ -6,9 +6,10 @@
 // The row's loss depends on the logits through l and H only, so
 //   dloss/dz_j = g (delta_ja - p_j) + w c p_j (ln p_j + H),
 //   g = w (-ratio A [not clipped] - kl_coef (exp(r - l) - 1)).
-// A power is 2^x with x = (z - m) log2 e rounded; the sum of what that rounding
-// leaves out, times e, goes into S as a correction, so that l (whose difference
-// with another log-probability is what counts) is good to a few 1e-8.
+// A power is 2^x with x = z log2 e - c in one rounding, c = m log2 e rounded; the
+// factor that the rounding of c puts on every power is taken out of ln S again.
+// (The rounding of x, at most 2^-25 |x|, moves S by at most about 4e-8: the
+// entries that weigh have small x, or are many.)
 //
 // What bounds it is the bytes: each logit is read once and its gradient written
 // once. A row stays in registers as it was loaded (16 bytes of logits and their
@@ -40,6 +41,17 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// x, no lower than what makes 2^x 0 in 32 bits: an entry that does not count (-inf) then adds 0 to every sum. NaN, and
+// +inf - inf, stay NaN.
+__device__ __forceinline__ float above(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, 0fC47A0000;" : "=f"(y) : "f"(x));  // -1000
+    return y;
+}
+
+// c of a maximum, the same number wherever it is formed (a product fused into a sum would not be rounded)
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, LOG2E); }
+
 // What a row needs besides its logits: loaded a row ahead, since the logits' loads wait for it (a row that is void
 // reads none)
 struct RowIn {
@@ -62,18 +74,20 @@ struct RowIn {
 // add to them is not.
 struct Row {
     float loss, l, H, kl;   // results
-    float m, inv, g, ce, k; // gradient: p = e inv;  d = p (ce ln 2 x + k) + [action] g,  k = ce (H - ln S) - g
+    float c, g, e, k;       // gradient: d = 2^x (e x + k) + [action] g
+    float ce;
     Row() = default;
-    __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float top, float S, float W, float za) : m(top) {
+    __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float m, float S, float W, float za) : c(scaled(m)) {
         const float mean = W / S;  // of x
+        const float off = fmaf(m, LOG2E, -c) * LN2;
         // ln S from S = 2^n f, f about 1; LOG2E as a float is 1.34e-8 (relative) low, which mean puts right to first order
         int n;
         float f = frexpf(S, &n);
         if (f < 0.75f) f *= 2.0f, --n;
-        const double lnS = (double)n * 0.6931471805599453 + (double)fmaf(mean, 9.25e-9f, logf(f));
+        const double lnS = (double)n * 0.6931471805599453 + (double)(fmaf(mean, 9.25e-9f, logf(f)) - off);
         const double ld = ((double)za - (double)m) - lnS;
         l = (float)ld;
-        H = (float)lnS - mean * LN2;
+        H = (float)lnS + (off - mean * LN2);
         const float lo = 1.0f - a.clip_low, hi = 1.0f + a.clip_high, A = in.A;
         const float ratio = expf((float)(ld - (double)in.old));
         const float free = ratio * A, clipped = fminf(fmaxf(ratio, lo), hi) * A;
@@ -84,29 +98,25 @@ struct Row {
         const float up = (a.upstream ? *a.upstream : 1.0f) * in.w;
         g = up * ((held ? 0.0f : -free) - a.kl_coef * em);
         ce = up * a.entropy_coef;
-        inv = 1.0f / S;
-        k = fmaf(ce, H - (float)lnS, -g);
+        // p = 2^x / S and ln p = x ln 2 - ln S - off
+        const float inv = 1.0f / S;
+        e = ce * LN2 * inv, k = fmaf(ce, H - (float)lnS - off, -g) * inv;
     }
     __device__ __forceinline__ void put(const wc_policy_loss_args& a, int64_t t) const {
         a.row_out[t] = loss, a.row_out[a.rows + t] = l, a.row_out[2 * a.rows + t] = H, a.row_out[3 * a.rows + t] = kl;
     }
-    // the gradient at an entry other than the action
+    // the gradient at an entry other than the action; one that does not count has 2^x = 0 (and needs a finite x where
+    // x is a factor)
+    template <bool ENTROPY>
     __device__ __forceinline__ float grad(float z) const {
-        const float x = fmaxf((z - m) * LOG2E, -1000.0f);
-        return isnan(z) ? z : ex2(x) * inv * fmaf(ce * LN2, x, k);
+        const float x = fmaf(z, LOG2E, -c);
+        if (!ENTROPY) return ex2(x) * k;
+        const float y = above(x);
+        return ex2(y) * fmaf(y, e, k);
     }
 };
 __device__ __forceinline__ void put_void(const wc_policy_loss_args& a, int64_t t) {
     a.row_out[t] = 0.0f, a.row_out[a.rows + t] = 0.0f, a.row_out[2 * a.rows + t] = 0.0f, a.row_out[3 * a.rows + t] = 0.0f;
-}
-
-using umma::f2;
-using umma::f2_add;
-using umma::f2_fma;
-__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
-    unsigned long long d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 
 // 16 bytes of logits as they lie in memory, what does not count as -inf
@@ -157,55 +167,34 @@ __device__ __forceinline__ float local_max(const Chunk<T>* q) {
         return fmaxf(to_f(m.x), to_f(m.y));
     }
 }
-// z - m, no lower than what makes e 0 in 32 bits: an entry that does not count (-inf) then adds 0 to every sum. NaN, and
-// +inf - inf, stay NaN.
-__device__ __forceinline__ float above(float d) {
-    float y;
-    asm("max.NaN.f32 %0, %1, 0fC42C8000;" : "=f"(y) : "f"(d));  // -690
-    return y;
-}
-// One entry's share of the sums
-__device__ __forceinline__ void add_entry(float v, float m, float& s, float& w) {
-    const float d = above(v - m), x = __fmul_rn(d, LOG2E), e = ex2(x);
-    s += fmaf(e * LN2, fmaf(d, LOG2E, -x), e);
+// One entry's share of the sums from c on
+__device__ __forceinline__ void add_entry(float z, float c, float& s, float& w) {
+    const float x = above(fmaf(z, LOG2E, -c)), e = ex2(x);
+    s += e;
     w = fmaf(e, x, w);
 }
-__device__ __forceinline__ unsigned long long twice(float v) { return f2(v, v); }
-__device__ __forceinline__ unsigned long long distance(float2 z, unsigned long long minus_m) {
-    const unsigned long long d = f2_add(f2(z.x, z.y), minus_m);
-    return f2(above(umma::f2_lo(d)), above(umma::f2_hi(d)));
-}
-__device__ __forceinline__ unsigned long long powers(unsigned long long x) { return f2(ex2(umma::f2_lo(x)), ex2(umma::f2_hi(x))); }
-// ... of NV chunks, two entries at a time
+// ... of NV chunks; two accumulators each
 template <class T, int NV>
 __device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
-    const unsigned long long L = twice(LOG2E), minus_L = twice(-LOG2E), M = twice(-m);
-    unsigned long long s = 0, w = 0, c = 0;  // pairs of zeros; c: what the rounding of x added to s, over ln 2
+    const float c = scaled(m);
+    float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < Chunk<T>::N / 2; ++k) {
-            const unsigned long long d = distance(q[i].pair(k), M), x = f2_mul(d, L), e = powers(x);
-            s = f2_add(s, e);
-            c = f2_fma(e, f2_fma(d, minus_L, x), c);
-            w = f2_fma(e, x, w);
+            const float2 v = q[i].pair(k);
+            add_entry(v.x, c, s0, w0), add_entry(v.y, c, s1, w1);
         }
-    const float S = umma::f2_lo(s) + umma::f2_hi(s);
-    return make_float2(fmaf(umma::f2_lo(c) + umma::f2_hi(c), -LN2, S), umma::f2_lo(w) + umma::f2_hi(w));
+    return make_float2(s0 + s1, w0 + w1);
 }
 // The gradient of a chunk whose first entry is `at`
 template <class T, bool ENTROPY>
 __device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, T* out, int at, int act) {
-    const unsigned long long L = twice(LOG2E), M = twice(-r.m);
-    const unsigned long long E = twice(r.ce * LN2 * r.inv), K = twice(r.k * r.inv);
     float v[Chunk<T>::N];
 #pragma unroll
     for (int k = 0; k < Chunk<T>::N / 2; ++k) {
         const float2 z = q.pair(k);
-        // (an entry that does not count has e = 0 with or without a bound on its x, where no product needs x)
-        const unsigned long long x = f2_mul(ENTROPY ? distance(z, M) : f2_add(f2(z.x, z.y), M), L);
-        const unsigned long long d = f2_mul(powers(x), ENTROPY ? f2_fma(x, E, K) : K);
-        v[2 * k] = umma::f2_lo(d), v[2 * k + 1] = umma::f2_hi(d);
+        v[2 * k] = r.grad<ENTROPY>(z.x), v[2 * k + 1] = r.grad<ENTROPY>(z.y);
     }
     if ((unsigned)(act - at) < (unsigned)Chunk<T>::N)
 #pragma unroll
@@ -252,9 +241,9 @@ __device__ __forceinline__ void join(const float4* parts, int n, float& M, float
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         const bool none = p[i].x == -INFINITY;
-        const float d = none ? 0.0f : p[i].x - M, f = none ? 0.0f : expf(d);
+        const float d = none ? 0.0f : scaled(p[i].x) - scaled(M), f = none ? 0.0f : exp2f(d);
         S = fmaf(p[i].y, f, S);
-        W = fmaf(fmaf(p[i].y, d * LOG2E, p[i].z), f, W);
+        W = fmaf(fmaf(p[i].y, d, p[i].z), f, W);
     }
     S = warp_sum(S), W = warp_sum(W);
 }
@@ -321,26 +310,29 @@ __global__ void __launch_bounds__(256, NV <= 4 ? 4 : 2) k_policy_warp(wc_policy_
 // gradient is written: while a row's parts go round the cluster and its first
 // warp forms the loss, the other warps write the gradient of the row before and
 // sum up the row after. In the order of a CTA's rows, step by step:
-//   sums of row i + 1;  its parts sent, the cluster's barrier entered
+//   sums of row i + 1, its parts sent
 //   gradient of row i
-//   the barrier left; the first warp joins the parts of row i + 1
+//   the first warp joins the parts of row i + 1
 constexpr int SLICES = 3;
-template <int CTAS>
-__device__ __forceinline__ void cluster_arrive() {
-    if (CTAS > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+// 16 bytes into the shared memory of a CTA of the cluster (both addresses mapped to it), counted by its barrier. No
+// fence: a cluster barrier's release would wait for the gradient's stores as well.
+__device__ __forceinline__ void send(uint32_t to, float4 v, uint32_t bar) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to), "f"(v.x),
+                 "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+                 : "memory");
 }
-template <int CTAS>
-__device__ __forceinline__ void cluster_wait() {
-    if (CTAS > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-    else __syncthreads();
+__device__ __forceinline__ uint32_t of_rank(uint32_t addr, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
 }
 template <class T, bool MASK, int NV, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_policy_loss_args a, int slice, double* part) {
     constexpr int N = Chunk<T>::N, WARPS = THREADS / 32;
     extern __shared__ __align__(128) uint8_t ring[];  // SLICES of the logits, then of the legal bytes
-    __shared__ float4 parts[2][CTAS * WARPS];         // of every warp of the cluster, two rows in turn
-    __shared__ Row rows[2];                           // what the first warp made of them, too
-    __shared__ uint64_t full[SLICES];
+    __shared__ float4 parts[3][CTAS * WARPS];         // of every warp of the cluster, three (live) rows in turn
+    __shared__ Row rows[2];                           // what the first warp made of them, two rows in turn
+    __shared__ uint64_t full[SLICES], joined[3];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -349,10 +341,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
     uint8_t* masks = ring + SLICES * slice * sizeof(T);
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLICES; ++i) umma::mbar_init(&full[i], 1);
+        for (int i = 0; i < 3; ++i) umma::mbar_init(&joined[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    cluster_arrive<CTAS>();
-    cluster_wait<CTAS>();
+    if (CTAS > 1) cluster.sync();
+    else __syncthreads();
     // thread 0: the slice of the CTA's row i
     auto copy = [&](int64_t i, int act) {
         const int64_t t = t0 + i * step;
@@ -387,6 +380,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
     double total = 0.0;
     bool bad = false, live0 = false;
     int act0 = -1;
+    int turn = 0;         // of parts[] and joined[]
+    uint32_t phases = 0;  // of joined[]
     for (int64_t i = -1, t = t0 - step; t < a.rows; ++i, t += step) {
         const int64_t t1 = t + step;
         const int slot1 = (int)((i + 1) % SLICES), turn1 = (int)(i + 1) & 1;
@@ -408,12 +403,14 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
             float2 v = local_sums<T, NV>(q, m);
             v.x = warp_sum(v.x), v.y = warp_sum(v.y);
             if (bad) v.x = __uint_as_float(0x7fffffffu);
-            if (lane < CTAS) {
-                float4* to = CTAS > 1 ? cluster.map_shared_rank(parts[turn1], lane) : parts[turn1];
-                to[rank * WARPS + warp] = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
-            }
+            const float4 mine = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
+            float4* to = &parts[turn][rank * WARPS + warp];
+            // This warp's CTA has by now joined the live row before last (past the last __syncthreads). That took a part
+            // from the first warp of every CTA, sent after it had joined the row before that one: of three places in
+            // turn, the one written here has been read everywhere.
+            if (CTAS == 1 && lane == 0) *to = mine;
+            if (CTAS > 1 && lane < CTAS) send(of_rank(umma::smem_u32(to), lane), mine, of_rank(umma::smem_u32(&joined[turn]), lane));
         }
-        cluster_arrive<CTAS>();
         __syncthreads();  // rows[] of row i is there, and the slice of row i - 1 has been read by all
         if (threadIdx.x == 0 && i >= 0 && !bad) copy(i + 2, in2.act);
         if (t >= 0 && i >= 0 && a.dlogits) {
@@ -432,11 +429,17 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
                 for (int at = threadIdx.x * N; at < width; at += THREADS * N) __stcs(reinterpret_cast<uint4*>(out + at), make_uint4(0, 0, 0, 0));
             }
         }
-        cluster_wait<CTAS>();
+        if (CTAS == 1) __syncthreads();
         if (warp == 0 && t1 < a.rows) {
             if (live1) {
+                if (CTAS > 1) {
+                    if (lane == 0) umma::expect_tx(&joined[turn], CTAS * WARPS * 16);
+                    if (!umma::mbar_wait(&joined[turn], phases >> turn & 1)) bad = true;
+                    phases ^= 1u << turn;
+                }
                 float M, S, W;
-                join<(CTAS * WARPS + 31) / 32>(parts[turn1], CTAS * WARPS, M, S, W);
+                join<(CTAS * WARPS + 31) / 32>(parts[turn], CTAS * WARPS, M, S, W);
+                if (bad) S = __uint_as_float(0x7fffffffu);
                 const Row row(a, in1, M, S, W, za1);
                 if (lane == 0) rows[turn1] = row;
                 if (rank == 0 && lane == 0) row.put(a, t1), total += (double)(in1.w * row.loss);
@@ -444,6 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
                 put_void(a, t1);
             }
         }
+        if (live1) turn = turn == 2 ? 0 : turn + 1;
         live0 = live1, act0 = in1.act;
         in1 = in2, in2 = in3, za1 = za2;
         za2 = logit(t1 + 2 * step, in2.act);
@@ -452,8 +456,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
     if (bad && threadIdx.x == 0)
         for (int k = 0; k < SLICES; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
     if (rank == 0 && threadIdx.x == 0) part[blockIdx.x / CTAS] = total;
-    cluster_arrive<CTAS>();  // no CTA leaves while another may still write to it
-    cluster_wait<CTAS>();
+    if (CTAS > 1) cluster.sync();  // no CTA leaves while another may still write to it
 }
 
 // Any row: one CTA reads it twice, an entry at a time.
@@ -486,16 +489,16 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
                 v[k] = i < V && (!legal || legal[i]) ? to_f(z[i]) : -INFINITY;
                 top = fmaxf(top, v[k]);
             }
-            const float from = top == -INFINITY ? 0.0f : top, d = m == -INFINITY ? 0.0f : m - top, f = expf(d);
-            w = fmaf(s, d * LOG2E, w) * f, s *= f, m = top;
+            const float c = top == -INFINITY ? 0.0f : scaled(top), d = m == -INFINITY ? 0.0f : scaled(m) - c, f = exp2f(d);
+            w = fmaf(s, d, w) * f, s *= f, m = top;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) add_entry(v[k], from, s, w);
+            for (int k = 0; k < 8; ++k) add_entry(v[k], c, s, w);
         }
         float top = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        const float d = m == -INFINITY ? 0.0f : m - top, f = expf(d);
-        w = warp_sum(fmaf(s, d * LOG2E, w) * f), s = warp_sum(s * f);
+        const float d = m == -INFINITY ? 0.0f : scaled(m) - scaled(top), f = exp2f(d);
+        w = warp_sum(fmaf(s, d, w) * f), s = warp_sum(s * f);
         __syncthreads();  // the last row's parts have been read
         if (lane == 0) parts[warp] = make_float4(top, s, w, 0.0f);
         __syncthreads();
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
         if (out)
             for (int64_t j = threadIdx.x; j < V; j += 512) {
                 const float v = !legal || legal[j] ? to_f(z[j]) : -INFINITY;
-                float d = v == -INFINITY ? 0.0f : row.grad(v);
+                float d = row.grad<true>(v);
                 if (j == r.act) d += row.g;
                 out[j] = from_f<T>(d);
             }
@@ -523,7 +526,7 @@ __global__ void k_policy_total(const double* part, int n, float* loss) {
     if (threadIdx.x == 0) *loss = (float)v;
 }
 
-constexpr int MOST_CTAS = 148 * 8;
+constexpr int MOST_CTAS = 148 * 12;
 
 template <class T, bool MASK, int THREADS, int CTAS>
 int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
@@ -552,15 +555,18 @@ int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
 template <class T, bool MASK, bool ENTROPY>
 int launch_warp(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     const int64_t chunks = a.width / Chunk<T>::N;
+    // up to 8 chunks a lane of a 16-bit type (4 of 32 bits): the more rows a warp has, the less their scalars cost
+    constexpr int MOST = sizeof(T) == 2 ? 8 : 4;
     int lanes = 1;
-    while (lanes < 32 && lanes * 4 < chunks) lanes *= 2;
+    while (lanes < 32 && lanes * MOST < chunks) lanes *= 2;
     const int64_t per = 256 / lanes;
-    const int n = (int)std::min<int64_t>(MOST_CTAS, (a.rows + per - 1) / per);
+    const int n = (int)std::min<int64_t>(148 * 12, (a.rows + per - 1) / per);
     const int nv = (int)((chunks + lanes - 1) / lanes);
     if (nv <= 1) k_policy_warp<T, MASK, ENTROPY, 1><<<n, 256, 0, s>>>(a, lanes, part);
     else if (nv == 2) k_policy_warp<T, MASK, ENTROPY, 2><<<n, 256, 0, s>>>(a, lanes, part);
-    else if (nv == 3) k_policy_warp<T, MASK, ENTROPY, 3><<<n, 256, 0, s>>>(a, lanes, part);
-    else k_policy_warp<T, MASK, ENTROPY, 4><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv <= 4) k_policy_warp<T, MASK, ENTROPY, 4><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv <= 6) k_policy_warp<T, MASK, ENTROPY, MOST == 8 ? 6 : 4><<<n, 256, 0, s>>>(a, lanes, part);
+    else k_policy_warp<T, MASK, ENTROPY, MOST><<<n, 256, 0, s>>>(a, lanes, part);
     return n;
 }
 
