@@ -19,7 +19,7 @@ constexpr int THREADS = 256;
 template <class T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, int64_t c, int64_t width, float* v) {
     if (VEC && c + 8 <= width) {
-        T e[8];
+        alignas(16) T e[8];
         if constexpr (sizeof(T) == 2) {
             *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p + c);
         } else {
@@ -36,7 +36,7 @@ __device__ __forceinline__ void load8(const T* p, int64_t c, int64_t width, floa
 template <class T, bool VEC>
 __device__ __forceinline__ void store8(T* p, int64_t c, int64_t width, const float* v) {
     if (VEC && c + 8 <= width) {
-        T e[8];
+        alignas(16) T e[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
         *reinterpret_cast<uint4*>(p + c) = *reinterpret_cast<const uint4*>(e);
@@ -48,25 +48,6 @@ __device__ __forceinline__ void store8(T* p, int64_t c, int64_t width, const flo
     }
 }
 
-// The 8 values' bytes under the block's code, which every thread of the block gets.
-__device__ __forceinline__ uint2 quantise8(const float* v, uint32_t* code) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    *code = act8_code(__uint_as_float(top));
-    if (*code == 255) return make_uint2(0, 0);
-    const float inv = act8_inverse(*code);
-    uint32_t b[8];
-    // adding 1.5 2^23 rounds to a whole number, ties to even, and leaves its two's complement in the low bits
-#pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(v[i], inv, 12582912.0f));
-    uint2 r;
-    r.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    r.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
-    return r;
-}
 __device__ __forceinline__ void dequantise8(uint2 q, uint32_t code, float* v) {
     const float unit = act8_unit(code);
 #pragma unroll

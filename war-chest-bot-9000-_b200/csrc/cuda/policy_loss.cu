@@ -124,7 +124,7 @@ template <class T>
 struct Chunk {
     static constexpr int N = 16 / sizeof(T);
     static constexpr uint32_t INF = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-    uint32_t z[4];
+    alignas(16) uint32_t z[4];
     __device__ __forceinline__ void load(const T* at) { *reinterpret_cast<uint4*>(z) = __ldcs(reinterpret_cast<const uint4*>(at)); }
     __device__ __forceinline__ void none() { z[0] = z[1] = z[2] = z[3] = INF; }
     // legal bytes, in the order of the entries

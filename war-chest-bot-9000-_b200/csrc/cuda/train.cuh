@@ -59,6 +59,27 @@ __device__ __forceinline__ float act8_unit(uint32_t code) {
 // 2^-e of a code; the product with a block's value is exact (or too small to round to anything but 0)
 __device__ __forceinline__ float act8_inverse(uint32_t code) { return __uint_as_float((254u - code) << 23); }
 
+// A thread's 8 values of a block (4 threads next to each other hold one) as bytes, and the block's code.
+// Magnitudes are compared as integers, where NaN is above infinity above the rest, so either shows in the code.
+__device__ __forceinline__ uint2 quantise8(const float* v, uint32_t* code) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    *code = act8_code(__uint_as_float(top));
+    if (*code == 255) return make_uint2(0, 0);
+    const float inv = act8_inverse(*code);
+    uint32_t b[8];
+    // adding 1.5 2^23 rounds to a whole number, ties to even, and leaves its two's complement in the low bits
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(fmaf(v[i], inv, 12582912.0f));
+    uint2 r;
+    r.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    r.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+    return r;
+}
+
 // GELU (tanh form) as x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3):
 // no cancellation for negative x. The exponent is held below 126 so that the
 // divisor stays finite.
