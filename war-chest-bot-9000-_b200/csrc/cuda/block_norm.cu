@@ -237,6 +237,19 @@ struct Unit {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
     }
+    // the same in pairs
+    __device__ __forceinline__ void get(unsigned long long* v) const {
+        float f[8];
+        get(f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = umma::f2(f[2 * i], f[2 * i + 1]);
+    }
+    __device__ __forceinline__ static void put(T* p, const unsigned long long* v) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = umma::f2_lo(v[i]), f[2 * i + 1] = umma::f2_hi(v[i]);
+        put(p, f);
+    }
     __device__ __forceinline__ static void put(T* p, const float* v) {
         alignas(16) T e[8];
 #pragma unroll
@@ -284,7 +297,7 @@ struct Group {
 // WARPS = 0: `lanes` threads of a warp a row, else a CTA of up to WARPS warps;
 // NV units a thread, `lanes` (or blockDim.x) apart.
 template <class T, int WARPS, int NV>
-__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256) k_norm_units(wc_block_norm_args a, int lanes) {
+__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 ? 40 / (WARPS ? WARPS : 1) : 1) : 4) k_norm_units(wc_block_norm_args a, int lanes) {
     __shared__ float2 s[2][32];
     Group<WARPS> group{s, lanes};
     const int D = (int)a.width, at = WARPS ? threadIdx.x : (int)(threadIdx.x & (lanes - 1)), apart = WARPS ? (int)blockDim.x : lanes;
@@ -420,17 +433,42 @@ struct Items {
     }
 };
 
+// Arithmetic on pairs of 32-bit numbers (umma.cuh), each rounded as the scalar form: the backward pass has some 30
+// operations a column, which would bound it before the bytes do.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair twice(float v) { return umma::f2(v, v); }
+__device__ __forceinline__ Pair mul(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair add(Pair a, Pair b) { return umma::f2_add(a, b); }
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) { return umma::f2_fma(a, b, c); }
+__device__ __forceinline__ float both(Pair a) { return umma::f2_lo(a) + umma::f2_hi(a); }
+
 // What a thread keeps of its unit: the parameters and their gradients' sums.
 struct Column {
-    float wp[8], bp[8], wn[8], g[8];
-    float dwp[8], dbp[8], dwn[8], dbn[8], dg[8];
+    Pair wp[4], bp[4], wn[4], g[4];
+    Pair dwp[4], dbp[4], dwn[4], dbn[4], dg[4];
+    __device__ __forceinline__ static void fill(Pair* v, float x) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = twice(x);
+    }
+    __device__ __forceinline__ static void load(Pair* v, const float* p) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = umma::f2(a.x, a.y), v[1] = umma::f2(a.z, a.w), v[2] = umma::f2(b.x, b.y), v[3] = umma::f2(b.z, b.w);
+    }
+    __device__ __forceinline__ static void unpack(const Pair* v, float* f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[2 * k] = umma::f2_lo(v[k]), f[2 * k + 1] = umma::f2_hi(v[k]);
+    }
     __device__ __forceinline__ void load(const wc_block_norm_args& a, int c, bool in) {
-        fill8(wp, 1.0f), fill8(bp, 0.0f), fill8(wn, 0.0f), fill8(g, 1.0f);
-        fill8(dwp, 0.0f), fill8(dbp, 0.0f), fill8(dwn, 0.0f), fill8(dbn, 0.0f), fill8(dg, 0.0f);
+        fill(wp, 1.0f), fill(bp, 0.0f), fill(wn, 0.0f), fill(g, 1.0f);
+        fill(dwp, 0.0f), fill(dbp, 0.0f), fill(dwn, 0.0f), fill(dbn, 0.0f), fill(dg, 0.0f);
         if (!in) return;
-        if (a.post_weight) load8(a.post_weight + c, wp);
-        if (a.post_bias) load8(a.post_bias + c, bp);
-        if (a.pre_weight) load8(a.pre_weight + c, wn);
+        if (a.post_weight) load(wp, a.post_weight + c);
+        if (a.post_bias) load(bp, a.post_bias + c);
+        if (a.pre_weight) load(wn, a.pre_weight + c);
     }
     // A row's unit. get(i, v) reads its x, h, dy or dn (i = 0 .. 3; zeros past the width and for a gradient that is not
     // there), when it is needed: what is not held meanwhile leaves room for the sums. put(i, v) takes dx, then dh.
@@ -438,50 +476,49 @@ struct Column {
     __device__ __forceinline__ void row(const wc_block_norm_args& a, const float4& st, bool pre, bool in, float inv, G& group, Get&& get,
                                         Put&& put) {
         const bool layer = a.kind == WC_NORM_LAYER;
-        float hh[8], yh[8], d[8];
+        Pair hh[4], yh[4], d[4];
         get(1, hh), get(0, yh);
+        const Pair pr = twice(st.y), pm = twice(-st.x), nr = twice(st.w), nm = twice(-st.z), rs = twice(a.residual_scale);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            hh[k] = (hh[k] - st.x) * st.y;
-            yh[k] = (fmaf(a.residual_scale, yh[k], g[k] * fmaf(hh[k], wp[k], bp[k])) - st.z) * st.w;
+        for (int k = 0; k < 4; ++k) {
+            hh[k] = mul(add(hh[k], pm), pr);
+            yh[k] = mul(add(fma(rs, yh[k], mul(g[k], fma(hh[k], wp[k], bp[k]))), nm), nr);
         }
-        float2 m = make_float2(0.0f, 0.0f);
         if (pre) {
+            Pair m0 = 0, m1 = 0;  // pairs of zeros
             get(3, d);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                dwn[k] = fmaf(d[k], yh[k], dwn[k]), dbn[k] += d[k];
-                const float w = d[k] * wn[k];
-                m.x += w, m.y = fmaf(w, yh[k], m.y);
+            for (int k = 0; k < 4; ++k) {
+                dwn[k] = fma(d[k], yh[k], dwn[k]), dbn[k] = add(dbn[k], d[k]);
+                d[k] = mul(d[k], wn[k]);
+                m0 = add(m0, d[k]), m1 = fma(d[k], yh[k], m1);
             }
-            m = group.sum(m);
-            m.x = layer ? m.x * inv : 0.0f, m.y *= inv;
+            const float2 m = group.sum(make_float2(both(m0), both(m1)));
+            const Pair a0 = twice(layer ? -m.x * inv : 0.0f), a1 = twice(-m.y * inv);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) yh[k] = fmaf(yh[k], m.y, m.x);
-            get(3, d);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) yh[k] = st.w * fmaf(d[k], wn[k], -yh[k]);
+            for (int k = 0; k < 4; ++k) yh[k] = mul(nr, fma(yh[k], a1, add(d[k], a0)));
         } else {
-            fill8(yh, 0.0f);
+            fill(yh, 0.0f);
         }
         get(2, d);
+        const Pair live = twice(in ? 1.0f : 0.0f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) yh[k] = in ? d[k] + yh[k] : 0.0f, d[k] = a.residual_scale * yh[k];  // dY
+        for (int k = 0; k < 4; ++k) yh[k] = mul(live, add(d[k], yh[k])), d[k] = mul(rs, yh[k]);  // dY
         put(0, d);
-        float2 c = make_float2(0.0f, 0.0f);
+        Pair c0 = 0, c1 = 0;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            dg[k] = fmaf(yh[k], fmaf(hh[k], wp[k], bp[k]), dg[k]);
-            const float du = yh[k] * g[k];
-            dwp[k] = fmaf(du, hh[k], dwp[k]), dbp[k] += du;
-            yh[k] = du * wp[k];
-            c.x += yh[k], c.y = fmaf(yh[k], hh[k], c.y);
+        for (int k = 0; k < 4; ++k) {
+            dg[k] = fma(yh[k], fma(hh[k], wp[k], bp[k]), dg[k]);
+            const Pair du = mul(yh[k], g[k]);
+            dwp[k] = fma(du, hh[k], dwp[k]), dbp[k] = add(dbp[k], du);
+            yh[k] = mul(du, wp[k]);
+            c0 = add(c0, yh[k]), c1 = fma(yh[k], hh[k], c1);
         }
         if (a.post_weight) {
-            c = group.sum(c);
-            c.x = layer ? c.x * inv : 0.0f, c.y *= inv;
+            const float2 c = group.sum(make_float2(both(c0), both(c1)));
+            const Pair a0 = twice(layer ? -c.x * inv : 0.0f), a1 = twice(-c.y * inv);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) yh[k] = st.y * (yh[k] - c.x - hh[k] * c.y);
+            for (int k = 0; k < 4; ++k) yh[k] = mul(pr, fma(hh[k], a1, add(yh[k], a0)));
         }
         put(1, yh);
     }
@@ -503,52 +540,53 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
         if (a.gate && in) {
-            Unit<T> u;
-            u.load(static_cast<const T*>(a.gate) + item_group * D + c);
-            u.get(col.g);
+            Unit<T> gate;
+            gate.load(static_cast<const T*>(a.gate) + item_group * D + c);
+            gate.get(col.g);
         }
-        // the next row's loads are under way while a row is worked on
-        Unit<T> nx, nh, ndy, ndn;
-        float4 nst = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        Unit<T> u[4];  // x, h, dy, dn: the next row's from when dx is out
+        float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto fetch = [&](int64_t t) {
             const bool here = in && t < last;
-            const Unit<T> zero{};
-            nx = nh = ndy = ndn = zero;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) u[k] = Unit<T>{};
             if (here) {
-                nx.stream(static_cast<const T*>(a.x) + t * a.ld_x + c);
-                nh.stream(static_cast<const T*>(a.h) + t * a.ld_h + c);
-                if (g.dy) ndy.stream(static_cast<const T*>(g.dy) + t * g.ld_dy + c);
-                if (g.dn) ndn.stream(static_cast<const T*>(g.dn) + t * g.ld_dn + c);
+                u[0].stream(static_cast<const T*>(a.x) + t * a.ld_x + c);
+                u[1].stream(static_cast<const T*>(a.h) + t * a.ld_h + c);
+                if (g.dy) u[2].stream(static_cast<const T*>(g.dy) + t * g.ld_dy + c);
+                if (g.dn) u[3].stream(static_cast<const T*>(g.dn) + t * g.ld_dn + c);
             }
-            if (t < last) nst = reinterpret_cast<const float4*>(a.stats)[t];
+            if (t < last) next = reinterpret_cast<const float4*>(a.stats)[t];
         };
         fetch(first + slot);
         for (int64_t t0 = first; t0 < last; t0 += slots) {
             const int64_t t = t0 + slot;
-            const Unit<T> now[4] = {nx, nh, ndy, ndn};
-            const float4 st = nst;
+            const float4 st = next;
             const bool here = in && t < last;
-            fetch(t + slots);
-            col.row(a, st, pre, here, inv, group, [&](int i, float* v) { now[i].get(v); },
-                    [&](int i, const float* v) {
-                        if (!here) return;
-                        if (i == 0 && g.dx) Unit<T>::put(static_cast<T*>(g.dx) + t * g.ld_dx + c, v);
-                        if (i == 1 && g.dh) Unit<T>::put(static_cast<T*>(g.dh) + t * g.ld_dh + c, v);
+            col.row(a, st, pre, here, inv, group, [&](int i, Pair* v) { u[i].get(v); },
+                    [&](int i, const Pair* v) {
+                        if (i == 0 && here && g.dx) Unit<T>::put(static_cast<T*>(g.dx) + t * g.ld_dx + c, v);
+                        if (i == 0) fetch(t + slots);
+                        if (i == 1 && here && g.dh) Unit<T>::put(static_cast<T*>(g.dh) + t * g.ld_dh + c, v);
                     });
         }
         if (g.dgate) {
+            float dg[8];
+            Column::unpack(col.dg, dg);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                for (int o = 16; o >= lanes; o >>= 1) col.dg[k] += __shfl_xor_sync(~0u, col.dg[k], o);
+                for (int o = 16; o >= lanes; o >>= 1) dg[k] += __shfl_xor_sync(~0u, dg[k], o);
             if (slot == 0 && in) {
-                if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, col.dg);
-                else store8(gate_part + i * D + c, col.dg);
+                if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, dg);
+                else store8(gate_part + i * D + c, dg);
             }
-            fill8(col.dg, 0.0f);
+            Column::fill(col.dg, 0.0f);
         }
     }
     // the slots of a warp, then the warps
-    auto flush = [&](float* v, int which) {
+    auto flush = [&](const Pair* sum, int which) {
+        float v[8];
+        Column::unpack(sum, v);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -628,31 +666,37 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
             __syncthreads();  // all have done with the row before this one: its stage takes another
             if (threadIdx.x == 0 && !bad) copy();
             col.row(a, st, pre, in, inv, group,
-                    [&](int i, float* v) {
-                        fill8(v, 0.0f);
+                    [&](int i, Pair* v) {
+                        Column::fill(v, 0.0f);
                         if (!in || (i == 2 && !g.dy) || (i == 3 && !g.dn)) return;
                         Unit<T> u;
                         u.load(from + i * D + c), u.get(v);
                     },
-                    [&](int i, const float* v) {
+                    [&](int i, const Pair* v) {
                         if (!in) return;
                         if (i == 0 && g.dx) Unit<T>::put(static_cast<T*>(g.dx) + t * g.ld_dx + c, v);
                         if (i == 1 && g.dh) Unit<T>::put(static_cast<T*>(g.dh) + t * g.ld_dh + c, v);
                     });
         }
         if (g.dgate && in) {
-            if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, col.dg);
-            else store8(gate_part + i * D + c, col.dg);
+            float dg[8];
+            Column::unpack(col.dg, dg);
+            if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, dg);
+            else store8(gate_part + i * D + c, dg);
         }
-        fill8(col.dg, 0.0f);
+        Column::fill(col.dg, 0.0f);
     }
     if (bad && threadIdx.x == 0)
         for (int k = 0; k < stages; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
     if (in) {
         float* to = weight_part + (int64_t)blockIdx.x * 4 * D + c;
-        const float* v[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
+        const Pair* sums[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) store8(to + k * D, v[k]);
+        for (int k = 0; k < 4; ++k) {
+            float v[8];
+            Column::unpack(sums[k], v);
+            store8(to + k * D, v);
+        }
     }
 }
 
