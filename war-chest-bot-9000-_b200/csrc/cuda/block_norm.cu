@@ -10,16 +10,19 @@
 //   dwn = sum dn yhat, dbn = sum dn, dwp = sum dU hhat, dbp = sum dU
 //
 // Both directions are bound by the bytes of the [rows, width] matrices (two in
-// and two out; four in and two out), each read and written once here. A unit is
-// 8 columns of a row (16 bytes of a 16-bit type).
+// and two out; four in and two out), read and written once. A thread has units
+// of 8 columns: next to each other, 16 bytes of a 16-bit type at a time, where
+// addresses and strides allow, else one column of each of 8 runs, so that the
+// threads of a warp still read and write next to each other.
 //   forward: a row in the registers of a part of a warp, or of a CTA; means and
 //     deviations from the registers, in two passes.
 //   backward, widths up to 256: a part of a warp a row, a unit a thread, which
 //     also keeps that unit's sums over the rows (weights' and gate's).
-//   backward, widths up to 4096: a CTA a row, a unit a thread, rows brought to
-//     shared memory by bulk copies some rows ahead.
-//   other widths, strides and addresses: kernels that read an element at a
-//     time, and in the backward pass all inputs twice (rows, then columns).
+//   backward, widths up to 4096: a CTA a row, a unit a thread; rows come to
+//     shared memory by bulk copies some rows ahead where their addresses allow.
+//   backward, wider: the sums of a CTA no longer fit its registers: the rows
+//     first (dx, dh and two means a row), then the sums column by column, which
+//     reads the inputs a second time.
 #include <algorithm>
 
 #include "colsum.cuh"
@@ -30,182 +33,9 @@ namespace wctrain {
 
 namespace {
 
-constexpr int THREADS = 256;
-
 struct Row {
     float pm, pr, nm, nr;
 };
-
-template <class T>
-struct Args {
-    wc_block_norm_args a;
-    __device__ const T* gate(int64_t t) const {
-        return a.gate ? static_cast<const T*>(a.gate) + t / a.rows_per_gate * a.width : nullptr;
-    }
-    __device__ float hhat(int64_t t, int64_t j, const Row& r) const {
-        return (to_f(static_cast<const T*>(a.h)[t * a.ld_h + j]) - r.pm) * r.pr;
-    }
-    __device__ float u(float hh, int64_t j) const {
-        return a.post_weight ? fmaf(hh, a.post_weight[j], a.post_bias ? a.post_bias[j] : 0.0f) : hh;
-    }
-    __device__ float y(int64_t t, int64_t j, float u, const T* gate) const {
-        return a.residual_scale * to_f(static_cast<const T*>(a.x)[t * a.ld_x + j]) + (gate ? to_f(gate[j]) * u : u);
-    }
-};
-
-template <class T>
-__global__ void __launch_bounds__(THREADS) k_block_norm(Args<T> q) {
-    __shared__ float s[32];
-    const wc_block_norm_args& a = q.a;
-    const int64_t D = a.width, blocks = (D + 31) / 32;
-    const float inv = 1.0f / (float)D;
-    for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
-        Row r{0.0f, 1.0f, 0.0f, 1.0f};
-        const T* gate = q.gate(t);
-        if (a.post_weight) {
-            float v = 0.0f;
-            if (a.kind == WC_NORM_LAYER) {
-                for (int64_t j = threadIdx.x; j < D; j += THREADS) v += q.hhat(t, j, r);
-                r.pm = cta_sum(v, s) * inv;
-            }
-            v = 0.0f;
-            for (int64_t j = threadIdx.x; j < D; j += THREADS) v += q.hhat(t, j, r) * q.hhat(t, j, r);
-            r.pr = rsqrtf(cta_sum(v, s) * inv + a.eps);
-        }
-        auto y_at = [&](int64_t j) { return q.y(t, j, q.u(q.hhat(t, j, r), j), gate); };
-        if (a.pre_weight) {
-            float v = 0.0f;
-            if (a.kind == WC_NORM_LAYER) {
-                for (int64_t j = threadIdx.x; j < D; j += THREADS) v += y_at(j);
-                r.nm = cta_sum(v, s) * inv;
-            }
-            v = 0.0f;
-            for (int64_t j = threadIdx.x; j < D; j += THREADS) v += (y_at(j) - r.nm) * (y_at(j) - r.nm);
-            r.nr = rsqrtf(cta_sum(v, s) * inv + a.eps);
-        }
-        for (int64_t b = threadIdx.x / 32; b < blocks; b += THREADS / 32) {
-            const int64_t j = b * 32 + (threadIdx.x & 31);
-            float n = 0.0f;
-            if (j < D) {
-                const float y = y_at(j);
-                static_cast<T*>(a.y)[t * a.ld_y + j] = from_f<T>(y);
-                if (a.pre_weight) {
-                    n = fmaf((y - r.nm) * r.nr, a.pre_weight[j], a.pre_bias ? a.pre_bias[j] : 0.0f);
-                    if (a.n) static_cast<T*>(a.n)[t * a.ld_n + j] = from_f<T>(n);
-                }
-            }
-            if (a.n_q) {
-                const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(n) & 0x7fffffffu)));
-                a.n_q[(t * blocks + b) * 32 + (threadIdx.x & 31)] =
-                    code == 255 ? (int8_t)0 : (int8_t)__float2int_rn(n * act8_inverse(code));
-                if ((threadIdx.x & 31) == 0) a.n_scale[t * blocks + b] = (uint8_t)code;
-            }
-        }
-        if (threadIdx.x == 0) reinterpret_cast<float4*>(a.stats)[t] = make_float4(r.pm, r.pr, r.nm, r.nr);
-    }
-}
-
-template <class T>
-__device__ float at(const void* p, int64_t ld, int64_t t, int64_t j) {
-    return p ? to_f(static_cast<const T*>(p)[t * ld + j]) : 0.0f;
-}
-
-// dx and dh, and per row the two means that dY needs
-template <class T>
-__global__ void __launch_bounds__(THREADS) k_block_norm_rows(Args<T> q, wc_block_norm_grads g, float2* means) {
-    __shared__ float s[32];
-    const wc_block_norm_args& a = q.a;
-    const int64_t D = a.width;
-    const float inv = 1.0f / (float)D;
-    const bool layer = a.kind == WC_NORM_LAYER, pre = a.pre_weight && g.dn;
-    for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
-        const float4 st = reinterpret_cast<const float4*>(a.stats)[t];
-        const Row r{st.x, st.y, st.z, st.w};
-        const T* gate = q.gate(t);
-        auto yhat = [&](int64_t j) { return (q.y(t, j, q.u(q.hhat(t, j, r), j), gate) - r.nm) * r.nr; };
-        float m0 = 0.0f, m1 = 0.0f;
-        if (pre) {
-            for (int64_t j = threadIdx.x; j < D; j += THREADS) {
-                const float d = at<T>(g.dn, g.ld_dn, t, j) * a.pre_weight[j];
-                m0 += d, m1 += d * yhat(j);
-            }
-            m0 = layer ? cta_sum(m0, s) * inv : 0.0f;
-            m1 = cta_sum(m1, s) * inv;
-        }
-        if (threadIdx.x == 0) means[t] = make_float2(m0, m1);
-        auto dY = [&](int64_t j) {
-            float d = at<T>(g.dy, g.ld_dy, t, j);
-            if (pre) d += r.nr * (at<T>(g.dn, g.ld_dn, t, j) * a.pre_weight[j] - m0 - yhat(j) * m1);
-            return d;
-        };
-        auto dU = [&](int64_t j) { return dY(j) * (gate ? to_f(gate[j]) : 1.0f) * (a.post_weight ? a.post_weight[j] : 1.0f); };
-        float c0 = 0.0f, c1 = 0.0f;
-        if (a.post_weight && g.dh) {
-            for (int64_t j = threadIdx.x; j < D; j += THREADS) {
-                const float d = dU(j);
-                c0 += d, c1 += d * q.hhat(t, j, r);
-            }
-            c0 = layer ? cta_sum(c0, s) * inv : 0.0f;
-            c1 = cta_sum(c1, s) * inv;
-        }
-        for (int64_t j = threadIdx.x; j < D; j += THREADS) {
-            if (g.dx) static_cast<T*>(g.dx)[t * g.ld_dx + j] = from_f<T>(a.residual_scale * dY(j));
-            if (g.dh) static_cast<T*>(g.dh)[t * g.ld_dh + j] =
-                from_f<T>(a.post_weight ? r.pr * (dU(j) - c0 - q.hhat(t, j, r) * c1) : dU(j));
-        }
-    }
-}
-
-// Items are (group, segment of its rows); a CTA column y takes items y, y +
-// gridDim.y, ... It keeps the weights' sums over all of them and writes the
-// gate's sum of each.
-template <class T>
-__global__ void __launch_bounds__(THREADS) k_block_norm_cols(Args<T> q, wc_block_norm_grads g, const float2* means,
-                                                             int64_t items, int segments, int64_t per, float* gate_part,
-                                                             float* weight_part) {
-    __shared__ float s[5][8][32];
-    const wc_block_norm_args& a = q.a;
-    const int64_t D = a.width, j = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int w = threadIdx.x / 32;
-    const int64_t R = a.gate ? a.rows_per_gate : a.rows;
-    float acc[4] = {};
-    for (int64_t i = blockIdx.y; i < items; i += gridDim.y) {
-        const int64_t group = i / segments, first = group * R + (i - group * segments) * per;
-        const int64_t last = min(min(first + per, (group + 1) * R), a.rows);
-        float dg = 0.0f;
-        if (j < D)
-            for (int64_t t = first + w; t < last; t += 8) {
-                const float4 st = reinterpret_cast<const float4*>(a.stats)[t];
-                const Row r{st.x, st.y, st.z, st.w};
-                const T* gate = q.gate(t);
-                const float hh = q.hhat(t, j, r), u = q.u(hh, j), yh = (q.y(t, j, u, gate) - r.nm) * r.nr;
-                const float dn = at<T>(g.dn, g.ld_dn, t, j);
-                float d = at<T>(g.dy, g.ld_dy, t, j);
-                if (a.pre_weight && g.dn) d += r.nr * (dn * a.pre_weight[j] - means[t].x - yh * means[t].y);
-                dg += d * u;
-                const float du = d * (gate ? to_f(gate[j]) : 1.0f);
-                acc[0] += du * hh, acc[1] += du, acc[2] += dn * yh, acc[3] += dn;
-            }
-        if (g.dgate) {
-            __syncthreads();
-            s[4][w][threadIdx.x & 31] = dg;
-            __syncthreads();
-            if (w == 0 && j < D) {
-                for (int k = 1; k < 8; ++k) dg += s[4][k][threadIdx.x];
-                if (segments == 1) static_cast<T*>(g.dgate)[group * D + j] = from_f<T>(dg);
-                else gate_part[i * D + j] = dg;
-            }
-        }
-    }
-    for (int k = 0; k < 4; ++k) s[k][w][threadIdx.x & 31] = acc[k];
-    __syncthreads();
-    if (w == 0 && j < D)
-        for (int k = 0; k < 4; ++k) {
-            float v = acc[k];
-            for (int i = 1; i < 8; ++i) v += s[k][i][threadIdx.x];
-            weight_part[(blockIdx.y * 4 + k) * D + j] = v;
-        }
-}
 
 // the segments of a group joined
 template <class T>
@@ -219,56 +49,117 @@ __global__ void k_gate_sum(const float* part, int segments, int64_t D, int64_t t
 }
 
 // ---- units -------------------------------------------------------------------
-template <class T>
-struct Unit {
-    uint4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+using Pair = unsigned long long;  // two 32-bit numbers for the packed forms (umma.cuh)
+
+// How a thread's 8 columns lie: next to each other; or one of each of 8 runs, the runs as long as the threads that share
+// the row (of a warp or less), or 32 (a warp's 256 columns next to each other: offsets known to the compiler).
+enum { VEC, LANES, RUNS };
+// A thread's i-th unit of a row: `at` of `apart` threads.
+template <class T, int LAY>
+struct Cols {
+    int D, at, apart;
+    __device__ __forceinline__ int col(int i, int k) const {
+        return LAY == VEC ? (i * apart + at) * 8 + k : LAY == RUNS ? (i * apart + (at & ~31)) * 8 + (at & 31) + k * 32 : (i * 8 + k) * apart + at;
     }
-    __device__ __forceinline__ void stream(const T* p) {
+    __device__ __forceinline__ bool in(int i, int k) const { return col(i, LAY == VEC ? 0 : k) < D; }
+    __device__ __forceinline__ bool any(int i) const { return col(i, 0) < D; }
+};
+template <class T, int LAY>
+struct Unit {
+    T e[8];
+    __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        for (int k = 0; k < 8; ++k) e[k] = from_f<T>(0.0f);
+    }
+    __device__ __forceinline__ void load(const T* row, const Cols<T, LAY>& c, int i) {
+        const T* p = row + c.col(i, 0);
+        const int left = c.D - c.col(i, 0), step = c.col(i, 1) - c.col(i, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) e[k] = k * step < left ? p[k * step] : from_f<T>(0.0f);
+    }
+    __device__ __forceinline__ void stream(const T* row, const Cols<T, LAY>& c, int i) { load(row, c, i); }
+    __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = to_f(e[k]);
+    }
+    __device__ __forceinline__ static void put(T* row, const Cols<T, LAY>& c, int i, const float* v) {
+        T* p = row + c.col(i, 0);
+        const int left = c.D - c.col(i, 0), step = c.col(i, 1) - c.col(i, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k * step < left) p[k * step] = from_f<T>(v[k]);
+    }
+};
+template <class T>
+struct Unit<T, VEC> {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void load(const T* row, const Cols<T, VEC>& c, int i) {
+        const T* p = row + c.col(i, 0);
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) w[j] = reinterpret_cast<const uint4*>(p)[j];
+    }
+    __device__ __forceinline__ void stream(const T* row, const Cols<T, VEC>& c, int i) {
+        const T* p = row + c.col(i, 0);
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) w[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j);
     }
     __device__ __forceinline__ void get(float* v) const {
         alignas(16) T e[8];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(e)[i] = w[i];
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(e)[j] = w[j];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
+        for (int k = 0; k < 8; ++k) v[k] = to_f(e[k]);
     }
-    // the same in pairs
-    __device__ __forceinline__ void get(unsigned long long* v) const {
-        float f[8];
-        get(f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = umma::f2(f[2 * i], f[2 * i + 1]);
-    }
-    __device__ __forceinline__ static void put(T* p, const unsigned long long* v) {
-        float f[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[2 * i] = umma::f2_lo(v[i]), f[2 * i + 1] = umma::f2_hi(v[i]);
-        put(p, f);
-    }
-    __device__ __forceinline__ static void put(T* p, const float* v) {
+    __device__ __forceinline__ static void put(T* row, const Cols<T, VEC>& c, int i, const float* v) {
+        T* p = row + c.col(i, 0);
         alignas(16) T e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
+        for (int k = 0; k < 8; ++k) e[k] = from_f<T>(v[k]);
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(e)[i]);
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) __stcs(reinterpret_cast<uint4*>(p) + j, reinterpret_cast<const uint4*>(e)[j]);
     }
 };
-__device__ __forceinline__ void load8(const float* p, float* v) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+// the same columns of a 32-bit vector
+template <class T, int LAY>
+__device__ __forceinline__ void load8(const float* p, const Cols<T, LAY>& c, int i, float* v) {
+    if constexpr (LAY == VEC) {
+        const float4 a = *reinterpret_cast<const float4*>(p + c.col(i, 0)), b = *reinterpret_cast<const float4*>(p + c.col(i, 0) + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const int left = c.D - c.col(i, 0), step = c.col(i, 1) - c.col(i, 0);
+        p += c.col(i, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k * step < left ? p[k * step] : 0.0f;
+    }
 }
-__device__ __forceinline__ void store8(float* p, const float* v) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+template <class T, int LAY>
+__device__ __forceinline__ void store8(float* p, const Cols<T, LAY>& c, int i, const float* v) {
+    if constexpr (LAY == VEC) {
+        *reinterpret_cast<float4*>(p + c.col(i, 0)) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + c.col(i, 0) + 4) = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        const int left = c.D - c.col(i, 0), step = c.col(i, 1) - c.col(i, 0);
+        p += c.col(i, 0);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k * step < left) p[k * step] = v[k];
+    }
 }
 __device__ __forceinline__ void fill8(float* v, float x) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = x;
+}
+__device__ __forceinline__ void pairs(const float* f, Pair* v) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = umma::f2(f[2 * k], f[2 * k + 1]);
+}
+__device__ __forceinline__ void unpairs(const Pair* v, float* f) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[2 * k] = umma::f2_lo(v[k]), f[2 * k + 1] = umma::f2_hi(v[k]);
 }
 
 // Sums over the threads that share a row: `lanes` of a warp, or the CTA (each
@@ -295,12 +186,13 @@ struct Group {
 };
 
 // WARPS = 0: `lanes` threads of a warp a row, else a CTA of up to WARPS warps;
-// NV units a thread, `lanes` (or blockDim.x) apart.
-template <class T, int WARPS, int NV>
-__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 ? 40 / (WARPS ? WARPS : 1) : 1) : 4) k_norm_units(wc_block_norm_args a, int lanes) {
+// NV units a thread.
+template <class T, int LAY, int WARPS, int NV>
+__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS ? WARPS : 1) : 4) k_norm_units(wc_block_norm_args a, int lanes) {
     __shared__ float2 s[2][32];
     Group<WARPS> group{s, lanes};
-    const int D = (int)a.width, at = WARPS ? threadIdx.x : (int)(threadIdx.x & (lanes - 1)), apart = WARPS ? (int)blockDim.x : lanes;
+    const int D = (int)a.width;
+    const Cols<T, LAY> cols{D, WARPS ? (int)threadIdx.x : (int)(threadIdx.x & (lanes - 1)), WARPS ? (int)blockDim.x : lanes};
     const int per = WARPS ? 1 : 256 / lanes, slot = WARPS ? 0 : (int)threadIdx.x / lanes;
     const int blocks = (D + 31) / 32;
     const float inv = 1.0f / (float)D;
@@ -308,16 +200,15 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
     for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < a.rows; t0 += (int64_t)gridDim.x * per) {
         const int64_t t = t0 + slot;
         const bool in = t < a.rows;
-        Unit<T> x[NV];
+        Unit<T, LAY> x[NV];
         float v[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * apart + at) * 8;
             fill8(v[i], 0.0f);
-            if (in && c < D) {
-                Unit<T> h;
-                h.stream(static_cast<const T*>(a.h) + t * a.ld_h + c);
-                x[i].stream(static_cast<const T*>(a.x) + t * a.ld_x + c);
+            if (in && cols.any(i)) {
+                Unit<T, LAY> h;
+                h.stream(static_cast<const T*>(a.h) + t * a.ld_h, cols, i);
+                x[i].stream(static_cast<const T*>(a.x) + t * a.ld_x, cols, i);
                 h.get(v[i]);
             }
         }
@@ -334,9 +225,9 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
             float q = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if ((i * apart + at) * 8 < D)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) q = fmaf(v[i][k] - mean, v[i][k] - mean, q);
+                for (int k = 0; k < 8; ++k)
+                    if (cols.in(i, k)) q = fmaf(v[i][k] - mean, v[i][k] - mean, q);
             r = rsqrtf(group.sum(q) * inv + a.eps);
         };
         Row r{0.0f, 1.0f, 0.0f, 1.0f};
@@ -344,12 +235,11 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
         const T* gate = a.gate && in ? static_cast<const T*>(a.gate) + t / a.rows_per_gate * D : nullptr;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * apart + at) * 8;
-            if (!in || c >= D) continue;
+            if (!in || !cols.any(i)) continue;
             if (a.post_weight) {
                 float w[8], b[8];
-                load8(a.post_weight + c, w);
-                if (a.post_bias) load8(a.post_bias + c, b);
+                load8(a.post_weight, cols, i, w);
+                if (a.post_bias) load8(a.post_bias, cols, i, b);
                 else fill8(b, 0.0f);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[i][k] = fmaf((v[i][k] - r.pm) * r.pr, w[k], b[k]);
@@ -357,8 +247,8 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
             float xf[8];
             x[i].get(xf);
             if (gate) {
-                Unit<T> gu;
-                gu.load(gate + c);
+                Unit<T, LAY> gu;
+                gu.load(gate, cols, i);
                 float g[8];
                 gu.get(g);
 #pragma unroll
@@ -367,34 +257,48 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[i][k] = fmaf(a.residual_scale, xf[k], v[i][k]);
             }
-            Unit<T>::put(static_cast<T*>(a.y) + t * a.ld_y + c, v[i]);
+            if (LAY != VEC)  // (whose columns past the width had weights of 0 but no x)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (!cols.in(i, k)) v[i][k] = 0.0f;
+            Unit<T, LAY>::put(static_cast<T*>(a.y) + t * a.ld_y, cols, i, v[i]);
         }
         if (a.pre_weight) {
             moments(r.nm, r.nr);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (i * apart + at) * 8;
-                const bool here = in && c < D;
-                if (here) {
+                if (in && cols.any(i)) {
                     float w[8], b[8];
-                    load8(a.pre_weight + c, w);
-                    if (a.pre_bias) load8(a.pre_bias + c, b);
+                    load8(a.pre_weight, cols, i, w);
+                    if (a.pre_bias) load8(a.pre_bias, cols, i, b);
                     else fill8(b, 0.0f);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[i][k] = fmaf((v[i][k] - r.nm) * r.nr, w[k], b[k]);
-                    if (a.n) Unit<T>::put(static_cast<T*>(a.n) + t * a.ld_n + c, v[i]);
+                    for (int k = 0; k < 8; ++k) v[i][k] = cols.in(i, k) ? fmaf((v[i][k] - r.nm) * r.nr, w[k], b[k]) : 0.0f;
+                    if (a.n) Unit<T, LAY>::put(static_cast<T*>(a.n) + t * a.ld_n, cols, i, v[i]);
                 }
-                if (a.n_q) {  // 4 threads next to each other hold a block (lanes is at least 4 then)
+                if (!a.n_q) continue;
+                if constexpr (LAY == VEC) {  // 4 threads next to each other hold a block (lanes is at least 4 then)
                     uint32_t code;
                     const uint2 q = quantise8(v[i], &code);
+                    const int c = cols.col(i, 0);
                     if (in && c < blocks * 32) {
                         *reinterpret_cast<uint2*>(a.n_q + t * blocks * 32 + c) = q;
                         if ((c & 31) == 0) a.n_scale[t * blocks + c / 32] = (uint8_t)code;
                     }
+                } else {  // a warp does (lanes is 32 then)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(v[i][k]) & 0x7fffffffu)));
+                        const int c = cols.col(i, k);
+                        if (in && c < blocks * 32) {
+                            a.n_q[t * blocks * 32 + c] = code == 255 ? (int8_t)0 : (int8_t)__float2int_rn(v[i][k] * act8_inverse(code));
+                            if ((c & 31) == 0) a.n_scale[t * blocks + c / 32] = (uint8_t)code;
+                        }
+                    }
                 }
             }
         }
-        if (in && at == 0) reinterpret_cast<float4*>(a.stats)[t] = make_float4(r.pm, r.pr, r.nm, r.nr);
+        if (in && cols.at == 0) reinterpret_cast<float4*>(a.stats)[t] = make_float4(r.pm, r.pr, r.nm, r.nr);
     }
 }
 
@@ -404,14 +308,15 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? (WARPS < 32 
 // and hands on the gate's sum of each.
 struct Plan {
     int64_t R, groups, per, items;
-    int segments, workers, lanes, parts;  // lanes of a warp a row (0: a CTA a row, -1: the general kernels)
-    Plan(const wc_block_norm_args& a, bool units) {
+    int width, segments, workers, lanes, parts;  // lanes of a warp a row (0: a CTA a row, -1: rows, then columns)
+    Plan(const wc_block_norm_args& a) {
+        width = (int)a.width;
         R = a.gate ? a.rows_per_gate : a.rows;
         groups = a.rows ? (a.rows + R - 1) / R : 0;
-        lanes = !units || a.width > 4096 ? -1 : 0;
-        if (units && a.width <= 256)
+        lanes = a.width > 4096 ? -1 : 0;
+        if (a.width <= 256)
             for (lanes = 1; lanes * 8 < a.width;) lanes *= 2;
-        const int64_t most = lanes > 0 ? 148 * 2 * 8 : lanes == 0 ? (a.width <= 2048 ? 296 : 148) : 512;
+        const int64_t most = lanes > 0 ? 148 * 2 * 8 : lanes == 0 ? 148 * (512 / threads()) : 296;
         const int64_t longest = R < a.rows ? R : a.rows, want = groups ? (most + groups - 1) / groups : 1;
         const int64_t fit = (longest + 7) / 8;
         segments = (int)(fit < 1 ? 1 : fit < want ? fit : want);
@@ -420,6 +325,7 @@ struct Plan {
         workers = (int)(items < most ? items : most);
         parts = lanes > 0 ? (workers + 7) / 8 : workers;  // partial sums of the weights
     }
+    int threads() const { return (width + 255) / 256 * 32; }  // of a CTA that has a row
     uint64_t floats(const wc_block_norm_args& a) const {
         return 2 * (uint64_t)(a.rows + 1) + (uint64_t)parts * 4 * a.width + (segments > 1 ? (uint64_t)items * a.width : 0);
     }
@@ -433,9 +339,8 @@ struct Items {
     }
 };
 
-// Arithmetic on pairs of 32-bit numbers (umma.cuh), each rounded as the scalar form: the backward pass has some 30
-// operations a column, which would bound it before the bytes do.
-using Pair = unsigned long long;
+// Arithmetic on pairs, each rounded as the scalar form: the backward pass has some 30 operations a column, which would
+// bound it before the bytes do.
 __device__ __forceinline__ Pair twice(float v) { return umma::f2(v, v); }
 __device__ __forceinline__ Pair mul(Pair a, Pair b) {
     Pair d;
@@ -445,45 +350,56 @@ __device__ __forceinline__ Pair mul(Pair a, Pair b) {
 __device__ __forceinline__ Pair add(Pair a, Pair b) { return umma::f2_add(a, b); }
 __device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) { return umma::f2_fma(a, b, c); }
 __device__ __forceinline__ float both(Pair a) { return umma::f2_lo(a) + umma::f2_hi(a); }
+__device__ __forceinline__ void fill(Pair* v, float x) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = twice(x);
+}
+
+__device__ __forceinline__ void bulk_copy(uint32_t to, uint64_t from, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes),
+                 "r"(umma::smem_u32(bar))
+                 : "memory");
+}
 
 // What a thread keeps of its unit: the parameters and their gradients' sums.
+// Columns past the width have weights, gate and inputs of 0, and so add 0 to
+// everything.
 struct Column {
     Pair wp[4], bp[4], wn[4], g[4];
     Pair dwp[4], dbp[4], dwn[4], dbn[4], dg[4];
-    __device__ __forceinline__ static void fill(Pair* v, float x) {
+    template <class T, int LAY>
+    __device__ __forceinline__ void load(const wc_block_norm_args& a, const Cols<T, LAY>& c, int i) {
+        float v[8];
+        auto param = [&](const float* p, float otherwise, Pair* to) {
+            fill8(v, 0.0f);
+            if (c.any(i)) {
+                if (p) load8(p, c, i, v);
+                else
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = twice(x);
-    }
-    __device__ __forceinline__ static void load(Pair* v, const float* p) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-        v[0] = umma::f2(a.x, a.y), v[1] = umma::f2(a.z, a.w), v[2] = umma::f2(b.x, b.y), v[3] = umma::f2(b.z, b.w);
-    }
-    __device__ __forceinline__ static void unpack(const Pair* v, float* f) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) f[2 * k] = umma::f2_lo(v[k]), f[2 * k + 1] = umma::f2_hi(v[k]);
-    }
-    __device__ __forceinline__ void load(const wc_block_norm_args& a, int c, bool in) {
-        fill(wp, 1.0f), fill(bp, 0.0f), fill(wn, 0.0f), fill(g, 1.0f);
+                    for (int k = 0; k < 8; ++k) v[k] = c.in(i, k) ? otherwise : 0.0f;
+            }
+            pairs(v, to);
+        };
+        param(a.post_weight, 1.0f, wp), param(a.post_bias, 0.0f, bp), param(a.pre_weight, 0.0f, wn), param(nullptr, 1.0f, g);
         fill(dwp, 0.0f), fill(dbp, 0.0f), fill(dwn, 0.0f), fill(dbn, 0.0f), fill(dg, 0.0f);
-        if (!in) return;
-        if (a.post_weight) load(wp, a.post_weight + c);
-        if (a.post_bias) load(bp, a.post_bias + c);
-        if (a.pre_weight) load(wn, a.pre_weight + c);
+    }
+    template <class T, int LAY>
+    __device__ __forceinline__ void gate(const T* row, const Cols<T, LAY>& c, int i) {
+        Unit<T, LAY> u;
+        u.zero();
+        if (c.any(i)) u.load(row, c, i);
+        float v[8];
+        u.get(v);
+        pairs(v, g);
     }
     // A row's unit. get(i, v) reads its x, h, dy or dn (i = 0 .. 3; zeros past the width and for a gradient that is not
     // there), when it is needed: what is not held meanwhile leaves room for the sums. put(i, v) takes dx, then dh.
     template <class G, class Get, class Put>
-    __device__ __forceinline__ void row(const wc_block_norm_args& a, const float4& st, bool pre, bool in, float inv, G& group, Get&& get,
-                                        Put&& put) {
+    __device__ __forceinline__ void row(const wc_block_norm_args& a, const float4& st, bool pre, float inv, G& group, Get&& get, Put&& put) {
         const bool layer = a.kind == WC_NORM_LAYER;
         Pair hh[4], yh[4], d[4];
         get(1, hh), get(0, yh);
-        const Pair pr = twice(st.y), pm = twice(-st.x), nr = twice(st.w), nm = twice(-st.z), rs = twice(a.residual_scale);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            hh[k] = mul(add(hh[k], pm), pr);
-            yh[k] = mul(add(fma(rs, yh[k], mul(g[k], fma(hh[k], wp[k], bp[k]))), nm), nr);
-        }
+        hats(a, st, hh, yh);
         if (pre) {
             Pair m0 = 0, m1 = 0;  // pairs of zeros
             get(3, d);
@@ -494,99 +410,115 @@ struct Column {
                 m0 = add(m0, d[k]), m1 = fma(d[k], yh[k], m1);
             }
             const float2 m = group.sum(make_float2(both(m0), both(m1)));
-            const Pair a0 = twice(layer ? -m.x * inv : 0.0f), a1 = twice(-m.y * inv);
+            const Pair a0 = twice(layer ? -m.x * inv : 0.0f), a1 = twice(-m.y * inv), nr = twice(st.w);
 #pragma unroll
             for (int k = 0; k < 4; ++k) yh[k] = mul(nr, fma(yh[k], a1, add(d[k], a0)));
         } else {
             fill(yh, 0.0f);
         }
         get(2, d);
-        const Pair live = twice(in ? 1.0f : 0.0f);
+        const Pair rs = twice(a.residual_scale);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) yh[k] = mul(live, add(d[k], yh[k])), d[k] = mul(rs, yh[k]);  // dY
+        for (int k = 0; k < 4; ++k) yh[k] = add(d[k], yh[k]), d[k] = mul(rs, yh[k]);  // dY
         put(0, d);
         Pair c0 = 0, c1 = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            dg[k] = fma(yh[k], fma(hh[k], wp[k], bp[k]), dg[k]);
-            const Pair du = mul(yh[k], g[k]);
-            dwp[k] = fma(du, hh[k], dwp[k]), dbp[k] = add(dbp[k], du);
-            yh[k] = mul(du, wp[k]);
+            sums(k, yh[k], hh[k]);
+            yh[k] = mul(mul(yh[k], g[k]), wp[k]);
             c0 = add(c0, yh[k]), c1 = fma(yh[k], hh[k], c1);
         }
         if (a.post_weight) {
             const float2 c = group.sum(make_float2(both(c0), both(c1)));
-            const Pair a0 = twice(layer ? -c.x * inv : 0.0f), a1 = twice(-c.y * inv);
+            const Pair a0 = twice(layer ? -c.x * inv : 0.0f), a1 = twice(-c.y * inv), pr = twice(st.y);
 #pragma unroll
             for (int k = 0; k < 4; ++k) yh[k] = mul(pr, fma(hh[k], a1, add(yh[k], a0)));
         }
         put(1, yh);
     }
+    // h and x to hhat and yhat
+    __device__ __forceinline__ void hats(const wc_block_norm_args& a, const float4& st, Pair* hh, Pair* yh) const {
+        const Pair pr = twice(st.y), pm = twice(-st.x), nr = twice(st.w), nm = twice(-st.z), rs = twice(a.residual_scale);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            hh[k] = mul(add(hh[k], pm), pr);
+            yh[k] = mul(add(fma(rs, yh[k], mul(g[k], fma(hh[k], wp[k], bp[k]))), nm), nr);
+        }
+    }
+    // the gate's and the post norm's sums
+    __device__ __forceinline__ void sums(int k, Pair dY, Pair hh) {
+        dg[k] = fma(dY, fma(hh, wp[k], bp[k]), dg[k]);
+        const Pair du = mul(dY, g[k]);
+        dwp[k] = fma(du, hh, dwp[k]), dbp[k] = add(dbp[k], du);
+    }
 };
 
 // A part of a warp a row; a warp is a worker.
-template <class T>
+template <class T, int LAY>
 __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_args a, wc_block_norm_grads g, Items q, int lanes,
                                                                float* gate_part, float* weight_part) {
     __shared__ float s[8][8][33];
-    const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = lane & (lanes - 1), c = at * 8;
+    const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int slots = 32 / lanes, slot = lane / lanes, worker = blockIdx.x * 8 + warp;
-    const bool in = c < D, pre = a.pre_weight && g.dn;
+    const Cols<T, LAY> cols{D, lane & (lanes - 1), lanes};
+    const bool any = cols.any(0), pre = a.pre_weight && g.dn;
     const float inv = 1.0f / (float)D;
     Group<0> group{nullptr, lanes};
     Column col;
-    col.load(a, c, in);
+    col.load(a, cols, 0);
     for (int64_t i = worker; i < q.items; i += q.workers) {
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
-        if (a.gate && in) {
-            Unit<T> gate;
-            gate.load(static_cast<const T*>(a.gate) + item_group * D + c);
-            gate.get(col.g);
-        }
-        Unit<T> u[4];  // x, h, dy, dn: the next row's from when dx is out
+        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
+        Unit<T, LAY> u[4];  // x, h, dy, dn: the next row's from when dx is out
         float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto fetch = [&](int64_t t) {
-            const bool here = in && t < last;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) u[k] = Unit<T>{};
-            if (here) {
-                u[0].stream(static_cast<const T*>(a.x) + t * a.ld_x + c);
-                u[1].stream(static_cast<const T*>(a.h) + t * a.ld_h + c);
-                if (g.dy) u[2].stream(static_cast<const T*>(g.dy) + t * g.ld_dy + c);
-                if (g.dn) u[3].stream(static_cast<const T*>(g.dn) + t * g.ld_dn + c);
-            }
-            if (t < last) next = reinterpret_cast<const float4*>(a.stats)[t];
+            for (int k = 0; k < 4; ++k) u[k].zero();
+            if (t >= last) return;
+            next = reinterpret_cast<const float4*>(a.stats)[t];
+            if (!any) return;
+            u[0].stream(static_cast<const T*>(a.x) + t * a.ld_x, cols, 0);
+            u[1].stream(static_cast<const T*>(a.h) + t * a.ld_h, cols, 0);
+            if (g.dy) u[2].stream(static_cast<const T*>(g.dy) + t * g.ld_dy, cols, 0);
+            if (g.dn) u[3].stream(static_cast<const T*>(g.dn) + t * g.ld_dn, cols, 0);
         };
         fetch(first + slot);
         for (int64_t t0 = first; t0 < last; t0 += slots) {
             const int64_t t = t0 + slot;
+            const bool here = any && t < last;  // (a row past the last has gradients of 0: it adds 0 to every sum)
             const float4 st = next;
-            const bool here = in && t < last;
-            col.row(a, st, pre, here, inv, group, [&](int i, Pair* v) { u[i].get(v); },
-                    [&](int i, const Pair* v) {
-                        if (i == 0 && here && g.dx) Unit<T>::put(static_cast<T*>(g.dx) + t * g.ld_dx + c, v);
-                        if (i == 0) fetch(t + slots);
-                        if (i == 1 && here && g.dh) Unit<T>::put(static_cast<T*>(g.dh) + t * g.ld_dh + c, v);
+            col.row(a, st, pre, inv, group,
+                    [&](int k, Pair* v) {
+                        float f[8];
+                        u[k].get(f);
+                        pairs(f, v);
+                    },
+                    [&](int k, const Pair* v) {
+                        float f[8];
+                        unpairs(v, f);
+                        if (k == 0 && here && g.dx) Unit<T, LAY>::put(static_cast<T*>(g.dx) + t * g.ld_dx, cols, 0, f);
+                        if (k == 0) fetch(t + slots);
+                        if (k == 1 && here && g.dh) Unit<T, LAY>::put(static_cast<T*>(g.dh) + t * g.ld_dh, cols, 0, f);
                     });
         }
         if (g.dgate) {
             float dg[8];
-            Column::unpack(col.dg, dg);
+            unpairs(col.dg, dg);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 for (int o = 16; o >= lanes; o >>= 1) dg[k] += __shfl_xor_sync(~0u, dg[k], o);
-            if (slot == 0 && in) {
-                if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, dg);
-                else store8(gate_part + i * D + c, dg);
+            if (slot == 0 && any) {
+                if (q.segments == 1) Unit<T, LAY>::put(static_cast<T*>(g.dgate) + item_group * D, cols, 0, dg);
+                else store8(gate_part + i * D, cols, 0, dg);
             }
-            Column::fill(col.dg, 0.0f);
+            fill(col.dg, 0.0f);
         }
     }
     // the slots of a warp, then the warps
     auto flush = [&](const Pair* sum, int which) {
         float v[8];
-        Column::unpack(sum, v);
+        unpairs(sum, v);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -595,36 +527,48 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
         }
         __syncthreads();
         const int k = warp;
-        if (slot == 0 && in) {
+        if (slot == 0 && cols.in(0, k)) {
             float t = 0.0f;
 #pragma unroll
             for (int w = 0; w < 8; ++w) t += s[w][k][lane];
-            weight_part[((int64_t)blockIdx.x * 4 + which) * D + c + k] = t;
+            weight_part[((int64_t)blockIdx.x * 4 + which) * D + cols.col(0, k)] = t;
         }
     };
     flush(col.dwp, 0), flush(col.dbp, 1), flush(col.dwn, 2), flush(col.dbn, 3);
 }
 
 // A CTA a row, one unit a thread; a CTA is a worker. Its rows in order come to
-// shared memory by bulk copies: x, h, dy, dn and the statistics.
+// shared memory by bulk copies: x, h, dy, dn and the statistics. A bulk copy
+// moves whole 16-byte pieces: of rows that do not end on them (LAY != VEC) it
+// takes the pieces they lie in, parts of the rows before and after; the
+// matrices' first and last rows, which have none, are read where they are.
 constexpr int MAX_RING = 8;
-template <class T>
+template <class T, int LAY>
 __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a, wc_block_norm_grads g, Items q, int stages,
                                                            float* gate_part, float* weight_part) {
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 s[2][32];
     __shared__ uint64_t full[MAX_RING];
-    const int D = (int)a.width, c = threadIdx.x * 8, row_bytes = D * (int)sizeof(T), stage_bytes = 4 * row_bytes + 16;
-    const bool in = c < D, pre = a.pre_weight && g.dn;
+    const int D = (int)a.width, row_bytes = D * (int)sizeof(T), piece = LAY == VEC ? row_bytes : (row_bytes + 15) / 16 * 16 + 16;
+    const int stage_bytes = 4 * piece + 16;
+    const Cols<T, LAY> cols{D, (int)threadIdx.x, (int)blockDim.x};
+    const bool any = cols.any(0), pre = a.pre_weight && g.dn;
     const float inv = 1.0f / (float)D;
     Group<16> group{s, 32};
     Column col;
-    col.load(a, c, in);
+    col.load(a, cols, 0);
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) umma::mbar_init(&full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    auto row_of = [&](int k, int64_t t) -> const T* {
+        return k == 0   ? static_cast<const T*>(a.x) + t * a.ld_x
+               : k == 1 ? static_cast<const T*>(a.h) + t * a.ld_h
+               : k == 2 ? (g.dy ? static_cast<const T*>(g.dy) + t * g.ld_dy : nullptr)
+                        : (g.dn ? static_cast<const T*>(g.dn) + t * g.ld_dn : nullptr);
+    };
+    auto edge = [&](int64_t t) { return LAY != VEC && (t == 0 || t == a.rows - 1); };
     // thread 0 walks ahead of the rows
     int64_t copy_item = blockIdx.x, copy_row = 0, copy_last = 0, copy_group;
     int copied = 0;
@@ -635,13 +579,21 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
             copy_item += q.workers;
         }
         const int slot = copied % stages;
-        uint8_t* to = ring + slot * stage_bytes;
-        umma::expect_tx(&full[slot], (2 + (g.dy != nullptr) + (g.dn != nullptr)) * row_bytes + 16);
-        umma::bulk_g2s(to, static_cast<const T*>(a.x) + copy_row * a.ld_x, row_bytes, &full[slot]);
-        umma::bulk_g2s(to + row_bytes, static_cast<const T*>(a.h) + copy_row * a.ld_h, row_bytes, &full[slot]);
-        if (g.dy) umma::bulk_g2s(to + 2 * row_bytes, static_cast<const T*>(g.dy) + copy_row * g.ld_dy, row_bytes, &full[slot]);
-        if (g.dn) umma::bulk_g2s(to + 3 * row_bytes, static_cast<const T*>(g.dn) + copy_row * g.ld_dn, row_bytes, &full[slot]);
-        umma::bulk_g2s(to + 4 * row_bytes, a.stats + copy_row * 4, 16, &full[slot]);
+        const uint32_t to = umma::smem_u32(ring + slot * stage_bytes);
+        uint64_t from[4];
+        uint32_t bytes[4], total = 16;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint64_t p = reinterpret_cast<uint64_t>(row_of(k, copy_row));
+            from[k] = p & ~15ull;
+            bytes[k] = !p || edge(copy_row) ? 0 : (uint32_t)(((p + row_bytes + 15) & ~15ull) - from[k]);
+            total += bytes[k];
+        }
+        umma::expect_tx(&full[slot], total);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (bytes[k]) bulk_copy(to + k * piece, from[k], bytes[k], &full[slot]);
+        bulk_copy(to + 4 * piece, reinterpret_cast<uint64_t>(a.stats + copy_row * 4), 16, &full[slot]);
         ++copied, ++copy_row;
     };
     if (threadIdx.x == 0)
@@ -651,52 +603,220 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
     for (int64_t i = blockIdx.x; i < q.items; i += q.workers) {
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
-        if (a.gate && in) {
-            Unit<T> u;
-            u.load(static_cast<const T*>(a.gate) + item_group * D + c);
-            u.get(col.g);
-        }
+        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
         for (int64_t t = first; t < last; ++t, ++done) {
             const int slot = done % stages;
             // a copy that does not come (umma.cuh) leaves NaN from here on
             if (!bad && !umma::mbar_wait(&full[slot], (uint32_t)(done / stages) & 1)) bad = true;
-            const T* from = reinterpret_cast<const T*>(ring + slot * stage_bytes);
-            float4 st = *reinterpret_cast<const float4*>(ring + slot * stage_bytes + 4 * row_bytes);
+            float4 st = *reinterpret_cast<const float4*>(ring + slot * stage_bytes + 4 * piece);
             if (bad) st.y = st.w = __uint_as_float(0x7fffffffu);
+            const bool here = !edge(t);
             __syncthreads();  // all have done with the row before this one: its stage takes another
             if (threadIdx.x == 0 && !bad) copy();
-            col.row(a, st, pre, in, inv, group,
-                    [&](int i, Pair* v) {
-                        Column::fill(v, 0.0f);
-                        if (!in || (i == 2 && !g.dy) || (i == 3 && !g.dn)) return;
-                        Unit<T> u;
-                        u.load(from + i * D + c), u.get(v);
+            col.row(a, st, pre, inv, group,
+                    [&](int k, Pair* v) {
+                        Unit<T, LAY> u;
+                        u.zero();
+                        const T* p = row_of(k, t);
+                        if (any && p) {
+                            const T* copied = reinterpret_cast<const T*>(ring + slot * stage_bytes + k * piece + (reinterpret_cast<uintptr_t>(p) & 15));
+                            if (here) u.load(copied, cols, 0);
+                            else u.load(p, cols, 0);
+                        }
+                        float f[8];
+                        u.get(f);
+                        pairs(f, v);
                     },
-                    [&](int i, const Pair* v) {
-                        if (!in) return;
-                        if (i == 0 && g.dx) Unit<T>::put(static_cast<T*>(g.dx) + t * g.ld_dx + c, v);
-                        if (i == 1 && g.dh) Unit<T>::put(static_cast<T*>(g.dh) + t * g.ld_dh + c, v);
+                    [&](int k, const Pair* v) {
+                        if (!any) return;
+                        float f[8];
+                        unpairs(v, f);
+                        if (k == 0 && g.dx) Unit<T, LAY>::put(static_cast<T*>(g.dx) + t * g.ld_dx, cols, 0, f);
+                        if (k == 1 && g.dh) Unit<T, LAY>::put(static_cast<T*>(g.dh) + t * g.ld_dh, cols, 0, f);
                     });
         }
-        if (g.dgate && in) {
+        if (g.dgate && any) {
             float dg[8];
-            Column::unpack(col.dg, dg);
-            if (q.segments == 1) Unit<T>::put(static_cast<T*>(g.dgate) + item_group * D + c, dg);
-            else store8(gate_part + i * D + c, dg);
+            unpairs(col.dg, dg);
+            if (q.segments == 1) Unit<T, LAY>::put(static_cast<T*>(g.dgate) + item_group * D, cols, 0, dg);
+            else store8(gate_part + i * D, cols, 0, dg);
         }
-        Column::fill(col.dg, 0.0f);
+        fill(col.dg, 0.0f);
     }
     if (bad && threadIdx.x == 0)
         for (int k = 0; k < stages; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
-    if (in) {
-        float* to = weight_part + (int64_t)blockIdx.x * 4 * D + c;
+    if (any) {
+        float* to = weight_part + (int64_t)blockIdx.x * 4 * D;
         const Pair* sums[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float v[8];
-            Column::unpack(sums[k], v);
-            store8(to + k * D, v);
+            unpairs(sums[k], v);
+            store8(to + k * D, cols, 0, v);
         }
+    }
+}
+
+// Wide rows: a CTA a row, two units a thread; what it does is Column::row
+// without the sums over rows.
+template <class T, int LAY, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32) k_norm_backward_rows(wc_block_norm_args a, wc_block_norm_grads g, float2* means) {
+    __shared__ float2 s[2][32];
+    const int D = (int)a.width;
+    const Cols<T, LAY> cols{D, (int)threadIdx.x, (int)blockDim.x};
+    const bool layer = a.kind == WC_NORM_LAYER, pre = a.pre_weight && g.dn;
+    const float inv = 1.0f / (float)D;
+    Group<WARPS> group{s, 32};
+    for (int64_t t = blockIdx.x; t < a.rows; t += gridDim.x) {
+        const float4 st = reinterpret_cast<const float4*>(a.stats)[t];
+        const T* gate = a.gate ? static_cast<const T*>(a.gate) + t / a.rows_per_gate * D : nullptr;
+        auto get = [&](const void* p, int64_t ld, int i, float* v) {
+            Unit<T, LAY> u;
+            u.zero();
+            if (p && cols.any(i)) u.load(static_cast<const T*>(p) + t * ld, cols, i);
+            u.get(v);
+        };
+        float hh[2][8], d[2][8], yh[2][8];  // hhat; dY, then the gradient at the post norm's output times its weight; yhat
+        float2 m = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            get(a.h, a.ld_h, i, hh[i]);
+            get(a.x, a.ld_x, i, yh[i]);
+            get(g.dn, g.ld_dn, i, d[i]);
+            if (!cols.any(i)) continue;
+            float w[8], b[8], ga[8];
+            fill8(w, 1.0f), fill8(b, 0.0f), fill8(ga, 1.0f);
+            if (a.post_weight) load8(a.post_weight, cols, i, w);
+            if (a.post_bias) load8(a.post_bias, cols, i, b);
+            if (gate) {
+                Unit<T, LAY> u;
+                u.load(gate, cols, i), u.get(ga);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                hh[i][k] = (hh[i][k] - st.x) * st.y;
+                yh[i][k] = (fmaf(a.residual_scale, yh[i][k], ga[k] * fmaf(hh[i][k], w[k], b[k])) - st.z) * st.w;
+            }
+            if (pre) {
+                load8(a.pre_weight, cols, i, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[i][k] = cols.in(i, k) ? d[i][k] * w[k] : 0.0f, m.x += d[i][k], m.y = fmaf(d[i][k], yh[i][k], m.y);
+            }
+        }
+        if (pre) {
+            m = group.sum(m);
+            m.x = layer ? m.x * inv : 0.0f, m.y *= inv;
+        }
+        if (threadIdx.x == 0) means[t] = m;
+        float2 c = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (!cols.any(i)) continue;
+            float dy[8], w[8];
+            get(g.dy, g.ld_dy, i, dy);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                d[i][k] = dy[k] + (pre ? st.w * (d[i][k] - m.x - yh[i][k] * m.y) : 0.0f);
+                dy[k] = a.residual_scale * d[i][k];
+            }
+            if (g.dx) Unit<T, LAY>::put(static_cast<T*>(g.dx) + t * g.ld_dx, cols, i, dy);
+            if (gate) {
+                Unit<T, LAY> u;
+                u.load(gate, cols, i), u.get(w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[i][k] *= w[k];
+            }
+            if (a.post_weight) {
+                load8(a.post_weight, cols, i, w);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    d[i][k] = cols.in(i, k) ? d[i][k] * w[k] : 0.0f;
+                    c.x += d[i][k], c.y = fmaf(d[i][k], hh[i][k], c.y);
+                }
+            }
+        }
+        if (a.post_weight) {
+            c = group.sum(c);
+            c.x = layer ? c.x * inv : 0.0f, c.y *= inv;
+        }
+        if (g.dh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (!cols.any(i)) continue;
+                if (a.post_weight)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) d[i][k] = st.y * (d[i][k] - c.x - hh[i][k] * c.y);
+                Unit<T, LAY>::put(static_cast<T*>(g.dh) + t * g.ld_dh, cols, i, d[i]);
+            }
+    }
+}
+
+// ... and the sums: a warp has 256 columns and every eighth row of an item, the
+// CTA's eight warps are joined at the end of one.
+template <class T, int LAY>
+__global__ void __launch_bounds__(256, 2) k_norm_backward_cols(wc_block_norm_args a, wc_block_norm_grads g, Items q, const float2* means,
+                                                            float* gate_part, float* weight_part) {
+    __shared__ float s[8][8][33];
+    const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // the columns as one unit of `apart` threads' row, of which this CTA has 32
+    const int all = gridDim.x * 32;
+    const Cols<T, LAY> cols{D, (int)blockIdx.x * 32 + lane, all};
+    const bool any = cols.any(0), pre = a.pre_weight && g.dn;
+    Column col;
+    col.load(a, cols, 0);
+    // v summed over the warps: thread (warp k, lane) gets column k of lane's unit
+    auto over_warps = [&](const Pair* sum) {
+        float v[8];
+        unpairs(sum, v);
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[warp][k][lane] = v[k];
+        __syncthreads();
+        float t = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) t += s[w][warp][lane];
+        return t;
+    };
+    for (int64_t i = blockIdx.y; i < q.items; i += q.workers) {
+        int64_t item_group, first, last;
+        q.range(i, item_group, first, last);
+        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
+        for (int64_t t = first + warp; t < last; t += 8) {
+            const float4 st = reinterpret_cast<const float4*>(a.stats)[t];
+            const float2 m = means[t];
+            Pair hh[4], yh[4], dn[4], dY[4];
+            auto get = [&](const void* p, int64_t ld, Pair* v) {
+                Unit<T, LAY> u;
+                u.zero();
+                if (p && any) u.stream(static_cast<const T*>(p) + t * ld, cols, 0);
+                float f[8];
+                u.get(f);
+                pairs(f, v);
+            };
+            get(a.h, a.ld_h, hh), get(a.x, a.ld_x, yh), get(g.dn, g.ld_dn, dn), get(g.dy, g.ld_dy, dY);
+            col.hats(a, st, hh, yh);
+            const Pair a0 = twice(-m.x), a1 = twice(-m.y), nr = twice(st.w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                if (pre) dY[k] = fma(nr, fma(yh[k], a1, fma(dn[k], col.wn[k], a0)), dY[k]);
+                col.dwn[k] = fma(dn[k], yh[k], col.dwn[k]), col.dbn[k] = add(col.dbn[k], dn[k]);
+                col.sums(k, dY[k], hh[k]);
+            }
+        }
+        if (g.dgate) {
+            const float v = over_warps(col.dg);
+            if (cols.in(0, warp)) {
+                if (q.segments == 1) static_cast<T*>(g.dgate)[item_group * D + cols.col(0, warp)] = from_f<T>(v);
+                else gate_part[i * D + cols.col(0, warp)] = v;
+            }
+            fill(col.dg, 0.0f);
+        }
+    }
+    const Pair* sums[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float v = over_warps(sums[k]);
+        if (cols.in(0, warp)) weight_part[((int64_t)blockIdx.y * 4 + k) * D + cols.col(0, warp)] = v;
     }
 }
 
@@ -709,29 +829,29 @@ bool units_ok(const wc_block_norm_args& a) {
            fine(a.post_weight) && fine(a.post_bias) && fine(a.pre_weight) && fine(a.pre_bias);
 }
 
-template <class T>
-void backward(const wc_block_norm_args& a, const wc_block_norm_grads& g, cudaStream_t s) {
-    const size_t e = sizeof(T);
-    const bool units = units_ok(a) && unit_rows(g.dy, g.ld_dy, e) && unit_rows(g.dn, g.ld_dn, e) && unit_rows(g.dx, g.ld_dx, e) &&
-                       unit_rows(g.dh, g.ld_dh, e) && unit_rows(g.dgate, a.width, e);
-    const Plan p(a, units);
+template <class T, bool UNITS>
+void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cudaStream_t s) {
+    const Plan p(a);
+    const int64_t D = a.width, e = sizeof(T);
     float* ws = static_cast<float*>(g.workspace);
-    const int64_t D = a.width;
     float2* means = reinterpret_cast<float2*>(ws);
     float *weights = ws + (a.rows + 1) / 2 * 4, *gates = weights + (int64_t)p.parts * 4 * D;  // both 16-byte aligned where D is a multiple of 4
+    constexpr int WIDE = UNITS ? VEC : RUNS, NARROW = UNITS ? VEC : LANES;
     if (a.rows) {
         const Items q{p.items, p.per, p.R, a.rows, p.segments, p.workers};
         if (p.lanes > 0) {
-            k_norm_backward_warp<T><<<p.parts, 256, 0, s>>>(a, g, q, p.lanes, gates, weights);
+            k_norm_backward_warp<T, NARROW><<<p.parts, 256, 0, s>>>(a, g, q, p.lanes, gates, weights);
         } else if (p.lanes == 0) {
-            const int stage = 4 * (int)D * (int)e + 16, threads = (int)(D / 8 + 31) / 32 * 32;
-            const int stages = std::min(MAX_RING, (D <= 2048 ? 100 : 200) * 1024 / stage);
-            if (wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_norm_backward_cta<T>), 200 * 1024))
-                k_norm_backward_cta<T><<<p.workers, threads, (size_t)stages * stage, s>>>(a, g, q, stages, gates, weights);
+            const int stage = (int)(4 * (UNITS ? D * e : (D * e + 15) / 16 * 16 + 16) + 16), threads = p.threads();
+            const int stages = (int)std::min<int64_t>(MAX_RING, 200 * 1024 / (512 / threads) / stage);
+            if (wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_norm_backward_cta<T, WIDE>), 200 * 1024))
+                k_norm_backward_cta<T, WIDE><<<p.workers, threads, (size_t)stages * stage, s>>>(a, g, q, stages, gates, weights);
         } else {
-            k_block_norm_rows<T><<<(unsigned)(a.rows < 148 * 8 ? a.rows : 148 * 8), THREADS, 0, s>>>(Args<T>{a}, g, means);
-            k_block_norm_cols<T><<<dim3((unsigned)((D + 31) / 32), p.workers), THREADS, 0, s>>>(
-                Args<T>{a}, g, means, p.items, p.segments, p.per, gates, weights);
+            const unsigned threads = (unsigned)((D + 511) / 512 * 32);
+            const unsigned n = (unsigned)std::min<int64_t>(a.rows, 148 * (1024 / threads));
+            if (threads <= 512) k_norm_backward_rows<T, WIDE, 16><<<n, threads, 0, s>>>(a, g, means);
+            else k_norm_backward_rows<T, WIDE, 32><<<n, threads, 0, s>>>(a, g, means);
+            k_norm_backward_cols<T, WIDE><<<dim3((unsigned)((D + 255) / 256), p.workers), 256, 0, s>>>(a, g, q, means, gates, weights);
         }
         if (g.dgate && p.segments > 1)
             k_gate_sum<T><<<148 * 4, 256, 0, s>>>(gates, p.segments, D, p.groups * D, static_cast<T*>(g.dgate));
@@ -740,41 +860,48 @@ void backward(const wc_block_norm_args& a, const wc_block_norm_grads& g, cudaStr
     for (int k = 0; k < 4; ++k)
         if (to[k]) launch_colsum<float>(weights + k * D, p.parts, 4 * D, D, to[k], s);
 }
-
 template <class T>
-void forward(const wc_block_norm_args& a, cudaStream_t s) {
-    if (!a.rows) return;
+void backward(const wc_block_norm_args& a, const wc_block_norm_grads& g, cudaStream_t s) {
     const size_t e = sizeof(T);
-    if (!units_ok(a) || !unit_rows(a.y, a.ld_y, e) || !unit_rows(a.n, a.ld_n, e)) {
-        k_block_norm<T><<<(unsigned)(a.rows < 148 * 8 ? a.rows : 148 * 8), THREADS, 0, s>>>(Args<T>{a});
-        return;
-    }
+    const bool vec = units_ok(a) && unit_rows(g.dy, g.ld_dy, e) && unit_rows(g.dn, g.ld_dn, e) && unit_rows(g.dx, g.ld_dx, e) &&
+                     unit_rows(g.dh, g.ld_dh, e) && unit_rows(g.dgate, a.width, e);
+    if (vec) backward_as<T, true>(a, g, s);
+    else backward_as<T, false>(a, g, s);
+}
+
+template <class T, bool UNITS>
+void forward_as(const wc_block_norm_args& a, cudaStream_t s) {
     // units of a row, whole blocks of 32 columns where it is packed
-    const int units = (int)(a.n_q ? (a.width + 31) / 32 * 4 : a.width / 8);
+    constexpr int WIDE = UNITS ? VEC : RUNS, NARROW = UNITS ? VEC : LANES;
+    const int units = (int)(a.n_q ? (a.width + 31) / 32 * 4 : (a.width + 7) / 8);
     if (units <= 64) {
-        int lanes = a.n_q ? 4 : 1;
+        int lanes = !a.n_q ? 1 : UNITS ? 4 : 32;
         while (lanes < 32 && lanes * 2 < units) lanes *= 2;
         const int64_t per = 256 / lanes;
         const unsigned n = (unsigned)std::min<int64_t>(148 * 16, (a.rows + per - 1) / per);
-        if (units <= lanes) k_norm_units<T, 0, 1><<<n, 256, 0, s>>>(a, lanes);
-        else k_norm_units<T, 0, 2><<<n, 256, 0, s>>>(a, lanes);
+        if (units <= lanes) k_norm_units<T, NARROW, 0, 1><<<n, 256, 0, s>>>(a, lanes);
+        else k_norm_units<T, NARROW, 0, 2><<<n, 256, 0, s>>>(a, lanes);
         return;
     }
-    // two units a thread
+    // two units a thread (one a thread was slower: 157 against 123 us at 16384 x 4096 in bf16)
     const int threads = (units + 63) / 64 * 32;
     const unsigned n = (unsigned)std::min<int64_t>(148 * std::max(1, 2048 / threads), a.rows);
-    if (threads <= 128) k_norm_units<T, 4, 2><<<n, threads, 0, s>>>(a, 32);
-    else if (threads <= 256) k_norm_units<T, 8, 2><<<n, threads, 0, s>>>(a, 32);
-    else if (threads <= 512) k_norm_units<T, 16, 2><<<n, threads, 0, s>>>(a, 32);
-    else k_norm_units<T, 32, 2><<<n, threads, 0, s>>>(a, 32);
+    if (threads <= 128) k_norm_units<T, WIDE, 4, 2><<<n, threads, 0, s>>>(a, 32);
+    else if (threads <= 256) k_norm_units<T, WIDE, 8, 2><<<n, threads, 0, s>>>(a, 32);
+    else if (threads <= 512) k_norm_units<T, WIDE, 16, 2><<<n, threads, 0, s>>>(a, 32);
+    else k_norm_units<T, WIDE, 32, 2><<<n, threads, 0, s>>>(a, 32);
+}
+template <class T>
+void forward(const wc_block_norm_args& a, cudaStream_t s) {
+    const size_t e = sizeof(T);
+    if (!a.rows) return;
+    if (units_ok(a) && unit_rows(a.y, a.ld_y, e) && unit_rows(a.n, a.ld_n, e)) forward_as<T, true>(a, s);
+    else forward_as<T, false>(a, s);
 }
 
 }  // namespace
 
-// for either path: which one the gradients' addresses decide
-uint64_t block_norm_workspace(const wc_block_norm_args& a) {
-    return std::max(Plan(a, true).floats(a), Plan(a, false).floats(a)) * sizeof(float) + 16;
-}
+uint64_t block_norm_workspace(const wc_block_norm_args& a) { return Plan(a).floats(a) * sizeof(float) + 16; }
 
 void launch_block_norm(const wc_block_norm_args& a, cudaStream_t s) {
     if (a.type == WC_F32) forward<float>(a, s);
