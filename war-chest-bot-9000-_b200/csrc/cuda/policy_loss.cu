@@ -12,12 +12,13 @@
 // entries that weigh have small x, or are many.)
 //
 // What bounds it is the bytes: each logit is read once and its gradient written
-// once. A row stays in registers as it was loaded (16 bytes of logits and their
-// legal bytes a chunk): a part of a warp for the narrowest rows, then a warp, a
-// CTA, and for long rows a cluster of CTAs, which exchange (m, S, sum) through
-// distributed shared memory. Rows that no cluster can hold, and rows whose
-// stride or address keeps 16-byte loads off them, are read twice by one CTA
-// (the second time mostly from L2).
+// once. Rows of up to 1024 entries (512 of 32 bits) stay in the registers of a
+// part of a warp; longer ones in the shared memory of a CTA, or of a cluster of
+// CTAs that exchange (m, S, sum) through distributed shared memory, until the
+// gradient is written. Entries are handled in chunks of 16 bytes; rows that
+// chunks do not fit have the chunks they lie in, or (short ones) entries one by
+// one, a warp's next to each other. Rows that no cluster can hold are read twice
+// by one CTA (the second time mostly from L2).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -187,42 +188,60 @@ __device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
         }
     return make_float2(s0 + s1, w0 + w1);
 }
-// The gradient of a chunk whose first entry is `at`
+// The gradient of a chunk, of which entry `hit` is the action
 template <class T, bool ENTROPY>
-__device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, T* out, int at, int act) {
+__device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, int hit, T* e) {
     float v[Chunk<T>::N];
 #pragma unroll
     for (int k = 0; k < Chunk<T>::N / 2; ++k) {
         const float2 z = q.pair(k);
         v[2 * k] = r.grad<ENTROPY>(z.x), v[2 * k + 1] = r.grad<ENTROPY>(z.y);
     }
-    if ((unsigned)(act - at) < (unsigned)Chunk<T>::N)
+    if ((unsigned)hit < (unsigned)Chunk<T>::N)
 #pragma unroll
         for (int k = 0; k < Chunk<T>::N; ++k)
-            if (at + k == act) v[k] += r.g;
-    alignas(16) T e[Chunk<T>::N];
+            if (k == hit) v[k] += r.g;
 #pragma unroll
     for (int k = 0; k < Chunk<T>::N; ++k) e[k] = from_f<T>(v[k]);
-    __stcs(reinterpret_cast<uint4*>(out + at), *reinterpret_cast<const uint4*>(e));
 }
-// A row's logits in registers: NV chunks, `step` entries apart
-template <class T, bool MASK, int NV>
-__device__ __forceinline__ void load_row(Chunk<T>* q, const T* z, const uint8_t* legal, bool read, int first, int step, int width) {
-    uint2 on[MASK ? NV : 1];
+template <class T>
+__device__ __forceinline__ void put_chunk(T* out, const T* e) {
+    __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(e));
+}
+// A row's logits in registers: NV chunks of `lanes` threads. VEC: 16 bytes at a time; else an entry at a time, chunk i's
+// k-th being the row's ((i N + k) lanes + at)-th.
+template <class T, bool MASK, bool VEC, int NV>
+__device__ __forceinline__ void load_row(Chunk<T>* q, const T* z, const uint8_t* legal, bool read, int at, int lanes, int width) {
+    constexpr int N = Chunk<T>::N;
+    if constexpr (VEC) {
+        uint2 on[MASK ? NV : 1];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int at = first + i * step;
-        if (read && at < width) {
-            q[i].load(z + at);
-            if constexpr (MASK) on[i] = Chunk<T>::load_legal(legal + at);
-        } else {
-            q[i].none();
-            if constexpr (MASK) on[i] = make_uint2(0, 0);
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * lanes + at) * N;
+            if (read && c < width) {
+                q[i].load(z + c);
+                if constexpr (MASK) on[i] = Chunk<T>::load_legal(legal + c);
+            } else {
+                q[i].none();
+                if constexpr (MASK) on[i] = make_uint2(0, 0);
+            }
+        }
+        if constexpr (MASK)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) q[i].mask(on[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            alignas(16) T e[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int c = (i * N + k) * lanes + at;
+                e[k] = from_f<T>(-INFINITY);
+                if (read && c < width && (!MASK || legal[c])) e[k] = z[c];
+            }
+            *reinterpret_cast<uint4*>(q[i].z) = *reinterpret_cast<const uint4*>(e);
         }
     }
-    if constexpr (MASK)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) q[i].mask(on[i]);
 }
 // Parts of a row (m, s, w: sums relative to the part's own maximum), up to 4 a lane, joined over the warp.
 template <int EACH>
@@ -248,9 +267,24 @@ __device__ __forceinline__ void join(const float4* parts, int n, float& M, float
     S = warp_sum(S), W = warp_sum(W);
 }
 
+template <bool VEC, class T>
+__device__ __forceinline__ void put(T* out, const T* e, int i, int at, int lanes, int width) {
+    constexpr int N = Chunk<T>::N;
+    if constexpr (VEC) {
+        const int c = (i * lanes + at) * N;
+        if (c < width) put_chunk(out + c, e);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int c = (i * N + k) * lanes + at;
+            if (c < width) out[c] = e[k];
+        }
+    }
+}
+
 // Rows of up to 32 NV chunks: `lanes` threads of a warp a row (a power of two).
-template <class T, bool MASK, bool ENTROPY, int NV>
-__global__ void __launch_bounds__(256, NV <= 4 ? 4 : 2) k_policy_warp(wc_policy_loss_args a, int lanes, double* part) {
+template <class T, bool MASK, bool ENTROPY, bool VEC, int NV>
+__global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss_args a, int lanes, double* part) {
     constexpr int N = Chunk<T>::N;
     __shared__ double s[8];
     const int lane = threadIdx.x & 31, at = lane & (lanes - 1), per = 256 / lanes, width = (int)a.width;
@@ -266,7 +300,7 @@ __global__ void __launch_bounds__(256, NV <= 4 ? 4 : 2) k_policy_warp(wc_policy_
         Chunk<T> q[NV];
         float za = -INFINITY;
         if (r.act >= 0 && (!MASK || legal[r.act])) za = to_f(z[r.act]);
-        load_row<T, MASK, NV>(q, z, legal, r.act >= 0, at * N, lanes * N, width);
+        load_row<T, MASK, VEC, NV>(q, z, legal, r.act >= 0, at, lanes, width);
         next = RowIn(a, t + stride);
         const bool live = za != -INFINITY;
         float m = local_max<T, NV>(q);
@@ -278,21 +312,23 @@ __global__ void __launch_bounds__(256, NV <= 4 ? 4 : 2) k_policy_warp(wc_policy_
         if (live) {
             const Row row(a, r, m, sw.x, sw.y, za);
             if (at == 0) row.put(a, t), total += (double)(r.w * row.loss);
-            if (out)
+            if (!out) continue;
+            // the action's place among this thread's entries
+            const int unit = VEC ? r.act / N : r.act, mine = (unit & (lanes - 1)) != at ? -1 : VEC ? unit / lanes * N + r.act % N : unit / lanes;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int c = (i * lanes + at) * N;
-                    if (c >= width) break;
-                    chunk_grad<T, ENTROPY>(q[i], row, out, c, r.act);
-                }
+            for (int i = 0; i < NV; ++i) {
+                alignas(16) T e[N];
+                chunk_grad<T, ENTROPY>(q[i], row, mine < 0 ? -1 : mine - i * N, e);
+                put<VEC>(out, e, i, at, lanes, width);
+            }
         } else {
             if (at == 0) put_void(a, t);
+            alignas(16) T e[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) e[k] = from_f<T>(0.0f);
             if (out)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int c = (i * lanes + at) * N;
-                    if (c < width) __stcs(reinterpret_cast<uint4*>(out + c), make_uint4(0, 0, 0, 0));
-                }
+                for (int i = 0; i < NV; ++i) put<VEC>(out, e, i, at, lanes, width);
         }
     }
 #pragma unroll
@@ -326,8 +362,9 @@ __device__ __forceinline__ uint32_t of_rank(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-template <class T, bool MASK, int NV, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_policy_loss_args a, int slice, double* part) {
+// FIT: every row starts and ends with a chunk (of the legal bytes: with 16).
+template <class T, bool MASK, bool FIT, int NV, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_policy_cluster(wc_policy_loss_args a, int slice, double* part) {
     constexpr int N = Chunk<T>::N, WARPS = THREADS / 32;
     extern __shared__ __align__(128) uint8_t ring[];  // SLICES of the logits, then of the legal bytes
     __shared__ float4 parts[3][CTAS * WARPS];         // of every warp of the cluster, three (live) rows in turn
@@ -336,8 +373,19 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int first = rank * slice, width = min(slice, max(0, (int)a.width - first));  // this CTA's entries
+    const int first = rank * slice;
     const int64_t t0 = blockIdx.x / CTAS, step = gridDim.x / CTAS;
+    // A row starts `before` entries into its first chunk, and its chunks are dealt to the CTAs: this one's are the entries
+    // from first - before on, `width` of them (of which the row's first and last chunk may have fewer). Bulk copies take
+    // whole chunks, with what lies there of the rows before and after; the matrix's first and last row, which have none,
+    // are read where they are if they do not fill theirs.
+    auto row_at = [&](int64_t t) { return static_cast<const T*>(a.logits) + t * a.ld_logits; };
+    auto before = [&](int64_t t) { return FIT ? 0 : (int)((reinterpret_cast<uintptr_t>(row_at(t)) & 15) / sizeof(T)); };
+    auto width_of = [&](int b) { return min(slice, max(0, (int)a.width + b - first)); };
+    auto in_place = [&](int64_t t) {
+        if (FIT || (t != 0 && t != a.rows - 1)) return false;
+        return before(t) != 0 || (a.width + before(t)) % N != 0 || (MASK && (((uintptr_t)(a.legal + t * a.ld_legal) & 15) != 0 || a.width % 16 != 0));
+    };
     uint8_t* masks = ring + SLICES * slice * sizeof(T);
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLICES; ++i) umma::mbar_init(&full[i], 1);
@@ -350,22 +398,56 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
     auto copy = [&](int64_t i, int act) {
         const int64_t t = t0 + i * step;
         if (t >= a.rows) return;
-        const int slot = (int)(i % SLICES);
-        if (act < 0 || !width) {
+        const int slot = (int)(i % SLICES), b = before(t), width = width_of(b);
+        if (act < 0 || !width || in_place(t)) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(&full[slot])) : "memory");
             return;
         }
-        umma::expect_tx(&full[slot], width * (sizeof(T) + (MASK ? 1 : 0)));
-        umma::bulk_g2s(ring + slot * slice * sizeof(T), static_cast<const T*>(a.logits) + t * a.ld_logits + first, width * sizeof(T), &full[slot]);
-        if (MASK) umma::bulk_g2s(masks + slot * slice, a.legal + t * a.ld_legal + first, width, &full[slot]);
+        const uint32_t bytes = (width + N - 1) / N * 16;
+        const uint8_t* on = MASK ? a.legal + t * a.ld_legal + max(0, first - b) : nullptr;
+        const uint32_t skew = (uint32_t)((uintptr_t)on & 15), on_bytes = MASK ? (skew + width - (first ? 0 : b) + 15) / 16 * 16 : 0;
+        umma::expect_tx(&full[slot], bytes + on_bytes);
+        umma::bulk_g2s(ring + slot * slice * sizeof(T), row_at(t) - b + first, bytes, &full[slot]);
+        if (MASK) umma::bulk_g2s(masks + slot * (slice + 32), on - skew, on_bytes, &full[slot]);
     };
-    auto chunk = [&](int slot, int at) {
+    // The chunk at `at` of the CTA's share of row t
+    auto chunk = [&](int64_t t, int slot, int b, int at) {
         Chunk<T> q;
+        const int col = first + at - b;
+        const bool whole = FIT || (col >= 0 && col + N <= a.width);
+        if (in_place(t)) {
+            alignas(16) T e[N];
+            for (int k = 0; k < N; ++k) {
+                e[k] = from_f<T>(-INFINITY);
+                if (col + k >= 0 && col + k < a.width && (!MASK || a.legal[t * a.ld_legal + col + k])) e[k] = row_at(t)[col + k];
+            }
+            *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(e);
+            return q;
+        }
         *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(ring + (slot * slice + at) * sizeof(T));
         if constexpr (MASK) {
-            const uint8_t* on = masks + slot * slice + at;
-            if constexpr (N == 8) q.mask(*reinterpret_cast<const uint2*>(on));
-            else q.mask(make_uint2(*reinterpret_cast<const uint32_t*>(on), 0));
+            // the bytes of the chunk's entries start anywhere
+            const uint8_t* on = a.legal + t * a.ld_legal + max(0, first - b);
+            const int from = (int)((uintptr_t)on & 15) + col - max(0, first - b);
+            const uint8_t* base = masks + slot * (slice + 32);
+            if (FIT) {
+                if constexpr (N == 8) q.mask(*reinterpret_cast<const uint2*>(base + at));
+                else q.mask(make_uint2(*reinterpret_cast<const uint32_t*>(base + at), 0));
+            } else if (whole) {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(base + (from & ~3));
+                const int by = 8 * (from & 3);
+                q.mask(make_uint2(__funnelshift_r(w[0], w[1], by), N == 8 ? __funnelshift_r(w[1], w[2], by) : 0u));
+            } else {
+                uint32_t m[2] = {0, 0};
+                for (int k = 0; k < N; ++k)
+                    if (col + k >= 0 && col + k < a.width) m[k >> 2] |= (uint32_t)base[from + k] << (8 * (k & 3));
+                q.mask(make_uint2(m[0], m[1]));
+            }
+        } else if (!whole) {
+            uint32_t m[2] = {0, 0};
+            for (int k = 0; k < N; ++k)
+                if (col + k >= 0 && col + k < a.width) m[k >> 2] |= 1u << (8 * (k & 3));
+            q.mask(make_uint2(m[0], m[1]));
         }
         return q;
     };
@@ -390,10 +472,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
         if (t1 < a.rows && !bad && !umma::mbar_wait(&full[slot1], (uint32_t)((i + 1) / SLICES) & 1)) bad = true;
         if (live1) {
             Chunk<T> q[NV];
+            const int b = before(t1), width = width_of(b);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
                 const int at = (k * THREADS + (int)threadIdx.x) * N;
-                if (at < width) q[k] = chunk(slot1, at);
+                if (at < width) q[k] = chunk(t1, slot1, b, at);
                 else q[k].none();
             }
             float m = local_max<T, NV>(q);
@@ -414,19 +497,33 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_policy_cluster(wc_p
         __syncthreads();  // rows[] of row i is there, and the slice of row i - 1 has been read by all
         if (threadIdx.x == 0 && i >= 0 && !bad) copy(i + 2, in2.act);
         if (t >= 0 && i >= 0 && a.dlogits) {
-            T* out = static_cast<T*>(a.dlogits) + t * a.ld_dlogits + first;
+            T* out = static_cast<T*>(a.dlogits) + t * a.ld_dlogits;
             const Row& r = rows[turn1 ^ 1];
-            const int slot = (int)(i % SLICES), act = act0 - first;
+            const int slot = (int)(i % SLICES), b = before(t), width = width_of(b);
+            // the gradient's chunks are the logits' if they start at the same place of 16 bytes
+            const bool same = FIT || (reinterpret_cast<uintptr_t>(out) & 15) == b * sizeof(T);
+            auto write = [&](int at, const T* e) {
+                const int col = first + at - b;
+                if (FIT || (same && col >= 0 && col + N <= a.width)) put_chunk(out + col, e);
+                else
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        if (col + k >= 0 && col + k < a.width) out[col + k] = e[k];
+            };
+            alignas(16) T e[N];
             if (live0 && r.ce != 0.0f) {
-                for (int at = threadIdx.x * N; at < width; at += THREADS * N) chunk_grad<T, true>(chunk(slot, at), r, out, at, act);
+                for (int at = threadIdx.x * N; at < width; at += THREADS * N)
+                    chunk_grad<T, true>(chunk(t, slot, b, at), r, act0 - (first + at - b), e), write(at, e);
             } else if (live0) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     const int at = (k * THREADS + (int)threadIdx.x) * N;
-                    if (at < width) chunk_grad<T, false>(chunk(slot, at), r, out, at, act);
+                    if (at < width) chunk_grad<T, false>(chunk(t, slot, b, at), r, act0 - (first + at - b), e), write(at, e);
                 }
             } else {
-                for (int at = threadIdx.x * N; at < width; at += THREADS * N) __stcs(reinterpret_cast<uint4*>(out + at), make_uint4(0, 0, 0, 0));
+#pragma unroll
+                for (int k = 0; k < N; ++k) e[k] = from_f<T>(0.0f);
+                for (int at = threadIdx.x * N; at < width; at += THREADS * N) write(at, e);
             }
         }
         if (CTAS == 1) __syncthreads();
@@ -526,15 +623,16 @@ __global__ void k_policy_total(const double* part, int n, float* loss) {
     if (threadIdx.x == 0) *loss = (float)v;
 }
 
-constexpr int MOST_CTAS = 148 * 12;
+constexpr int MOST_CTAS = 148 * 8;
 
-template <class T, bool MASK, int THREADS, int CTAS>
+template <class T, bool MASK, bool FIT, int THREADS, int CTAS>
 int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    // slices of whole chunks, and of 16 entries so that the legal bytes' are of 16 bytes
-    const int slice = (int)(((a.width + CTAS - 1) / CTAS + 15) / 16 * 16);
-    const size_t smem = SLICES * slice * (sizeof(T) + (MASK ? 1 : 0));
-    const auto kernel = k_policy_cluster<T, MASK, 4, THREADS, CTAS>;
-    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(kernel), SLICES * THREADS * 4 * Chunk<T>::N * (sizeof(T) + 1))) return 0;
+    // slices of whole chunks of a row that may start up to N - 1 entries into its first; legal bytes with room for the 16s
+    // that they start and end in
+    const int slice = (int)(((a.width + (FIT ? 0 : Chunk<T>::N - 1) + CTAS - 1) / CTAS + 15) / 16 * 16);
+    const size_t smem = SLICES * (slice * sizeof(T) + (MASK ? slice + 32 : 0));
+    const auto kernel = k_policy_cluster<T, MASK, FIT, 4, THREADS, CTAS>;
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(kernel), SLICES * (THREADS * 4 * Chunk<T>::N * (sizeof(T) + 1) + 64))) return 0;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -542,9 +640,10 @@ int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     cfg.blockDim = THREADS, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1, cfg.dynamicSmemBytes = smem;
     // As many clusters as are resident at a time: they do not fill the SMs of every GPC, and the ones left over would
     // start only when the others have ended (37 of 8 CTAs, of which 32 fit, took 2.1 times as long).
-    cfg.gridDim = CTAS * 1024 / THREADS;
+    constexpr int SM = (FIT ? 1024 : 512) / THREADS;  // CTAs of one
+    cfg.gridDim = CTAS * SM;
     int most = 0;
-    if (CTAS == 1) most = 148 * 1024 / THREADS;
+    if (CTAS == 1) most = 148 * SM;
     else if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) most = 1;
     const int n = (int)std::min<int64_t>(most, a.rows);
     cfg.gridDim = n * CTAS;
@@ -552,52 +651,56 @@ int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     return n;
 }
 
-template <class T, bool MASK, bool ENTROPY>
+template <class T, bool MASK, bool ENTROPY, bool VEC>
 int launch_warp(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    const int64_t chunks = a.width / Chunk<T>::N;
-    // up to 8 chunks a lane of a 16-bit type (4 of 32 bits): the more rows a warp has, the less their scalars cost
-    constexpr int MOST = sizeof(T) == 2 ? 8 : 4;
+    const int64_t chunks = (a.width + Chunk<T>::N - 1) / Chunk<T>::N;
+    // up to 4 chunks a lane (8 a lane and half the warps took 106 against 98 us at 131072 x 512 in bf16)
     int lanes = 1;
-    while (lanes < 32 && lanes * MOST < chunks) lanes *= 2;
+    while (lanes < 32 && lanes * 4 < chunks) lanes *= 2;
     const int64_t per = 256 / lanes;
-    const int n = (int)std::min<int64_t>(148 * 12, (a.rows + per - 1) / per);
+    const int n = (int)std::min<int64_t>(MOST_CTAS, (a.rows + per - 1) / per);
     const int nv = (int)((chunks + lanes - 1) / lanes);
-    if (nv <= 1) k_policy_warp<T, MASK, ENTROPY, 1><<<n, 256, 0, s>>>(a, lanes, part);
-    else if (nv == 2) k_policy_warp<T, MASK, ENTROPY, 2><<<n, 256, 0, s>>>(a, lanes, part);
-    else if (nv <= 4) k_policy_warp<T, MASK, ENTROPY, 4><<<n, 256, 0, s>>>(a, lanes, part);
-    else if (nv <= 6) k_policy_warp<T, MASK, ENTROPY, MOST == 8 ? 6 : 4><<<n, 256, 0, s>>>(a, lanes, part);
-    else k_policy_warp<T, MASK, ENTROPY, MOST><<<n, 256, 0, s>>>(a, lanes, part);
+    if (nv <= 1) k_policy_warp<T, MASK, ENTROPY, VEC, 1><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv == 2) k_policy_warp<T, MASK, ENTROPY, VEC, 2><<<n, 256, 0, s>>>(a, lanes, part);
+    else if (nv == 3) k_policy_warp<T, MASK, ENTROPY, VEC, 3><<<n, 256, 0, s>>>(a, lanes, part);
+    else k_policy_warp<T, MASK, ENTROPY, VEC, 4><<<n, 256, 0, s>>>(a, lanes, part);
     return n;
 }
 
 template <class T, bool MASK>
-int launch_vec(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
+int launch_rows(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     constexpr int N = Chunk<T>::N;
-    const int64_t chunks = a.width / N;
-    if (chunks <= 32 * 4) return a.entropy_coef != 0.0f ? launch_warp<T, MASK, true>(a, part, s) : launch_warp<T, MASK, false>(a, part, s);
+    const auto fits = [&](const void* p, int64_t ld, size_t e, int to) { return ((uintptr_t)p & (to - 1)) == 0 && (ld * e) % to == 0; };
+    const int64_t chunks = (a.width + N - 1) / N;
+    const bool is_short = chunks <= 32 * 4;
+    const bool fit = a.width % N == 0 && fits(a.logits, a.ld_logits, sizeof(T), 16) && (!a.dlogits || fits(a.dlogits, a.ld_dlogits, sizeof(T), 16)) &&
+                     (!a.legal || (is_short ? fits(a.legal, a.ld_legal, 1, 8) : a.width % 16 == 0 && fits(a.legal, a.ld_legal, 1, 16)));
+    if (is_short) {
+        if (a.entropy_coef != 0.0f) return fit ? launch_warp<T, MASK, true, true>(a, part, s) : launch_warp<T, MASK, true, false>(a, part, s);
+        return fit ? launch_warp<T, MASK, false, true>(a, part, s) : launch_warp<T, MASK, false, false>(a, part, s);
+    }
     // 4 chunks a thread, up to 8 CTAs a row
-    if (chunks <= 128 * 4) return launch_cluster<T, MASK, 128, 1>(a, part, s);
-    if (chunks <= 512 * 4) return launch_cluster<T, MASK, 512, 1>(a, part, s);
-    if (chunks <= 512 * 8) return launch_cluster<T, MASK, 512, 2>(a, part, s);
-    if (chunks <= 512 * 16) return launch_cluster<T, MASK, 512, 4>(a, part, s);
-    return launch_cluster<T, MASK, 512, 8>(a, part, s);
+    const auto slice = [&](int ctas) { return ((a.width + (fit ? 0 : N - 1) + ctas - 1) / ctas + 15) / 16 * 16; };
+    const int64_t most = 512 * 4 * N;
+    if (fit) {
+        if (slice(1) <= most / 4) return launch_cluster<T, MASK, true, 128, 1>(a, part, s);
+        if (slice(1) <= most) return launch_cluster<T, MASK, true, 512, 1>(a, part, s);
+        if (slice(2) <= most) return launch_cluster<T, MASK, true, 512, 2>(a, part, s);
+        if (slice(4) <= most) return launch_cluster<T, MASK, true, 512, 4>(a, part, s);
+        if (slice(8) <= most) return launch_cluster<T, MASK, true, 512, 8>(a, part, s);
+    } else {
+        if (slice(1) <= most / 4) return launch_cluster<T, MASK, false, 128, 1>(a, part, s);
+        if (slice(1) <= most) return launch_cluster<T, MASK, false, 512, 1>(a, part, s);
+        if (slice(8) <= most) return launch_cluster<T, MASK, false, 512, 8>(a, part, s);
+    }
+    const int n = (int)std::min<int64_t>(148 * 4, a.rows);
+    k_policy_long<T><<<n, 512, 0, s>>>(a, part);
+    return n;
 }
 
 template <class T>
 int launch_type(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    constexpr int N = 16 / sizeof(T);
-    const auto fits = [&](const void* p, int64_t ld, size_t e) { return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0; };
-    const bool vec = a.width % N == 0 && fits(a.logits, a.ld_logits, sizeof(T)) &&
-                     (!a.dlogits || fits(a.dlogits, a.ld_dlogits, sizeof(T)));
-    // short rows load 4 or 8 legal bytes at a time, slices of longer ones come in 16s
-    const bool is_short = a.width / N <= 32 * 4;
-    const bool mask = !a.legal || (is_short ? ((uintptr_t)a.legal & 7) == 0 && a.ld_legal % 8 == 0
-                                            : a.width % 16 == 0 && fits(a.legal, a.ld_legal, 1));
-    if (vec && mask && a.width / N <= 8 * 512 * 4)
-        return a.legal ? launch_vec<T, true>(a, part, s) : launch_vec<T, false>(a, part, s);
-    const int n = (int)std::min<int64_t>(148 * 4, a.rows);
-    k_policy_long<T><<<n, 512, 0, s>>>(a, part);
-    return n;
+    return a.legal ? launch_rows<T, true>(a, part, s) : launch_rows<T, false>(a, part, s);
 }
 
 }  // namespace
