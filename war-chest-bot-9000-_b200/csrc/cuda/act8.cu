@@ -2,11 +2,13 @@
 // unit (train.cuh act8_code), so a stored value is a whole number times that
 // unit and is exact in bf16.
 //
-// All of these are bound by the bytes they move. A thread holds 8 consecutive
-// values (16 bytes of a 16-bit type in one load, 8 bytes of q in one store)
-// and 4 threads a block: the largest magnitude takes two shuffles. Magnitudes
-// are compared as integers, where NaN is above infinity above the rest, so
-// either shows in the block's code.
+// All of these are bound by the bytes they move. Where addresses and strides
+// allow, a thread holds 8 consecutive values (16 bytes of a 16-bit type in one
+// load, 8 bytes of q in one store) and 4 threads a block: the largest magnitude
+// takes two shuffles. Elsewhere a warp holds a block, one value a thread, so
+// that its loads and stores are still next to each other.
+#include <algorithm>
+
 #include "colsum.cuh"
 
 namespace wctrain {
@@ -15,37 +17,24 @@ namespace {
 
 constexpr int THREADS = 256;
 
-// 8 values of a row from column c on; past the width they are 0
-template <class T, bool VEC>
+// 8 values of a row from column c on; those past the width (a whole number of 8s) are 0
+template <class T>
 __device__ __forceinline__ void load8(const T* p, int64_t c, int64_t width, float* v) {
-    if (VEC && c + 8 <= width) {
-        alignas(16) T e[8];
-        if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p + c);
-        } else {
-            *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p + c);
-            *reinterpret_cast<uint4*>(e + 4) = *reinterpret_cast<const uint4*>(p + c + 4);
-        }
+    alignas(16) T e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
-    } else {
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4*>(e)[i] = c < width ? __ldcs(reinterpret_cast<const uint4*>(p + c) + i) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < width ? to_f(p[c + i]) : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
 }
-template <class T, bool VEC>
+template <class T>
 __device__ __forceinline__ void store8(T* p, int64_t c, int64_t width, const float* v) {
-    if (VEC && c + 8 <= width) {
-        alignas(16) T e[8];
+    if (c >= width) return;
+    alignas(16) T e[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
-        *reinterpret_cast<uint4*>(p + c) = *reinterpret_cast<const uint4*>(e);
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p + c + 4) = *reinterpret_cast<const uint4*>(e + 4);
-    } else {
+    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (c + i < width) p[c + i] = from_f<T>(v[i]);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p + c) + i, reinterpret_cast<const uint4*>(e)[i]);
 }
 
 __device__ __forceinline__ void dequantise8(uint2 q, uint32_t code, float* v) {
@@ -56,7 +45,7 @@ __device__ __forceinline__ void dequantise8(uint2 q, uint32_t code, float* v) {
 
 enum { PACK, UNPACK, GELU };
 
-template <class T, bool VEC, int WHAT>
+template <class T, int WHAT>
 __global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, uint32_t chunks, uint32_t total) {
     const uint32_t i = blockIdx.x * THREADS + threadIdx.x;
     const bool in = i < total;  // total is a multiple of 4: a block's threads are in or out together
@@ -66,21 +55,18 @@ __global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, uint32_t chunk
     if constexpr (WHAT == UNPACK) {
         if (!in) return;
         dequantise8(reinterpret_cast<const uint2*>(a.q)[i], a.scale[i >> 2], v);
-        store8<T, VEC>(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, v);
+        store8(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, v);
     } else {
-        if (in) load8<T, VEC>(static_cast<const T*>(a.x) + row * a.ld_x, c, a.width, v);
-        else
-            for (float& x : v) x = 0.0f;
+        load8(static_cast<const T*>(a.x) + row * a.ld_x, in ? c : a.width, a.width, v);
         if constexpr (WHAT == GELU) {
-            if (a.bias && in)
+            if (in && c < a.width) {
+                if (a.bias)
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (c + k < a.width) v[k] += a.bias[c + k];
-            if (in) {
+                    for (int k = 0; k < 8; ++k) v[k] += a.bias[c + k];
                 float y[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) y[k] = gelu(v[k]);
-                store8<T, VEC>(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, y);
+                store8(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, y);
             }
         }
         uint32_t code;
@@ -92,27 +78,82 @@ __global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, uint32_t chunk
     }
 }
 
+// The same, a warp a run of 4 blocks of a row.
+template <class T, int WHAT>
+__global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, uint32_t blocks, uint32_t runs, uint32_t total) {
+    const uint32_t i = (blockIdx.x * THREADS + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+    if (i >= total) return;
+    const int64_t row = i / runs;
+    const uint32_t first = (i - (uint32_t)row * runs) * 4;
+    float v[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t c = (int64_t)(first + k) * 32 + lane;
+        v[k] = 0.0f;
+        if (WHAT != UNPACK && c < a.width) v[k] = to_f(static_cast<const T*>(a.x)[row * a.ld_x + c]);
+        if (WHAT == UNPACK && first + k < blocks) {
+            const int64_t b = row * blocks + first + k;
+            v[k] = (float)a.q[b * 32 + lane] * act8_unit(a.scale[b]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int64_t c = (int64_t)(first + k) * 32 + lane, b = row * blocks + first + k;
+        if (first + k >= blocks) break;
+        if (WHAT == UNPACK) {
+            if (c < a.width) static_cast<T*>(a.out)[row * a.ld_out + c] = from_f<T>(v[k]);
+            continue;
+        }
+        if (WHAT == GELU && c < a.width) {
+            if (a.bias) v[k] += a.bias[c];
+            static_cast<T*>(a.out)[row * a.ld_out + c] = from_f<T>(gelu(v[k]));
+        }
+        const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu)));
+        a.q[b * 32 + lane] = code == 255 ? (int8_t)0 : (int8_t)__float2int_rn(v[k] * act8_inverse(code));
+        if (lane == 0) a.scale[b] = (uint8_t)code;
+    }
+}
+
 // dz = da GELU'(z8). The CTA's threads keep their columns and walk down the
 // rows [blockIdx.y * chunk_rows, ...): `lanes` threads a row, each 8 columns.
-template <class T, bool VEC>
-__global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int chunks, int lanes, int64_t chunk_rows,
-                                                            float* part) {
+// UNITS: consecutive ones. Else `lanes` is a number of warps times 32, and a
+// warp has 256 columns, thread by thread next to each other.
+template <class T, bool UNITS>
+__global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int blocks, int lanes, int64_t chunk_rows, float* part) {
     __shared__ float s[THREADS][9];
     const int per = THREADS / lanes, r = threadIdx.x / lanes, at = blockIdx.x * lanes + threadIdx.x % lanes;
-    const bool in = r < per && at < chunks;
-    const int64_t c = (int64_t)at * 8, first = blockIdx.y * chunk_rows, last = min(first + chunk_rows, a.rows);
+    const int step = UNITS ? 1 : 32, c = UNITS ? at * 8 : (at & ~31) * 8 + (at & 31);
+    const bool in = r < per && c < a.width;
+    const int64_t first = blockIdx.y * chunk_rows, last = min(first + chunk_rows, a.rows);
     float acc[8] = {};
     if (in)
         for (int64_t t = first + r; t < last; t += per) {
+            const T* x = static_cast<const T*>(a.x) + t * a.ld_x;
+            T* out = static_cast<T*>(a.out) + t * a.ld_out;
             float d[8], z[8];
-            load8<T, VEC>(static_cast<const T*>(a.x) + t * a.ld_x, c, a.width, d);
-            dequantise8(reinterpret_cast<const uint2*>(a.q)[t * chunks + at], a.scale[(t * chunks + at) >> 2], z);
+            if constexpr (UNITS) {
+                load8(x, c, a.width, d);
+                dequantise8(*reinterpret_cast<const uint2*>(a.q + t * blocks * 32 + c), a.scale[t * blocks + c / 32], z);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const bool here = c + k * 32 < a.width;
+                    d[k] = here ? to_f(x[c + k * 32]) : 0.0f;
+                    z[k] = here ? (float)a.q[t * blocks * 32 + c + k * 32] * act8_unit(a.scale[t * blocks + c / 32 + k]) : 0.0f;
+                }
+            }
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 d[k] *= gelu_slope(z[k]);
                 acc[k] += d[k];
             }
-            store8<T, VEC>(static_cast<T*>(a.out) + t * a.ld_out, c, a.width, d);
+            if constexpr (UNITS) {
+                store8(out, c, a.width, d);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k * 32 < a.width) out[c + k * 32] = from_f<T>(d[k]);
+            }
         }
     if (!part) return;
 #pragma unroll
@@ -123,7 +164,7 @@ __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int 
         for (int k = 0; k < 8; ++k) {
             float v = acc[k];
             for (int j = 1; j < per; ++j) v += s[threadIdx.x + j * lanes][k];
-            if (c + k < a.width) part[blockIdx.y * a.width + c + k] = v;
+            if (c + k * step < a.width) part[blockIdx.y * a.width + c + k * step] = v;
         }
 }
 
@@ -140,11 +181,15 @@ void launch_as(const wc_act8_args& a, cudaStream_t s) {
         if (a.x) b.x = static_cast<const T*>(a.x) + t * a.ld_x;
         if (a.out) b.out = static_cast<T*>(a.out) + t * a.ld_out;
         b.q += t * chunks * 8, b.scale += t * chunks / 4;
-        const uint32_t total = (uint32_t)(b.rows * chunks), n = (total + THREADS - 1) / THREADS;
-        const bool vec = (WHAT == UNPACK || aligned(b.x, a.ld_x, sizeof(T))) &&
-                         (WHAT == PACK || aligned(b.out, a.ld_out, sizeof(T)));
-        if (vec) k_act8<T, true, WHAT><<<n, THREADS, 0, s>>>(b, (uint32_t)chunks, total);
-        else k_act8<T, false, WHAT><<<n, THREADS, 0, s>>>(b, (uint32_t)chunks, total);
+        const bool units = a.width % 8 == 0 && (WHAT == UNPACK || aligned(b.x, a.ld_x, sizeof(T))) &&
+                           (WHAT == PACK || aligned(b.out, a.ld_out, sizeof(T)));
+        if (units) {
+            const uint32_t total = (uint32_t)(b.rows * chunks);
+            k_act8<T, WHAT><<<(total + THREADS - 1) / THREADS, THREADS, 0, s>>>(b, (uint32_t)chunks, total);
+        } else {
+            const uint32_t runs = (uint32_t)(chunks + 15) / 16, total = (uint32_t)(b.rows * runs);
+            k_act8_runs<T, WHAT><<<(unsigned)((total + 7ull) / 8), THREADS, 0, s>>>(b, (uint32_t)(chunks / 4), runs, total);
+        }
     }
 }
 template <int WHAT>
@@ -155,12 +200,13 @@ void launch_type(const wc_act8_args& a, cudaStream_t s) {
 }
 
 struct Shape {
-    int chunks, tiles, lanes, splits;
+    int blocks, tiles, lanes, splits;
     int64_t chunk_rows;
-    Shape(int64_t rows, int64_t width) {
-        chunks = (int)((width + 31) / 32 * 4);
-        tiles = (chunks + THREADS - 1) / THREADS;
-        lanes = (chunks + tiles - 1) / tiles;
+    Shape(int64_t rows, int64_t width, bool units) {
+        blocks = (int)((width + 31) / 32);
+        const int threads = units ? (int)(width / 8) : (int)((width + 255) / 256 * 32), whole = units ? 1 : 32;
+        tiles = (threads + THREADS - 1) / THREADS;
+        lanes = (threads / whole + tiles - 1) / tiles * whole;
         const int per = THREADS / lanes;
         const int64_t want = (148 * 8 + tiles - 1) / tiles, most = (rows + 2 * per - 1) / (2 * per);
         splits = (int)(most < 1 ? 1 : most < want ? most : want);
@@ -170,12 +216,12 @@ struct Shape {
 
 template <class T>
 void launch_backward(const wc_act8_args& a, cudaStream_t s) {
-    const Shape g(a.rows, a.width);
+    const bool units = a.width % 8 == 0 && aligned(a.x, a.ld_x, sizeof(T)) && aligned(a.out, a.ld_out, sizeof(T));
+    const Shape g(a.rows, a.width, units);
     float* part = a.dbias ? static_cast<float*>(a.workspace) : nullptr;
-    const bool vec = aligned(a.x, a.ld_x, sizeof(T)) && aligned(a.out, a.ld_out, sizeof(T));
     const dim3 grid(g.tiles, g.splits);
-    if (vec) k_gelu8_backward<T, true><<<grid, THREADS, 0, s>>>(a, g.chunks, g.lanes, g.chunk_rows, part);
-    else k_gelu8_backward<T, false><<<grid, THREADS, 0, s>>>(a, g.chunks, g.lanes, g.chunk_rows, part);
+    if (units) k_gelu8_backward<T, true><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
+    else k_gelu8_backward<T, false><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
     if (part) launch_colsum<float>(part, g.splits, a.width, a.width, a.dbias, s);
 }
 
@@ -185,7 +231,10 @@ void launch_act8_pack(const wc_act8_args& a, cudaStream_t s) { launch_type<PACK>
 void launch_act8_unpack(const wc_act8_args& a, cudaStream_t s) { launch_type<UNPACK>(a, s); }
 void launch_gelu8(const wc_act8_args& a, cudaStream_t s) { launch_type<GELU>(a, s); }
 uint64_t gelu8_workspace(int64_t rows, int64_t width) {
-    return width ? (uint64_t)Shape(rows, width).splits * width * sizeof(float) : 0;
+    if (!width) return 0;
+    const Shape one(rows, width, false);
+    const int splits = width % 8 ? one.splits : std::max(one.splits, Shape(rows, width, true).splits);
+    return (uint64_t)splits * width * sizeof(float);
 }
 void launch_gelu8_backward(const wc_act8_args& a, cudaStream_t s) {
     if (a.type == WC_F32) launch_backward<float>(a, s);

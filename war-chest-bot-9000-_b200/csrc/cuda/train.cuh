@@ -80,23 +80,28 @@ __device__ __forceinline__ uint2 quantise8(const float* v, uint32_t* code) {
     return r;
 }
 
-// GELU (tanh form) as x / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3):
-// no cancellation for negative x. The exponent is held below 126 so that the
-// divisor stays finite.
-__device__ __forceinline__ float gelu(float x) {
-    const float u = x * fmaf(0.044715f * 0.7978845608f, x * x, 0.7978845608f);
-    const float e = exp2f(fminf(-2.8853900817779268f * u, 126.0f));
-    return x / (1.0f + e);
+// 1 / (1 + exp(-2u)), u = sqrt(2/pi) (x + 0.044715 x^3): GELU (tanh form) is x times it, with no cancellation for
+// negative x. The hardware's power and reciprocal are good to a few 2^-23. Where the power overflows the reciprocal is 0.
+__device__ __forceinline__ float gelu_gate(float x2, float x, float* e) {
+    const float u = x * fmaf(0.044715f * 0.7978845608f, x2, 0.7978845608f);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(*e) : "f"(-2.8853900817779268f * u));
+    float s;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + *e));
+    return s;
 }
-// Its derivative: s + 2 x s (1 - s) u'(x) with s = 1 / (1 + exp(-2u)); 1 - s
-// is e s, again without cancellation.
+// (x = -inf has u = -inf and a gate of 0: GELU there is its limit 0, not -inf 0)
+__device__ __forceinline__ float gelu(float x) {
+    float e;
+    const float s = gelu_gate(x * x, x, &e);
+    return s == 0.0f ? s * 0.0f : x * s;
+}
+// Its derivative s + 2 x s (1 - s) u'(x); 1 - s is e s, again without cancellation. Beyond |x| = 10 it is 0 or 1 in 32
+// bits, and the products of what grows with what vanishes are left out.
 __device__ __forceinline__ float gelu_slope(float x) {
     const float x2 = x * x;
-    const float u = x * fmaf(0.044715f * 0.7978845608f, x2, 0.7978845608f);
-    const float du = fmaf(3.0f * 0.044715f * 0.7978845608f, x2, 0.7978845608f);
-    const float e = exp2f(fminf(-2.8853900817779268f * u, 60.0f));
-    const float s = 1.0f / (1.0f + e);
-    return s + 2.0f * x * du * (e * s) * s;
+    float e;
+    const float s = gelu_gate(x2, x, &e), du = fmaf(3.0f * 0.044715f * 0.7978845608f, x2, 0.7978845608f);
+    return fabsf(x) > 10.0f ? s : fmaf(2.0f * x * du, (e * s) * s, s);
 }
 
 }  // namespace wctrain
