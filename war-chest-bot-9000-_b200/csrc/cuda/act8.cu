@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, uint32_t 
             static_cast<T*>(a.out)[row * a.ld_out + c] = from_f<T>(gelu(v[k]));
         }
         const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu)));
-        a.q[b * 32 + lane] = code == 255 ? (int8_t)0 : (int8_t)__float2int_rn(v[k] * act8_inverse(code));
+        a.q[b * 32 + lane] = act8_whole(v[k], code);
         if (lane == 0) a.scale[b] = (uint8_t)code;
     }
 }

@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS 
                         const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(~0u, __float_as_uint(v[i][k]) & 0x7fffffffu)));
                         const int c = cols.col(i, k);
                         if (in && c < blocks * 32) {
-                            a.n_q[t * blocks * 32 + c] = code == 255 ? (int8_t)0 : (int8_t)__float2int_rn(v[i][k] * act8_inverse(code));
+                            a.n_q[t * blocks * 32 + c] = act8_whole(v[i][k], code);
                             if ((c & 31) == 0) a.n_scale[t * blocks + c / 32] = (uint8_t)code;
                         }
                     }

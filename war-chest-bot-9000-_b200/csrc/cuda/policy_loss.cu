@@ -6,10 +6,13 @@
 // The row's loss depends on the logits through l and H only, so
 //   dloss/dz_j = g (delta_ja - p_j) + w c p_j (ln p_j + H),
 //   g = w (-ratio A [not clipped] - kl_coef (exp(r - l) - 1)).
-// A power is 2^x with x = z log2 e - c in one rounding, c = m log2 e rounded; the
-// factor that the rounding of c puts on every power is taken out of ln S again.
-// (The rounding of x, at most 2^-25 |x|, moves S by at most about 4e-8: the
-// entries that weigh have small x, or are many.)
+// A power is 2^x with x = z log2 e - c in one rounding, c = m log2 e rounded. The
+// maximum's own x is what c was rounded by: S is divided by its power, which takes
+// the rounding out again and, with it, the error of the hardware's power there (one
+// entry left of a row has l = 0 and H = 0 exactly). The rounding of x, at most
+// 2^-25 |x|, moves S by at most about 4e-8: the entries that weigh have small x, or
+// are many. Where m log2 e would overflow (a row of nothing but the type's lowest
+// value) x is z - m: such logits are equal or too far apart for a power to show.
 //
 // What bounds it is the bytes: each logit is read once and its gradient written
 // once. Rows of up to 1024 entries (512 of 32 bits) stay in the registers of a
@@ -50,8 +53,14 @@ __device__ __forceinline__ float above(float x) {
     return y;
 }
 
-// c of a maximum, the same number wherever it is formed (a product fused into a sum would not be rounded)
-__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, LOG2E); }
+// The factor of the logits, and c of a maximum: the same number wherever it is formed (a product fused into a sum would
+// not be rounded)
+__device__ __forceinline__ float factor(float m) { return fabsf(m) < 2e38f ? LOG2E : 1.0f; }
+__device__ __forceinline__ float scaled(float m) { return __fmul_rn(m, factor(m)); }
+// what sums from the maximum m on lack to those from `top` on, as a power of 2
+__device__ __forceinline__ float shift(float m, float top) {
+    return m == -INFINITY ? 0.0f : above(__fmul_rn(m, factor(top)) - scaled(top));
+}
 
 // What a row needs besides its logits: loaded a row ahead, since the logits' loads wait for it (a row that is void
 // reads none)
@@ -75,20 +84,20 @@ struct RowIn {
 // add to them is not.
 struct Row {
     float loss, l, H, kl;   // results
-    float c, g, e, k;       // gradient: d = 2^x (e x + k) + [action] g
+    float c, f, g, e, k;    // gradient: d = 2^x (e x + k) + [action] g, x = z f - c
     float ce;
     Row() = default;
-    __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float m, float S, float W, float za) : c(scaled(m)) {
-        const float mean = W / S;  // of x
-        const float off = fmaf(m, LOG2E, -c) * LN2;
-        // ln S from S = 2^n f, f about 1; LOG2E as a float is 1.34e-8 (relative) low, which mean puts right to first order
+    __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float m, float S, float W, float za) : c(scaled(m)), f(factor(m)) {
+        const float top = fmaf(m, f, -c), eTop = ex2(top);  // x and the power of the maximum
+        const float mean = S == eTop ? 0.0f : W / S - top;  // of x, from the maximum's on
+        // ln of S / eTop = 2^n q, q about 1; LOG2E as a float is 1.34e-8 (relative) low, which mean puts right to first order
         int n;
-        float f = frexpf(S, &n);
-        if (f < 0.75f) f *= 2.0f, --n;
-        const double lnS = (double)n * 0.6931471805599453 + (double)(fmaf(mean, 9.25e-9f, logf(f)) - off);
+        float q = frexpf(S / eTop, &n);
+        if (q < 0.75f) q *= 2.0f, --n;
+        const double lnS = (double)n * 0.6931471805599453 + (double)fmaf(mean, 9.25e-9f, logf(q));
         const double ld = ((double)za - (double)m) - lnS;
         l = (float)ld;
-        H = (float)lnS + (off - mean * LN2);
+        H = fmaf(mean, -LN2, (float)lnS);
         const float lo = 1.0f - a.clip_low, hi = 1.0f + a.clip_high, A = in.A;
         const float ratio = expf((float)(ld - (double)in.old));
         const float free = ratio * A, clipped = fminf(fmaxf(ratio, lo), hi) * A;
@@ -99,9 +108,9 @@ struct Row {
         const float up = (a.upstream ? *a.upstream : 1.0f) * in.w;
         g = up * ((held ? 0.0f : -free) - a.kl_coef * em);
         ce = up * a.entropy_coef;
-        // p = 2^x / S and ln p = x ln 2 - ln S - off
+        // p = 2^x / S and ln p = (x - top) ln 2 - ln (S / eTop)
         const float inv = 1.0f / S;
-        e = ce * LN2 * inv, k = fmaf(ce, H - (float)lnS - off, -g) * inv;
+        e = ce * LN2 * inv, k = fmaf(ce, -LN2 * (mean + top), -g) * inv;
     }
     __device__ __forceinline__ void put(const wc_policy_loss_args& a, int64_t t) const {
         a.row_out[t] = loss, a.row_out[a.rows + t] = l, a.row_out[2 * a.rows + t] = H, a.row_out[3 * a.rows + t] = kl;
@@ -110,7 +119,7 @@ struct Row {
     // x is a factor)
     template <bool ENTROPY>
     __device__ __forceinline__ float grad(float z) const {
-        const float x = fmaf(z, LOG2E, -c);
+        const float x = fmaf(z, f, -c);
         if (!ENTROPY) return ex2(x) * k;
         const float y = above(x);
         return ex2(y) * fmaf(y, e, k);
@@ -169,22 +178,22 @@ __device__ __forceinline__ float local_max(const Chunk<T>* q) {
     }
 }
 // One entry's share of the sums from c on
-__device__ __forceinline__ void add_entry(float z, float c, float& s, float& w) {
-    const float x = above(fmaf(z, LOG2E, -c)), e = ex2(x);
+__device__ __forceinline__ void add_entry(float z, float f, float c, float& s, float& w) {
+    const float x = above(fmaf(z, f, -c)), e = ex2(x);
     s += e;
     w = fmaf(e, x, w);
 }
 // ... of NV chunks; two accumulators each
 template <class T, int NV>
 __device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
-    const float c = scaled(m);
+    const float f = factor(m), c = scaled(m);
     float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < Chunk<T>::N / 2; ++k) {
             const float2 v = q[i].pair(k);
-            add_entry(v.x, c, s0, w0), add_entry(v.y, c, s1, w1);
+            add_entry(v.x, f, c, s0, w0), add_entry(v.y, f, c, s1, w1);
         }
     return make_float2(s0 + s1, w0 + w1);
 }
@@ -259,8 +268,7 @@ __device__ __forceinline__ void join(const float4* parts, int n, float& M, float
     S = W = 0.0f;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const bool none = p[i].x == -INFINITY;
-        const float d = none ? 0.0f : scaled(p[i].x) - scaled(M), f = none ? 0.0f : exp2f(d);
+        const float d = shift(p[i].x, M), f = p[i].x == -INFINITY ? 0.0f : exp2f(d);
         S = fmaf(p[i].y, f, S);
         W = fmaf(fmaf(p[i].y, d, p[i].z), f, W);
     }
@@ -586,15 +594,15 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
                 v[k] = i < V && (!legal || legal[i]) ? to_f(z[i]) : -INFINITY;
                 top = fmaxf(top, v[k]);
             }
-            const float c = top == -INFINITY ? 0.0f : scaled(top), d = m == -INFINITY ? 0.0f : scaled(m) - c, f = exp2f(d);
+            const float from = top == -INFINITY ? 0.0f : top, c = scaled(from), d = shift(m, from), f = exp2f(d);
             w = fmaf(s, d, w) * f, s *= f, m = top;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) add_entry(v[k], c, s, w);
+            for (int k = 0; k < 8; ++k) add_entry(v[k], factor(from), c, s, w);
         }
         float top = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        const float d = m == -INFINITY ? 0.0f : scaled(m) - scaled(top), f = exp2f(d);
+        const float d = shift(m, top), f = exp2f(d);
         w = warp_sum(fmaf(s, d, w) * f), s = warp_sum(s * f);
         __syncthreads();  // the last row's parts have been read
         if (lane == 0) parts[warp] = make_float4(top, s, w, 0.0f);
@@ -639,7 +647,8 @@ int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     attr.val.clusterDim = {CTAS, 1, 1};
     cfg.blockDim = THREADS, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1, cfg.dynamicSmemBytes = smem;
     // As many clusters as are resident at a time: they do not fill the SMs of every GPC, and the ones left over would
-    // start only when the others have ended (37 of 8 CTAs, of which 32 fit, took 2.1 times as long).
+    // start only when the others have ended (37 of 8 CTAs, of which 33 fit, took 560 us
+    // at 2048 x 131072 in bf16, 33 took 387).
     constexpr int SM = (FIT ? 1024 : 512) / THREADS;  // CTAs of one
     cfg.gridDim = CTAS * SM;
     int most = 0;

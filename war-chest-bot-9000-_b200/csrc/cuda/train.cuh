@@ -59,16 +59,31 @@ __device__ __forceinline__ float act8_unit(uint32_t code) {
 // 2^-e of a code; the product with a block's value is exact (or too small to round to anything but 0)
 __device__ __forceinline__ float act8_inverse(uint32_t code) { return __uint_as_float((254u - code) << 23); }
 
+// At the largest unit a whole number stops at 63: 64 times it would be no number of 32 bits.
+constexpr uint32_t ACT8_LARGEST = 249;
+constexpr float ACT8_MOST = 0x1.f8p127f;
+// one value of a block
+__device__ __forceinline__ int8_t act8_whole(float v, uint32_t code) {
+    if (code == 255) return 0;
+    return (int8_t)__float2int_rn((code == ACT8_LARGEST ? fminf(fmaxf(v, -ACT8_MOST), ACT8_MOST) : v) * act8_inverse(code));
+}
+
 // A thread's 8 values of a block (4 threads next to each other hold one) as bytes, and the block's code.
 // Magnitudes are compared as integers, where NaN is above infinity above the rest, so either shows in the code.
-__device__ __forceinline__ uint2 quantise8(const float* v, uint32_t* code) {
+__device__ __forceinline__ uint2 quantise8(const float* in, uint32_t* code) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(in[i]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     *code = act8_code(__uint_as_float(top));
     if (*code == 255) return make_uint2(0, 0);
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = in[i];
+    if (*code == ACT8_LARGEST)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -ACT8_MOST), ACT8_MOST);
     const float inv = act8_inverse(*code);
     uint32_t b[8];
     // adding 1.5 2^23 rounds to a whole number, ties to even, and leaves its two's complement in the low bits

@@ -103,7 +103,7 @@ int wc_block_norm_backward(const wc_block_norm_args* a, const wc_block_norm_grad
     if (const int rc = check_norm(me, a)) return rc;
     if (!g) return bad(me, "null arguments");
     if (g->dn && !a->pre_weight) return bad(me, "dn needs a pre norm");
-    if (!g->dy && !g->dn) return bad(me, "neither dy nor dn");
+    if (a->rows && !g->dy && !g->dn) return bad(me, "neither dy nor dn");
     if (g->dgate && !a->gate) return bad(me, "dgate without a gate");
     if ((g->dpost_weight && !a->post_weight) || (g->dpost_bias && !a->post_bias) || (g->dpre_weight && !a->pre_weight) ||
         (g->dpre_bias && !a->pre_bias))

@@ -1,0 +1,118 @@
+"""The training operators (train_ops) as differentiable functions: torch's
+autograd calls their backward entries. What a backward pass needs of an
+activation is kept in 8 bits where the operator has that form."""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from . import train_ops as ops
+from .train_ops import Act8, PolicyLoss
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, args, options):
+        r = ops.policy_loss(logits, *args, want_grad=False, **options)
+        ctx.save_for_backward(logits)
+        ctx.args, ctx.options = args, options
+        ctx.mark_non_differentiable(r.row_loss, r.logp, r.entropy, r.kl)
+        return r.loss, r.row_loss, r.logp, r.entropy, r.kl
+
+    @staticmethod
+    def backward(ctx, g, *unused):
+        (logits,) = ctx.saved_tensors
+        r = ops.policy_loss(logits, *ctx.args, upstream=g.to(torch.float32), **ctx.options)
+        return r.dlogits, None, None
+
+
+def policy_loss(logits, actions, old_logp, advantages, **options) -> PolicyLoss:
+    """train_ops.policy_loss with a differentiable loss (the other results are not, and dlogits is None): the logits are
+    read again in the backward pass, which keeps no gradient between the two."""
+    return PolicyLoss(*_PolicyLoss.apply(logits, (actions, old_logp, advantages), options), None)
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, h, gate, post, post_bias, pre, pre_bias, options, pack):
+        pair = lambda w, b: None if w is None else (w, b)  # noqa: E731
+        weights = {"post": pair(post, post_bias), "pre": pair(pre, pre_bias)}
+        r = ops.block_norm(x, h, gate=gate, pack=pack, **weights, **options)
+        ctx.save_for_backward(x, h, gate, post, post_bias, pre, pre_bias, r.stats)
+        ctx.options = options
+        out = (r.y,) + ((r.n,) if r.n is not None else ())
+        if pack:
+            ctx.mark_non_differentiable(r.n8.q, r.n8.scale)
+            out += (r.n8.q, r.n8.scale)
+        ctx.set_materialize_grads(False)
+        return out
+
+    @staticmethod
+    def backward(ctx, dy, dn=None, *unused):
+        x, h, gate, post, post_bias, pre, pre_bias, stats = ctx.saved_tensors
+        if dy is None and dn is None:
+            return (None,) * 9
+        flat = lambda d: None if d is None else d.contiguous()  # noqa: E731
+        g = ops.block_norm_backward(flat(dy), flat(dn), x, h, stats, gate=gate,
+                                    post=None if post is None else (post, post_bias),
+                                    pre=None if pre is None else (pre, pre_bias), **ctx.options)
+        return g.dx, g.dh, g.dgate, g.dpost, g.dpost_bias, g.dpre, g.dpre_bias, None, None
+
+
+def block_norm(x, h, *, gate=None, post=None, pre=None, pack=False, **options):
+    """train_ops.block_norm with gradients at x, h, gate and the norms' weights and biases: y, then n where there is a
+    pre norm, then n in 8 bits where `pack` asks for it."""
+    split = lambda w: w if isinstance(w, tuple) else (w, None)  # noqa: E731
+    out = _BlockNorm.apply(x, h, gate, *split(post), *split(pre), options, pack)
+    if pack:
+        return out[0], out[1], Act8(out[2], out[3], x.shape[1])
+    return out if len(out) > 1 else out[0]
+
+
+class _Gelu8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, z, bias):
+        a, z8 = ops.gelu8(z, bias)
+        ctx.save_for_backward(z8.q, z8.scale)
+        ctx.has_bias = bias is not None
+        return a
+
+    @staticmethod
+    def backward(ctx, da):
+        q, scale = ctx.saved_tensors
+        dz, dbias = ops.gelu8_backward(da.contiguous(), Act8(q, scale, da.shape[1]), want_bias=ctx.has_bias)
+        return dz, dbias
+
+
+def gelu8(z, bias=None) -> torch.Tensor:
+    """GELU (tanh form) of z + bias; what its backward pass needs is kept in 8 bits."""
+    return _Gelu8.apply(z, bias)
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, q, scale):
+        x8 = ops.act8_pack(x) if q is None else Act8(q, scale, x.shape[1])
+        ctx.save_for_backward(w, x8.q, x8.scale)
+        ctx.has_bias = bias is not None
+        out = x @ w.to(x.dtype)
+        return out if bias is None else out + bias.to(x.dtype)
+
+    @staticmethod
+    def backward(ctx, dy):
+        w, q, scale = ctx.saved_tensors
+        dy = dy.contiguous()
+        dx = dy @ w.to(dy.dtype).t() if ctx.needs_input_grad[0] else None
+        dw, db = ops.act8_wgrad(Act8(q, scale, w.shape[0]), dy, dtype=w.dtype, want_bias=ctx.has_bias)
+        return dx, dw, db, None, None
+
+
+def linear8(x, w, bias=None, x8: Optional[Act8] = None) -> torch.Tensor:
+    """x w + bias with w [in, out]. The input is kept in 8 bits for w's gradient: as `x8` has it (block_norm's pack, say),
+    or packed here. The product is the library's; the weight gradient is act8_wgrad's, in w's type."""
+    q, scale = (None, None) if x8 is None else x8[:2]
+    return _Linear8.apply(x, w, bias, q, scale)
+
+
+__all__ = ["policy_loss", "block_norm", "gelu8", "linear8"]
