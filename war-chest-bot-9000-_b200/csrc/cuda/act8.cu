@@ -2,12 +2,16 @@
 // unit (train.cuh act8_code), so a stored value is a whole number times that
 // unit and is exact in bf16.
 //
-// All of these are bound by the bytes they move. Where addresses and strides
+// All of these move few bytes a value, and what comes first is the instructions:
+// at 30 to 55 a value (measured, of earlier forms) the SMs issue for longer than
+// the memory takes. So arithmetic is on pairs, index divisions are products, and
+// what is a block's alone is computed once for it. Where addresses and strides
 // allow, a thread holds 8 consecutive values (16 bytes of a 16-bit type in one
 // load, 8 bytes of q in one store) and 4 threads a block: the largest magnitude
-// takes two shuffles. Elsewhere a warp holds a block, one value a thread, so
-// that its loads and stores are still next to each other.
+// takes two shuffles. Elsewhere a warp holds 8 blocks, one value of each a
+// thread, so that its loads and stores are still next to each other.
 #include <algorithm>
+#include <type_traits>
 
 #include "colsum.cuh"
 
@@ -19,54 +23,86 @@ constexpr int THREADS = 256;
 
 // 8 values of a row from column c on; those past the width (a whole number of 8s) are 0
 template <class T>
-__device__ __forceinline__ void load8(const T* p, int64_t c, int64_t width, float* v) {
-    alignas(16) T e[8];
+struct Raw {
+    alignas(16) uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p, bool in) {
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-        reinterpret_cast<uint4*>(e)[i] = c < width ? __ldcs(reinterpret_cast<const uint4*>(p + c) + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = in ? __ldcs(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(Pair* v) const {
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f(e[i]);
-}
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = umma::f2(u[2 * i], u[2 * i + 1]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) v[i] = umma::f2(u[i] << 16, u[i] & 0xffff0000u);
+            else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+                v[i] = umma::f2(f.x, f.y);
+            }
+        }
+    }
+};
 template <class T>
-__device__ __forceinline__ void store8(T* p, int64_t c, int64_t width, const float* v) {
-    if (c >= width) return;
-    alignas(16) T e[8];
+__device__ __forceinline__ void store8(T* p, const Pair* v) {
+    alignas(16) uint32_t u[2 * sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f<T>(v[i]);
+    for (int i = 0; i < 4; ++i) {
+        const float lo = umma::f2_lo(v[i]), hi = umma::f2_hi(v[i]);
+        if constexpr (sizeof(T) == 4) u[2 * i] = __float_as_uint(lo), u[2 * i + 1] = __float_as_uint(hi);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&u[i]) = __floats2bfloat162_rn(lo, hi);
+        else *reinterpret_cast<__half2*>(&u[i]) = __floats2half2_rn(lo, hi);
+    }
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p + c) + i, reinterpret_cast<const uint4*>(e)[i]);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) __stcs(reinterpret_cast<uint4*>(p) + i, reinterpret_cast<const uint4*>(u)[i]);
+}
+__device__ __forceinline__ void load_bias8(const float* p, Pair* v) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = umma::f2(a.x, a.y), v[1] = umma::f2(a.z, a.w), v[2] = umma::f2(b.x, b.y), v[3] = umma::f2(b.z, b.w);
 }
 
-__device__ __forceinline__ void dequantise8(uint2 q, uint32_t code, float* v) {
-    const float unit = act8_unit(code);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3))) * unit;
-}
+// i / d for i < 2^31 by a product with floor(2^32 / d), which gives the quotient or one less
+struct Divisor {
+    uint32_t d, m;
+    explicit Divisor(uint32_t v) : d(v), m(v > 1 ? (uint32_t)((1ull << 32) / v) : 0xffffffffu) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t i, uint32_t* rest) const {
+        uint32_t q = __umulhi(i, m), r = i - q * d;
+        if (r >= d) ++q, r -= d;
+        *rest = r;
+        return q;
+    }
+};
 
 enum { PACK, UNPACK, GELU };
 
 template <class T, int WHAT>
-__global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, uint32_t chunks, uint32_t total) {
+__global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, Divisor chunks, uint32_t total) {
     const uint32_t i = blockIdx.x * THREADS + threadIdx.x;
     const bool in = i < total;  // total is a multiple of 4: a block's threads are in or out together
-    const uint32_t row = in ? i / chunks : 0, chunk = in ? i - row * chunks : 0;
+    uint32_t chunk;
+    const uint32_t row = chunks(in ? i : 0, &chunk);
     const int64_t c = (int64_t)chunk * 8;
-    float v[8];
+    const bool here = in && c < a.width;
+    Pair v[4];
     if constexpr (WHAT == UNPACK) {
-        if (!in) return;
-        dequantise8(reinterpret_cast<const uint2*>(a.q)[i], a.scale[i >> 2], v);
-        store8(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, v);
+        if (!here) return;
+        dequantise8(__ldcs(reinterpret_cast<const uint2*>(a.q) + i), a.scale[i >> 2], v);
+        store8(static_cast<T*>(a.out) + row * a.ld_out + c, v);
     } else {
-        load8(static_cast<const T*>(a.x) + row * a.ld_x, in ? c : a.width, a.width, v);
+        Raw<T> x;
+        x.load(static_cast<const T*>(a.x) + row * a.ld_x + c, here);
+        x.get(v);
         if constexpr (WHAT == GELU) {
-            if (in && c < a.width) {
-                if (a.bias)
+            if (here) {
+                if (a.bias) {
+                    Pair b[4];
+                    load_bias8(a.bias + c, b);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] += a.bias[c + k];
-                float y[8];
+                    for (int k = 0; k < 4; ++k) v[k] = add(v[k], b[k]);
+                }
+                Pair y[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) y[k] = gelu(v[k]);
-                store8(static_cast<T*>(a.out) + row * a.ld_out, c, a.width, y);
+                for (int k = 0; k < 4; ++k) y[k] = gelu(v[k]);
+                store8(static_cast<T*>(a.out) + row * a.ld_out + c, y);
             }
         }
         uint32_t code;
@@ -78,39 +114,63 @@ __global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, uint32_t chunk
     }
 }
 
-// The same, a warp a run of 4 blocks of a row.
+// The same, a warp a run of 8 blocks of a row; lane k keeps what is the k-th block's.
 template <class T, int WHAT>
-__global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, uint32_t blocks, uint32_t runs, uint32_t total) {
+__global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int blocks, Divisor runs, uint32_t total) {
     const uint32_t i = (blockIdx.x * THREADS + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     if (i >= total) return;
-    const int64_t row = i / runs;
-    const uint32_t first = (i - (uint32_t)row * runs) * 4;
-    float v[4];
+    uint32_t run;
+    const int64_t row = runs(i, &run), b0 = row * blocks + run * 8;
+    const int left = blocks - (int)run * 8, cols = (int)(a.width - (int64_t)run * 256) - (int)lane;  // from this lane's first on
+    int8_t* q = a.q + b0 * 32 + lane;
+    uint8_t* scale = a.scale + b0;
+    if constexpr (WHAT == UNPACK) {
+        T* out = static_cast<T*>(a.out) + row * a.ld_out + run * 256 + lane;
+        uint32_t w[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t c = (int64_t)(first + k) * 32 + lane;
-        v[k] = 0.0f;
-        if (WHAT != UNPACK && c < a.width) v[k] = to_f(static_cast<const T*>(a.x)[row * a.ld_x + c]);
-        if (WHAT == UNPACK && first + k < blocks) {
-            const int64_t b = row * blocks + first + k;
-            v[k] = (float)a.q[b * 32 + lane] * act8_unit(a.scale[b]);
-        }
-    }
+        for (int k = 0; k < 8; ++k) w[k] = k < left ? (uint32_t)(uint8_t)__ldcs(q + k * 32) : 0;
+        const float unit = act8_unit((int)lane < min(left, 8) ? scale[lane] : 1);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int64_t c = (int64_t)(first + k) * 32 + lane, b = row * blocks + first + k;
-        if (first + k >= blocks) break;
-        if (WHAT == UNPACK) {
-            if (c < a.width) static_cast<T*>(a.out)[row * a.ld_out + c] = from_f<T>(v[k]);
-            continue;
+        for (int k = 0; k < 8; ++k) {
+            const float v = act8_number(w[k]) * __shfl_sync(0xffffffffu, unit, k);
+            if (k * 32 < cols) __stcs(out + k * 32, from_f<T>(v));
         }
-        if (WHAT == GELU && c < a.width) {
-            if (a.bias) v[k] += a.bias[c];
-            static_cast<T*>(a.out)[row * a.ld_out + c] = from_f<T>(gelu(v[k]));
+    } else {
+        const T* x = static_cast<const T*>(a.x) + row * a.ld_x + run * 256 + lane;
+        T* out = static_cast<T*>(a.out) + row * a.ld_out + run * 256 + lane;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = k * 32 < cols ? to_f(__ldcs(x + k * 32)) : 0.0f;
+        if constexpr (WHAT == GELU)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k * 32 < cols) {
+                    if (a.bias) v[k] += a.bias[(int64_t)run * 256 + lane + k * 32];
+                    __stcs(out + k * 32, from_f<T>(gelu(v[k])));
+                }
+        // magnitudes are compared as integers, where NaN is above infinity above the rest, so either shows in the code
+        uint32_t top = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu);
+            if (lane == k) top = m;
         }
-        const uint32_t code = act8_code(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v[k]) & 0x7fffffffu)));
-        a.q[b * 32 + lane] = act8_whole(v[k], code);
-        if (lane == 0) a.scale[b] = (uint8_t)code;
+        const uint32_t code = act8_code(__uint_as_float(top));
+        if ((int)lane < min(left, 8)) scale[lane] = (uint8_t)code;
+        if (__any_sync(0xffffffffu, code >= ACT8_LARGEST)) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t mine = __shfl_sync(0xffffffffu, code, k);
+                if (k < left) q[k * 32] = act8_whole(v[k], mine);
+            }
+        } else {
+            const float inv = act8_inverse(code);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float mine = __shfl_sync(0xffffffffu, inv, k);
+                if (k < left) q[k * 32] = (int8_t)__float_as_uint(fmaf(v[k], mine, 12582912.0f));
+            }
+        }
     }
 }
 
@@ -125,44 +185,70 @@ __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int 
     const int step = UNITS ? 1 : 32, c = UNITS ? at * 8 : (at & ~31) * 8 + (at & 31);
     const bool in = r < per && c < a.width;
     const int64_t first = blockIdx.y * chunk_rows, last = min(first + chunk_rows, a.rows);
-    float acc[8] = {};
-    if (in)
-        for (int64_t t = first + r; t < last; t += per) {
-            const T* x = static_cast<const T*>(a.x) + t * a.ld_x;
-            T* out = static_cast<T*>(a.out) + t * a.ld_out;
-            float d[8], z[8];
-            if constexpr (UNITS) {
-                load8(x, c, a.width, d);
-                dequantise8(*reinterpret_cast<const uint2*>(a.q + t * blocks * 32 + c), a.scale[t * blocks + c / 32], z);
-            } else {
+    Pair acc[4] = {0, 0, 0, 0};  // (pairs of zeros)
+    if constexpr (UNITS) {
+        if (in) {
+            const int64_t row_q = (int64_t)blocks * 32;
+            const T* x = static_cast<const T*>(a.x) + (first + r) * a.ld_x + c;
+            T* out = static_cast<T*>(a.out) + (first + r) * a.ld_out + c;
+            const int8_t* q = a.q + (first + r) * row_q + c;
+            const uint8_t* scale = a.scale + (first + r) * blocks + c / 32;
+            Raw<T> d;
+            uint2 w = make_uint2(0, 0);
+            uint32_t code = 1;
+            auto fetch = [&](int64_t t) {
+                if (t >= last) return;
+                d.load(x, true), w = __ldcs(reinterpret_cast<const uint2*>(q)), code = *scale;
+                x += per * a.ld_x, q += per * row_q, scale += per * blocks;
+            };
+            fetch(first + r);
+            for (int64_t t = first + r; t < last; t += per) {
+                Pair z[4], g[4];
+                d.get(g), dequantise8(w, code, z), gelu_cut(code, z, 4);
+                fetch(t + per);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const bool here = c + k * 32 < a.width;
-                    d[k] = here ? to_f(x[c + k * 32]) : 0.0f;
-                    z[k] = here ? (float)a.q[t * blocks * 32 + c + k * 32] * act8_unit(a.scale[t * blocks + c / 32 + k]) : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                d[k] *= gelu_slope(z[k]);
-                acc[k] += d[k];
-            }
-            if constexpr (UNITS) {
-                store8(out, c, a.width, d);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (c + k * 32 < a.width) out[c + k * 32] = from_f<T>(d[k]);
+                for (int k = 0; k < 4; ++k) g[k] = mul(g[k], gelu_slope(z[k])), acc[k] = add(acc[k], g[k]);
+                store8(out, g);
+                out += per * a.ld_out;
             }
         }
+    } else if (in) {
+        for (int64_t t = first + r; t < last; t += per) {
+            const T* x = static_cast<const T*>(a.x) + t * a.ld_x + c;
+            T* out = static_cast<T*>(a.out) + t * a.ld_out + c;
+            const int8_t* q = a.q + t * blocks * 32 + c;
+            const uint8_t* scale = a.scale + t * blocks + c / 32;
+            const int left = (int)(a.width - c);
+            float d[8];
+            uint32_t w[8], code[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const bool here = k * 32 < left;
+                d[k] = here ? to_f(__ldcs(x + k * 32)) : 0.0f, w[k] = here ? (uint32_t)(uint8_t)__ldcs(q + k * 32) : 0, code[k] = here ? scale[k] : 1;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                Pair z = mul(umma::f2(act8_number(w[2 * k]), act8_number(w[2 * k + 1])), umma::f2(act8_unit(code[2 * k]), act8_unit(code[2 * k + 1])));
+                if (max(code[2 * k], code[2 * k + 1]) > 147) {
+                    Pair lo = umma::f2(umma::f2_lo(z), 0.0f), hi = umma::f2(umma::f2_hi(z), 0.0f);
+                    gelu_cut(code[2 * k], &lo, 1), gelu_cut(code[2 * k + 1], &hi, 1);
+                    z = umma::f2(umma::f2_lo(lo), umma::f2_lo(hi));
+                }
+                const Pair g = mul(umma::f2(d[2 * k], d[2 * k + 1]), gelu_slope(z));
+                acc[k] = add(acc[k], g);
+                if (2 * k * 32 < left) __stcs(out + 2 * k * 32, from_f<T>(umma::f2_lo(g)));
+                if ((2 * k + 1) * 32 < left) __stcs(out + (2 * k + 1) * 32, from_f<T>(umma::f2_hi(g)));
+            }
+        }
+    }
     if (!part) return;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) s[threadIdx.x][k] = acc[k];
+    for (int k = 0; k < 8; ++k) s[threadIdx.x][k] = k & 1 ? umma::f2_hi(acc[k / 2]) : umma::f2_lo(acc[k / 2]);
     __syncthreads();
     if (in && r == 0)
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            float v = acc[k];
+            float v = s[threadIdx.x][k];
             for (int j = 1; j < per; ++j) v += s[threadIdx.x + j * lanes][k];
             if (c + k * step < a.width) part[blockIdx.y * a.width + c + k * step] = v;
         }
@@ -182,13 +268,13 @@ void launch_as(const wc_act8_args& a, cudaStream_t s) {
         if (a.out) b.out = static_cast<T*>(a.out) + t * a.ld_out;
         b.q += t * chunks * 8, b.scale += t * chunks / 4;
         const bool units = a.width % 8 == 0 && (WHAT == UNPACK || aligned(b.x, a.ld_x, sizeof(T))) &&
-                           (WHAT == PACK || aligned(b.out, a.ld_out, sizeof(T)));
+                           (WHAT == PACK || aligned(b.out, a.ld_out, sizeof(T))) && ((uintptr_t)a.bias & 15) == 0;
         if (units) {
             const uint32_t total = (uint32_t)(b.rows * chunks);
-            k_act8<T, WHAT><<<(total + THREADS - 1) / THREADS, THREADS, 0, s>>>(b, (uint32_t)chunks, total);
+            k_act8<T, WHAT><<<(total + THREADS - 1) / THREADS, THREADS, 0, s>>>(b, Divisor((uint32_t)chunks), total);
         } else {
-            const uint32_t runs = (uint32_t)(chunks + 15) / 16, total = (uint32_t)(b.rows * runs);
-            k_act8_runs<T, WHAT><<<(unsigned)((total + 7ull) / 8), THREADS, 0, s>>>(b, (uint32_t)(chunks / 4), runs, total);
+            const uint32_t runs = (uint32_t)(chunks + 31) / 32, total = (uint32_t)(b.rows * runs);
+            k_act8_runs<T, WHAT><<<(unsigned)((total + 7ull) / 8), THREADS, 0, s>>>(b, (int)(chunks / 4), Divisor(runs), total);
         }
     }
 }
@@ -222,7 +308,7 @@ void launch_backward(const wc_act8_args& a, cudaStream_t s) {
     const dim3 grid(g.tiles, g.splits);
     if (units) k_gelu8_backward<T, true><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
     else k_gelu8_backward<T, false><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
-    if (part) launch_colsum<float>(part, g.splits, a.width, a.width, a.dbias, s);
+    if (part) launch_colsum(part, g.splits, a.width, a.width, 1, ColSums{{a.dbias}}, s);
 }
 
 }  // namespace

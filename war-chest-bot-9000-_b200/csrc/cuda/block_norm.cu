@@ -49,7 +49,6 @@ __global__ void k_gate_sum(const float* part, int segments, int64_t D, int64_t t
 }
 
 // ---- units -------------------------------------------------------------------
-using Pair = unsigned long long;  // two 32-bit numbers for the packed forms (umma.cuh)
 
 // How a thread's 8 columns lie: next to each other; or one of each of 8 runs, the runs as long as the threads that share
 // the row (of a warp or less), or 32 (a warp's 256 columns next to each other: offsets known to the compiler).
@@ -341,15 +340,6 @@ struct Items {
 
 // Arithmetic on pairs, each rounded as the scalar form: the backward pass has some 30 operations a column, which would
 // bound it before the bytes do.
-__device__ __forceinline__ Pair twice(float v) { return umma::f2(v, v); }
-__device__ __forceinline__ Pair mul(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ Pair add(Pair a, Pair b) { return umma::f2_add(a, b); }
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) { return umma::f2_fma(a, b, c); }
-__device__ __forceinline__ float both(Pair a) { return umma::f2_lo(a) + umma::f2_hi(a); }
 __device__ __forceinline__ void fill(Pair* v, float x) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) v[k] = twice(x);
@@ -856,9 +846,8 @@ void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cuda
         if (g.dgate && p.segments > 1)
             k_gate_sum<T><<<148 * 4, 256, 0, s>>>(gates, p.segments, D, p.groups * D, static_cast<T*>(g.dgate));
     }
-    float* to[4] = {g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias};
-    for (int k = 0; k < 4; ++k)
-        if (to[k]) launch_colsum<float>(weights + k * D, p.parts, 4 * D, D, to[k], s);
+    if (g.dpost_weight || g.dpost_bias || g.dpre_weight || g.dpre_bias)
+        launch_colsum(weights, p.parts, 4 * D, D, 4, ColSums{{g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias}}, s);
 }
 template <class T>
 void backward(const wc_block_norm_args& a, const wc_block_norm_grads& g, cudaStream_t s) {

@@ -627,12 +627,20 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
     if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
-// the CTAs' totals, in order
-__global__ void k_policy_total(const double* part, int n, float* loss) {
+// the CTAs' totals, in a fixed order
+__global__ void __launch_bounds__(1024) k_policy_total(const double* part, int n, float* loss) {
+    __shared__ double s[32];
     double v = 0.0;
-    for (int i = threadIdx.x; i < n; i += 32) v += part[i];
+    for (int i = threadIdx.x; i < n; i += blockDim.x) v += part[i];
+    for (int stage = 0; stage < 2; ++stage) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+        if (stage) break;
+        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
+        __syncthreads();
+        if (threadIdx.x >= 32) return;
+        v = threadIdx.x < blockDim.x / 32 ? s[threadIdx.x] : 0.0;
+    }
     if (threadIdx.x == 0) *loss = (float)v;
 }
 
@@ -727,7 +735,7 @@ void launch_policy_loss(const wc_policy_loss_args& a, cudaStream_t s) {
     if (a.rows) n = a.type == WC_F32   ? launch_type<float>(a, part, s)
                     : a.type == WC_F16 ? launch_type<__half>(a, part, s)
                                        : launch_type<__nv_bfloat16>(a, part, s);
-    k_policy_total<<<1, 32, 0, s>>>(part, n, a.loss);
+    k_policy_total<<<1, std::min(1024, std::max(32, (n + 31) / 32 * 32)), 0, s>>>(part, n, a.loss);
 }
 
 }  // namespace wctrain
