@@ -89,7 +89,7 @@ struct Row {
     Row() = default;
     __device__ __forceinline__ Row(const wc_policy_loss_args& a, const RowIn& in, float m, float S, float W, float za) : c(scaled(m)), f(factor(m)) {
         const float top = fmaf(m, f, -c), eTop = ex2(top);  // x and the power of the maximum
-        const float mean = S == eTop ? 0.0f : W / S - top;  // of x, from the maximum's on
+        const float inv = __frcp_rn(S), mean = S == eTop ? 0.0f : fmaf(W, inv, -top);  // of x, from the maximum's on
         // ln of S / eTop = 2^n q, q about 1; LOG2E as a float is 1.34e-8 (relative) low, which mean puts right to first order
         int n;
         float q = frexpf(S / eTop, &n);
@@ -114,7 +114,6 @@ struct Row {
         g = up * ((held ? 0.0f : -free) - a.kl_coef * em);
         ce = up * a.entropy_coef;
         // p = 2^x / S and ln p = (x - top) ln 2 - ln (S / eTop)
-        const float inv = 1.0f / S;
         e = ce * LN2 * inv, k = fmaf(ce, -LN2 * (mean + top), -g) * inv;
     }
     __device__ __forceinline__ void put(const wc_policy_loss_args& a, int64_t t) const {
@@ -144,22 +143,33 @@ struct Chunk {
     __device__ __forceinline__ void none() { z[0] = z[1] = z[2] = z[3] = INF; }
     // legal bytes, in the order of the entries
     __device__ __forceinline__ void mask(uint2 legal) {
-        const uint32_t off[2] = {__vcmpeq4(legal.x, 0), __vcmpeq4(legal.y, 0)};
+        // a byte that is not 0 gets its top bit, which the permutation spreads over the entry's bytes
+        const uint32_t on[2] = {((legal.x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | legal.x, ((legal.y & 0x7f7f7f7fu) + 0x7f7f7f7fu) | legal.y};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t m = N == 8 ? __byte_perm(off[i >> 1], 0, i & 1 ? 0x3322 : 0x1100) : __byte_perm(off[0], 0, 0x1111 * i);
-            z[i] = (z[i] & ~m) | (INF & m);
+            const uint32_t m = N == 8 ? spread(on[i >> 1], i & 1 ? 0xbbaa : 0x9988) : spread(on[0], 0x8888 + 0x1111 * i);
+            z[i] = (z[i] & m) | (INF & ~m);
         }
     }
     __device__ __forceinline__ static uint2 load_legal(const uint8_t* at) {
         if constexpr (N == 8) return __ldcs(reinterpret_cast<const uint2*>(at));
         return make_uint2(__ldcs(reinterpret_cast<const unsigned int*>(at)), 0);
     }
+    __device__ __forceinline__ static uint32_t spread(uint32_t v, uint32_t how) {
+        uint32_t r;
+        asm("prmt.b32 %0, %1, 0, %2;" : "=r"(r) : "r"(v), "r"(how));
+        return r;
+    }
     // entries 2 i and 2 i + 1
-    __device__ __forceinline__ float2 pair(int i) const {
-        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1]));
-        else if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&z[i]));
-        else return make_float2(__uint_as_float(z[i] << 16), __uint_as_float(z[i] & 0xffff0000u));
+    __device__ __forceinline__ Pair pair(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return umma::f2(z[2 * i], z[2 * i + 1]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&z[i]));
+            return umma::f2(f.x, f.y);
+        } else {
+            return umma::f2(z[i] << 16, z[i] & 0xffff0000u);
+        }
     }
 };
 
@@ -188,35 +198,40 @@ __device__ __forceinline__ void add_entry(float z, float f, float c, float& s, f
     s += e;
     w = fmaf(e, x, w);
 }
-// ... of NV chunks; two accumulators each
+// ... of NV chunks, by pairs
 template <class T, int NV>
 __device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
-    const float f = factor(m), c = scaled(m);
-    float s0 = 0.0f, s1 = 0.0f, w0 = 0.0f, w1 = 0.0f;
+    const Pair f = twice(factor(m)), c = twice(-scaled(m));
+    Pair s = 0, w = 0;  // (pairs of zeros)
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int k = 0; k < Chunk<T>::N / 2; ++k) {
-            const float2 v = q[i].pair(k);
-            add_entry(v.x, f, c, s0, w0), add_entry(v.y, f, c, s1, w1);
+            const Pair t = fma(q[i].pair(k), f, c), x = umma::f2(above(umma::f2_lo(t)), above(umma::f2_hi(t)));
+            const Pair e = umma::f2(ex2(umma::f2_lo(x)), ex2(umma::f2_hi(x)));
+            s = add(s, e), w = fma(e, x, w);
         }
-    return make_float2(s0 + s1, w0 + w1);
+    return make_float2(both(s), both(w));
 }
-// The gradient of a chunk, of which entry `hit` is the action
+// The gradient of a chunk. (At the action it is not all: the thread that writes the action's chunk writes that entry
+// after it, which costs one store a row and nothing an entry.)
 template <class T, bool ENTROPY>
-__device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, int hit, T* e) {
-    float v[Chunk<T>::N];
+__device__ __forceinline__ void chunk_grad(const Chunk<T>& q, const Row& r, T* e) {
+    const Pair f = twice(r.f), c = twice(-r.c);
 #pragma unroll
     for (int k = 0; k < Chunk<T>::N / 2; ++k) {
-        const float2 z = q.pair(k);
-        v[2 * k] = r.grad<ENTROPY>(z.x), v[2 * k + 1] = r.grad<ENTROPY>(z.y);
+        const Pair t = fma(q.pair(k), f, c);
+        Pair d;
+        if constexpr (ENTROPY) {
+            const Pair y = umma::f2(above(umma::f2_lo(t)), above(umma::f2_hi(t)));
+            d = mul(umma::f2(ex2(umma::f2_lo(y)), ex2(umma::f2_hi(y))), fma(y, twice(r.e), twice(r.k)));
+        } else {
+            d = mul(umma::f2(ex2(umma::f2_lo(t)), ex2(umma::f2_hi(t))), twice(r.k));
+        }
+        if constexpr (sizeof(T) == 4) e[2 * k] = umma::f2_lo(d), e[2 * k + 1] = umma::f2_hi(d);
+        else if constexpr (std::is_same<T, __half>::value) reinterpret_cast<__half2*>(e)[k] = __floats2half2_rn(umma::f2_lo(d), umma::f2_hi(d));
+        else reinterpret_cast<__nv_bfloat162*>(e)[k] = __floats2bfloat162_rn(umma::f2_lo(d), umma::f2_hi(d));
     }
-    if ((unsigned)hit < (unsigned)Chunk<T>::N)
-#pragma unroll
-        for (int k = 0; k < Chunk<T>::N; ++k)
-            if (k == hit) v[k] += r.g;
-#pragma unroll
-    for (int k = 0; k < Chunk<T>::N; ++k) e[k] = from_f<T>(v[k]);
 }
 template <class T>
 __device__ __forceinline__ void put_chunk(T* out, const T* e) {
@@ -326,14 +341,13 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss
             const Row row(a, r, m, sw.x, sw.y, za);
             if (at == 0) row.put(a, t), total += (double)(r.w * row.loss);
             if (!out) continue;
-            // the action's place among this thread's entries
-            const int unit = VEC ? r.act / N : r.act, mine = (unit & (lanes - 1)) != at ? -1 : VEC ? unit / lanes * N + r.act % N : unit / lanes;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 alignas(16) T e[N];
-                chunk_grad<T, ENTROPY>(q[i], row, mine < 0 ? -1 : mine - i * N, e);
+                chunk_grad<T, ENTROPY>(q[i], row, e);
                 put<VEC>(out, e, i, at, lanes, width);
             }
+            if (((VEC ? r.act / N : r.act) & (lanes - 1)) == at) out[r.act] = from_f<T>(row.grad<ENTROPY>(za) + row.g);
         } else {
             if (at == 0) put_void(a, t);
             alignas(16) T e[N];
@@ -475,6 +489,7 @@ __global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_polic
     double total = 0.0;
     bool bad = false, live0 = false;
     int act0 = -1;
+    float za0 = 0.0f;
     int turn = 0;         // of parts[] and joined[]
     uint32_t phases = 0;  // of joined[]
     for (int64_t i = -1, t = t0 - step; t < a.rows; ++i, t += step) {
@@ -526,18 +541,20 @@ __global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_polic
             alignas(16) T e[N];
             if (live0 && r.ce != 0.0f) {
                 for (int at = threadIdx.x * N; at < width; at += THREADS * N)
-                    chunk_grad<T, true>(chunk(t, slot, b, at), r, act0 - (first + at - b), e), write(at, e);
+                    chunk_grad<T, true>(chunk(t, slot, b, at), r, e), write(at, e);
             } else if (live0) {
 #pragma unroll
                 for (int k = 0; k < NV; ++k) {
                     const int at = (k * THREADS + (int)threadIdx.x) * N;
-                    if (at < width) chunk_grad<T, false>(chunk(t, slot, b, at), r, act0 - (first + at - b), e), write(at, e);
+                    if (at < width) chunk_grad<T, false>(chunk(t, slot, b, at), r, e), write(at, e);
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < N; ++k) e[k] = from_f<T>(0.0f);
                 for (int at = threadIdx.x * N; at < width; at += THREADS * N) write(at, e);
             }
+            const int mine = act0 + b - first;
+            if (live0 && mine >= 0 && mine < width && mine / N % THREADS == threadIdx.x) out[act0] = from_f<T>(r.grad<true>(za0) + r.g);
         }
         if (CTAS == 1) __syncthreads();
         if (warp == 0 && t1 < a.rows) {
@@ -558,7 +575,7 @@ __global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_polic
             }
         }
         if (live1) turn = turn == 2 ? 0 : turn + 1;
-        live0 = live1, act0 = in1.act;
+        live0 = live1, act0 = in1.act, za0 = za1;
         in1 = in2, in2 = in3, za1 = za2;
         za2 = logit(t1 + 2 * step, in2.act);
         in3 = RowIn(a, t1 + 3 * step);

@@ -707,9 +707,7 @@ void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
     if (p.parts == 3) launch_split<3, float>(a, p, split, s);
     else if (p.parts == 2) launch_split<2, __half>(a, p, split, s);
     else if (p.split_ld) launch_split<1, __nv_bfloat16>(a, p, split, s);
-    const auto launch = p.parts == 3   ? (p.mt == 2 ? launch_tile<3, 2> : launch_tile<3, 1>)
-                        : p.parts == 2 ? (p.mt == 2 ? launch_tile<2, 2> : launch_tile<2, 1>)
-                                       : (p.mt == 2 ? launch_tile<1, 2> : launch_tile<1, 1>);
+    const auto launch = p.parts == 3 ? launch_tile<3, 1> : p.parts == 2 ? launch_tile<2, 1> : p.mt == 2 ? launch_tile<1, 2> : launch_tile<1, 1>;
     launch(a, p, split, part, part_db, s);
     if (!p.joined && !a.db) return;
     if (a.out_type == WC_F32) launch_join<float>(a, p, part, part_db, s);

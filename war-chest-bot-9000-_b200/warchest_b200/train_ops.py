@@ -100,13 +100,14 @@ def _row_stride(what: str, name: str, t: torch.Tensor) -> int:
 def _vector(what: str, name: str, t: Optional[torch.Tensor], n: int, like: torch.Tensor) -> int:
     if t is None:
         return 0
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != n or t.device != like.device or not t.is_contiguous():
+    if t.dtype != torch.float32 or t.dim() != 1 or t.numel() != n or t.get_device() != like.get_device() or not t.is_contiguous():
         _fail(what, f"{name} must be {n} contiguous float32 values on {like.device}")
     return t.data_ptr()
 
 
-def _scratch(n: int, device: torch.device) -> torch.Tensor:
-    return torch.empty(max(16, n), dtype=torch.uint8, device=device)
+# (Tensor.new_empty takes half as long as torch.empty, which is given a type and a device to look up.)
+def _scratch(n: int, like: torch.Tensor) -> torch.Tensor:
+    return like.new_empty(max(16, n), dtype=torch.uint8)
 
 
 def _call(fn, index: int, *args) -> None:
@@ -141,10 +142,10 @@ def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp
     me = "policy_loss"
     ld = _matrix(me, "logits", logits)
     rows, width = logits.shape
-    device = logits.device
-    if actions.dtype not in (torch.int64, torch.int32) or actions.dim() != 1 or actions.shape[0] != rows or \
-            actions.device != device or not actions.is_contiguous():
-        _fail(me, f"actions must be {rows} contiguous int64 or int32 values on {device}")
+    index = logits.get_device()
+    if actions.dtype not in (torch.int64, torch.int32) or actions.dim() != 1 or actions.numel() != rows or \
+            actions.get_device() != index or not actions.is_contiguous():
+        _fail(me, f"actions must be {rows} contiguous int64 or int32 values on {logits.device}")
     if old_logp is None or advantages is None:
         _fail(me, "old_logp and advantages are needed")
     old = _vector(me, "old_logp", old_logp, rows, logits)
@@ -153,18 +154,18 @@ def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp
     ref = _vector(me, "ref_logp", ref_logp, rows, logits)
     up = on = ld_legal = 0
     if upstream is not None:
-        if upstream.dtype != torch.float32 or upstream.numel() != 1 or upstream.device != device:
+        if upstream.dtype != torch.float32 or upstream.numel() != 1 or upstream.get_device() != index:
             _fail(me, "upstream must be one float32 value on the logits' device")
         up = upstream.data_ptr()
     if legal is not None:
-        if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or legal.device != device:
+        if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or legal.get_device() != index:
             _fail(me, "legal must be a bool or uint8 matrix of the logits' shape and device")
         on, ld_legal = legal.data_ptr(), _row_stride(me, "legal", legal)
     space = _policy_workspace(rows, width)
-    flat = torch.empty(space + 4 * rows + 1, dtype=torch.float32, device=device)  # workspace, rows, loss
-    grad = torch.empty((rows, width), dtype=logits.dtype, device=device) if want_grad else None
+    flat = old_logp.new_empty(space + 4 * rows + 1)  # workspace, rows, loss
+    grad = logits.new_empty(rows, width) if want_grad else None
     at = flat.data_ptr()
-    _call(lib().wc_policy_loss, device.index, _POLICY_LOSS.pack(
+    _call(lib().wc_policy_loss, index, _POLICY_LOSS.pack(
         logits.data_ptr(), on, actions.data_ptr(), old, adv, wts, ref, up, at + 4 * (space + 4 * rows), at + 4 * space,
         grad.data_ptr() if want_grad else 0, at, rows, width, ld, ld_legal, max(1, width), clip_low, clip_high, kl_coef,
         entropy_coef, _TYPES[logits.dtype], actions.element_size()))
@@ -194,8 +195,8 @@ def _norm_args(me, x, h, gate, rows_per_gate, residual_scale, post, pre, kind, e
         per = rows_per_gate if rows_per_gate is not None else max(1, rows)
         if per < 1:
             _fail(me, "rows_per_gate below 1")
-        if gate.dim() != 2 or tuple(gate.shape) != (-(-rows // per), width) or gate.dtype != x.dtype or \
-                gate.device != x.device or not gate.is_contiguous():
+        if gate.shape != (-(-rows // per), width) or gate.dtype != x.dtype or \
+                gate.get_device() != x.get_device() or not gate.is_contiguous():
             _fail(me, f"gate must be a contiguous {-(-rows // per)} x {width} matrix of x's type and device")
         gp = gate.data_ptr()
     there = _weight(me, "post", post, x) + _weight(me, "pre", pre, x)
@@ -219,19 +220,18 @@ def block_norm(x, h, *, gate=None, rows_per_gate=None, residual_scale=1.0, post=
     me = "block_norm"
     args, there = _norm_args(me, x, h, gate, rows_per_gate, residual_scale, post, pre, kind, eps)
     rows, width = x.shape
-    device = x.device
-    y = torch.empty((rows, width), dtype=x.dtype, device=device)
-    stats = torch.empty((rows, 4), dtype=torch.float32, device=device)
+    y = x.new_empty(rows, width)
+    stats = x.new_empty((rows, 4), dtype=torch.float32)
     n = n8 = None
     if there[2]:
-        n = torch.empty((rows, width), dtype=x.dtype, device=device)
+        n = x.new_empty(rows, width)
         if pack:
             n8 = _new_act8(x)
     elif pack:
         _fail(me, "pack needs a pre norm")
-    _call(lib().wc_block_norm, device.index, args(y.data_ptr(), n.data_ptr() if n is not None else 0,
-                                                  n8.q.data_ptr() if n8 else 0, n8.scale.data_ptr() if n8 else 0,
-                                                  stats.data_ptr()))
+    _call(lib().wc_block_norm, x.get_device(), args(y.data_ptr(), n.data_ptr() if n is not None else 0,
+                                                    n8.q.data_ptr() if n8 else 0, n8.scale.data_ptr() if n8 else 0,
+                                                    stats.data_ptr()))
     return BlockNorm(y, n, n8, stats)
 
 
@@ -242,20 +242,17 @@ def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, r
     me = "block_norm_backward"
     args, there = _norm_args(me, x, h, gate, rows_per_gate, residual_scale, post, pre, kind, eps)
     rows, width = x.shape
-    device = x.device
-    if stats.dtype != torch.float32 or tuple(stats.shape) != (rows, 4) or stats.device != device or \
+    if stats.dtype != torch.float32 or stats.shape != (rows, 4) or stats.get_device() != x.get_device() or \
             not stats.is_contiguous():
         _fail(me, f"stats must be the forward's contiguous float32 {rows} x 4 matrix")
     packed = args(0, 0, 0, 0, stats.data_ptr())
     ld_dy = _matrix(me, "dy", dy, x) if dy is not None else 0
     ld_dn = _matrix(me, "dn", dn, x) if dn is not None else 0
-    dx = torch.empty((rows, width), dtype=x.dtype, device=device)
-    dh = torch.empty((rows, width), dtype=x.dtype, device=device)
+    dx, dh = x.new_empty(rows, width), x.new_empty(rows, width)
     dgate = torch.empty_like(gate) if gate is not None else None
-    flat = torch.empty((4, width), dtype=torch.float32, device=device)
-    grads = [g if w else None for g, w in zip(flat.unbind(0), there)]
-    scratch = _scratch(lib().wc_block_norm_workspace(packed), device)
-    _call(lib().wc_block_norm_backward, device.index, packed, _BLOCK_NORM_GRADS.pack(
+    grads = [x.new_empty(width, dtype=torch.float32) if w else None for w in there]
+    scratch = _scratch(lib().wc_block_norm_workspace(packed), x)
+    _call(lib().wc_block_norm_backward, x.get_device(), packed, _BLOCK_NORM_GRADS.pack(
         dy.data_ptr() if dy is not None else 0, dn.data_ptr() if dn is not None else 0, dx.data_ptr(), dh.data_ptr(),
         dgate.data_ptr() if dgate is not None else 0, *[g.data_ptr() if g is not None else 0 for g in grads],
         scratch.data_ptr(), ld_dy, ld_dn, max(1, width), max(1, width)))
@@ -267,17 +264,15 @@ def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, r
 def _new_act8(like: torch.Tensor) -> Act8:
     rows, width = like.shape
     blocks = -(-width // BLOCK)
-    device = like.device
-    return Act8(torch.empty((rows, blocks * BLOCK), dtype=torch.int8, device=device),
-                torch.empty((rows, blocks), dtype=torch.uint8, device=device), width)
+    return Act8(like.new_empty((rows, blocks * BLOCK), dtype=torch.int8), like.new_empty((rows, blocks), dtype=torch.uint8), width)
 
 
 def _check_act8(what: str, a: Act8) -> None:
     q, scale, width = a
     blocks = -(-width // BLOCK)
-    if q.dtype != torch.int8 or scale.dtype != torch.uint8 or not q.is_cuda or q.device != scale.device or \
-            q.dim() != 2 or scale.dim() != 2 or tuple(q.shape) != (scale.shape[0], blocks * BLOCK) or \
-            scale.shape[1] != blocks or not q.is_contiguous() or not scale.is_contiguous():
+    if q.dtype != torch.int8 or scale.dtype != torch.uint8 or not q.is_cuda or q.get_device() != scale.get_device() or \
+            scale.dim() != 2 or q.shape != (scale.shape[0], blocks * BLOCK) or scale.shape[1] != blocks or \
+            not q.is_contiguous() or not scale.is_contiguous():
         _fail(what, "not an 8-bit matrix: q int8 [rows, 32 blocks] and scale uint8 [rows, blocks], contiguous")
 
 
@@ -286,7 +281,7 @@ def act8_pack(x) -> Act8:
     ld = _matrix("act8_pack", "x", x)
     rows, width = x.shape
     p = _new_act8(x)
-    _call(lib().wc_act8_pack, x.device.index, _ACT8.pack(
+    _call(lib().wc_act8_pack, x.get_device(), _ACT8.pack(
         x.data_ptr(), 0, p.q.data_ptr(), p.scale.data_ptr(), 0, 0, 0, rows, width, ld, 0, _TYPES[x.dtype]))
     return p
 
@@ -296,9 +291,9 @@ def act8_unpack(p: Act8, dtype=torch.bfloat16) -> torch.Tensor:
     _check_act8("act8_unpack", p)
     if dtype not in _TYPES:
         _fail("act8_unpack", "dtype must be float32, float16 or bfloat16")
-    rows, width, device = p.q.shape[0], p.width, p.q.device
-    out = torch.empty((rows, width), dtype=dtype, device=device)
-    _call(lib().wc_act8_unpack, device.index, _ACT8.pack(
+    rows, width = p.q.shape[0], p.width
+    out = p.q.new_empty((rows, width), dtype=dtype)
+    _call(lib().wc_act8_unpack, p.q.get_device(), _ACT8.pack(
         0, 0, p.q.data_ptr(), p.scale.data_ptr(), out.data_ptr(), 0, 0, rows, width, 0, max(1, width), _TYPES[dtype]))
     return out
 
@@ -309,8 +304,8 @@ def gelu8(z, bias=None) -> Tuple[torch.Tensor, Act8]:
     rows, width = z.shape
     b = _vector("gelu8", "bias", bias, width, z)
     p = _new_act8(z)
-    out = torch.empty((rows, width), dtype=z.dtype, device=z.device)
-    _call(lib().wc_gelu8, z.device.index, _ACT8.pack(
+    out = z.new_empty(rows, width)
+    _call(lib().wc_gelu8, z.get_device(), _ACT8.pack(
         z.data_ptr(), b, p.q.data_ptr(), p.scale.data_ptr(), out.data_ptr(), 0, 0, rows, width, ld, max(1, width),
         _TYPES[z.dtype]))
     return out, p
@@ -327,15 +322,14 @@ def gelu8_backward(da, z8: Act8, want_bias=True):
     ld = _matrix(me, "da", da)
     _check_act8(me, z8)
     rows, width = da.shape
-    device = da.device
-    if z8.width != width or z8.q.shape[0] != rows or z8.q.device != device:
+    if z8.width != width or z8.q.shape[0] != rows or z8.q.get_device() != da.get_device():
         _fail(me, "da and the 8-bit activations differ in shape or device")
-    dz = torch.empty((rows, width), dtype=da.dtype, device=device)
+    dz = da.new_empty(rows, width)
     dbias = scratch = None
     if want_bias:
-        dbias = torch.empty(width, dtype=torch.float32, device=device)
-        scratch = _scratch(_gelu8_workspace(rows, width), device)
-    _call(lib().wc_gelu8_backward, device.index, _ACT8.pack(
+        dbias = da.new_empty(width, dtype=torch.float32)
+        scratch = _scratch(_gelu8_workspace(rows, width), da)
+    _call(lib().wc_gelu8_backward, da.get_device(), _ACT8.pack(
         da.data_ptr(), 0, z8.q.data_ptr(), z8.scale.data_ptr(), dz.data_ptr(), dbias.data_ptr() if want_bias else 0,
         scratch.data_ptr() if want_bias else 0, rows, width, ld, max(1, width), _TYPES[da.dtype]))
     return dz, dbias
@@ -349,19 +343,18 @@ def act8_wgrad(x8: Act8, dy, *, dtype=torch.float32, want_bias=True):
     ld = _matrix(me, "dy", dy)
     _check_act8(me, x8)
     rows, n = dy.shape
-    device = dy.device
-    if x8.q.shape[0] != rows or x8.q.device != device:
+    if x8.q.shape[0] != rows or x8.q.get_device() != dy.get_device():
         _fail(me, "dy and the 8-bit activations differ in rows or device")
     if dtype not in _TYPES:
         _fail(me, "dtype must be float32, float16 or bfloat16")
-    dw = torch.empty((x8.width, n), dtype=dtype, device=device)
-    db = torch.empty(n, dtype=torch.float32, device=device) if want_bias else None
+    dw = dy.new_empty((x8.width, n), dtype=dtype)
+    db = dy.new_empty(n, dtype=torch.float32) if want_bias else None
 
     def args(workspace):
         return _ACT8_WGRAD.pack(x8.q.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), dw.data_ptr(),
                                 db.data_ptr() if want_bias else 0, workspace, rows, x8.width, n, ld, _TYPES[dy.dtype],
                                 _TYPES[dtype])
 
-    scratch = _scratch(lib().wc_act8_wgrad_workspace(args(0)), device)
-    _call(lib().wc_act8_wgrad, device.index, args(scratch.data_ptr()))
+    scratch = _scratch(lib().wc_act8_wgrad_workspace(args(0)), dy)
+    _call(lib().wc_act8_wgrad, dy.get_device(), args(scratch.data_ptr()))
     return dw, db
