@@ -19,9 +19,8 @@
 // part of a warp; longer ones in the shared memory of a CTA, or of a cluster of
 // CTAs that exchange (m, S, sum) through distributed shared memory, until the
 // gradient is written. Entries are handled in chunks of 16 bytes; rows that
-// chunks do not fit have the chunks they lie in, or (short ones) entries one by
-// one, a warp's next to each other. Rows that no cluster can hold are read twice
-// by one CTA (the second time mostly from L2).
+// chunks do not fit have the chunks they lie in. Rows that no cluster can hold
+// are read twice by one CTA (the second time mostly from L2).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -140,6 +139,13 @@ struct Chunk {
     static constexpr uint32_t INF = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
     alignas(16) uint32_t z[4];
     __device__ __forceinline__ void load(const T* at) { *reinterpret_cast<uint4*>(z) = __ldcs(reinterpret_cast<const uint4*>(at)); }
+    // from and to shared memory, by its own addresses
+    __device__ __forceinline__ void read(uint32_t at) {
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(z[0]), "=r"(z[1]), "=r"(z[2]), "=r"(z[3]) : "r"(at) : "memory");
+    }
+    __device__ __forceinline__ void write(uint32_t at) const {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(z[0]), "r"(z[1]), "r"(z[2]), "r"(z[3]) : "memory");
+    }
     __device__ __forceinline__ void none() { z[0] = z[1] = z[2] = z[3] = INF; }
     // legal bytes, in the order of the entries
     __device__ __forceinline__ void mask(uint2 legal) {
@@ -173,45 +179,45 @@ struct Chunk {
     }
 };
 
-template <class T, int NV>
-__device__ __forceinline__ float local_max(const Chunk<T>* q) {
-    if constexpr (sizeof(T) == 4) {
-        float m = -INFINITY;
+// The largest entry of chunks (NaN is left to the sums)
+template <class T>
+struct Largest {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    static constexpr bool WIDE = sizeof(T) == 4;
+    uint32_t m = Chunk<T>::INF;
+    __device__ __forceinline__ void add(const Chunk<T>& q) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m = fmaxf(m, __uint_as_float(q[i].z[k]));
-        return m;
-    } else {
-        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-        T2 m = *reinterpret_cast<const T2*>(&q[0].z[0]);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) m = __hmax2(m, *reinterpret_cast<const T2*>(&q[i].z[k]));
-        return fmaxf(to_f(m.x), to_f(m.y));
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (WIDE) m = __float_as_uint(fmaxf(__uint_as_float(m), __uint_as_float(q.z[k])));
+            else {
+                const T2 v = __hmax2(*reinterpret_cast<const T2*>(&m), *reinterpret_cast<const T2*>(&q.z[k]));
+                m = *reinterpret_cast<const uint32_t*>(&v);
+            }
+        }
     }
-}
+    __device__ __forceinline__ float get() const {
+        if constexpr (WIDE) return __uint_as_float(m);
+        else {
+            const T2 v = *reinterpret_cast<const T2*>(&m);
+            return fmaxf(to_f(v.x), to_f(v.y));
+        }
+    }
+};
 // One entry's share of the sums from c on
 __device__ __forceinline__ void add_entry(float z, float f, float c, float& s, float& w) {
     const float x = above(fmaf(z, f, -c)), e = ex2(x);
     s += e;
     w = fmaf(e, x, w);
 }
-// ... of NV chunks, by pairs
-template <class T, int NV>
-__device__ __forceinline__ float2 local_sums(const Chunk<T>* q, float m) {
-    const Pair f = twice(factor(m)), c = twice(-scaled(m));
-    Pair s = 0, w = 0;  // (pairs of zeros)
+// ... of a chunk, by pairs
+template <class T>
+__device__ __forceinline__ void add_chunk(const Chunk<T>& q, Pair f, Pair c, Pair& s, Pair& w) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int k = 0; k < Chunk<T>::N / 2; ++k) {
-            const Pair t = fma(q[i].pair(k), f, c), x = umma::f2(above(umma::f2_lo(t)), above(umma::f2_hi(t)));
-            const Pair e = umma::f2(ex2(umma::f2_lo(x)), ex2(umma::f2_hi(x)));
-            s = add(s, e), w = fma(e, x, w);
-        }
-    return make_float2(both(s), both(w));
+    for (int k = 0; k < Chunk<T>::N / 2; ++k) {
+        const Pair t = fma(q.pair(k), f, c), x = umma::f2(above(umma::f2_lo(t)), above(umma::f2_hi(t)));
+        const Pair e = umma::f2(ex2(umma::f2_lo(x)), ex2(umma::f2_hi(x)));
+        s = add(s, e), w = fma(e, x, w);
+    }
 }
 // The gradient of a chunk. (At the action it is not all: the thread that writes the action's chunk writes that entry
 // after it, which costs one store a row and nothing an entry.)
@@ -237,38 +243,58 @@ template <class T>
 __device__ __forceinline__ void put_chunk(T* out, const T* e) {
     __stcs(reinterpret_cast<uint4*>(out), *reinterpret_cast<const uint4*>(e));
 }
-// A row's logits in registers: NV chunks of `lanes` threads. VEC: 16 bytes at a time; else an entry at a time, chunk i's
-// k-th being the row's ((i N + k) lanes + at)-th.
+// The bytes of entries col .. col + 7 that lie in a row: all bits, or none
+__device__ __forceinline__ uint2 inside(int col, int width) {
+    const uint64_t m = (~0ull << (8 * max(0, -col))) & (~0ull >> (8 * max(0, min(7, col + 8 - width))));
+    return make_uint2((uint32_t)m, (uint32_t)(m >> 32));
+}
+// A row's logits in registers: NV chunks of `lanes` threads. VEC: the row starts and ends with a chunk. Else it starts
+// `before` entries into its first, and chunks are read with what lies there of the rows before and after (`edge`: a row
+// that has too little of them around is read entry by entry); the legal bytes of a chunk start anywhere.
 template <class T, bool MASK, bool VEC, int NV>
-__device__ __forceinline__ void load_row(Chunk<T>* q, const T* z, const uint8_t* legal, bool read, int at, int lanes, int width) {
+__device__ __forceinline__ void load_row(Chunk<T>* q, const T* z, const uint8_t* legal, bool read, int at, int lanes, int width, int before, bool edge) {
     constexpr int N = Chunk<T>::N;
-    if constexpr (VEC) {
-        uint2 on[MASK ? NV : 1];
+    if (!VEC && edge) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (i * lanes + at) * N;
-            if (read && c < width) {
-                q[i].load(z + c);
-                if constexpr (MASK) on[i] = Chunk<T>::load_legal(legal + c);
-            } else {
-                q[i].none();
-                if constexpr (MASK) on[i] = make_uint2(0, 0);
-            }
-        }
-        if constexpr (MASK)
-#pragma unroll
-            for (int i = 0; i < NV; ++i) q[i].mask(on[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
+            const int c = (i * lanes + at) * N - before;
             alignas(16) T e[N];
 #pragma unroll
             for (int k = 0; k < N; ++k) {
-                const int c = (i * N + k) * lanes + at;
                 e[k] = from_f<T>(-INFINITY);
-                if (read && c < width && (!MASK || legal[c])) e[k] = z[c];
+                if (read && c + k >= 0 && c + k < width && (!MASK || legal[c + k])) e[k] = z[c + k];
             }
             *reinterpret_cast<uint4*>(q[i].z) = *reinterpret_cast<const uint4*>(e);
+        }
+        return;
+    }
+    uint2 on[MASK ? NV : 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * lanes + at) * N - before;
+        if (read && c < width) {
+            q[i].load(z + c);
+            if constexpr (MASK && VEC) on[i] = Chunk<T>::load_legal(legal + c);
+            if constexpr (MASK && !VEC) {
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(legal + c) & ~3ull);
+                const int by = 8 * (int)(reinterpret_cast<uintptr_t>(legal + c) & 3);
+                const uint32_t w1 = __ldg(w + 1);
+                on[i] = make_uint2(__funnelshift_r(__ldg(w), w1, by), N == 8 ? __funnelshift_r(w1, __ldg(w + 2), by) : 0u);
+            }
+        } else {
+            q[i].none();
+            if constexpr (MASK) on[i] = make_uint2(0, 0);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if constexpr (VEC) {
+            if constexpr (MASK) q[i].mask(on[i]);
+        } else {
+            const int c = (i * lanes + at) * N - before;
+            uint2 m = inside(c, width);
+            if constexpr (MASK) m.x &= on[i].x, m.y &= on[i].y;
+            if (MASK || c < 0 || c + N > width) q[i].mask(m);
         }
     }
 }
@@ -296,17 +322,15 @@ __device__ __forceinline__ void join(const float4* parts, int n, float& M, float
 }
 
 template <bool VEC, class T>
-__device__ __forceinline__ void put(T* out, const T* e, int i, int at, int lanes, int width) {
+__device__ __forceinline__ void put(T* out, const T* e, int i, int at, int lanes, int width, int before, bool same) {
     constexpr int N = Chunk<T>::N;
-    if constexpr (VEC) {
-        const int c = (i * lanes + at) * N;
+    const int c = (i * lanes + at) * N - before;
+    if (VEC || (same && c >= 0 && c + N <= width)) {
         if (c < width) put_chunk(out + c, e);
     } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const int c = (i * N + k) * lanes + at;
-            if (c < width) out[c] = e[k];
-        }
+        for (int k = 0; k < N; ++k)
+            if (c + k >= 0 && c + k < width) out[c + k] = e[k];
     }
 }
 
@@ -328,15 +352,27 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss
         Chunk<T> q[NV];
         float za = -INFINITY;
         if (r.act >= 0 && (!MASK || legal[r.act])) za = to_f(z[r.act]);
-        load_row<T, MASK, VEC, NV>(q, z, legal, r.act >= 0, at, lanes, width);
+        const int before = VEC ? 0 : (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+        const int64_t row = in ? t : 0, rest = a.rows - 1 - row, ld = MASK ? min(a.ld_logits, a.ld_legal) : a.ld_logits;
+        const bool edge = !VEC && (row * ld < 16 || rest * ld < 16);
+        load_row<T, MASK, VEC, NV>(q, z, legal, r.act >= 0, at, lanes, width, before, edge);
         next = RowIn(a, t + stride);
         const bool live = za != -INFINITY;
-        float m = local_max<T, NV>(q);
+        Largest<T> most;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) most.add(q[i]);
+        float m = most.get();
         for (int o = lanes >> 1; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        float2 sw = local_sums<T, NV>(q, live ? m : 0.0f);
+        const Pair f = twice(factor(live ? m : 0.0f)), c = twice(-scaled(live ? m : 0.0f));
+        Pair sum = 0, mean = 0;  // (pairs of zeros)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) add_chunk(q[i], f, c, sum, mean);
+        float2 sw = make_float2(both(sum), both(mean));
         for (int o = lanes >> 1; o; o >>= 1) sw.x += __shfl_xor_sync(~0u, sw.x, o), sw.y += __shfl_xor_sync(~0u, sw.y, o);
         if (!in) continue;
         T* out = a.dlogits ? static_cast<T*>(a.dlogits) + t * a.ld_dlogits : nullptr;
+        // the gradient's chunks are the logits' if they start at the same place of 16 bytes
+        const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == before * sizeof(T);
         if (live) {
             const Row row(a, r, m, sw.x, sw.y, za);
             if (at == 0) row.put(a, t), total += (double)(r.w * row.loss);
@@ -345,9 +381,9 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss
             for (int i = 0; i < NV; ++i) {
                 alignas(16) T e[N];
                 chunk_grad<T, ENTROPY>(q[i], row, e);
-                put<VEC>(out, e, i, at, lanes, width);
+                put<VEC>(out, e, i, at, lanes, width, before, same);
             }
-            if (((VEC ? r.act / N : r.act) & (lanes - 1)) == at) out[r.act] = from_f<T>(row.grad<ENTROPY>(za) + row.g);
+            if ((((r.act + before) / N) & (lanes - 1)) == at) out[r.act] = from_f<T>(row.grad<ENTROPY>(za) + row.g);
         } else {
             if (at == 0) put_void(a, t);
             alignas(16) T e[N];
@@ -355,7 +391,7 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss
             for (int k = 0; k < N; ++k) e[k] = from_f<T>(0.0f);
             if (out)
 #pragma unroll
-                for (int i = 0; i < NV; ++i) put<VEC>(out, e, i, at, lanes, width);
+                for (int i = 0; i < NV; ++i) put<VEC>(out, e, i, at, lanes, width, before, same);
         }
     }
 #pragma unroll
@@ -369,14 +405,12 @@ __global__ void __launch_bounds__(256, VEC ? 4 : 2) k_policy_warp(wc_policy_loss
 }
 
 // Longer rows: one CTA, or the CTAs of a cluster, a row, each with a slice of
-// it. Slices come into shared memory by bulk copies, and stay until the
-// gradient is written: while a row's parts go round the cluster and its first
-// warp forms the loss, the other warps write the gradient of the row before and
-// sum up the row after. In the order of a CTA's rows, step by step:
-//   sums of row i + 1, its parts sent
-//   gradient of row i
-//   the first warp joins the parts of row i + 1
-constexpr int SLICES = 3;
+// it, which bulk copies bring into shared memory and which stays there until
+// the gradient is written. A warp of its own starts the copies, joins the
+// cluster's parts of a row and forms its loss (some thousand cycles in a chain)
+// while the other warps, in the order of the CTA's rows, take the sums of row
+// i + 1 and write the gradient of row i. With that done by the first of the
+// working warps instead, 2048 x 131072 in bf16 took 325 us.
 // 16 bytes into the shared memory of a CTA of the cluster (both addresses mapped to it), counted by its barrier. No
 // fence: a cluster barrier's release would wait for the gradient's stores as well.
 __device__ __forceinline__ void send(uint32_t to, float4 v, uint32_t bar) {
@@ -389,14 +423,17 @@ __device__ __forceinline__ uint32_t of_rank(uint32_t addr, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
-// FIT: every row starts and ends with a chunk (of the legal bytes: with 16).
-template <class T, bool MASK, bool FIT, int NV, int THREADS, int CTAS>
-__global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_policy_cluster(wc_policy_loss_args a, int slice, double* part) {
-    constexpr int N = Chunk<T>::N, WARPS = THREADS / 32;
-    extern __shared__ __align__(128) uint8_t ring[];  // SLICES of the logits, then of the legal bytes
-    __shared__ float4 parts[3][CTAS * WARPS];         // of every warp of the cluster, three (live) rows in turn
-    __shared__ Row rows[2];                           // what the first warp made of them, two rows in turn
-    __shared__ uint64_t full[SLICES], joined[3];
+constexpr int MAX_SLICES = 4;
+template <class T, bool MASK, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 ? 4 : 6) k_policy_cluster(wc_policy_loss_args a, int slice, int slices, double* part) {
+    constexpr int N = Chunk<T>::N, THREADS = WARPS * 32;
+    constexpr int TOGETHER = 1;
+    extern __shared__ __align__(128) uint8_t ring[];  // `slices` of the logits, then of the legal bytes
+    __shared__ float4 parts[4][CTAS * WARPS];         // of every warp of the cluster, four (live) rows in turn
+    __shared__ Row rows[2];                           // what was made of them, two in turn
+    __shared__ float2 meta[MAX_SLICES];               // a slice's row: its action (-1: void) and the logit there
+    __shared__ uint64_t full[MAX_SLICES], empty[MAX_SLICES], joined[4], ready[2];
+    __shared__ int failed;
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = CTAS > 1 ? (int)cluster.block_rank() : 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -407,182 +444,270 @@ __global__ void __launch_bounds__(THREADS, (FIT ? 1024 : 512) / THREADS) k_polic
     // whole chunks, with what lies there of the rows before and after; the matrix's first and last row, which have none,
     // are read where they are if they do not fill theirs.
     auto row_at = [&](int64_t t) { return static_cast<const T*>(a.logits) + t * a.ld_logits; };
-    auto before = [&](int64_t t) { return FIT ? 0 : (int)((reinterpret_cast<uintptr_t>(row_at(t)) & 15) / sizeof(T)); };
+    auto before = [&](int64_t t) { return (int)((reinterpret_cast<uintptr_t>(row_at(t)) & 15) / sizeof(T)); };
     auto width_of = [&](int b) { return min(slice, max(0, (int)a.width + b - first)); };
     auto in_place = [&](int64_t t) {
-        if (FIT || (t != 0 && t != a.rows - 1)) return false;
+        if (t != 0 && t != a.rows - 1) return false;
         return before(t) != 0 || (a.width + before(t)) % N != 0 || (MASK && (((uintptr_t)(a.legal + t * a.ld_legal) & 15) != 0 || a.width % 16 != 0));
     };
-    uint8_t* masks = ring + SLICES * slice * sizeof(T);
+    uint8_t* masks = ring + slices * slice * sizeof(T);
+    auto arrive = [](uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory"); };
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLICES; ++i) umma::mbar_init(&full[i], 1);
-        for (int i = 0; i < 3; ++i) umma::mbar_init(&joined[i], 1);
+        for (int i = 0; i < slices; ++i) umma::mbar_init(&full[i], 1), umma::mbar_init(&empty[i], WARPS);
+        for (int i = 0; i < 4; ++i) umma::mbar_init(&joined[i], CTAS > 1 ? 1 : WARPS);
+        for (int i = 0; i < 2; ++i) umma::mbar_init(&ready[i], 1);
+        failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (CTAS > 1) cluster.sync();
     else __syncthreads();
-    // thread 0: the slice of the CTA's row i
-    auto copy = [&](int64_t i, int act) {
-        const int64_t t = t0 + i * step;
-        if (t >= a.rows) return;
-        const int slot = (int)(i % SLICES), b = before(t), width = width_of(b);
-        if (act < 0 || !width || in_place(t)) {
-            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(&full[slot])) : "memory");
-            return;
-        }
-        const uint32_t bytes = (width + N - 1) / N * 16;
-        const uint8_t* on = MASK ? a.legal + t * a.ld_legal + max(0, first - b) : nullptr;
-        const uint32_t skew = (uint32_t)((uintptr_t)on & 15), on_bytes = MASK ? (skew + width - (first ? 0 : b) + 15) / 16 * 16 : 0;
-        umma::expect_tx(&full[slot], bytes + on_bytes);
-        umma::bulk_g2s(ring + slot * slice * sizeof(T), row_at(t) - b + first, bytes, &full[slot]);
-        if (MASK) umma::bulk_g2s(masks + slot * (slice + 32), on - skew, on_bytes, &full[slot]);
-    };
-    // The chunk at `at` of the CTA's share of row t
-    auto chunk = [&](int64_t t, int slot, int b, int at) {
-        Chunk<T> q;
-        const int col = first + at - b;
-        const bool whole = FIT || (col >= 0 && col + N <= a.width);
-        if (in_place(t)) {
-            alignas(16) T e[N];
-            for (int k = 0; k < N; ++k) {
-                e[k] = from_f<T>(-INFINITY);
-                if (col + k >= 0 && col + k < a.width && (!MASK || a.legal[t * a.ld_legal + col + k])) e[k] = row_at(t)[col + k];
-            }
-            *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(e);
-            return q;
-        }
-        *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(ring + (slot * slice + at) * sizeof(T));
-        if constexpr (MASK) {
-            // the bytes of the chunk's entries start anywhere
-            const uint8_t* on = a.legal + t * a.ld_legal + max(0, first - b);
-            const int from = (int)((uintptr_t)on & 15) + col - max(0, first - b);
-            const uint8_t* base = masks + slot * (slice + 32);
-            if (FIT) {
-                if constexpr (N == 8) q.mask(*reinterpret_cast<const uint2*>(base + at));
-                else q.mask(make_uint2(*reinterpret_cast<const uint32_t*>(base + at), 0));
-            } else if (whole) {
-                const uint32_t* w = reinterpret_cast<const uint32_t*>(base + (from & ~3));
-                const int by = 8 * (from & 3);
-                q.mask(make_uint2(__funnelshift_r(w[0], w[1], by), N == 8 ? __funnelshift_r(w[1], w[2], by) : 0u));
-            } else {
-                uint32_t m[2] = {0, 0};
-                for (int k = 0; k < N; ++k)
-                    if (col + k >= 0 && col + k < a.width) m[k >> 2] |= (uint32_t)base[from + k] << (8 * (k & 3));
-                q.mask(make_uint2(m[0], m[1]));
-            }
-        } else if (!whole) {
-            uint32_t m[2] = {0, 0};
-            for (int k = 0; k < N; ++k)
-                if (col + k >= 0 && col + k < a.width) m[k >> 2] |= 1u << (8 * (k & 3));
-            q.mask(make_uint2(m[0], m[1]));
-        }
-        return q;
-    };
-    auto logit = [&](int64_t t, int act) {
-        if (act < 0 || (MASK && !a.legal[t * a.ld_legal + act])) return -INFINITY;
-        return to_f(static_cast<const T*>(a.logits)[t * a.ld_logits + act]);
-    };
-    // The scalars of rows i + 1, i + 2 and i + 3: a load's result is asked for a row later, so that nothing waits for it.
-    RowIn in1(a, t0), in2(a, t0 + step), in3(a, t0 + 2 * step);
-    float za1 = logit(t0, in1.act), za2 = logit(t0 + step, in2.act);
-    if (threadIdx.x == 0) copy(0, in1.act), copy(1, in2.act);
     double total = 0.0;
-    bool bad = false, live0 = false;
-    int act0 = -1;
-    float za0 = 0.0f;
-    int turn = 0;         // of parts[] and joined[]
-    uint32_t phases = 0;  // of joined[]
-    for (int64_t i = -1, t = t0 - step; t < a.rows; ++i, t += step) {
-        const int64_t t1 = t + step;
-        const int slot1 = (int)((i + 1) % SLICES), turn1 = (int)(i + 1) & 1;
-        const bool live1 = za1 != -INFINITY;
-        // a copy that does not come (umma.cuh) leaves NaN in the rows from here on, after those in flight have landed
-        if (t1 < a.rows && !bad && !umma::mbar_wait(&full[slot1], (uint32_t)((i + 1) / SLICES) & 1)) bad = true;
-        if (live1) {
-            Chunk<T> q[NV];
-            const int b = before(t1), width = width_of(b);
-#pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int at = (k * THREADS + (int)threadIdx.x) * N;
-                if (at < width) q[k] = chunk(t1, slot1, b, at);
-                else q[k].none();
-            }
-            float m = local_max<T, NV>(q);
-#pragma unroll
-            for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-            if (m == -INFINITY) m = 0.0f;  // nothing here counts (or is a number): its sums are 0 (or NaN)
-            float2 v = local_sums<T, NV>(q, m);
-            v.x = warp_sum(v.x), v.y = warp_sum(v.y);
-            if (bad) v.x = __uint_as_float(0x7fffffffu);
-            const float4 mine = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
-            float4* to = &parts[turn][rank * WARPS + warp];
-            // This warp's CTA has by now joined the live row before last (past the last __syncthreads). That took a part
-            // from the first warp of every CTA, sent after it had joined the row before that one: of three places in
-            // turn, the one written here has been read everywhere.
-            if (CTAS == 1 && lane == 0) *to = mine;
-            if (CTAS > 1 && lane < CTAS) send(of_rank(umma::smem_u32(to), lane), mine, of_rank(umma::smem_u32(&joined[turn]), lane));
+    // A wait that runs out (umma.cuh) leaves NaN in the rows from here on; the copies in flight land before the end.
+    bool bad = false;
+    auto wait = [&](uint64_t* bar, int64_t use) {
+        if (!bad && !umma::mbar_wait(bar, (uint32_t)use & 1)) bad = true, failed = 1;
+        bad = __any_sync(~0u, bad);  // (a warp's lanes go on together)
+    };
+    // the slice of a row, and how often it had others before
+    struct Place {
+        int slot = 0;
+        uint32_t use = 0;
+        __device__ __forceinline__ void next(int slices) {
+            if (++slot == slices) slot = 0, ++use;
         }
-        __syncthreads();  // rows[] of row i is there, and the slice of row i - 1 has been read by all
-        if (threadIdx.x == 0 && i >= 0 && !bad) copy(i + 2, in2.act);
-        if (t >= 0 && i >= 0 && a.dlogits) {
-            T* out = static_cast<T*>(a.dlogits) + t * a.ld_dlogits;
-            const Row& r = rows[turn1 ^ 1];
-            const int slot = (int)(i % SLICES), b = before(t), width = width_of(b);
-            // the gradient's chunks are the logits' if they start at the same place of 16 bytes
-            const bool same = FIT || (reinterpret_cast<uintptr_t>(out) & 15) == b * sizeof(T);
-            auto write = [&](int at, const T* e) {
-                const int col = first + at - b;
-                if (FIT || (same && col >= 0 && col + N <= a.width)) put_chunk(out + col, e);
-                else
-#pragma unroll
-                    for (int k = 0; k < N; ++k)
-                        if (col + k >= 0 && col + k < a.width) out[col + k] = e[k];
-            };
-            alignas(16) T e[N];
-            if (live0 && r.ce != 0.0f) {
-                for (int at = threadIdx.x * N; at < width; at += THREADS * N)
-                    chunk_grad<T, true>(chunk(t, slot, b, at), r, e), write(at, e);
-            } else if (live0) {
-#pragma unroll
-                for (int k = 0; k < NV; ++k) {
-                    const int at = (k * THREADS + (int)threadIdx.x) * N;
-                    if (at < width) chunk_grad<T, false>(chunk(t, slot, b, at), r, e), write(at, e);
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) e[k] = from_f<T>(0.0f);
-                for (int at = threadIdx.x * N; at < width; at += THREADS * N) write(at, e);
+    };
+    if (warp == WARPS) {
+        // Lane k has the scalars of the k-th of 32 rows, loaded 32 rows ahead of their use.
+        struct Batch {
+            RowIn in;
+            float za;
+        };
+        auto load = [&](int64_t i) {
+            const int64_t t = t0 + (i + lane) * step;
+            Batch v{RowIn(a, t), -INFINITY};
+            if (v.in.act >= 0 && (!MASK || a.legal[t * a.ld_legal + v.in.act])) v.za = to_f(row_at(t)[v.in.act]);
+            return v;
+        };
+        Batch now = load(0), next = load(32);
+        // the slice of the CTA's row i, of the batch now or next
+        auto copy = [&](int64_t i, int slot, bool later) {
+            const int from = (int)i & 31;
+            const int act = __shfl_sync(~0u, later ? next.in.act : now.in.act, from);
+            const float za = __shfl_sync(~0u, later ? next.za : now.za, from);
+            const int64_t t = t0 + i * step;
+            if (lane || t >= a.rows) return;
+            const int b = before(t), width = width_of(b);
+            const bool live = za != -INFINITY;
+            meta[slot] = make_float2(__int_as_float(live ? act : -1), za);
+            if (!live || !width || in_place(t)) {
+                arrive(&full[slot]);
+                return;
             }
-            const int mine = act0 + b - first;
-            if (live0 && mine >= 0 && mine < width && mine / N % THREADS == threadIdx.x) out[act0] = from_f<T>(r.grad<true>(za0) + r.g);
-        }
-        if (CTAS == 1) __syncthreads();
-        if (warp == 0 && t1 < a.rows) {
-            if (live1) {
-                if (CTAS > 1) {
-                    if (lane == 0) umma::expect_tx(&joined[turn], CTAS * WARPS * 16);
-                    if (!umma::mbar_wait(&joined[turn], phases >> turn & 1)) bad = true;
-                    phases ^= 1u << turn;
-                }
+            const uint32_t bytes = (width + N - 1) / N * 16;
+            const uint8_t* on = MASK ? a.legal + t * a.ld_legal + max(0, first - b) : nullptr;
+            const uint32_t skew = (uint32_t)((uintptr_t)on & 15), on_bytes = MASK ? (skew + width - (first ? 0 : b) + 15) / 16 * 16 : 0;
+            umma::expect_tx(&full[slot], bytes + on_bytes);
+            umma::bulk_g2s(ring + slot * slice * sizeof(T), row_at(t) - b + first, bytes, &full[slot]);
+            if (MASK) umma::bulk_g2s(masks + slot * (slice + 32), on - skew, on_bytes, &full[slot]);
+        };
+        for (int i = 0; i < slices; ++i) copy(i, i, false);
+        Place done;  // of the row before
+        int64_t live = 0;
+        for (int64_t i = 0, t = t0; t < a.rows; ++i, t += step) {
+            const int at = (int)i & 31;
+            if (at == 0 && i) now = next, next = load(i + 32);
+            const float za = __shfl_sync(~0u, now.za, at);
+            if (za != -INFINITY) {
+                const int turn = (int)live & 3;
+                RowIn in = now.in;
+                in.w = __shfl_sync(~0u, in.w, at), in.old = __shfl_sync(~0u, in.old, at), in.A = __shfl_sync(~0u, in.A, at), in.r = __shfl_sync(~0u, in.r, at);
+                if (CTAS > 1 && lane == 0) umma::expect_tx(&joined[turn], CTAS * WARPS * 16);
+                wait(&joined[turn], live >> 2);
                 float M, S, W;
                 join<(CTAS * WARPS + 31) / 32>(parts[turn], CTAS * WARPS, M, S, W);
                 if (bad) S = __uint_as_float(0x7fffffffu);
-                const Row row(a, in1, M, S, W, za1);
-                if (lane == 0) rows[turn1] = row;
-                if (rank == 0 && lane == 0) row.put(a, t1), total += (double)(in1.w * row.loss);
+                const Row row(a, in, M, S, W, za);
+                if (lane == 0) {
+                    rows[live & 1] = row;
+                    arrive(&ready[live & 1]);
+                    if (rank == 0) row.put(a, t), total += (double)(in.w * row.loss);
+                }
+                ++live;
             } else if (rank == 0 && lane == 0) {
-                put_void(a, t1);
+                put_void(a, t);
             }
+            // The slice of row i - 1 is free once its gradient is written, which is before the next row's parts are all
+            // here: this wait holds nothing up.
+            const int64_t ahead = i - 1 + slices;
+            if (i && t + (slices - 1) * step < a.rows) {
+                wait(&empty[done.slot], done.use);
+                if (!bad) copy(ahead, done.slot, (ahead >> 5) != (i >> 5));
+                done.next(slices);
+            }
+            __syncwarp();
         }
-        if (live1) turn = turn == 2 ? 0 : turn + 1;
-        live0 = live1, act0 = in1.act, za0 = za1;
-        in1 = in2, in2 = in3, za1 = za2;
-        za2 = logit(t1 + 2 * step, in2.act);
-        in3 = RowIn(a, t1 + 3 * step);
+    } else {
+        int64_t live = 0;  // rows with parts sent
+        int act0 = -1;
+        float za0 = 0.0f;
+        Place read, written;
+        for (int64_t i = -1, t = t0 - step; t < a.rows; ++i, t += step) {
+            const int64_t t1 = t + step;
+            int act1 = -1;
+            float za1 = 0.0f;
+            if (t1 < a.rows) {
+                const int slot = read.slot;
+                wait(&full[slot], read.use);
+                read.next(slices);
+                const float2 about = meta[slot];
+                act1 = bad ? -1 : __float_as_int(about.x), za1 = about.y;
+                if (act1 >= 0) {
+                    const int b = before(t1), width = width_of(b);
+                    const uint32_t z = umma::smem_u32(ring) + (uint32_t)(slot * slice * sizeof(T));
+                    const bool here = in_place(t1);
+                    const uint8_t* on = MASK ? a.legal + t1 * a.ld_legal + max(0, first - b) : nullptr;
+                    // legal byte of column col: base[skew + col]
+                    const uint8_t* base = masks + slot * (slice + 32);
+                    const int skew = (int)((uintptr_t)on & 15) - max(0, first - b);
+                    const bool even = ((skew + first - b) & (N - 1)) == 0;  // a chunk's bytes are one word, or two
+                    // First the maximum; a chunk whose entries do not all count goes back as what does.
+                    const int from = b - first, last = (int)a.width + from - N;  // where chunks lie in the row
+                    Largest<T> most;
+                    auto some = [&](int at) {
+                        const int col = at - from;
+                        const bool whole = at >= from && at <= last;
+                        Chunk<T> q;
+                        if (here) {
+                            alignas(16) T e[N];
+#pragma unroll
+                            for (int k = 0; k < N; ++k) {
+                                e[k] = from_f<T>(-INFINITY);
+                                if (col + k >= 0 && col + k < a.width && (!MASK || a.legal[t1 * a.ld_legal + col + k])) e[k] = row_at(t1)[col + k];
+                            }
+                            *reinterpret_cast<uint4*>(q.z) = *reinterpret_cast<const uint4*>(e);
+                        } else {
+                            q.read(z + at * sizeof(T));
+                            uint2 m = make_uint2(0, 0);
+                            if (!whole) {
+                                for (int k = 0; k < N; ++k)
+                                    if (col + k >= 0 && col + k < a.width && (!MASK || base[skew + col + k])) (k < 4 ? m.x : m.y) |= 1u << (8 * (k & 3));
+                            } else if (MASK && even) {
+                                if constexpr (N == 8) m = *reinterpret_cast<const uint2*>(base + skew + col);
+                                else m.x = *reinterpret_cast<const uint32_t*>(base + skew + col);
+                            } else if (MASK) {
+                                const uint32_t* w = reinterpret_cast<const uint32_t*>(base + ((skew + col) & ~3));
+                                const int by = 8 * ((skew + col) & 3);
+                                m = make_uint2(__funnelshift_r(w[0], w[1], by), N == 8 ? __funnelshift_r(w[1], w[2], by) : 0u);
+                            }
+                            q.mask(m);
+                        }
+                        q.write(z + at * sizeof(T));
+                        // ... before the copy that takes its place
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        most.add(q);
+                    };
+                    if (MASK || here) {
+                        for (int at = threadIdx.x * N; at < width; at += THREADS * N) some(at);
+                    } else {
+                        for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
+                            Chunk<T> q[TOGETHER];
+#pragma unroll
+                            for (int k = 0; k < TOGETHER; ++k) {
+                                const int to = at + k * THREADS * N;
+                                q[k].none();
+                                if (to < width && to >= from && to <= last) q[k].read(z + to * sizeof(T));
+                                else if (to < width) some(to);
+                            }
+#pragma unroll
+                            for (int k = 0; k < TOGETHER; ++k) most.add(q[k]);
+                        }
+                    }
+                    float m = most.get();
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+                    if (m == -INFINITY) m = 0.0f;  // nothing here counts (or is a number): its sums are 0 (or NaN)
+                    const Pair f = twice(factor(m)), c = twice(-scaled(m));
+                    Pair sum = 0, mean = 0;
+                    for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
+                        Chunk<T> q[TOGETHER];
+#pragma unroll
+                        for (int k = 0; k < TOGETHER; ++k)
+                            if (at + k * THREADS * N < width) q[k].read(z + (at + k * THREADS * N) * sizeof(T));
+#pragma unroll
+                        for (int k = 0; k < TOGETHER; ++k)
+                            if (at + k * THREADS * N < width) add_chunk(q[k], f, c, sum, mean);
+                    }
+                    const float2 v = make_float2(warp_sum(both(sum)), warp_sum(both(mean)));
+                    const float4 mine = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
+                    // Of four places in turn this one has been read everywhere: before this row a warp has written the
+                    // gradient of the live row before last, for which every CTA's parts of it were joined; they were sent
+                    // after the gradients of the live row two before that, for which each CTA had joined its parts.
+                    const int turn = (int)live & 3;
+                    float4* to = &parts[turn][rank * WARPS + warp];
+                    if (CTAS == 1 && lane == 0) *to = mine, arrive(&joined[turn]);
+                    if (CTAS > 1 && lane < CTAS) send(of_rank(umma::smem_u32(to), lane), mine, of_rank(umma::smem_u32(&joined[turn]), lane));
+                    ++live;
+                }
+            }
+            if (i >= 0) {
+                const int64_t mine = live - 1 - (act1 >= 0);  // this row among the live ones
+                if (act0 >= 0) wait(&ready[mine & 1], mine >> 1);
+                const int slot = written.slot;
+                if (a.dlogits) {
+                    const int b = before(t), width = width_of(b);
+                    const uint32_t z = umma::smem_u32(ring) + (uint32_t)(slot * slice * sizeof(T));
+                    T* out = static_cast<T*>(a.dlogits) + t * a.ld_dlogits;
+                    // the gradient's chunks are the logits' if they start at the same place of 16 bytes
+                    const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == b * sizeof(T);
+                    const int from = b - first, last = (int)a.width + from - N;  // where chunks lie in the row
+                    T* const o = out - from;
+                    auto chunks = [&](auto&& make) {
+                        for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
+                            Chunk<T> q[TOGETHER];
+#pragma unroll
+                            for (int k = 0; k < TOGETHER; ++k)
+                                if (at + k * THREADS * N < width) q[k].read(z + (at + k * THREADS * N) * sizeof(T));
+#pragma unroll
+                            for (int k = 0; k < TOGETHER; ++k) {
+                                const int to = at + k * THREADS * N;
+                                if (to >= width) continue;
+                                alignas(16) T e[N];
+                                make(q[k], e);
+                                if (same && to >= from && to <= last) put_chunk(o + to, e);
+                                else
+#pragma unroll
+                                    for (int j = 0; j < N; ++j)
+                                        if (to + j >= from && to + j < last + N) o[to + j] = e[j];
+                            }
+                        }
+                    };
+                    const Row r = rows[mine & 1];
+                    if (act0 >= 0 && !bad) {
+                        if (r.ce != 0.0f)
+                            chunks([&](const Chunk<T>& q, T* e) { chunk_grad<T, true>(q, r, e); });
+                        else
+                            chunks([&](const Chunk<T>& q, T* e) { chunk_grad<T, false>(q, r, e); });
+                        const int own = act0 + b - first;
+                        if (own >= 0 && own < width && own / N % THREADS == (int)threadIdx.x) out[act0] = from_f<T>(r.grad<true>(za0) + r.g);
+                    } else {
+                        const T fill = from_f<T>(bad ? __uint_as_float(0x7fffffffu) : 0.0f);
+                        chunks([&](const Chunk<T>&, T* e) {
+#pragma unroll
+                            for (int k = 0; k < N; ++k) e[k] = fill;
+                        });
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) arrive(&empty[slot]);
+                written.next(slices);
+            }
+            act0 = act1, za0 = za1;
+        }
     }
-    if (bad && threadIdx.x == 0)
-        for (int k = 0; k < SLICES; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
-    if (rank == 0 && threadIdx.x == 0) part[blockIdx.x / CTAS] = total;
+    __syncthreads();
+    if (failed && threadIdx.x == 0)
+        for (int k = 0; k < slices; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
+    if (rank == 0 && threadIdx.x == THREADS) part[blockIdx.x / CTAS] = total;
     if (CTAS > 1) cluster.sync();  // no CTA leaves while another may still write to it
 }
 
@@ -663,36 +788,46 @@ __global__ void __launch_bounds__(1024) k_policy_total(const double* part, int n
 
 constexpr int MOST_CTAS = 148 * 8;
 
-template <class T, bool MASK, bool FIT, int THREADS, int CTAS>
-int launch_cluster(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    // slices of whole chunks of a row that may start up to N - 1 entries into its first; legal bytes with room for the 16s
-    // that they start and end in
-    const int slice = (int)(((a.width + (FIT ? 0 : Chunk<T>::N - 1) + CTAS - 1) / CTAS + 15) / 16 * 16);
-    const size_t smem = SLICES * (slice * sizeof(T) + (MASK ? slice + 32 : 0));
-    const auto kernel = k_policy_cluster<T, MASK, FIT, 4, THREADS, CTAS>;
-    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(kernel), SLICES * (THREADS * 4 * Chunk<T>::N * (sizeof(T) + 1) + 64))) return 0;
+constexpr size_t RING = 208 * 1024;  // of an SM's shared memory (the cluster's parts take 8 KB more of each CTA's)
+// Slices are whole chunks of a row that may start up to N - 1 entries into its first
+template <class T>
+int64_t slice_of(const wc_policy_loss_args& a, int ctas) {
+    return ((a.width + Chunk<T>::N - 1 + ctas - 1) / ctas + 15) / 16 * 16;
+}
+// ... and their bytes, with legal bytes' room for the 16s that they start and end in
+template <class T, bool MASK>
+int64_t slice_bytes(int64_t slice) {
+    return slice * sizeof(T) + (MASK ? slice + 32 : 0);
+}
+// `sm`: CTAs of one SM
+template <class T, bool MASK, int WARPS, int CTAS>
+int launch_cluster(const wc_policy_loss_args& a, int sm, double* part, cudaStream_t s) {
+    const int slice = (int)slice_of<T>(a, CTAS);
+    const int64_t bytes = slice_bytes<T, MASK>(slice);
+    const int slices = (int)std::min<int64_t>(MAX_SLICES, (int64_t)RING / sm / bytes);
+    const auto kernel = k_policy_cluster<T, MASK, WARPS, CTAS>;
+    if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(kernel), RING)) return 0;
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {CTAS, 1, 1};
-    cfg.blockDim = THREADS, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1, cfg.dynamicSmemBytes = smem;
+    cfg.blockDim = WARPS * 32 + 32, cfg.stream = s, cfg.attrs = &attr, cfg.numAttrs = 1, cfg.dynamicSmemBytes = (size_t)(slices * bytes);
     // As many clusters as are resident at a time: they do not fill the SMs of every GPC, and the ones left over would
-    // start only when the others have ended (37 of 8 CTAs, of which 33 fit, took 560 us
-    // at 2048 x 131072 in bf16, 33 took 387).
-    constexpr int SM = (FIT ? 1024 : 512) / THREADS;  // CTAs of one
-    cfg.gridDim = CTAS * SM;
+    // start only when the others have ended (37 of 8 CTAs, of which 33 fit, took 560 us at 2048 x 131072 in bf16, 33
+    // took 387).
+    cfg.gridDim = CTAS * sm;
     int most = 0;
-    if (CTAS == 1) most = 148 * SM;
+    if (CTAS == 1) most = 148 * sm;
     else if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) most = 1;
     const int n = (int)std::min<int64_t>(most, a.rows);
     cfg.gridDim = n * CTAS;
-    cudaLaunchKernelEx(&cfg, kernel, a, slice, part);
+    cudaLaunchKernelEx(&cfg, kernel, a, slice, slices, part);
     return n;
 }
 
 template <class T, bool MASK, bool ENTROPY, bool VEC>
 int launch_warp(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
-    const int64_t chunks = (a.width + Chunk<T>::N - 1) / Chunk<T>::N;
+    const int64_t chunks = (a.width + (VEC ? 1 : 2) * (Chunk<T>::N - 1)) / Chunk<T>::N;
     // up to 4 chunks a lane (8 a lane and half the warps took 106 against 98 us at 131072 x 512 in bf16)
     int lanes = 1;
     while (lanes < 32 && lanes * 4 < chunks) lanes *= 2;
@@ -710,28 +845,23 @@ template <class T, bool MASK>
 int launch_rows(const wc_policy_loss_args& a, double* part, cudaStream_t s) {
     constexpr int N = Chunk<T>::N;
     const auto fits = [&](const void* p, int64_t ld, size_t e, int to) { return ((uintptr_t)p & (to - 1)) == 0 && (ld * e) % to == 0; };
-    const int64_t chunks = (a.width + N - 1) / N;
-    const bool is_short = chunks <= 32 * 4;
     const bool fit = a.width % N == 0 && fits(a.logits, a.ld_logits, sizeof(T), 16) && (!a.dlogits || fits(a.dlogits, a.ld_dlogits, sizeof(T), 16)) &&
-                     (!a.legal || (is_short ? fits(a.legal, a.ld_legal, 1, 8) : a.width % 16 == 0 && fits(a.legal, a.ld_legal, 1, 16)));
+                     (!a.legal || fits(a.legal, a.ld_legal, 1, 8));
+    const bool is_short = (a.width + (fit ? 1 : 2) * (N - 1)) / N <= 32 * 4;
     if (is_short) {
         if (a.entropy_coef != 0.0f) return fit ? launch_warp<T, MASK, true, true>(a, part, s) : launch_warp<T, MASK, true, false>(a, part, s);
         return fit ? launch_warp<T, MASK, false, true>(a, part, s) : launch_warp<T, MASK, false, false>(a, part, s);
     }
-    // 4 chunks a thread, up to 8 CTAs a row
-    const auto slice = [&](int ctas) { return ((a.width + (fit ? 0 : N - 1) + ctas - 1) / ctas + 15) / 16 * 16; };
-    const int64_t most = 512 * 4 * N;
-    if (fit) {
-        if (slice(1) <= most / 4) return launch_cluster<T, MASK, true, 128, 1>(a, part, s);
-        if (slice(1) <= most) return launch_cluster<T, MASK, true, 512, 1>(a, part, s);
-        if (slice(2) <= most) return launch_cluster<T, MASK, true, 512, 2>(a, part, s);
-        if (slice(4) <= most) return launch_cluster<T, MASK, true, 512, 4>(a, part, s);
-        if (slice(8) <= most) return launch_cluster<T, MASK, true, 512, 8>(a, part, s);
-    } else {
-        if (slice(1) <= most / 4) return launch_cluster<T, MASK, false, 128, 1>(a, part, s);
-        if (slice(1) <= most) return launch_cluster<T, MASK, false, 512, 1>(a, part, s);
-        if (slice(8) <= most) return launch_cluster<T, MASK, false, 512, 8>(a, part, s);
-    }
+    // The smallest CTA, then the smallest cluster, of which an SM's memory takes as many as its registers with three
+    // slices each; of the longest rows one CTA, with two or more
+    const auto fits_sm = [&](int ctas, int sm, int slices) { return slices * slice_bytes<T, MASK>(slice_of<T>(a, ctas)) <= (int64_t)RING / sm; };
+    if (fits_sm(1, 6, 3)) return launch_cluster<T, MASK, 4, 1>(a, 6, part, s);
+    if (fits_sm(1, 4, 3)) return launch_cluster<T, MASK, 8, 1>(a, 4, part, s);
+    if (fits_sm(1, 2, 3)) return launch_cluster<T, MASK, 16, 1>(a, 2, part, s);
+    if (fits_sm(2, 2, 3)) return launch_cluster<T, MASK, 16, 2>(a, 2, part, s);
+    if (fits_sm(4, 2, 3)) return launch_cluster<T, MASK, 16, 4>(a, 2, part, s);
+    if (fits_sm(8, 2, 3)) return launch_cluster<T, MASK, 16, 8>(a, 2, part, s);
+    if (fits_sm(8, 1, 2)) return launch_cluster<T, MASK, 16, 8>(a, 1, part, s);
     const int n = (int)std::min<int64_t>(148 * 4, a.rows);
     k_policy_long<T><<<n, 512, 0, s>>>(a, part);
     return n;
