@@ -24,6 +24,7 @@
 //     first (dx, dh and two means a row), then the sums column by column, which
 //     reads the inputs a second time.
 #include <algorithm>
+#include <type_traits>
 
 #include "colsum.cuh"
 #include "kernels.h"
@@ -107,17 +108,26 @@ struct Unit<T, VEC> {
         for (int j = 0; j < (int)sizeof(T) / 2; ++j) w[j] = __ldcs(reinterpret_cast<const uint4*>(p) + j);
     }
     __device__ __forceinline__ void get(float* v) const {
-        alignas(16) T e[8];
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(w);
 #pragma unroll
-        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(e)[j] = w[j];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = to_f(e[k]);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) v[2 * j] = __uint_as_float(u[2 * j]), v[2 * j + 1] = __uint_as_float(u[2 * j + 1]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) v[2 * j] = __uint_as_float(u[j] << 16), v[2 * j + 1] = __uint_as_float(u[j] & 0xffff0000u);
+            else {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
+                v[2 * j] = f.x, v[2 * j + 1] = f.y;
+            }
+        }
     }
     __device__ __forceinline__ static void put(T* row, const Cols<T, VEC>& c, int i, const float* v) {
         T* p = row + c.col(i, 0);
-        alignas(16) T e[8];
+        alignas(16) uint32_t e[2 * sizeof(T)];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) e[k] = from_f<T>(v[k]);
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (sizeof(T) == 4) e[2 * j] = __float_as_uint(v[2 * j]), e[2 * j + 1] = __float_as_uint(v[2 * j + 1]);
+            else if constexpr (std::is_same<T, __nv_bfloat16>::value) *reinterpret_cast<__nv_bfloat162*>(&e[j]) = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            else *reinterpret_cast<__half2*>(&e[j]) = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        }
 #pragma unroll
         for (int j = 0; j < (int)sizeof(T) / 2; ++j) __stcs(reinterpret_cast<uint4*>(p) + j, reinterpret_cast<const uint4*>(e)[j]);
     }
@@ -353,34 +363,78 @@ __device__ __forceinline__ void bulk_copy(uint32_t to, uint64_t from, uint32_t b
 
 // What a thread keeps of its unit: the parameters and their gradients' sums.
 // Columns past the width have weights, gate and inputs of 0, and so add 0 to
-// everything.
+// everything. Over the rows of an item the gate g is the same, so with A = g wp
+// and B = g bp its rows need
+//   y = c x + A hhat + B, dU wp = A dY, s1 = sum dY, s2 = sum dY hhat,
+// and its end dg = wp s2 + bp s1, dwp += g s2, dbp += g s1. The last two wait
+// in shared memory (`kept`: a thread's 16 numbers, a thread apart): with them in
+// registers, and a sum a row for each of the three, the kernels spilled.
 struct Column {
-    Pair wp[4], bp[4], wn[4], g[4];
-    Pair dwp[4], dbp[4], dwn[4], dbn[4], dg[4];
+    Pair A[4], B[4], wn[4];
+    Pair s1[4], s2[4], dwn[4], dbn[4];
+    float* kept;
+    int apart;
     template <class T, int LAY>
-    __device__ __forceinline__ void load(const wc_block_norm_args& a, const Cols<T, LAY>& c, int i) {
+    __device__ __forceinline__ static void param(const float* p, float otherwise, const Cols<T, LAY>& c, int i, Pair* to) {
         float v[8];
-        auto param = [&](const float* p, float otherwise, Pair* to) {
-            fill8(v, 0.0f);
-            if (c.any(i)) {
-                if (p) load8(p, c, i, v);
-                else
+        fill8(v, 0.0f);
+        if (c.any(i)) {
+            if (p) load8(p, c, i, v);
+            else
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = c.in(i, k) ? otherwise : 0.0f;
-            }
-            pairs(v, to);
-        };
-        param(a.post_weight, 1.0f, wp), param(a.post_bias, 0.0f, bp), param(a.pre_weight, 0.0f, wn), param(nullptr, 1.0f, g);
-        fill(dwp, 0.0f), fill(dbp, 0.0f), fill(dwn, 0.0f), fill(dbn, 0.0f), fill(dg, 0.0f);
+                for (int k = 0; k < 8; ++k) v[k] = c.in(i, k) ? otherwise : 0.0f;
+        }
+        pairs(v, to);
     }
     template <class T, int LAY>
-    __device__ __forceinline__ void gate(const T* row, const Cols<T, LAY>& c, int i) {
+    __device__ __forceinline__ static void gate(const wc_block_norm_args& a, int64_t group, const Cols<T, LAY>& c, int i, Pair* to) {
+        if (!a.gate) {
+            param(nullptr, 1.0f, c, i, to);
+            return;
+        }
         Unit<T, LAY> u;
         u.zero();
-        if (c.any(i)) u.load(row, c, i);
+        if (c.any(i)) u.load(static_cast<const T*>(a.gate) + group * c.D, c, i);
         float v[8];
         u.get(v);
-        pairs(v, g);
+        pairs(v, to);
+    }
+    template <class T, int LAY>
+    __device__ __forceinline__ void load(const wc_block_norm_args& a, const Cols<T, LAY>& c, int i, float* to, int threads) {
+        kept = to, apart = threads;
+        param(a.pre_weight, 0.0f, c, i, wn);
+        fill(dwn, 0.0f), fill(dbn, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) kept[k * apart] = 0.0f;
+    }
+    // an item begins
+    template <class T, int LAY>
+    __device__ __forceinline__ void begin(const wc_block_norm_args& a, int64_t group, const Cols<T, LAY>& c, int i) {
+        Pair g[4];
+        gate(a, group, c, i, g), param(a.post_weight, 1.0f, c, i, A), param(a.post_bias, 0.0f, c, i, B);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) A[k] = mul(g[k], A[k]), B[k] = mul(g[k], B[k]);
+        fill(s1, 0.0f), fill(s2, 0.0f);
+    }
+    // ... and ends, with the gate's gradient
+    template <class T, int LAY>
+    __device__ __forceinline__ void end(const wc_block_norm_args& a, int64_t group, const Cols<T, LAY>& c, int i, float* dg) {
+        Pair g[4], w[4], b[4];
+        gate(a, group, c, i, g), param(a.post_weight, 1.0f, c, i, w), param(a.post_bias, 0.0f, c, i, b);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const Pair d = fma(w[k], s2[k], mul(b[k], s1[k])), dw = mul(g[k], s2[k]), db = mul(g[k], s1[k]);
+            dg[2 * k] = umma::f2_lo(d), dg[2 * k + 1] = umma::f2_hi(d);
+            float* at = kept + 2 * k * apart;
+            at[0] += umma::f2_lo(dw), at[apart] += umma::f2_hi(dw), at[8 * apart] += umma::f2_lo(db), at[9 * apart] += umma::f2_hi(db);
+        }
+    }
+    // the sums over all items: dwp, dbp, dwn, dbn
+    __device__ __forceinline__ void sums(int which, float* v) const {
+        if (which < 2)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = kept[(which * 8 + k) * apart];
+        else unpairs(which == 2 ? dwn : dbn, v);
     }
     // A row's unit. get(i, v) reads its x, h, dy or dn (i = 0 .. 3; zeros past the width and for a gradient that is not
     // there), when it is needed: what is not held meanwhile leaves room for the sums. put(i, v) takes dx, then dh.
@@ -414,8 +468,8 @@ struct Column {
         Pair c0 = 0, c1 = 0;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            sums(k, yh[k], hh[k]);
-            yh[k] = mul(mul(yh[k], g[k]), wp[k]);
+            add_to(k, yh[k], hh[k]);
+            yh[k] = mul(yh[k], A[k]);
             c0 = add(c0, yh[k]), c1 = fma(yh[k], hh[k], c1);
         }
         if (a.post_weight) {
@@ -432,22 +486,18 @@ struct Column {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             hh[k] = mul(add(hh[k], pm), pr);
-            yh[k] = mul(add(fma(rs, yh[k], mul(g[k], fma(hh[k], wp[k], bp[k]))), nm), nr);
+            yh[k] = mul(add(fma(hh[k], A[k], fma(rs, yh[k], B[k])), nm), nr);
         }
     }
     // the gate's and the post norm's sums
-    __device__ __forceinline__ void sums(int k, Pair dY, Pair hh) {
-        dg[k] = fma(dY, fma(hh, wp[k], bp[k]), dg[k]);
-        const Pair du = mul(dY, g[k]);
-        dwp[k] = fma(du, hh, dwp[k]), dbp[k] = add(dbp[k], du);
-    }
+    __device__ __forceinline__ void add_to(int k, Pair dY, Pair hh) { s1[k] = add(s1[k], dY), s2[k] = fma(dY, hh, s2[k]); }
 };
 
 // A part of a warp a row; a warp is a worker.
 template <class T, int LAY>
 __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_args a, wc_block_norm_grads g, Items q, int lanes,
                                                                float* gate_part, float* weight_part) {
-    __shared__ float s[8][8][33];
+    __shared__ float s[8][8][33], kept[16][256];
     const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int slots = 32 / lanes, slot = lane / lanes, worker = blockIdx.x * 8 + warp;
     const Cols<T, LAY> cols{D, lane & (lanes - 1), lanes};
@@ -455,11 +505,11 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
     const float inv = 1.0f / (float)D;
     Group<0> group{nullptr, lanes};
     Column col;
-    col.load(a, cols, 0);
+    col.load(a, cols, 0, &kept[0][threadIdx.x], 256);
     for (int64_t i = worker; i < q.items; i += q.workers) {
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
-        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
+        col.begin(a, item_group, cols, 0);
         Unit<T, LAY> u[4];  // x, h, dy, dn: the next row's from when dx is out
         float4 next = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         auto fetch = [&](int64_t t) {
@@ -492,9 +542,9 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
                         if (k == 1 && here && g.dh) Unit<T, LAY>::put(static_cast<T*>(g.dh) + t * g.ld_dh, cols, 0, f);
                     });
         }
+        float dg[8];
+        col.end(a, item_group, cols, 0, dg);
         if (g.dgate) {
-            float dg[8];
-            unpairs(col.dg, dg);
 #pragma unroll
             for (int k = 0; k < 8; ++k)
                 for (int o = 16; o >= lanes; o >>= 1) dg[k] += __shfl_xor_sync(~0u, dg[k], o);
@@ -502,13 +552,12 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
                 if (q.segments == 1) Unit<T, LAY>::put(static_cast<T*>(g.dgate) + item_group * D, cols, 0, dg);
                 else store8(gate_part + i * D, cols, 0, dg);
             }
-            fill(col.dg, 0.0f);
         }
     }
     // the slots of a warp, then the warps
-    auto flush = [&](const Pair* sum, int which) {
+    auto flush = [&](int which) {
         float v[8];
-        unpairs(sum, v);
+        col.sums(which, v);
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -524,7 +573,7 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
             weight_part[((int64_t)blockIdx.x * 4 + which) * D + cols.col(0, k)] = t;
         }
     };
-    flush(col.dwp, 0), flush(col.dbp, 1), flush(col.dwn, 2), flush(col.dbn, 3);
+    flush(0), flush(1), flush(2), flush(3);
 }
 
 // A CTA a row, one unit a thread; a CTA is a worker. Its rows in order come to
@@ -536,7 +585,8 @@ constexpr int MAX_RING = 8;
 template <class T, int LAY>
 __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a, wc_block_norm_grads g, Items q, int stages,
                                                            float* gate_part, float* weight_part) {
-    extern __shared__ __align__(128) uint8_t ring[];
+    extern __shared__ __align__(128) uint8_t shared[];  // what Column keeps, then the ring
+    uint8_t* const ring = shared + 64 * blockDim.x;
     __shared__ float2 s[2][32];
     __shared__ uint64_t full[MAX_RING];
     const int D = (int)a.width, row_bytes = D * (int)sizeof(T), piece = LAY == VEC ? row_bytes : (row_bytes + 15) / 16 * 16 + 16;
@@ -546,7 +596,7 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
     const float inv = 1.0f / (float)D;
     Group<16> group{s, 32};
     Column col;
-    col.load(a, cols, 0);
+    col.load(a, cols, 0, reinterpret_cast<float*>(shared) + threadIdx.x, blockDim.x);
     if (threadIdx.x == 0) {
         for (int i = 0; i < stages; ++i) umma::mbar_init(&full[i], 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -559,50 +609,45 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
                         : (g.dn ? static_cast<const T*>(g.dn) + t * g.ld_dn : nullptr);
     };
     auto edge = [&](int64_t t) { return LAY != VEC && (t == 0 || t == a.rows - 1); };
-    // thread 0 walks ahead of the rows
+    // The first warp walks ahead of the rows: lanes 0 to 3 copy x, h, dy and dn, lane 4 the statistics.
+    const int array = threadIdx.x < 4 ? threadIdx.x : 0;
+    const uint64_t base = reinterpret_cast<uint64_t>(row_of(array, 0));
+    const int64_t pitch = (array == 0 ? a.ld_x : array == 1 ? a.ld_h : array == 2 ? g.ld_dy : g.ld_dn) * (int64_t)sizeof(T);
     int64_t copy_item = blockIdx.x, copy_row = 0, copy_last = 0, copy_group;
-    int copied = 0;
+    int copy_slot = 0;
     auto copy = [&] {
         while (copy_row >= copy_last) {
             if (copy_item >= q.items) return;
             q.range(copy_item, copy_group, copy_row, copy_last);
             copy_item += q.workers;
         }
-        const int slot = copied % stages;
-        const uint32_t to = umma::smem_u32(ring + slot * stage_bytes);
-        uint64_t from[4];
-        uint32_t bytes[4], total = 16;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint64_t p = reinterpret_cast<uint64_t>(row_of(k, copy_row));
-            from[k] = p & ~15ull;
-            bytes[k] = !p || edge(copy_row) ? 0 : (uint32_t)(((p + row_bytes + 15) & ~15ull) - from[k]);
-            total += bytes[k];
-        }
-        umma::expect_tx(&full[slot], total);
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (bytes[k]) bulk_copy(to + k * piece, from[k], bytes[k], &full[slot]);
-        bulk_copy(to + 4 * piece, reinterpret_cast<uint64_t>(a.stats + copy_row * 4), 16, &full[slot]);
-        ++copied, ++copy_row;
+        const uint64_t p = base + copy_row * pitch;
+        const uint64_t from = threadIdx.x < 4 ? p & ~15ull : reinterpret_cast<uint64_t>(a.stats + copy_row * 4);
+        const uint32_t bytes = threadIdx.x == 4 ? 16 : threadIdx.x > 4 || !base || edge(copy_row) ? 0 : (uint32_t)(((p + row_bytes + 15) & ~15ull) - from);
+        const uint32_t total = __reduce_add_sync(~0u, bytes);
+        if (threadIdx.x == 0) umma::expect_tx(&full[copy_slot], total);
+        __syncwarp();
+        if (bytes) bulk_copy(umma::smem_u32(ring + copy_slot * stage_bytes) + threadIdx.x * piece, from, bytes, &full[copy_slot]);
+        copy_slot = copy_slot + 1 == stages ? 0 : copy_slot + 1;
+        ++copy_row;
     };
-    if (threadIdx.x == 0)
+    if (threadIdx.x < 32)
         for (int i = 0; i + 1 < stages; ++i) copy();
-    int done = 0;
+    int slot = 0;
+    uint32_t turns = 0;  // of the ring
     bool bad = false;
     for (int64_t i = blockIdx.x; i < q.items; i += q.workers) {
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
-        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
-        for (int64_t t = first; t < last; ++t, ++done) {
-            const int slot = done % stages;
+        col.begin(a, item_group, cols, 0);
+        for (int64_t t = first; t < last; ++t) {
             // a copy that does not come (umma.cuh) leaves NaN from here on
-            if (!bad && !umma::mbar_wait(&full[slot], (uint32_t)(done / stages) & 1)) bad = true;
+            if (!bad && !umma::mbar_wait(&full[slot], turns & 1)) bad = true;
             float4 st = *reinterpret_cast<const float4*>(ring + slot * stage_bytes + 4 * piece);
             if (bad) st.y = st.w = __uint_as_float(0x7fffffffu);
             const bool here = !edge(t);
             __syncthreads();  // all have done with the row before this one: its stage takes another
-            if (threadIdx.x == 0 && !bad) copy();
+            if (threadIdx.x < 32 && __all_sync(~0u, !bad)) copy();
             col.row(a, st, pre, inv, group,
                     [&](int k, Pair* v) {
                         Unit<T, LAY> u;
@@ -624,24 +669,23 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
                         if (k == 0 && g.dx) Unit<T, LAY>::put(static_cast<T*>(g.dx) + t * g.ld_dx, cols, 0, f);
                         if (k == 1 && g.dh) Unit<T, LAY>::put(static_cast<T*>(g.dh) + t * g.ld_dh, cols, 0, f);
                     });
+            if (++slot == stages) slot = 0, ++turns;
         }
+        float dg[8];
+        col.end(a, item_group, cols, 0, dg);
         if (g.dgate && any) {
-            float dg[8];
-            unpairs(col.dg, dg);
             if (q.segments == 1) Unit<T, LAY>::put(static_cast<T*>(g.dgate) + item_group * D, cols, 0, dg);
             else store8(gate_part + i * D, cols, 0, dg);
         }
-        fill(col.dg, 0.0f);
     }
     if (bad && threadIdx.x == 0)
         for (int k = 0; k < stages; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
     if (any) {
         float* to = weight_part + (int64_t)blockIdx.x * 4 * D;
-        const Pair* sums[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             float v[8];
-            unpairs(sums[k], v);
+            col.sums(k, v);
             store8(to + k * D, cols, 0, v);
         }
     }
@@ -746,18 +790,16 @@ __global__ void __launch_bounds__(WARPS * 32) k_norm_backward_rows(wc_block_norm
 template <class T, int LAY>
 __global__ void __launch_bounds__(256, 2) k_norm_backward_cols(wc_block_norm_args a, wc_block_norm_grads g, Items q, const float2* means,
                                                             float* gate_part, float* weight_part) {
-    __shared__ float s[8][8][33];
+    __shared__ float s[8][8][33], kept[16][256];
     const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     // the columns as one unit of `apart` threads' row, of which this CTA has 32
     const int all = gridDim.x * 32;
     const Cols<T, LAY> cols{D, (int)blockIdx.x * 32 + lane, all};
     const bool any = cols.any(0), pre = a.pre_weight && g.dn;
     Column col;
-    col.load(a, cols, 0);
+    col.load(a, cols, 0, &kept[0][threadIdx.x], 256);
     // v summed over the warps: thread (warp k, lane) gets column k of lane's unit
-    auto over_warps = [&](const Pair* sum) {
-        float v[8];
-        unpairs(sum, v);
+    auto over_warps = [&](const float* v) {
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < 8; ++k) s[warp][k][lane] = v[k];
@@ -770,7 +812,7 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_cols(wc_block_norm_arg
     for (int64_t i = blockIdx.y; i < q.items; i += q.workers) {
         int64_t item_group, first, last;
         q.range(i, item_group, first, last);
-        if (a.gate) col.gate(static_cast<const T*>(a.gate) + item_group * D, cols, 0);
+        col.begin(a, item_group, cols, 0);
         for (int64_t t = first + warp; t < last; t += 8) {
             const float4 st = reinterpret_cast<const float4*>(a.stats)[t];
             const float2 m = means[t];
@@ -790,22 +832,24 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_cols(wc_block_norm_arg
             for (int k = 0; k < 4; ++k) {
                 if (pre) dY[k] = fma(nr, fma(yh[k], a1, fma(dn[k], col.wn[k], a0)), dY[k]);
                 col.dwn[k] = fma(dn[k], yh[k], col.dwn[k]), col.dbn[k] = add(col.dbn[k], dn[k]);
-                col.sums(k, dY[k], hh[k]);
+                col.add_to(k, dY[k], hh[k]);
             }
         }
+        float dg[8];
+        col.end(a, item_group, cols, 0, dg);
         if (g.dgate) {
-            const float v = over_warps(col.dg);
+            const float v = over_warps(dg);
             if (cols.in(0, warp)) {
                 if (q.segments == 1) static_cast<T*>(g.dgate)[item_group * D + cols.col(0, warp)] = from_f<T>(v);
                 else gate_part[i * D + cols.col(0, warp)] = v;
             }
-            fill(col.dg, 0.0f);
         }
     }
-    const Pair* sums[4] = {col.dwp, col.dbp, col.dwn, col.dbn};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float v = over_warps(sums[k]);
+        float sum[8];
+        col.sums(k, sum);
+        const float v = over_warps(sum);
         if (cols.in(0, warp)) weight_part[((int64_t)blockIdx.y * 4 + k) * D + cols.col(0, warp)] = v;
     }
 }
@@ -833,9 +877,9 @@ void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cuda
             k_norm_backward_warp<T, NARROW><<<p.parts, 256, 0, s>>>(a, g, q, p.lanes, gates, weights);
         } else if (p.lanes == 0) {
             const int stage = (int)(4 * (UNITS ? D * e : (D * e + 15) / 16 * 16 + 16) + 16), threads = p.threads();
-            const int stages = (int)std::min<int64_t>(MAX_RING, 200 * 1024 / (512 / threads) / stage);
+            const int stages = (int)std::min<int64_t>(MAX_RING, (200 * 1024 / (512 / threads) - 64 * threads) / stage);
             if (wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_norm_backward_cta<T, WIDE>), 200 * 1024))
-                k_norm_backward_cta<T, WIDE><<<p.workers, threads, (size_t)stages * stage, s>>>(a, g, q, stages, gates, weights);
+                k_norm_backward_cta<T, WIDE><<<p.workers, threads, (size_t)stages * stage + 64 * threads, s>>>(a, g, q, stages, gates, weights);
         } else {
             const unsigned threads = (unsigned)((D + 511) / 512 * 32);
             const unsigned n = (unsigned)std::min<int64_t>(a.rows, 148 * (1024 / threads));
