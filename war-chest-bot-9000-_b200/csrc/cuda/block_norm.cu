@@ -196,8 +196,8 @@ struct Group {
 
 // WARPS = 0: `lanes` threads of a warp a row, else a CTA of up to WARPS warps;
 // NV units a thread.
-template <class T, int LAY, int WARPS, int NV>
-__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS ? WARPS : 1) : 4) k_norm_units(wc_block_norm_args a, int lanes) {
+template <class T, int LAY, int WARPS, int NV, int lanes = 32>
+__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS ? WARPS : 1) : 4) k_norm_units(wc_block_norm_args a) {
     __shared__ float2 s[2][32];
     Group<WARPS> group{s, lanes};
     const int D = (int)a.width;
@@ -494,8 +494,8 @@ struct Column {
 };
 
 // A part of a warp a row; a warp is a worker.
-template <class T, int LAY>
-__global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_args a, wc_block_norm_grads g, Items q, int lanes,
+template <class T, int LAY, int lanes>
+__global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_args a, wc_block_norm_grads g, Items q,
                                                                float* gate_part, float* weight_part) {
     __shared__ float s[8][8][33], kept[16][256];
     const int D = (int)a.width, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -874,7 +874,13 @@ void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cuda
     if (a.rows) {
         const Items q{p.items, p.per, p.R, a.rows, p.segments, p.workers};
         if (p.lanes > 0) {
-            k_norm_backward_warp<T, NARROW><<<p.parts, 256, 0, s>>>(a, g, q, p.lanes, gates, weights);
+            const auto kernel = p.lanes == 1   ? k_norm_backward_warp<T, NARROW, 1>
+                                : p.lanes == 2 ? k_norm_backward_warp<T, NARROW, 2>
+                                : p.lanes == 4 ? k_norm_backward_warp<T, NARROW, 4>
+                                : p.lanes == 8 ? k_norm_backward_warp<T, NARROW, 8>
+                                : p.lanes == 16 ? k_norm_backward_warp<T, NARROW, 16>
+                                                : k_norm_backward_warp<T, NARROW, 32>;
+            kernel<<<p.parts, 256, 0, s>>>(a, g, q, gates, weights);
         } else if (p.lanes == 0) {
             const int stage = (int)(4 * (UNITS ? D * e : (D * e + 15) / 16 * 16 + 16) + 16), threads = p.threads();
             const int stages = (int)std::min<int64_t>(MAX_RING, (200 * 1024 / (512 / threads) - 64 * threads) / stage);
@@ -908,21 +914,28 @@ void forward_as(const wc_block_norm_args& a, cudaStream_t s) {
     constexpr int WIDE = UNITS ? VEC : RUNS, NARROW = UNITS ? VEC : LANES;
     const int units = (int)(a.n_q ? (a.width + 31) / 32 * 4 : (a.width + 7) / 8);
     if (units <= 64) {
-        int lanes = !a.n_q ? 1 : UNITS ? 4 : 32;
+        // (where units are runs, a whole warp from 129 columns on)
+        int lanes = UNITS ? (a.n_q ? 4 : 1) : a.n_q || a.width > 128 ? 32 : 1;
         while (lanes < 32 && lanes * 2 < units) lanes *= 2;
         const int64_t per = 256 / lanes;
         const unsigned n = (unsigned)std::min<int64_t>(148 * 16, (a.rows + per - 1) / per);
-        if (units <= lanes) k_norm_units<T, NARROW, 0, 1><<<n, 256, 0, s>>>(a, lanes);
-        else k_norm_units<T, NARROW, 0, 2><<<n, 256, 0, s>>>(a, lanes);
+        const auto kernel = lanes == 32  ? (units <= 32 ? k_norm_units<T, NARROW, 0, 1, 32> : k_norm_units<T, NARROW, 0, 2, 32>)
+                            : lanes == 16 ? k_norm_units<T, VEC, 0, 2, 16>
+                            : lanes == 8  ? k_norm_units<T, NARROW, 0, 2, 8>
+                            : lanes == 4  ? (units <= 4 ? k_norm_units<T, NARROW, 0, 1, 4> : k_norm_units<T, NARROW, 0, 2, 4>)
+                            : lanes == 2  ? k_norm_units<T, NARROW, 0, 2, 2>
+                            : units == 1  ? k_norm_units<T, NARROW, 0, 1, 1>
+                                          : k_norm_units<T, NARROW, 0, 2, 1>;
+        kernel<<<n, 256, 0, s>>>(a);
         return;
     }
     // two units a thread (one a thread was slower: 157 against 123 us at 16384 x 4096 in bf16)
     const int threads = (units + 63) / 64 * 32;
     const unsigned n = (unsigned)std::min<int64_t>(148 * std::max(1, 2048 / threads), a.rows);
-    if (threads <= 128) k_norm_units<T, WIDE, 4, 2><<<n, threads, 0, s>>>(a, 32);
-    else if (threads <= 256) k_norm_units<T, WIDE, 8, 2><<<n, threads, 0, s>>>(a, 32);
-    else if (threads <= 512) k_norm_units<T, WIDE, 16, 2><<<n, threads, 0, s>>>(a, 32);
-    else k_norm_units<T, WIDE, 32, 2><<<n, threads, 0, s>>>(a, 32);
+    if (threads <= 128) k_norm_units<T, WIDE, 4, 2><<<n, threads, 0, s>>>(a);
+    else if (threads <= 256) k_norm_units<T, WIDE, 8, 2><<<n, threads, 0, s>>>(a);
+    else if (threads <= 512) k_norm_units<T, WIDE, 16, 2><<<n, threads, 0, s>>>(a);
+    else k_norm_units<T, WIDE, 32, 2><<<n, threads, 0, s>>>(a);
 }
 template <class T>
 void forward(const wc_block_norm_args& a, cudaStream_t s) {
