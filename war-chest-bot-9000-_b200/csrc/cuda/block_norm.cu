@@ -197,7 +197,7 @@ struct Group {
 // WARPS = 0: `lanes` threads of a warp a row, else a CTA of up to WARPS warps;
 // NV units a thread.
 template <class T, int LAY, int WARPS, int NV, int lanes = 32>
-__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS ? WARPS : 1) : 4) k_norm_units(wc_block_norm_args a) {
+__global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS ? WARPS : 1) : LAY == VEC ? 4 : 3) k_norm_units(wc_block_norm_args a) {
     __shared__ float2 s[2][32];
     Group<WARPS> group{s, lanes};
     const int D = (int)a.width;
