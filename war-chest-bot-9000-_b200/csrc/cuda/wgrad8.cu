@@ -47,7 +47,7 @@ constexpr int RING = 230912;  // shared memory of the stages: 3 of the widest ti
 constexpr uint32_t TMEM_COLS = 512;
 
 struct Plan {
-    int mt, bk, ktiles, ntiles, ctas, joined, limit, parts, operands, dys, xs;
+    int mt, bk, ktiles, ntiles, ctas, joined, whole, limit, parts, operands, dys, xs;
     int steps;              // stages of a tile
     int64_t units;          // tiles x steps, below 2^31
     int64_t split_ld;       // elements of a row of dy's parts in the workspace; 0: dy as it is
@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (; walk.more(); walk.next(p), dy.next()) {
             if (walk.s == 0) turn = 0;
             ok = ok && wait_all(&sh.dy_full[dy.slot], dy.phase);
-            if (a.db && ok && turn == walk.kt) {
+            if (a.db && ok && walk.kt == (p.whole ? 0 : turn)) {
                 const uint32_t B = umma::smem_u32(dys) + dy.slot * p.dy_bytes() + lane * 128;
                 const int64_t left = a.n - (int64_t)walk.nt * (MT * 128);
 #pragma unroll
@@ -438,6 +438,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (!ok)
                     for (float& v : sum) v = __uint_as_float(0x7fffffffu);
                 // the slot of (column block, CTA): their sum grows along the walk
+                if (p.whole) {
+                    const int64_t n = (int64_t)walk.nt * (MT * 128) + lane * 2;
+#pragma unroll
+                    for (int h = 0; h < 4 * MT; ++h)
+                        if (walk.kt == 0 && n + h / 2 * 64 + (h & 1) < a.n) a.db[n + h / 2 * 64 + (h & 1)] = sum[h];
+                    continue;
+                }
                 float* to = part_db + (int64_t)(walk.nt + blockIdx.x) * 256 + lane * 2;
 #pragma unroll
                 for (int h = 0; h < 2 * MT; ++h) *reinterpret_cast<float2*>(to + h * 64) = make_float2(sum[2 * h], sum[2 * h + 1]);
@@ -621,7 +628,11 @@ Plan plan_of(const wc_act8_wgrad_args& a) {
     p.ktiles = (int)((a.k + p.bk - 1) / p.bk);
     p.ntiles = (int)((a.n + p.mt * 128 - 1) / (p.mt * 128));
     p.units = (int64_t)p.ktiles * p.ntiles * p.steps;
-    p.ctas = (int)std::max<int64_t>(1, std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
+    // Short sums take a CTA a tile: it has no partial results, and the second kernel is not launched (which takes as long
+    // as some three stages)
+    const int64_t tiles = (int64_t)p.ktiles * p.ntiles;
+    p.whole = p.steps <= 4 && tiles <= MAX_CTAS;
+    p.ctas = (int)std::max<int64_t>(1, p.whole ? tiles : std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
     p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
     // Converters work a stage or two ahead of the products; what is left holds copies in flight, of dy and x8 in turn
@@ -725,7 +736,7 @@ void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
     else if (p.split_ld) launch_split<1, __nv_bfloat16>(a, p, split, s);
     const auto launch = p.parts == 3 ? launch_tile<3, 1> : p.parts == 2 ? launch_tile<2, 1> : p.mt == 2 ? launch_tile<1, 2> : launch_tile<1, 1>;
     launch(a, p, split, part, part_db, s);
-    if (!p.joined && !a.db) return;
+    if (!p.joined && (!a.db || p.whole)) return;
     if (a.out_type == WC_F32) launch_join<float>(a, p, part, part_db, s);
     else if (a.out_type == WC_F16) launch_join<__half>(a, p, part, part_db, s);
     else launch_join<__nv_bfloat16>(a, p, part, part_db, s);
