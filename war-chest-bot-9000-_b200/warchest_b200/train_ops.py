@@ -335,6 +335,11 @@ def gelu8_backward(da, z8: Act8, want_bias=True):
     return dz, dbias
 
 
+@lru_cache(maxsize=256)
+def _wgrad_workspace(rows: int, k: int, n: int, ld: int, dy_offset: int, kind: int, out: int) -> int:
+    return lib().wc_act8_wgrad_workspace(_ACT8_WGRAD.pack(0, 0, dy_offset, 0, 0, 0, rows, k, n, ld, kind, out))
+
+
 def act8_wgrad(x8: Act8, dy, *, dtype=torch.float32, want_bias=True):
     """(dw, db): x8^T dy as [width of x8, width of dy] in `dtype`, and dy's column sums (float32, or None): the
     gradients of a linear layer's weight [in, out] and bias from its input as kept in 8 bits. A wait of the kernel
@@ -349,12 +354,8 @@ def act8_wgrad(x8: Act8, dy, *, dtype=torch.float32, want_bias=True):
         _fail(me, "dtype must be float32, float16 or bfloat16")
     dw = dy.new_empty((x8.width, n), dtype=dtype)
     db = dy.new_empty(n, dtype=torch.float32) if want_bias else None
-
-    def args(workspace):
-        return _ACT8_WGRAD.pack(x8.q.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), dw.data_ptr(),
-                                db.data_ptr() if want_bias else 0, workspace, rows, x8.width, n, ld, _TYPES[dy.dtype],
-                                _TYPES[dtype])
-
-    scratch = _scratch(lib().wc_act8_wgrad_workspace(args(0)), dy)
-    _call(lib().wc_act8_wgrad, dy.get_device(), args(scratch.data_ptr()))
+    scratch = _scratch(_wgrad_workspace(rows, x8.width, n, ld, dy.data_ptr() & 15, _TYPES[dy.dtype], _TYPES[dtype]), dy)
+    _call(lib().wc_act8_wgrad, dy.get_device(), _ACT8_WGRAD.pack(
+        x8.q.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), dw.data_ptr(), db.data_ptr() if want_bias else 0,
+        scratch.data_ptr(), rows, x8.width, n, ld, _TYPES[dy.dtype], _TYPES[dtype]))
     return dw, db
