@@ -389,7 +389,11 @@ int wc_replay_expand(const uint8_t* rows, size_t nrows, const uint8_t* cc, const
  * call do not overlap. Sums, statistics and gradients accumulate in 32 bits,
  * in an order fixed by the sizes: equal calls give equal bits. A workspace
  * (16-byte aligned) may be reused by the next call on the same stream; its
- * contents are not read. */
+ * contents are not read. Any address that is a multiple of its elements' size
+ * and any row stride will do; rows that start on 16 bytes are the fastest.
+ * Where a kernel waits for a copy of its own that does not come (which only a
+ * fault of the device would cause) it gives up after some seconds and leaves
+ * NaN in what was to follow. */
 enum { WC_F32 = 0, WC_F16 = 1, WC_BF16 = 2 };
 
 /* The clipped policy loss with a KL term, and its gradient, in one call.
@@ -482,11 +486,13 @@ int wc_block_norm_backward(const wc_block_norm_args* a, const wc_block_norm_grad
  * one byte per block: the exponent, plus 127, of the block's unit, the
  * smallest power of two (at least 2^-126) that its largest value allows. A
  * value reads back as q 2^(scale - 127), rounded to nearest-even when it was
- * stored: at most half a unit off, and exact in bf16. A block that holds an
- * infinity or NaN has scale 255 and q 0, and reads back as NaN.
+ * stored: at most half a unit off, and exact in bf16. (Where the unit is
+ * 2^122, the largest there is, q stops at 63, so that it stays a number.) A
+ * block that holds an infinity or NaN has scale 255 and q 0, and reads back as
+ * NaN.
  * wc_act8_pack:   x -> q, scale.            wc_act8_unpack: q, scale -> out.
- * wc_gelu8:       out = GELU(x + bias) (tanh form), and the 32-bit sum
- *                 x + bias to q, scale.
+ * wc_gelu8:       out = GELU(x + bias) (tanh form; 0 at -inf), and the 32-bit
+ *                 sum x + bias to q, scale.
  * wc_gelu8_backward: out = x GELU'(q, scale) with x the gradient at the
  *                 activation; dbias, if not NULL, the column sums of that
  *                 (before rounding). */
@@ -509,7 +515,10 @@ uint64_t wc_gelu8_workspace(int64_t rows, int64_t width);
 int wc_gelu8_backward(const wc_act8_args* a, void* stream);
 /* The weight gradient of a linear layer whose input was kept in 8 bits:
  * dw[k, n] = sum over t of x8[t, k] dy[t, n] (weights as [in, out]), and
- * db[n] = sum over t of dy[t, n] when db is not NULL. */
+ * db[n] = sum over t of dy[t, n] when db is not NULL; 0 where there are no
+ * rows. k is 1 to 2^20, n up to 2^20. The workspace also holds a dy in f16 or
+ * f32, or one whose rows do not start on 16 bytes, as its bf16 parts (2, 3 and
+ * 1 of them). */
 typedef struct wc_act8_wgrad_args {
     const int8_t* q;        /* rows x 32 blocks of k values */
     const uint8_t* scale;

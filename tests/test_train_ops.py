@@ -105,6 +105,17 @@ def test_act8_wgrad_refuses(change, match):
     refused(lib().wc_act8_wgrad, wgrad(**change), None, match=match)
 
 
+@pytest.mark.parametrize("entry,args", [
+    ("wc_policy_loss", [policy(logits=P + 2)]), ("wc_policy_loss", [policy(type=1, dlogits=P + 1)]),
+    ("wc_policy_loss", [policy(actions=P + 4)]), ("wc_policy_loss", [policy(old_logp=P + 2)]), ("wc_policy_loss", [policy(loss=P + 1)]),
+    ("wc_block_norm", [norm(type=2, x=P + 1)]), ("wc_block_norm", [norm(post_weight=P + 2)]),
+    ("wc_block_norm_backward", [norm(), grads(dx=P + 2)]), ("wc_block_norm_backward", [norm(), grads(dpost_weight=P + 1)]),
+    ("wc_act8_pack", [act8(x=P + 2)]), ("wc_act8_unpack", [act8(type=1, out=P + 1)]), ("wc_gelu8", [act8(bias=P + 2)]),
+    ("wc_act8_wgrad", [wgrad(dy=P + 2)]), ("wc_act8_wgrad", [wgrad(out_type=2, dw=P + 1)]), ("wc_act8_wgrad", [wgrad(db=P + 2)])])
+def test_addresses_between_elements_are_refused(entry, args):
+    refused(getattr(lib(), entry), *args, None, match="not aligned to its elements")
+
+
 def test_null_arguments_are_refused():
     for name in ("policy_loss", "block_norm", "act8_pack", "act8_unpack", "gelu8", "gelu8_backward", "act8_wgrad"):
         refused(getattr(lib(), "wc_" + name), None, None, match="null arguments")

@@ -2,6 +2,7 @@
 // checks, then the launch.
 #include <cmath>
 #include <exception>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/wc_b200.h"
@@ -35,6 +36,13 @@ bool type_ok(int t) { return t == WC_F32 || t == WC_F16 || t == WC_BF16; }
 bool size_ok(int64_t rows, int64_t width) { return rows >= 0 && width >= 0 && rows <= (1ll << 31) && width <= (1ll << 31); }
 bool off(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
+// elements at addresses that are no multiple of their size
+bool loose(int type, std::initializer_list<const void*> ps) {
+    for (const void* p : ps)
+        if (off(p, type == WC_F32 ? 4 : 2)) return true;
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -59,6 +67,9 @@ int wc_policy_loss(const wc_policy_loss_args* a, void* stream) {
                 return bad(me, "row stride below the width");
         }
     }
+    if (loose(a->type, {a->logits, a->dlogits}) || off(a->actions, a->action_bytes) ||
+        loose(WC_F32, {a->old_logp, a->advantages, a->weights, a->ref_logp, a->upstream, a->loss, a->row_out}))
+        return bad(me, "an address is not aligned to its elements");
     if (!(a->clip_low >= 0) || !(a->clip_high >= 0)) return bad(me, "a clip range below 0");
     if (!std::isfinite(a->kl_coef) || !std::isfinite(a->entropy_coef)) return bad(me, "a coefficient is not finite");
     return launched(me, [&] { wctrain::launch_policy_loss(*a, static_cast<cudaStream_t>(stream)); });
@@ -78,6 +89,8 @@ static int check_norm(const char* me, const wc_block_norm_args* a) {
         if (!a->x || !a->h || !a->stats) return bad(me, "null device pointer");
         if (a->ld_x < a->width || a->ld_h < a->width) return bad(me, "row stride below the width");
         if (off(a->stats, 16)) return bad(me, "stats is not 16-byte aligned");
+        if (loose(a->type, {a->x, a->h, a->gate, a->y, a->n}) || loose(WC_F32, {a->post_weight, a->post_bias, a->pre_weight, a->pre_bias}))
+            return bad(me, "an address is not aligned to its elements");
     }
     return WC_OK;
 }
@@ -113,6 +126,9 @@ int wc_block_norm_backward(const wc_block_norm_args* a, const wc_block_norm_grad
     if (a->rows && ((g->dy && g->ld_dy < a->width) || (g->dn && g->ld_dn < a->width) || (g->dx && g->ld_dx < a->width) ||
                     (g->dh && g->ld_dh < a->width)))
         return bad(me, "row stride below the width");
+    if (loose(a->type, {g->dy, g->dn, g->dx, g->dh, g->dgate}) ||
+        loose(WC_F32, {g->dpost_weight, g->dpost_bias, g->dpre_weight, g->dpre_bias}))
+        return bad(me, "an address is not aligned to its elements");
     return launched(me, [&] { wctrain::launch_block_norm_backward(*a, *g, static_cast<cudaStream_t>(stream)); });
 }
 
@@ -124,6 +140,8 @@ static int check_act8(const char* me, const wc_act8_args* a, bool x, bool out) {
     if (!a->q || !a->scale || (x && !a->x) || (out && !a->out)) return bad(me, "null device pointer");
     if ((x && a->ld_x < a->width) || (out && a->ld_out < a->width)) return bad(me, "row stride below the width");
     if (off(a->q, 16)) return bad(me, "q is not 16-byte aligned");
+    if (loose(a->type, {x ? a->x : nullptr, out ? a->out : nullptr}) || loose(WC_F32, {a->bias, a->dbias}))
+        return bad(me, "an address is not aligned to its elements");
     return WC_OK;
 }
 
@@ -183,6 +201,8 @@ int wc_act8_wgrad(const wc_act8_wgrad_args* a, void* stream) {
         if (a->ld_dy < a->n) return bad(me, "row stride below the width");
         if (off(a->q, 16)) return bad(me, "q is not 16-byte aligned");
     }
+    if (loose(a->type, {a->dy}) || loose(a->out_type, {a->dw}) || loose(WC_F32, {a->db}))
+        return bad(me, "an address is not aligned to its elements");
     return launched(me, [&] { wctrain::launch_wgrad8(*a, static_cast<cudaStream_t>(stream)); });
 }
 
