@@ -635,6 +635,15 @@ def test_layers_differentiate():
     assert abs(float(r.loss) - float(want)) < 1e-3 * (1 + abs(float(want)))
 
 
+def test_layers_notice_what_changed_before_the_backward_pass():
+    c = policy_case(20, 30, F32, seed=13)
+    z = c["logits"].clone().requires_grad_()
+    r = layers.policy_loss(z, c["actions"], c["old_logp"], c["advantages"], weights=c["weights"])
+    c["weights"].mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        r.loss.backward()
+
+
 def test_the_example_learns():
     import os
     import sys

@@ -13,24 +13,26 @@ from .train_ops import Act8, PolicyLoss
 
 class _PolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, args, options):
-        r = ops.policy_loss(logits, *args, want_grad=False, **options)
-        ctx.save_for_backward(logits)
-        ctx.args, ctx.options = args, options
+    def forward(ctx, logits, actions, old_logp, advantages, weights, ref_logp, legal, options):
+        r = ops.policy_loss(logits, actions, old_logp, advantages, weights=weights, ref_logp=ref_logp, legal=legal,
+                            want_grad=False, **options)
+        ctx.save_for_backward(logits, actions, old_logp, advantages, weights, ref_logp, legal)
+        ctx.options = options
         ctx.mark_non_differentiable(r.row_loss, r.logp, r.entropy, r.kl)
         return r.loss, r.row_loss, r.logp, r.entropy, r.kl
 
     @staticmethod
     def backward(ctx, g, *unused):
-        (logits,) = ctx.saved_tensors
-        r = ops.policy_loss(logits, *ctx.args, upstream=g.to(torch.float32), **ctx.options)
-        return r.dlogits, None, None
+        logits, actions, old_logp, advantages, weights, ref_logp, legal = ctx.saved_tensors
+        r = ops.policy_loss(logits, actions, old_logp, advantages, weights=weights, ref_logp=ref_logp, legal=legal,
+                            upstream=g.to(torch.float32), **ctx.options)
+        return (r.dlogits,) + (None,) * 7
 
 
-def policy_loss(logits, actions, old_logp, advantages, **options) -> PolicyLoss:
-    """train_ops.policy_loss with a differentiable loss (the other results are not, and dlogits is None): the logits are
-    read again in the backward pass, which keeps no gradient between the two."""
-    return PolicyLoss(*_PolicyLoss.apply(logits, (actions, old_logp, advantages), options), None)
+def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp=None, legal=None, **options) -> PolicyLoss:
+    """train_ops.policy_loss with a loss that is differentiable at the logits (the other results are not, and dlogits is
+    None): the logits are read again in the backward pass, which keeps no gradient between the two."""
+    return PolicyLoss(*_PolicyLoss.apply(logits, actions, old_logp, advantages, weights, ref_logp, legal, options), None)
 
 
 class _BlockNorm(torch.autograd.Function):
