@@ -24,7 +24,7 @@
 //     first (dx, dh and two means a row), then the sums column by column, which
 //     reads the inputs a second time.
 //
-// On a B200 16384 x 4096 in bf16 takes 124 us forward (4.3 TB/s of the 6.5 that a
+// On a B200 16384 x 4096 in bf16 takes 105 us forward (5.1 TB/s of the 6.5 that a
 // copy reaches: a CTA waits for its row's sums) and 251 us backward, 606208 x 96 in
 // f16 119 and 193 us (3.6 TB/s: instructions, and 12 units for 16 lanes).
 #include <algorithm>
@@ -210,20 +210,32 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS 
     const int blocks = (D + 31) / 32;
     const float inv = 1.0f / (float)D;
     const bool layer = a.kind == WC_NORM_LAYER;
-    for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < a.rows; t0 += (int64_t)gridDim.x * per) {
+    // The next row's h and x are read from when this one's are used up, where that leaves registers: CTAs and 16-bit
+    // types (16384 x 4096 in bf16 104 us for 119; parts of warps 127 for 119 at 606208 x 96, 32-bit types 108 for 100 at
+    // 32768 x 1024).
+    constexpr bool AHEAD = LAY == VEC && WARPS && sizeof(T) == 2;
+    Unit<T, LAY> h[AHEAD ? NV : 1], x[NV];
+    const int64_t step = (int64_t)gridDim.x * per;
+    auto fetch = [&](int64_t t, int i, Unit<T, LAY>& to) {
+        to.zero();
+        if (t >= a.rows || !cols.any(i)) return;
+        to.stream(static_cast<const T*>(a.h) + t * a.ld_h, cols, i);
+        x[i].stream(static_cast<const T*>(a.x) + t * a.ld_x, cols, i);
+    };
+    auto fetch_ahead = [&](int64_t t) {
+        if constexpr (AHEAD)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) fetch(t, i, h[i]);
+    };
+    fetch_ahead((int64_t)blockIdx.x * per + slot);
+    for (int64_t t0 = (int64_t)blockIdx.x * per; t0 < a.rows; t0 += step) {
         const int64_t t = t0 + slot;
         const bool in = t < a.rows;
-        Unit<T, LAY> x[NV];
         float v[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            fill8(v[i], 0.0f);
-            if (in && cols.any(i)) {
-                Unit<T, LAY> h;
-                h.stream(static_cast<const T*>(a.h) + t * a.ld_h, cols, i);
-                x[i].stream(static_cast<const T*>(a.x) + t * a.ld_x, cols, i);
-                h.get(v[i]);
-            }
+            if (!AHEAD) fetch(t, i, h[0]);
+            h[AHEAD ? i : 0].get(v[i]);
         }
         // moments of what is in v; columns past the width are 0 and count for nothing
         auto moments = [&](float& mean, float& r) {
@@ -276,6 +288,7 @@ __global__ void __launch_bounds__(WARPS ? WARPS * 32 : 256, WARPS ? 32 / (WARPS 
                     if (!cols.in(i, k)) v[i][k] = 0.0f;
             Unit<T, LAY>::put(static_cast<T*>(a.y) + t * a.ld_y, cols, i, v[i]);
         }
+        fetch_ahead(t + step);
         if (a.pre_weight) {
             moments(r.nm, r.nr);
 #pragma unroll
@@ -650,7 +663,8 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
             float4 st = *reinterpret_cast<const float4*>(ring + slot * stage_bytes + 4 * piece);
             if (bad) st.y = st.w = __uint_as_float(0x7fffffffu);
             const bool here = !edge(t);
-            __syncthreads();  // all have done with the row before this one: its stage takes another
+            // all have read the row before this one, whose stage takes another: with a post norm, before its last sum
+            if (!a.post_weight) __syncthreads();
             if (threadIdx.x < 32 && __all_sync(~0u, !bad)) copy();
             col.row(a, st, pre, inv, group,
                     [&](int k, Pair* v) {
