@@ -457,6 +457,22 @@ def test_act8_wgrad_long_sums_in_32_bits():
     assert float((dw.double() - want).norm() / want.norm()) < 2e-6
 
 
+@pytest.mark.parametrize("T,K,N,dtype", [(100000, 512, 336, F32), (150000, 192, 96, BF16), (100000, 320, 200, F16), (60000, 128, 384, F32)])
+def test_act8_wgrad_long_walks(T, K, N, dtype):
+    """Many stages a CTA, in rings of different lengths: every call's bits alike, and right."""
+    g = gen(T + K)
+    x8, dy = ops.act8_pack(randn(g, T, K, dtype=BF16)), randn(g, T, N, dtype=dtype)
+    x = ops.act8_unpack(x8, F32)
+    want = sum(a.double().t() @ b.double() for a, b in zip(x.split(20000), dy.split(20000)))
+    first, db = ops.act8_wgrad(x8, dy)
+    # as above relative to the whole: a run's bias, and the runs' own sums
+    assert float((first.double() - want).norm() / want.norm()) < 2e-6
+    near(db, dy.double().sum(0), 32 * U * dy.double().abs().sum(0), "db")
+    for i in range(30):
+        dw, other = ops.act8_wgrad(x8, dy, want_bias=i % 2 == 0)
+        assert torch.equal(dw, first) and (other is None or torch.equal(other, db))
+
+
 @pytest.mark.parametrize("ld,skip", [(104, 8), (97, 0), (99, 3)])
 def test_act8_wgrad_strides_and_addresses(ld, skip):
     g = gen(2)

@@ -394,9 +394,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
     } else if (warp == 3) {  // -------------------------------- column sums
         // Eight columns at a time as products with ones: 8 rows of 8 columns are a matrix fragment, and 4 products a stage
-        // replace 64 additions a column (606208 x 192 x 96 takes 87 us, with additions it took 92; without db 68). Lanes 4 j to 4 j + 3 keep the j-th eight of every 64 columns. The
-        // tiles of a column block take the stages in turn, so that no CTA has more of this than another; a CTA keeps its
-        // sums until the column block ends.
+        // replace 64 additions a column (606208 x 192 x 96 takes 87 us, with additions it took 92; without db 68). Lanes
+        // 4 j to 4 j + 3 keep the j-th eight of every 64 columns. The tiles of a column block take the stages in turn, so
+        // that no CTA has more of this than another; a CTA keeps its sums until the column block ends.
         bool ok = true;
         float sum[4 * MT] = {};
         int turn = walk.s % p.ktiles;  // the tile whose stage this is
@@ -635,16 +635,20 @@ Plan plan_of(const wc_act8_wgrad_args& a) {
     p.ctas = (int)std::max<int64_t>(1, p.whole ? tiles : std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
     p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
-    // Converters work a stage or two ahead of the products; what is left holds copies in flight, of dy and x8 in turn
+    // Converters work a stage or two ahead of the products; what is left holds copies in flight, of dy and x8 in turn.
+    // x8's ring has an even number of places, so that a place is always the same team's. With an odd one a team that is
+    // ahead could take the barrier's phase before last for the one it waits for, when the copy between the two (the
+    // other team's) is late: it would convert what is not there yet and free a place that is still in use.
     p.operands = 3, p.xs = 2, p.dys = 2;
     for (bool grew = true; grew;) {
         grew = false;
-        for (int* n : {&p.dys, &p.xs}) {
-            if (*n == MAX_STAGES) continue;
-            ++*n;
+        const auto grow = [&](int& n, int by) {
+            if (n + by > MAX_STAGES) return;
+            n += by;
             if (p.ring_bytes() <= RING) grew = true;
-            else --*n;
-        }
+            else n -= by;
+        };
+        grow(p.dys, 1), grow(p.dys, 1), grow(p.xs, 2);
     }
     return p;
 }
