@@ -118,18 +118,33 @@ __global__ void __launch_bounds__(THREADS) k_act8(wc_act8_args a, Divisor chunks
     }
 }
 
-// The same, a warp a run of 8 blocks of a row; lane k keeps what is the k-th block's.
-template <class T, int WHAT>
-__global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int blocks, Divisor runs, uint32_t total) {
+// The same, a warp 8 blocks, a column of each a lane; lane k keeps what is the k-th block's. FLAT: 8 next to each other in
+// the matrix, which end in a later row than they begin in (`units` is a row's blocks); else a run of a row's (`units` is a
+// row's runs), whose addresses are known from the first.
+template <class T, int WHAT, bool FLAT>
+__global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int blocks, Divisor units, uint32_t total) {
     const uint32_t i = (blockIdx.x * THREADS + threadIdx.x) >> 5, lane = threadIdx.x & 31;
-    if (i >= total) return;
+    if (FLAT ? i * 8 >= total : i >= total) return;
+    // this lane's block of the eight, and the place of the first one's q and scale
     uint32_t run;
-    const int64_t row = runs(i, &run), b0 = row * blocks + run * 8;
-    const int left = blocks - (int)run * 8, cols = (int)(a.width - (int64_t)run * 256) - (int)lane;  // from this lane's first on
+    const uint32_t mine = FLAT ? min(i * 8 + (lane & 7), total - 1) : i, line = units(mine, &run);
+    const int64_t b0 = FLAT ? (int64_t)i * 8 : (int64_t)line * blocks + run * 8;
+    const int left = FLAT ? (int)(total - i * 8) : blocks - (int)run * 8;
     int8_t* q = a.q + b0 * 32 + lane;
     uint8_t* scale = a.scale + b0;
+    // the k-th block's first column, how many are left in its row from this lane's on, and that one's address
+    auto first = [&](int k) { return FLAT ? __shfl_sync(0xffffffffu, run, k) * 32 : run * 256 + k * 32; };
+    auto cols = [&](int k) {
+        const uint32_t c = first(k);
+        return k < left ? (int)(a.width - c) - (int)lane : 0;
+    };
+    auto at = [&](auto* base, int64_t ld, int k) {
+        if constexpr (FLAT) return base + __shfl_sync(0xffffffffu, line, k) * ld + first(k) + lane;
+        else return base + (line * ld + run * 256 + lane) + k * 32;
+    };
+    const T* x = static_cast<const T*>(a.x);
+    T* out = static_cast<T*>(a.out);
     if constexpr (WHAT == UNPACK) {
-        T* out = static_cast<T*>(a.out) + row * a.ld_out + run * 256 + lane;
         uint32_t w[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[k] = k < left ? (uint32_t)(uint8_t)__ldcs(q + k * 32) : 0;
@@ -137,21 +152,26 @@ __global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int block
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             const float v = act8_number(w[k]) * __shfl_sync(0xffffffffu, unit, k);
-            if (k * 32 < cols) __stcs(out + k * 32, from_f<T>(v));
+            T* to = at(out, a.ld_out, k);
+            if (cols(k) > 0) __stcs(to, from_f<T>(v));
         }
     } else {
-        const T* x = static_cast<const T*>(a.x) + row * a.ld_x + run * 256 + lane;
-        T* out = static_cast<T*>(a.out) + row * a.ld_out + run * 256 + lane;
         float v[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = k * 32 < cols ? to_f(__ldcs(x + k * 32)) : 0.0f;
+        for (int k = 0; k < 8; ++k) {
+            const T* from = at(x, a.ld_x, k);
+            v[k] = cols(k) > 0 ? to_f(__ldcs(from)) : 0.0f;
+        }
         if constexpr (WHAT == GELU)
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (k * 32 < cols) {
-                    if (a.bias) v[k] += a.bias[(int64_t)run * 256 + lane + k * 32];
-                    __stcs(out + k * 32, from_f<T>(gelu(v[k])));
+            for (int k = 0; k < 8; ++k) {
+                T* to = at(out, a.ld_out, k);
+                const uint32_t c = first(k) + lane;
+                if (cols(k) > 0) {
+                    if (a.bias) v[k] += a.bias[c];
+                    __stcs(to, from_f<T>(gelu(v[k])));
                 }
+            }
         // magnitudes are compared as integers, where NaN is above infinity above the rest, so either shows in the code
         uint32_t top = 0;
 #pragma unroll
@@ -164,15 +184,15 @@ __global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int block
         if (__any_sync(0xffffffffu, code >= ACT8_LARGEST)) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const uint32_t mine = __shfl_sync(0xffffffffu, code, k);
-                if (k < left) q[k * 32] = act8_whole(v[k], mine);
+                const uint32_t its = __shfl_sync(0xffffffffu, code, k);
+                if (k < left) q[k * 32] = act8_whole(v[k], its);
             }
         } else {
             const float inv = act8_inverse(code);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const float mine = __shfl_sync(0xffffffffu, inv, k);
-                if (k < left) q[k * 32] = (int8_t)__float_as_uint(fmaf(v[k], mine, 12582912.0f));
+                const float its = __shfl_sync(0xffffffffu, inv, k);
+                if (k < left) q[k * 32] = (int8_t)__float_as_uint(fmaf(v[k], its, 12582912.0f));
             }
         }
     }
@@ -180,13 +200,15 @@ __global__ void __launch_bounds__(THREADS) k_act8_runs(wc_act8_args a, int block
 
 // dz = da GELU'(z8). The CTA's threads keep their columns and walk down the
 // rows [blockIdx.y * chunk_rows, ...): `lanes` threads a row, each 8 columns.
-// UNITS: consecutive ones. Else `lanes` is a number of warps times 32, and a
-// warp has 256 columns, thread by thread next to each other.
-template <class T, bool UNITS>
+// K = 0: consecutive ones. Else `lanes` is a number of warps times 32, and a
+// warp has 32 K columns, thread by thread next to each other.
+template <class T, int K>
 __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int blocks, int lanes, int64_t chunk_rows, float* part) {
+    constexpr bool UNITS = K == 0;
+    constexpr int EACH = UNITS ? 8 : K;  // columns of a thread
     __shared__ float s[THREADS][9];
     const int per = THREADS / lanes, r = threadIdx.x / lanes, at = blockIdx.x * lanes + threadIdx.x % lanes;
-    const int step = UNITS ? 1 : 32, c = UNITS ? at * 8 : (at & ~31) * 8 + (at & 31);
+    const int step = UNITS ? 1 : 32, c = UNITS ? at * 8 : (at & ~31) * K + (at & 31);
     const bool in = r < per && c < a.width;
     const int64_t first = blockIdx.y * chunk_rows, last = min(first + chunk_rows, a.rows);
     Pair acc[4] = {0, 0, 0, 0};  // (pairs of zeros)
@@ -223,15 +245,15 @@ __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int 
             const int8_t* q = a.q + t * blocks * 32 + c;
             const uint8_t* scale = a.scale + t * blocks + c / 32;
             const int left = (int)(a.width - c);
-            float d[8];
+            float d[8] = {};
             uint32_t w[8], code[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                const bool here = k * 32 < left;
+                const bool here = k < K && k * 32 < left;
                 d[k] = here ? to_f(__ldcs(x + k * 32)) : 0.0f, w[k] = here ? (uint32_t)(uint8_t)__ldcs(q + k * 32) : 0, code[k] = here ? scale[k] : 1;
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; 2 * k < K; ++k) {
                 Pair z = mul(umma::f2(act8_number(w[2 * k]), act8_number(w[2 * k + 1])), umma::f2(act8_unit(code[2 * k]), act8_unit(code[2 * k + 1])));
                 if (max(code[2 * k], code[2 * k + 1]) > 147) {
                     Pair lo = umma::f2(umma::f2_lo(z), 0.0f), hi = umma::f2(umma::f2_hi(z), 0.0f);
@@ -241,7 +263,7 @@ __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int 
                 const Pair g = mul(umma::f2(d[2 * k], d[2 * k + 1]), gelu_slope(z));
                 acc[k] = add(acc[k], g);
                 if (2 * k * 32 < left) __stcs(out + 2 * k * 32, from_f<T>(umma::f2_lo(g)));
-                if ((2 * k + 1) * 32 < left) __stcs(out + (2 * k + 1) * 32, from_f<T>(umma::f2_hi(g)));
+                if (2 * k + 1 < K && (2 * k + 1) * 32 < left) __stcs(out + (2 * k + 1) * 32, from_f<T>(umma::f2_hi(g)));
             }
         }
     }
@@ -251,7 +273,7 @@ __global__ void __launch_bounds__(THREADS) k_gelu8_backward(wc_act8_args a, int 
     __syncthreads();
     if (in && r == 0)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < EACH; ++k) {
             float v = s[threadIdx.x][k];
             for (int j = 1; j < per; ++j) v += s[threadIdx.x + j * lanes][k];
             if (c + k * step < a.width) part[blockIdx.y * a.width + c + k * step] = v;
@@ -277,8 +299,16 @@ void launch_as(const wc_act8_args& a, cudaStream_t s) {
             const uint32_t total = (uint32_t)(b.rows * chunks);
             k_act8<T, WHAT><<<(total + THREADS - 1) / THREADS, THREADS, 0, s>>>(b, Divisor((uint32_t)chunks), total);
         } else {
-            const uint32_t runs = (uint32_t)(chunks + 31) / 32, total = (uint32_t)(b.rows * runs);
-            k_act8_runs<T, WHAT><<<(unsigned)((total + 7ull) / 8), THREADS, 0, s>>>(b, (int)(chunks / 4), Divisor(runs), total);
+            // Runs of a row unless most of one is past it (1000000 x 31 in bf16 packs in 39 us, in runs with one block of
+            // eight it took 178; 100000 x 333, with 11 blocks of 16, in 44 us in runs, 47 without)
+            const uint32_t blocks = (uint32_t)(chunks / 4), runs = (blocks + 7) / 8;
+            if (blocks < 4) {
+                const uint32_t total = (uint32_t)(b.rows * blocks), warps = (total + 7) / 8;
+                k_act8_runs<T, WHAT, true><<<(warps + 7) / 8, THREADS, 0, s>>>(b, (int)blocks, Divisor(blocks), total);
+            } else {
+                const uint32_t total = (uint32_t)(b.rows * runs);
+                k_act8_runs<T, WHAT, false><<<(unsigned)((total + 7ull) / 8), THREADS, 0, s>>>(b, (int)blocks, Divisor(runs), total);
+            }
         }
     }
 }
@@ -292,9 +322,14 @@ void launch_type(const wc_act8_args& a, cudaStream_t s) {
 struct Shape {
     int blocks, tiles, lanes, splits;
     int64_t chunk_rows;
+    int each = 8;  // columns of a thread
     Shape(int64_t rows, int64_t width, bool units) {
         blocks = (int)((width + 31) / 32);
-        const int threads = units ? (int)(width / 8) : (int)((width + 255) / 256 * 32), whole = units ? 1 : 32;
+        // without units: the most columns a thread with little past the width (an eighth), else a warp's 32
+        const auto past = [&](int k) { return (blocks + k - 1) / k * k - blocks; };
+        if (!units)
+            while (each > 1 && past(each) * 8 > blocks) each /= 2;
+        const int threads = units ? (int)(width / 8) : (blocks + each - 1) / each * 32, whole = units ? 1 : 32;
         tiles = (threads + THREADS - 1) / THREADS;
         lanes = (threads / whole + tiles - 1) / tiles * whole;
         const int per = THREADS / lanes;
@@ -310,8 +345,12 @@ void launch_backward(const wc_act8_args& a, cudaStream_t s) {
     const Shape g(a.rows, a.width, units);
     float* part = a.dbias ? static_cast<float*>(a.workspace) : nullptr;
     const dim3 grid(g.tiles, g.splits);
-    if (units) k_gelu8_backward<T, true><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
-    else k_gelu8_backward<T, false><<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
+    const auto kernel = units ? k_gelu8_backward<T, 0>
+                        : g.each == 8 ? k_gelu8_backward<T, 8>
+                        : g.each == 4 ? k_gelu8_backward<T, 4>
+                        : g.each == 2 ? k_gelu8_backward<T, 2>
+                                      : k_gelu8_backward<T, 1>;
+    kernel<<<grid, THREADS, 0, s>>>(a, g.blocks, g.lanes, g.chunk_rows, part);
     if (part) launch_colsum(part, g.splits, a.width, a.width, 1, ColSums{{a.dbias}}, s);
 }
 
