@@ -25,8 +25,8 @@
 //     reads the inputs a second time.
 //
 // On a B200 16384 x 4096 in bf16 takes 105 us forward (5.1 TB/s of the 6.5 that a
-// copy reaches: a CTA waits for its row's sums) and 251 us backward, 606208 x 96 in
-// f16 119 and 193 us (3.6 TB/s: instructions, and 12 units for 16 lanes).
+// copy reaches: a CTA waits for its row's sums) and 237 us backward, 606208 x 96 in
+// f16 117 and 194 us (3.6 TB/s: instructions, and 12 units for 16 lanes).
 #include <algorithm>
 #include <type_traits>
 
@@ -42,15 +42,21 @@ struct Row {
     float pm, pr, nm, nr;
 };
 
-// the segments of a group joined
+// The segments of a group joined: 32 columns of group blockIdx.y a CTA, the segments dealt to its warps and those joined in
+// order. (With a thread a column, a chain of 2368 segments, the backward pass of one gate over 19184 x 25 took 174 us
+// for 49.)
 template <class T>
-__global__ void k_gate_sum(const float* part, int segments, int64_t D, int64_t total, T* out) {
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t group = i / D, j = i - group * D;
-        float v = 0.0f;
-        for (int k = 0; k < segments; ++k) v += part[(group * segments + k) * D + j];
-        out[i] = from_f<T>(v);
-    }
+__global__ void __launch_bounds__(1024) k_gate_sum(const float* part, int segments, int64_t D, T* out) {
+    __shared__ float s[32][33];
+    const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x, group = blockIdx.y;
+    float v = 0.0f;
+    if (c < D)
+        for (int k = threadIdx.y; k < segments; k += blockDim.y) v += part[(group * segments + k) * D + c];
+    s[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y || c >= D) return;
+    for (int j = 1; j < (int)blockDim.y; ++j) v += s[j][threadIdx.x];
+    out[group * D + c] = from_f<T>(v);
 }
 
 // ---- units -------------------------------------------------------------------
@@ -912,7 +918,9 @@ void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cuda
             k_norm_backward_cols<T, WIDE><<<dim3((unsigned)((D + 255) / 256), p.workers), 256, 0, s>>>(a, g, q, means, gates, weights);
         }
         if (g.dgate && p.segments > 1)
-            k_gate_sum<T><<<148 * 4, 256, 0, s>>>(gates, p.segments, D, p.groups * D, static_cast<T*>(g.dgate));
+            // (there are segments only where the groups are fewer than the workers)
+            k_gate_sum<T><<<dim3((unsigned)((D + 31) / 32), (unsigned)p.groups), dim3(32, p.segments >= 16 ? 32 : 4), 0, s>>>(
+                gates, p.segments, D, static_cast<T*>(g.dgate));
     }
     if (g.dpost_weight || g.dpost_bias || g.dpre_weight || g.dpre_bias)
         launch_colsum(weights, p.parts, 4 * D, D, 4, ColSums{{g.dpost_weight, g.dpost_bias, g.dpre_weight, g.dpre_bias}}, s);
