@@ -53,19 +53,6 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Sum over the CTA in a fixed order; every thread gets it. `s` holds one
-// float per warp; the call ends with the array free for the next one.
-__device__ __forceinline__ float cta_sum(float v, float* s) {
-    v = warp_sum(v);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    if (lane == 0) s[warp] = v;
-    __syncthreads();
-    float t = lane < nw ? s[lane] : 0.0f;
-    t = warp_sum(t);
-    __syncthreads();
-    return t;
-}
-
 // The unit of an 8-bit block whose largest magnitude is `top`: the smallest
 // power of two 2^e with top <= 127 2^e, as e + 127 (at least 1, so the unit
 // and its reciprocal are normal numbers). top = 1.M 2^(E - 127); 64 (1.M)
