@@ -669,3 +669,43 @@ def test_the_example_learns():
 
     gains = policy_step.train(32, 12)
     assert gains[-1] > gains[0] + 0.2, gains
+
+
+# ------------------------------------------------------------- sums of any length
+
+def act8_product(x8, dy):
+    want = torch.zeros(x8.width, dy.shape[1], dtype=torch.float64, device="cuda")
+    for t in range(0, len(dy), 16384):
+        part = ops.Act8(x8.q[t:t + 16384], x8.scale[t:t + 16384], x8.width)
+        want += ops.act8_unpack(part, F32).double().t() @ dy[t:t + 16384].double()
+    return want
+
+
+# Values of one sign, so that whatever a long sum loses shows in the mean; enough tiles that CTAs sum whole ones. Rounding
+# to the nearest is unbiased: the mean of K N of them, each at most EPS, lies within six deviations.
+
+def test_act8_wgrad_long_sums_in_f16():
+    g = gen(21)
+    T, K, N = 131072, 4096, 1280
+    positive = lambda n, scale: (0.5 + torch.rand(T, n, generator=g, device="cuda")) * scale  # noqa: E731
+    x8, dy = ops.act8_pack(positive(K, 1.0)), positive(N, 1.5 * 2.0 ** -7).to(F16)
+    dw, _ = ops.act8_wgrad(x8, dy, dtype=F16)  # about 1536, where places are 1 and values spread over 10
+    off = dw.double() / act8_product(x8, dy) - 1
+    # and a run's bias: at most 3.84e-6, a 64th of the least that the rounding can move a value by
+    assert abs(float(off.mean())) < 6 * EPS[F16] / math.sqrt(3 * K * N) + 3.84e-6
+    assert float(off.abs().max()) < EPS[F16] + 1e-5
+    # what is rounded is the 32-bit result
+    assert torch.equal(dw, ops.act8_wgrad(x8, dy)[0].to(F16))
+
+
+def test_act8_wgrad_long_sums_in_bf16():
+    g = gen(22)
+    T, K, N = 131072, 4096, 2560
+    positive = lambda n: 0.5 + torch.rand(T, n, generator=g, device="cuda")  # noqa: E731
+    octave = torch.linspace(0, 1, K, device="cuda").exp2()  # results over all places of a power of two
+    x8, dy = ops.act8_pack(positive(K) * octave), positive(N).to(BF16)
+    dw, _ = ops.act8_wgrad(x8, dy, dtype=BF16)
+    off = dw.double() / act8_product(x8, dy) - 1
+    # a run's bias: 1024 products, each half a last place of a sum that grows to the result (u of the result)
+    assert abs(float(off.mean())) < 6 * EPS[BF16] / math.sqrt(3 * K * N) + 1024 * U
+    assert float(off.abs().max()) < EPS[BF16] + 1e-4

@@ -47,7 +47,7 @@ constexpr int RING = 230912;  // shared memory of the stages: 3 of the widest ti
 constexpr uint32_t TMEM_COLS = 512;
 
 struct Plan {
-    int mt, bk, ktiles, ntiles, ctas, joined, whole, limit, parts, operands, dys, xs;
+    int mt, bk, ktiles, ntiles, ctas, joined, kept, whole, limit, parts, operands, dys, xs;
     int steps;              // stages of a tile
     int64_t units;          // tiles x steps, below 2^31
     int64_t split_ld;       // elements of a row of dy's parts in the workspace; 0: dy as it is
@@ -209,12 +209,16 @@ __device__ __forceinline__ void tmem_load(uint32_t at, float (&v)[16]) {
 }
 
 // A run of stages of one tile that is summed in TMEM. The tensor core's f32
-// accumulation drops the bits below the sum's last place, about 4e-9 of the
-// result for each product of 16 rows, always towards zero; a 32-bit dw
-// therefore takes runs of at most RUN stages (below 8e-7) and adds them up in
-// global memory, each thread the values it wrote itself. For a 16-bit dw a
-// whole segment is one run.
-constexpr int RUN = 40;
+// accumulation drops the bits below the sum's last place, always towards zero:
+// nothing while the products' bits still fit, up to 6e-8 of the result for each
+// product of 16 rows (4 a stage) of a long sum. Values of one sign lose 1.8e-6
+// in 40 stages, 4e-5 in 240, 4.7e-4 in 2048 (measured). A share therefore goes
+// in runs, which are added up in global memory, each thread the values it wrote
+// itself: at most RUN stages, and RUN_BF16 where the result is rounded to bf16
+// (at most 6e-5, a 32nd of the least that its rounding can move a value by).
+// Each run more is a tile written and read: 8192 x 4096 x 4096 takes 593 us in
+// f16 for 523 in one run, in bf16 332 in runs of 64 for 282 in one of 128.
+constexpr int RUN = 40, RUN_BF16 = 256;
 
 // The units (a stage of a tile each) that fall to a CTA, in order. A share is
 // what it has of one tile, cut into runs.
@@ -516,9 +520,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 if (!ok)
                     for (float& e : v) e = __uint_as_float(0x7fffffffu);
-                if (!walk.whole) {
-                    float* to = part + (((int64_t)(2 * blockIdx.x + (walk.head ? 0 : 1)) * MT + m) * p.bk + c) * 128 + row;
-                    put<W>(to, 128, v, W, !walk.begins);
+                // A share that is not the whole tile is left to the second kernel, in the CTA's first or second place. A
+                // 16-bit tile in several runs is summed up in the second (the CTA's last share comes after it), then rounded.
+                const bool wide = a.out_type == WC_F32;
+                float* kept = part + (((int64_t)(2 * blockIdx.x + (walk.head && !walk.whole ? 0 : 1)) * MT + m) * p.bk + c) * 128 + row;
+                if (!wide && walk.whole && !walk.begins && walk.share_ends(p))
+#pragma unroll
+                    for (int e = 0; e < W; ++e) v[channel(e)] += kept[e * 128];
+                if (!walk.whole || !(wide || walk.share_ends(p))) {
+                    put<W>(kept, 128, v, W, !walk.begins);
                 } else if (n < a.n) {
                     const int count = (int)min((int64_t)W, a.k - k0 - c);
                     const int64_t to = (k0 + c) * a.n + n;
@@ -634,7 +644,8 @@ Plan plan_of(const wc_act8_wgrad_args& a) {
     p.whole = p.steps <= 4 && tiles <= MAX_CTAS;
     p.ctas = (int)std::max<int64_t>(1, p.whole ? tiles : std::min<int64_t>(MAX_CTAS, p.steps == 1 ? p.units : (p.units + 1) / 2));
     p.joined = p.steps > 1 && (p.units % p.ctas != 0 || (p.units / p.ctas) % p.steps != 0);
-    p.limit = a.out_type == WC_F32 ? RUN : 1 << 30;
+    p.limit = a.out_type == WC_BF16 ? RUN_BF16 : RUN;
+    p.kept = p.joined || (a.out_type != WC_F32 && p.steps > p.limit);
     // Converters work a stage or two ahead of the products; what is left holds copies in flight, of dy and x8 in turn.
     // x8's ring has an even number of places, so that a place is always the same team's. With an odd one a team that is
     // ahead could take the barrier's phase before last for the one it waits for, when the copy between the two (the
@@ -722,7 +733,7 @@ void launch_join(const wc_act8_wgrad_args& a, const Plan& p, const float* part, 
 uint64_t wgrad8_workspace(const wc_act8_wgrad_args& a) {
     if (!a.n || !a.rows) return 0;
     const Plan p = plan_of(a);
-    return parts_bytes(a, p) + (uint64_t)(p.ntiles + p.ctas) * 1024 + (p.joined ? (uint64_t)2 * p.ctas * p.mt * 128 * p.bk * sizeof(float) : 0);
+    return parts_bytes(a, p) + (uint64_t)(p.ntiles + p.ctas) * 1024 + (p.kept ? (uint64_t)2 * p.ctas * p.mt * 128 * p.bk * sizeof(float) : 0);
 }
 
 void launch_wgrad8(const wc_act8_wgrad_args& a, cudaStream_t s) {
