@@ -709,3 +709,19 @@ def test_act8_wgrad_long_sums_in_bf16():
     # a run's bias: 1024 products, each half a last place of a sum that grows to the result (u of the result)
     assert abs(float(off.mean())) < 6 * EPS[BF16] / math.sqrt(3 * K * N) + 1024 * U
     assert float(off.abs().max()) < EPS[BF16] + 1e-4
+
+
+# --------------------------------------------------------------------- long gates
+
+@pytest.mark.parametrize("T", [1, 2, 3, 100])
+@pytest.mark.parametrize("D", [40, 300, 5000])
+def test_block_norm_one_gate_for_any_number_of_rows(T, D):
+    c = norm_case(T, D, F32, "layer", per=0, seed=T)
+    r, rest = ops.block_norm(**c), {k: v for k, v in c.items() if k not in ("x", "h")}
+    dy, dn = randn(gen(1), T, D), randn(gen(2), T, D)
+    want = [r.y, r.n, *ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest)]
+    for per in (2 ** 63 - 1, 2 ** 63 - T, T + 1):
+        s = ops.block_norm(**(c | {"rows_per_gate": per}))
+        got = [s.y, s.n, *ops.block_norm_backward(dy, dn, c["x"], c["h"], s.stats, **(rest | {"rows_per_gate": per}))]
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)

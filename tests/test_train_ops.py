@@ -142,3 +142,9 @@ def test_cpu_tensors_are_refused():
                  lambda: ops.policy_loss(x, torch.zeros(4, dtype=torch.int64), x[:, 0], x[:, 0])):
         with pytest.raises(SolveError, match="CUDA tensor"):
             call()
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 100])
+def test_a_gate_for_more_rows_than_there_are_is_one_for_all(rows):
+    space = lambda per: lib().wc_block_norm_workspace(norm(rows=rows, gate=P, rows_per_gate=per))  # noqa: E731
+    assert space((1 << 63) - 1) == space((1 << 63) - rows) == space(rows)

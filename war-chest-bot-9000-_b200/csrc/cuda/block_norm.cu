@@ -343,7 +343,8 @@ struct Plan {
     int width, segments, workers, lanes, parts;  // lanes of a warp a row (0: a CTA a row, -1: rows, then columns)
     Plan(const wc_block_norm_args& a) {
         width = (int)a.width;
-        R = a.gate ? a.rows_per_gate : a.rows;
+        // (a gate for more rows than there are is one for all of them, however many it says)
+        R = a.gate ? std::min(a.rows_per_gate, std::max<int64_t>(1, a.rows)) : a.rows;
         groups = a.rows ? (a.rows + R - 1) / R : 0;
         lanes = a.width > 4096 ? -1 : 0;
         if (a.width <= 256)
