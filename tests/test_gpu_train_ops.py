@@ -725,3 +725,15 @@ def test_block_norm_one_gate_for_any_number_of_rows(T, D):
         got = [s.y, s.n, *ops.block_norm_backward(dy, dn, c["x"], c["h"], s.stats, **(rest | {"rows_per_gate": per}))]
         for a, b in zip(want, got):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+def test_block_norm_one_gate_for_no_rows(kind):
+    c = norm_case(4, 16, F32, kind, per=0) | {"rows_per_gate": None}
+    c["x"], c["h"] = c["x"][:0], c["h"][:0]
+    r = ops.block_norm(**c)
+    assert r.y.shape == r.n.shape == (0, 16)
+    g = ops.block_norm_backward(r.y, r.n, c["x"], c["h"], r.stats, **{k: v for k, v in c.items() if k not in ("x", "h")})
+    assert g.dgate.shape == (1, 16) and not g.dgate.any()
+    with pytest.raises(SolveError, match="0 x 16"):
+        ops.block_norm(**(c | {"rows_per_gate": 4}))

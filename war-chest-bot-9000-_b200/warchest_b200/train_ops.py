@@ -195,9 +195,10 @@ def _norm_args(me, x, h, gate, rows_per_gate, residual_scale, post, pre, kind, e
         per = rows_per_gate if rows_per_gate is not None else max(1, rows)
         if per < 1:
             _fail(me, "rows_per_gate below 1")
-        if gate.shape != (-(-rows // per), width) or gate.dtype != x.dtype or \
-                gate.get_device() != x.get_device() or not gate.is_contiguous():
-            _fail(me, f"gate must be a contiguous {-(-rows // per)} x {width} matrix of x's type and device")
+        groups = -(-rows // per) if rows_per_gate is not None else 1
+        if gate.shape != (groups, width) or gate.dtype != x.dtype or gate.get_device() != x.get_device() or \
+                not gate.is_contiguous():
+            _fail(me, f"gate must be a contiguous {groups} x {width} matrix of x's type and device")
         gp = gate.data_ptr()
     there = _weight(me, "post", post, x) + _weight(me, "pre", pre, x)
 
@@ -249,7 +250,7 @@ def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, r
     ld_dy = _matrix(me, "dy", dy, x) if dy is not None else 0
     ld_dn = _matrix(me, "dn", dn, x) if dn is not None else 0
     dx, dh = x.new_empty(rows, width), x.new_empty(rows, width)
-    dgate = torch.empty_like(gate) if gate is not None else None
+    dgate = None if gate is None else torch.empty_like(gate) if rows else torch.zeros_like(gate)
     grads = [x.new_empty(width, dtype=torch.float32) if w else None for w in there]
     scratch = _scratch(lib().wc_block_norm_workspace(packed), x)
     _call(lib().wc_block_norm_backward, x.get_device(), packed, _BLOCK_NORM_GRADS.pack(
