@@ -737,3 +737,43 @@ def test_block_norm_one_gate_for_no_rows(kind):
     assert g.dgate.shape == (1, 16) and not g.dgate.any()
     with pytest.raises(SolveError, match="0 x 16"):
         ops.block_norm(**(c | {"rows_per_gate": 4}))
+
+
+# ------------------------------------------------------------------ waits that run out
+
+@pytest.fixture
+def wait_limit():
+    """Sets the limit of the kernels' waits for their own copies and products, which complete all the same."""
+    from warchest_b200 import _check, lib
+
+    yield lambda ns: _check(lib().wc_debug_set_train_wait_limit(ns))
+    torch.cuda.synchronize()
+    _check(lib().wc_debug_set_train_wait_limit(0))
+
+
+LIMITS = [1, 300, 1000, 3000, 10000]
+
+
+def gives_up(wait_limit, call):
+    """call's results under short limits: each element NaN or, to the bit, what it is without; at the shortest there is NaN.
+    Then as before."""
+    want = call()
+    for ns in LIMITS:
+        wait_limit(ns)
+        got = call()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert (b.isnan() | (a == b) | a.isnan()).all(), ns
+        assert ns > LIMITS[0] or any(b.isnan().any() for b in got)
+    wait_limit(0)
+    for a, b in zip(want, call()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,K,N,dtype,out", [
+    (40, 96, 64, BF16, F32), (150, 192, 96, BF16, F32), (150, 192, 96, F16, F16), (250, 300, 500, BF16, BF16), (1000, 64, 2000, F32, F32),
+    (2500, 1000, 1000, BF16, BF16), (60000, 192, 96, BF16, F32), (30000, 320, 200, F16, F16), (20000, 512, 336, F32, F32)])
+def test_act8_wgrad_waits_that_run_out(wait_limit, T, K, N, dtype, out):
+    g = gen(31)
+    x8, dy = ops.act8_pack(randn(g, T, K, dtype=BF16)), randn(g, T, N, dtype=dtype)
+    gives_up(wait_limit, lambda: ops.act8_wgrad(x8, dy, dtype=out))

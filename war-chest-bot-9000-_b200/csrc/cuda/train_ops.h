@@ -8,6 +8,8 @@
 
 namespace wctrain {
 
+// limit of each wait of a kernel for its own copies and products, ns of %globaltimer
+uint64_t wait_limit();
 // policy_loss.cu
 uint64_t policy_loss_workspace(int64_t rows, int64_t width);
 void launch_policy_loss(const wc_policy_loss_args& a, cudaStream_t s);

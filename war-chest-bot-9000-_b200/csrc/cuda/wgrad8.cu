@@ -63,7 +63,7 @@ struct Plan {
 
 struct Shared {
     uint64_t x_full[MAX_STAGES], x_empty[MAX_STAGES], dy_full[MAX_STAGES], dy_empty[MAX_STAGES];
-    uint64_t op_full[MAX_STAGES], op_empty[MAX_STAGES], acc_full, acc_empty;
+    uint64_t op_full[MAX_STAGES], op_empty[MAX_STAGES], acc_full, acc_empty, drained;
     uint32_t tmem;
     int failed;
 };
@@ -110,19 +110,6 @@ __device__ __forceinline__ void commit_one(uint64_t* bar) {
         "elect.sync _|e, 0xffffffff;\n\t"
         "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(umma::smem_u32(bar))
         : "memory");
-}
-// One test that may sleep for up to 100 us: a warp that polls instead takes issue slots and shared-memory cycles from
-// the warps it waits for.
-__device__ __forceinline__ bool mbar_sleep(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(umma::smem_u32(bar)), "r"(parity), "r"(100000u)
-        : "memory");
-    return done != 0;
 }
 __device__ __forceinline__ void arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(bar)) : "memory");
@@ -259,7 +246,7 @@ struct Walk {
 template <int P, int MT>
 __global__ void __launch_bounds__(THREADS, 1)
     k_wgrad8(wc_act8_wgrad_args a, Plan p, const __grid_constant__ CUtensorMap map_q,
-             const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db) {
+             const __grid_constant__ CUtensorMap map_dy, float* part, float* part_db, uint64_t wait_ns) {
     constexpr int GROUPS = 2 * MT;  // of 64 columns of dy
     extern __shared__ uint8_t raw[];
     __shared__ Shared sh;
@@ -281,6 +268,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         umma::mbar_init(&sh.acc_full, 1);
         umma::mbar_init(&sh.acc_empty, CONVERTERS / 32);
+        umma::mbar_init(&sh.drained, 1);
         sh.failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -291,11 +279,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t tmem = sh.tmem;
     Walk walk(p);
     Place x{p.xs}, dy{p.dys}, op{p.operands};
-    // A wait that runs out (umma.cuh) makes every role give up: products and copies in flight are waited for, what
-    // the CTA had still to write becomes NaN, and the tensor memory is released. wait_all: the same for a whole warp.
+    // A wait that runs out makes every role give up: products and copies in flight are waited for, what the CTA had still
+    // to write becomes NaN, and the tensor memory is released. What a role that gave up owes to others stays undone, so
+    // that their waits run out too. wait_all: the same for a whole warp.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        if (mbar_sleep(bar, parity)) return true;
-        if (!*failed && umma::mbar_wait(bar, parity)) return true;
+        if (sleep_on(bar, parity, wait_ns)) return true;
+        if (!*failed && wait_ns > SLEEP_NS && umma::mbar_wait(bar, parity, wait_ns)) return true;
         *failed = 1;
         return false;
     };
@@ -335,17 +324,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (ok) commit_one(&sh.acc_full), ++done;
             walk.skip(p, n);
         }
-        if (!ok) {  // every issued product has finished before TMEM is given back
-            commit_one(&sh.acc_full);
-            umma::mbar_wait(&sh.acc_full, done & 1, umma::DRAIN_NS);
-        }
+        // Every issued product has finished before TMEM is given back, also where no one waits for it any more. (On a barrier
+        // of its own: acc_full would tell of a whole run.)
+        commit_one(&sh.drained);
+        umma::mbar_wait(&sh.drained, 0, umma::DRAIN_NS);
     } else if (warp == 1) {  // ----------------------------- dy's producer
         if (lane == 0) {
             const uint32_t ring = umma::smem_u32(dys);
             int it = 0;
-            bool ok = true;
             for (; walk.more(); walk.next(p), dy.next(), ++it) {
-                if (it >= p.dys && !(ok = wait(&sh.dy_empty[dy.slot], dy.phase ^ 1))) break;
+                if (it >= p.dys && !wait(&sh.dy_empty[dy.slot], dy.phase ^ 1)) break;
                 const int n0 = walk.nt * (MT * 128);
                 umma::expect_tx(&sh.dy_full[dy.slot], p.dy_bytes());
                 uint32_t to = ring + dy.slot * p.dy_bytes();
@@ -355,9 +343,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int g = 0; g < GROUPS; ++g, to += GROUP)
                         tma_load(to, &map_dy, n0 + 64 * g, walk.s * BK, q, &sh.dy_full[dy.slot]);
             }
-            if (!ok)  // the copies in flight land before the CTA leaves
-                for (int i = it > p.dys ? it - p.dys : 0; i < it; ++i)
-                    umma::mbar_wait(&sh.dy_full[i % p.dys], (i / p.dys) & 1, umma::DRAIN_NS);
+            // the copies in flight land before the CTA leaves, also where no one waits for them any more
+            for (int i = it > p.dys ? it - p.dys : 0; i < it; ++i)
+                umma::mbar_wait(&sh.dy_full[i % p.dys], (i / p.dys) & 1, umma::DRAIN_NS);
         }
         __syncwarp();
     } else if (warp == 2) {  // ----------------------------- x8's producer
@@ -365,9 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int64_t blocks = (a.k + 31) / 32;
         const uint32_t ring = umma::smem_u32(xs);
         int it = 0;
-        bool ok = true;
         for (; walk.more(); walk.next(p), x.next(), ++it) {
-            if (it >= p.xs && !(ok = wait_all(&sh.x_empty[x.slot], x.phase ^ 1))) break;
+            if (it >= p.xs && !wait_all(&sh.x_empty[x.slot], x.phase ^ 1)) break;
             const uint32_t to = ring + x.slot * p.x_bytes();
             const int k0 = walk.kt * p.bk, t0 = walk.s * BK;
             if (lane == 0) {
@@ -392,7 +379,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(umma::smem_u32(&sh.x_full[x.slot])) : "memory");
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-        if (!ok && lane == 0)
+        if (lane == 0)
             for (int i = it > p.xs ? it - p.xs : 0; i < it; ++i)
                 umma::mbar_wait(&sh.x_full[i % p.xs], (i / p.xs) & 1, umma::DRAIN_NS);
         __syncwarp();
@@ -539,7 +526,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             umma::fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive(&sh.acc_empty);
+            if (ok && lane == 0) arrive(&sh.acc_empty);
             ++done;
         }
     }
@@ -713,7 +700,7 @@ void launch_tile(const wc_act8_wgrad_args& a, const Plan& p, const __nv_bfloat16
         : map_of(a.dy, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, a.n, a.rows, 1, a.ld_dy * 2, CU_TENSOR_MAP_SWIZZLE_128B);
     const size_t smem = (size_t)p.ring_bytes() + 1024;
     if (!wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_wgrad8<P, MT>), RING + 1024)) return;
-    k_wgrad8<P, MT><<<p.ctas, THREADS, smem, s>>>(a, p, q, dy, part, part_db);
+    k_wgrad8<P, MT><<<p.ctas, THREADS, smem, s>>>(a, p, q, dy, part, part_db, wait_limit());
 }
 
 template <class T>

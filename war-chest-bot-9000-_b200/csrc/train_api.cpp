@@ -1,5 +1,6 @@
 // The C entries of the training operators (include/wc_b200.h): argument
 // checks, then the launch.
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <initializer_list>
@@ -32,6 +33,8 @@ int launched(const char* what, F&& f) {
     return WC_E_CUDA;
 }
 
+std::atomic<uint64_t> g_wait_ns{wc::DEFAULT_WAIT_NS};
+
 bool type_ok(int t) { return t == WC_F32 || t == WC_F16 || t == WC_BF16; }
 bool size_ok(int64_t rows, int64_t width) { return rows >= 0 && width >= 0 && rows <= (1ll << 31) && width <= (1ll << 31); }
 bool off(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
@@ -45,7 +48,14 @@ bool loose(int type, std::initializer_list<const void*> ps) {
 
 }  // namespace
 
+uint64_t wctrain::wait_limit() { return g_wait_ns; }
+
 extern "C" {
+
+int wc_debug_set_train_wait_limit(uint64_t ns) {
+    g_wait_ns = ns ? ns : wc::DEFAULT_WAIT_NS;
+    return WC_OK;
+}
 
 uint64_t wc_policy_loss_workspace(int64_t rows, int64_t width) {
     return size_ok(rows, width) ? wctrain::policy_loss_workspace(rows, width) : 0;

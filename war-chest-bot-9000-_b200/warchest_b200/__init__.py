@@ -116,6 +116,7 @@ def _load() -> C.CDLL:
         "wc_job_from_wcj8": (I, [C.c_char_p, C.c_size_t, P(VP)]),
         "wc_debug_set_wait_limit": (I, [VP, U64]),
         "wc_replay_expand": (I, [VP, C.c_size_t, VP, VP, C.c_size_t, VP, VP, VP]),
+        "wc_debug_set_train_wait_limit": (I, [U64]),
         "wc_policy_loss_workspace": (U64, [C.c_int64, C.c_int64]),
         "wc_policy_loss": (I, [VP, VP]),
         "wc_block_norm": (I, [VP, VP]),
