@@ -461,9 +461,10 @@ struct Column {
         else unpairs(which == 2 ? dwn : dbn, v);
     }
     // A row's unit. get(i, v) reads its x, h, dy or dn (i = 0 .. 3; zeros past the width and for a gradient that is not
-    // there), when it is needed: what is not held meanwhile leaves room for the sums. put(i, v) takes dx, then dh.
+    // there), when it is needed: what is not held meanwhile leaves room for the sums. put(i, v) takes dx, then dh. `zero`
+    // stands for what the pre norm gives where there is none.
     template <class G, class Get, class Put>
-    __device__ __forceinline__ void row(const wc_block_norm_args& a, const float4& st, bool pre, float inv, G& group, Get&& get, Put&& put) {
+    __device__ __forceinline__ void row(const wc_block_norm_args& a, const float4& st, bool pre, float inv, float zero, G& group, Get&& get, Put&& put) {
         const bool layer = a.kind == WC_NORM_LAYER;
         Pair hh[4], yh[4], d[4];
         get(1, hh), get(0, yh);
@@ -482,7 +483,7 @@ struct Column {
 #pragma unroll
             for (int k = 0; k < 4; ++k) yh[k] = mul(nr, fma(yh[k], a1, add(d[k], a0)));
         } else {
-            fill(yh, 0.0f);
+            fill(yh, zero);
         }
         get(2, d);
         const Pair rs = twice(a.residual_scale);
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
             const int64_t t = t0 + slot;
             const bool here = any && t < last;  // (a row past the last has gradients of 0: it adds 0 to every sum)
             const float4 st = next;
-            col.row(a, st, pre, inv, group,
+            col.row(a, st, pre, inv, 0.0f, group,
                     [&](int k, Pair* v) {
                         float f[8];
                         u[k].get(f);
@@ -608,7 +609,7 @@ __global__ void __launch_bounds__(256, 2) k_norm_backward_warp(wc_block_norm_arg
 constexpr int MAX_RING = 8;
 template <class T, int LAY>
 __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a, wc_block_norm_grads g, Items q, int stages,
-                                                           float* gate_part, float* weight_part) {
+                                                           float* gate_part, float* weight_part, uint64_t wait_ns) {
     extern __shared__ __align__(128) uint8_t shared[];  // what Column keeps, then the ring
     uint8_t* const ring = shared + 64 * blockDim.x;
     __shared__ float2 s[2][32];
@@ -639,6 +640,7 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
     const int64_t pitch = (array == 0 ? a.ld_x : array == 1 ? a.ld_h : array == 2 ? g.ld_dy : g.ld_dn) * (int64_t)sizeof(T);
     int64_t copy_item = blockIdx.x, copy_row = 0, copy_last = 0, copy_group;
     int copy_slot = 0;
+    uint32_t copied = 0;
     auto copy = [&] {
         while (copy_row >= copy_last) {
             if (copy_item >= q.items) return;
@@ -653,7 +655,7 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
         __syncwarp();
         if (bytes) bulk_copy(umma::smem_u32(ring + copy_slot * stage_bytes) + threadIdx.x * piece, from, bytes, &full[copy_slot]);
         copy_slot = copy_slot + 1 == stages ? 0 : copy_slot + 1;
-        ++copy_row;
+        ++copy_row, ++copied;
     };
     if (threadIdx.x < 32)
         for (int i = 0; i + 1 < stages; ++i) copy();
@@ -665,15 +667,16 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
         q.range(i, item_group, first, last);
         col.begin(a, item_group, cols, 0);
         for (int64_t t = first; t < last; ++t) {
-            // a copy that does not come (umma.cuh) leaves NaN from here on
-            if (!bad && !umma::mbar_wait(&full[slot], turns & 1)) bad = true;
+            // a copy that does not come leaves NaN from here on: hhat and yhat are none, nor is 0
+            if (!bad && !wait_within(&full[slot], turns & 1, wait_ns)) bad = true;
             float4 st = *reinterpret_cast<const float4*>(ring + slot * stage_bytes + 4 * piece);
-            if (bad) st.y = st.w = __uint_as_float(0x7fffffffu);
+            const float zero = bad ? __uint_as_float(0x7fffffffu) : 0.0f;
+            if (bad) st.y = st.w = zero;
             const bool here = !edge(t);
             // all have read the row before this one, whose stage takes another: with a post norm, before its last sum
             if (!a.post_weight) __syncthreads();
             if (threadIdx.x < 32 && __all_sync(~0u, !bad)) copy();
-            col.row(a, st, pre, inv, group,
+            col.row(a, st, pre, inv, zero, group,
                     [&](int k, Pair* v) {
                         Unit<T, LAY> u;
                         u.zero();
@@ -703,8 +706,10 @@ __global__ void __launch_bounds__(512) k_norm_backward_cta(wc_block_norm_args a,
             else store8(gate_part + i * D, cols, 0, dg);
         }
     }
-    if (bad && threadIdx.x == 0)
-        for (int k = 0; k < stages; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
+    if (bad && threadIdx.x == 0)  // (the others' rows have all come where this thread's have)
+        for (uint32_t i = copied > (uint32_t)stages ? copied - stages : 0; i < copied; ++i)
+            umma::mbar_wait(&full[i % stages], (i / stages) & 1, umma::DRAIN_NS);
+    if (bad) fill(col.dbn, __uint_as_float(0x7fffffffu));  // (a sum of dn alone)
     if (any) {
         float* to = weight_part + (int64_t)blockIdx.x * 4 * D;
 #pragma unroll
@@ -910,7 +915,7 @@ void backward_as(const wc_block_norm_args& a, const wc_block_norm_grads& g, cuda
             const int stage = (int)(4 * (UNITS ? D * e : (D * e + 15) / 16 * 16 + 16) + 16), threads = p.threads();
             const int stages = (int)std::min<int64_t>(MAX_RING, (200 * 1024 / (512 / threads) - 64 * threads) / stage);
             if (wcdev::raise_smem_limit(reinterpret_cast<const void*>(k_norm_backward_cta<T, WIDE>), 200 * 1024))
-                k_norm_backward_cta<T, WIDE><<<p.workers, threads, (size_t)stages * stage + 64 * threads, s>>>(a, g, q, stages, gates, weights);
+                k_norm_backward_cta<T, WIDE><<<p.workers, threads, (size_t)stages * stage + 64 * threads, s>>>(a, g, q, stages, gates, weights, wait_limit());
         } else {
             const unsigned threads = (unsigned)((D + 511) / 512 * 32);
             const unsigned n = (unsigned)std::min<int64_t>(a.rows, 148 * (1024 / threads));

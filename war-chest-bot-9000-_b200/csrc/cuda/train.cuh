@@ -47,28 +47,35 @@ __device__ __forceinline__ float min_nan(float a, float b) {
     return d;
 }
 
-// One test of a barrier that may sleep for up to SLEEP_NS, or the limit of a wait if that is shorter (the whole wait, then;
-// below a microsecond it is one look, as a sleep's end is not that exact): a warp that polls instead takes issue slots
-// and shared-memory cycles from the warps it waits for.
+// Waits of at most `limit_ns`. A limit below a microsecond is one look, as the end of a sleep is not that exact.
+constexpr uint64_t LOOK_NS = 1000;
+__device__ __forceinline__ bool look_at(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(umma::smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool wait_within(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    return look_at(bar, parity) || (limit_ns >= LOOK_NS && umma::mbar_wait(bar, parity, limit_ns));
+}
+// ... the first part of a wait, up to SLEEP_NS, asleep: a warp that polls takes issue slots and shared-memory cycles from
+// the warps it waits for
 constexpr uint64_t SLEEP_NS = 100000;
 __device__ __forceinline__ bool sleep_on(uint64_t* bar, uint32_t parity, uint64_t limit_ns) {
+    if (limit_ns < LOOK_NS) return look_at(bar, parity);
     uint32_t done;
-    if (limit_ns < 1000)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(umma::smem_u32(bar)), "r"(parity)
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}\n"
-            : "=r"(done)
-            : "r"(umma::smem_u32(bar)), "r"(parity), "r"((uint32_t)min(limit_ns, SLEEP_NS))
-            : "memory");
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(umma::smem_u32(bar)), "r"(parity), "r"((uint32_t)min(limit_ns, SLEEP_NS))
+        : "memory");
     return done != 0;
 }
 
