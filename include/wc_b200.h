@@ -532,11 +532,11 @@ typedef struct wc_act8_wgrad_args {
 uint64_t wc_act8_wgrad_workspace(const wc_act8_wgrad_args* a);
 int wc_act8_wgrad(const wc_act8_wgrad_args* a, void* stream);
 
-/* The time limit of wc_act8_wgrad's and wc_block_norm_backward's waits in the
- * calls to come, in the whole process (ns of %globaltimer; 0 restores the
- * default, 2 s). A debug control: with a limit shorter than the work waited on, a kernel gives up, waits for
- * what it has in flight, releases its tensor memory and ends, and the device
- * stays usable; a result is then NaN or what it would have been. */
+/* The time limit of those waits in the calls to come, in the whole process (ns
+ * of %globaltimer; 0 restores the default, 2 s). A debug control: with a limit
+ * shorter than the work waited on, a kernel gives up, waits for what it has in
+ * flight, releases its tensor memory and ends, and the device stays usable; a
+ * result is then NaN or what it would have been. */
 int wc_debug_set_train_wait_limit(uint64_t ns);
 
 /* ---- streaming submit / wait ---------------------------------------------- */

@@ -790,3 +790,12 @@ def test_block_norm_backward_waits_that_run_out(wait_limit, T, D, dtype, per, po
     dy, dn = randn(gen(1), T, D, dtype=dtype), randn(gen(2), T, D, dtype=dtype) if pre else None
     gives_up(wait_limit, lambda: [g for g in ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest) if g is not None],
              sure=T * D > 1 << 26)
+
+
+@pytest.mark.parametrize("T,V,dtype,legal", [
+    (5, 1025, F32, None), (700, 2001, F16, 0.4), (600, 9000, BF16, None), (2000, 16384, BF16, None), (300, 40000, F32, 0.5), (500, 50001, BF16, None),
+    (300, 131072, BF16, None)])
+def test_policy_waits_that_run_out(wait_limit, T, V, dtype, legal):
+    c = policy_case(T, V, dtype, seed=41, legal=legal)
+    c["weights"][::7] = 0.0
+    gives_up(wait_limit, lambda: ops.policy_loss(**c, **OPTIONS), sure=T * V > 1 << 24)

@@ -431,7 +431,7 @@ __device__ __forceinline__ uint32_t of_rank(uint32_t addr, int rank) {
 }
 constexpr int MAX_SLICES = 4;
 template <class T, bool MASK, int WARPS, int CTAS>
-__global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 ? 4 : 6) k_policy_cluster(wc_policy_loss_args a, int slice, int slices, double* part) {
+__global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 ? 4 : 6) k_policy_cluster(wc_policy_loss_args a, int slice, int slices, double* part, uint64_t wait_ns) {
     constexpr int N = Chunk<T>::N, THREADS = WARPS * 32;
     constexpr int TOGETHER = 1;
     extern __shared__ __align__(128) uint8_t ring[];  // `slices` of the logits, then of the legal bytes
@@ -468,10 +468,11 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
     if (CTAS > 1) cluster.sync();
     else __syncthreads();
     double total = 0.0;
-    // A wait that runs out (umma.cuh) leaves NaN in the rows from here on; the copies in flight land before the end.
+    // A wait that runs out leaves NaN in the rows from here on. What a warp that gave up owes to others stays undone, so
+    // that their waits run out too and none takes a place for free, or a row's parts for whole, that is not.
     bool bad = false;
     auto wait = [&](uint64_t* bar, int64_t use) {
-        if (!bad && !umma::mbar_wait(bar, (uint32_t)use & 1)) bad = true, failed = 1;
+        if (!bad && !wait_within(bar, (uint32_t)use & 1, wait_ns)) bad = true, failed = 1;
         bad = __any_sync(~0u, bad);  // (a warp's lanes go on together)
     };
     // the slice of a row, and how often it had others before
@@ -527,15 +528,14 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                 const int turn = (int)live & 3;
                 RowIn in = now.in;
                 in.w = __shfl_sync(~0u, in.w, at), in.old = __shfl_sync(~0u, in.old, at), in.A = __shfl_sync(~0u, in.A, at), in.r = __shfl_sync(~0u, in.r, at);
-                if (CTAS > 1 && lane == 0) umma::expect_tx(&joined[turn], CTAS * WARPS * 16);
+                if (CTAS > 1 && lane == 0 && !bad) umma::expect_tx(&joined[turn], CTAS * WARPS * 16);
                 wait(&joined[turn], live >> 2);
                 float M, S, W;
                 join<(CTAS * WARPS + 31) / 32>(parts[turn], CTAS * WARPS, M, S, W);
                 if (bad) S = __uint_as_float(0x7fffffffu);
                 const Row row(a, in, M, S, W, za);
                 if (lane == 0) {
-                    rows[live & 1] = row;
-                    arrive(&ready[live & 1]);
+                    if (!bad) rows[live & 1] = row, arrive(&ready[live & 1]);
                     if (rank == 0) row.put(a, t), total += (double)(in.w * row.loss);
                 }
                 ++live;
@@ -547,11 +547,14 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
             const int64_t ahead = i - 1 + slices;
             if (i && t + (slices - 1) * step < a.rows) {
                 wait(&empty[done.slot], done.use);
-                if (!bad) copy(ahead, done.slot, (ahead >> 5) != (i >> 5));
-                done.next(slices);
+                if (!bad) copy(ahead, done.slot, (ahead >> 5) != (i >> 5)), done.next(slices);
             }
             __syncwarp();
         }
+        // the copies in flight land before the CTA leaves, also where no one waits for them any more
+        const int64_t copied = min((a.rows - t0 + step - 1) / step, (int64_t)(done.use + 1) * slices + done.slot);
+        if (lane == 0)
+            for (int64_t i = max((int64_t)0, copied - slices); i < copied; ++i) umma::mbar_wait(&full[i % slices], (uint32_t)(i / slices) & 1, umma::DRAIN_NS);
     } else {
         int64_t live = 0;  // rows with parts sent
         int act0 = -1;
@@ -704,17 +707,21 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                     }
                 }
                 __syncwarp();
-                if (lane == 0) arrive(&empty[slot]);
+                if (lane == 0 && !bad) arrive(&empty[slot]);
                 written.next(slices);
             }
             act0 = act1, za0 = za1;
         }
     }
     __syncthreads();
-    if (failed && threadIdx.x == 0)
-        for (int k = 0; k < slices; ++k) umma::mbar_wait(&full[k], 0, umma::DRAIN_NS / 4), umma::mbar_wait(&full[k], 1, umma::DRAIN_NS / 4);
     if (rank == 0 && threadIdx.x == THREADS) part[blockIdx.x / CTAS] = total;
-    if (CTAS > 1) cluster.sync();  // no CTA leaves while another may still write to it
+    if (CTAS > 1) {
+        cluster.sync();  // no CTA leaves while another may still write to it
+        // Where this CTA's warp has not waited for all that was sent to it, the last of that may still be on its way, for less
+        // than a few microseconds.
+        if (failed)
+            for (const uint64_t from = umma::now_ns(); umma::now_ns() - from < 100000;) {}
+    }
 }
 
 // Any row: one CTA reads it twice, an entry at a time.
@@ -827,7 +834,7 @@ int launch_cluster(const wc_policy_loss_args& a, int sm, double* part, cudaStrea
     else if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess || most < 1) most = 1;
     const int n = (int)std::min<int64_t>(most, a.rows);
     cfg.gridDim = n * CTAS;
-    cudaLaunchKernelEx(&cfg, kernel, a, slice, slices, part);
+    cudaLaunchKernelEx(&cfg, kernel, a, slice, slices, part, wait_limit());
     return n;
 }
 
