@@ -799,3 +799,17 @@ def test_policy_waits_that_run_out(wait_limit, T, V, dtype, legal):
     c = policy_case(T, V, dtype, seed=41, legal=legal)
     c["weights"][::7] = 0.0
     gives_up(wait_limit, lambda: ops.policy_loss(**c, **OPTIONS), sure=T * V > 1 << 24)
+
+
+# ----------------------------------------------------------------- equal bits, layers
+
+def test_layers_refuse_second_derivatives():
+    g = gen(14)
+    x, w = randn(g, 20, 40).requires_grad_(), randn(g, 40, 30).requires_grad_()
+    y = layers.gelu8(layers.linear8(layers.block_norm(x, x.detach(), pre=torch.ones(40, device="cuda"))[1], w))
+    want = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    got = torch.autograd.grad(y.sum(), (x, w), create_graph=True)
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+        with pytest.raises(SolveError, match="second derivative"):
+            torch.autograd.grad(b.square().sum() + w.sum(), w, retain_graph=True)
