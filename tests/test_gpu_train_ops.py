@@ -803,6 +803,13 @@ def test_policy_waits_that_run_out(wait_limit, T, V, dtype, legal):
 
 # ----------------------------------------------------------------- equal bits, layers
 
+def test_equal_calls_give_the_same_bits():
+    first = every_result(3)
+    for _ in range(3):
+        for a, b in zip(first, every_result(3)):
+            assert torch.equal(a, b) and not (a.is_floating_point() and a.isnan().any())
+
+
 def test_layers_refuse_second_derivatives():
     g = gen(14)
     x, w = randn(g, 20, 40).requires_grad_(), randn(g, 40, 30).requires_grad_()
