@@ -401,7 +401,8 @@ enum { WC_F32 = 0, WC_F16 = 1, WC_BF16 = 2 };
  * `legal` byte (all, when legal is NULL) and a value above -inf count. With
  * l = ln softmax(z)[action], ratio = exp(l - old_logp), A the advantage, H
  * the entropy of softmax(z), and k = exp(r - l) - (r - l) - 1 for the
- * reference log-probability r (0 when ref_logp is NULL):
+ * reference log-probability r (0 when ref_logp is NULL; with a kl_coef of 0 it
+ * is a result only):
  *   row_loss = -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A)
  *              + kl_coef k - entropy_coef H
  *   loss = sum of weight row_loss         (weight 1 when weights is NULL)

@@ -820,3 +820,14 @@ def test_layers_refuse_second_derivatives():
         assert torch.equal(a, b)
         with pytest.raises(SolveError, match="second derivative"):
             torch.autograd.grad(b.square().sum() + w.sum(), w, retain_graph=True)
+
+
+@pytest.mark.parametrize("V", [16, 600, 3000, 40000])
+def test_policy_kl_that_is_only_watched(V):
+    """With kl_coef 0 the loss and the gradient are those without a reference, however far off it is."""
+    c = policy_case(6, V, F32, seed=15)
+    c["ref_logp"] = c["ref_logp"] + torch.tensor([0.0, 50.0, 87.0, 95.0, 200.0, 1e6], device="cuda")
+    options = OPTIONS | {"kl_coef": 0.0}
+    r, s = ops.policy_loss(**c, **options), ops.policy_loss(**(c | {"ref_logp": None}), **options)
+    assert r.loss.isfinite() and torch.equal(r.loss, s.loss) and torch.equal(r.row_loss, s.row_loss) and torch.equal(r.dlogits, s.dlogits)
+    assert (r.kl[3:] == math.inf).all() and r.kl[:2].isfinite().all()

@@ -113,9 +113,9 @@ struct Row {
 #pragma unroll
         for (int i = 0; i < 8; ++i) series = fmaf(series, d, n1[i]);
         kl = fabsf(d) < 0.5f ? d * d * series : em - d;
-        loss = -(free < clipped || isnan(free) ? free : clipped) + a.kl_coef * kl - a.entropy_coef * H;
+        loss = -(free < clipped || isnan(free) ? free : clipped) + (a.kl_coef == 0.0f ? 0.0f : a.kl_coef * kl) - a.entropy_coef * H;  // (kl may be past 32 bits)
         const float up = (a.upstream ? *a.upstream : 1.0f) * in.w;
-        g = up * ((held ? 0.0f : -free) - a.kl_coef * em);
+        g = up * ((held ? 0.0f : -free) - (a.kl_coef == 0.0f ? 0.0f : a.kl_coef * em));
         ce = up * a.entropy_coef;
         // p = 2^x / S and ln p = (x - top) ln 2 - ln (S / eTop)
         e = ce * LN2 * inv, k = fmaf(ce, -LN2 * (mean + top), -g) * inv;
