@@ -831,3 +831,20 @@ def test_policy_kl_that_is_only_watched(V):
     r, s = ops.policy_loss(**c, **options), ops.policy_loss(**(c | {"ref_logp": None}), **options)
     assert r.loss.isfinite() and torch.equal(r.loss, s.loss) and torch.equal(r.row_loss, s.row_loss) and torch.equal(r.dlogits, s.dlogits)
     assert (r.kl[3:] == math.inf).all() and r.kl[:2].isfinite().all()
+
+
+def test_policy_results_are_the_users_own():
+    """They can be changed in place, and hold no more memory than they are."""
+    c = policy_case(40, 60, F32, seed=16)
+    z = c["logits"].clone().requires_grad_()
+    r = layers.policy_loss(z, c["actions"], c["old_logp"], c["advantages"], weights=c["weights"])
+    s = ops.policy_loss(c["logits"], c["actions"], c["old_logp"], c["advantages"], weights=c["weights"])
+    want, row = s.loss.clone(), s.row_loss.clone()
+    r.loss.div_(4)
+    r.row_loss.mul_(2)
+    s.loss.div_(4)
+    s.row_loss.mul_(2)
+    assert torch.equal(r.loss, want / 4) and torch.equal(s.loss, want / 4) and torch.equal(r.row_loss, 2 * row) and torch.equal(s.row_loss, 2 * row)
+    r.loss.backward()
+    near(z.grad, s.dlogits.double() / 4, 1e-7, "dlogits")
+    assert s.loss.untyped_storage().nbytes() == 4 and s.logp.untyped_storage().nbytes() == 4 * 4 * 40

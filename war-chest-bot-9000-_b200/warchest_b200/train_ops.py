@@ -124,7 +124,7 @@ def _call(fn, index: int, *args) -> None:
 
 @lru_cache(maxsize=256)
 def _policy_workspace(rows: int, width: int) -> int:
-    return (lib().wc_policy_loss_workspace(rows, width) + 15) // 16 * 4
+    return lib().wc_policy_loss_workspace(rows, width)
 
 
 def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp=None, legal=None, clip_low=0.2,
@@ -161,16 +161,14 @@ def policy_loss(logits, actions, old_logp, advantages, *, weights=None, ref_logp
         if legal.dtype not in (torch.bool, torch.uint8) or legal.shape != logits.shape or legal.get_device() != index:
             _fail(me, "legal must be a bool or uint8 matrix of the logits' shape and device")
         on, ld_legal = legal.data_ptr(), _row_stride(me, "legal", legal)
-    space = _policy_workspace(rows, width)
-    flat = old_logp.new_empty(space + 4 * rows + 1)  # workspace, rows, loss
+    scratch = _scratch(_policy_workspace(rows, width), logits)
+    loss, per_row = old_logp.new_empty(()), old_logp.new_empty((4, rows))
     grad = logits.new_empty(rows, width) if want_grad else None
-    at = flat.data_ptr()
     _call(lib().wc_policy_loss, index, _POLICY_LOSS.pack(
-        logits.data_ptr(), on, actions.data_ptr(), old, adv, wts, ref, up, at + 4 * (space + 4 * rows), at + 4 * space,
-        grad.data_ptr() if want_grad else 0, at, rows, width, ld, ld_legal, max(1, width), clip_low, clip_high, kl_coef,
-        entropy_coef, _TYPES[logits.dtype], actions.element_size()))
-    _, row_loss, logp, entropy, kl, loss = flat.split((space, rows, rows, rows, rows, 1))
-    return PolicyLoss(loss[0], row_loss, logp, entropy, kl, grad)
+        logits.data_ptr(), on, actions.data_ptr(), old, adv, wts, ref, up, loss.data_ptr(), per_row.data_ptr(),
+        grad.data_ptr() if want_grad else 0, scratch.data_ptr(), rows, width, ld, ld_legal, max(1, width), clip_low, clip_high,
+        kl_coef, entropy_coef, _TYPES[logits.dtype], actions.element_size()))
+    return PolicyLoss(loss, *per_row.unbind(), grad)
 
 
 # --------------------------------------------------------------- block norms
