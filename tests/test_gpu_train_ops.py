@@ -848,3 +848,16 @@ def test_policy_results_are_the_users_own():
     r.loss.backward()
     near(z.grad, s.dlogits.double() / 4, 1e-7, "dlogits")
     assert s.loss.untyped_storage().nbytes() == 4 and s.logp.untyped_storage().nbytes() == 4 * 4 * 40
+
+
+@pytest.mark.parametrize("T,D", [(40, 96), (40, 97), (50, 1000), (30, 5000)])
+def test_block_norm_gradients_one_at_a_time(T, D):
+    c = norm_case(T, D, BF16, "layer", per=7)
+    r, rest = ops.block_norm(**c), {k: v for k, v in c.items() if k not in ("x", "h")}
+    dy, dn = randn(gen(1), T, D, dtype=BF16), randn(gen(2), T, D, dtype=BF16)
+    full = ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest)
+    for i in range(7):
+        some = ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest, want=[j == i for j in range(7)])
+        assert torch.equal(some[i], full[i]) and all(some[j] is None for j in range(7) if j != i)
+    with pytest.raises(SolveError, match="seven"):
+        ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest, want=(True,))

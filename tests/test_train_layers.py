@@ -49,7 +49,8 @@ def asked(monkeypatch):
 
     @note
     def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, residual_scale=1.0, post=None, pre=None, kind="layer",
-                            eps=1e-5, **unused):
+                            eps=1e-5, want=None):
+        calls.append(want)
         y = residual_scale * x + h * (1 if post is None else post[0])
         d = (0 if dy is None else dy) + (0 if dn is None else 2 * dn * y * pre[0])
         return ops.BlockNormGrads(residual_scale * d, d * (1 if post is None else post[0]), None, None if post is None else (d * h).sum(0), None,
@@ -113,3 +114,38 @@ def test_gradients_under_create_graph_reach_the_leaves(asked):
         for t, g in zip(leaves, want):
             assert torch.equal(t.grad, g)
             t.grad = None
+
+
+def test_linear8_keeps_its_input_only_for_a_weight_gradient(asked):
+    x, w, b = leaf(5, 4, seed=1), leaf(4, 3, seed=3), leaf(3, seed=4)
+    want = torch.autograd.grad(layers.linear8(x, w, b).square().sum(), (x, b))
+    assert asked == ["act8_pack", "act8_wgrad"]
+    del asked[:]
+    frozen = w.detach()
+    for a, g in zip(want, torch.autograd.grad(layers.linear8(x, frozen, b).square().sum(), (x, b))):
+        assert torch.equal(a, g)
+    with torch.no_grad():
+        assert torch.equal(layers.linear8(x, w, b), x @ w + b)
+    assert layers.linear8(x.detach(), frozen).shape == (5, 3)
+    assert asked == []
+    g, = torch.autograd.grad(layers.linear8(x.detach(), w, b.detach(), x8=ops.Act8(x.detach(), torch.zeros(5, 1), 4)).sum(), w)
+    assert torch.equal(g, x.detach().t() @ torch.ones(5, 3)) and asked == ["act8_wgrad"]
+
+
+def test_block_norm_forms_the_gradients_that_are_wanted(asked):
+    x, h, post, pre = leaf(5, 4, seed=1), leaf(5, 4, seed=2), leaf(4, seed=5), leaf(4, seed=6)
+    for some in ((x,), (h, pre), (post,), (x, h, post, pre)):
+        del asked[:]
+        on = lambda t: t if any(t is s for s in some) else t.detach()  # noqa: E731
+        y, n = layers.block_norm(on(x), on(h), post=on(post), pre=on(pre))
+        torch.autograd.grad(y.sum() + n.sum(), some)
+        assert asked[1:] == ["block_norm_backward", tuple(any(t is s for s in some) for t in (x, h, None, post, None, pre, None))]
+
+
+def test_gelu8_sums_its_bias_only_for_a_gradient(asked, monkeypatch):
+    z, b = leaf(5, 4, seed=1), leaf(4, seed=2)
+    seen, real = [], ops.gelu8_backward
+    monkeypatch.setattr(ops, "gelu8_backward", lambda da, z8, want_bias=True: (seen.append(want_bias), real(da, z8, want_bias=want_bias))[1])
+    torch.autograd.grad(layers.gelu8(z, b).sum(), (z, b))
+    torch.autograd.grad(layers.gelu8(z, b.detach()).sum(), z)
+    assert seen == [True, False]

@@ -97,8 +97,8 @@ class _BlockNorm(torch.autograd.Function):
         flat = lambda d: None if d is None else d.contiguous()  # noqa: E731
         g = ops.block_norm_backward(flat(dy), flat(dn), x, h, stats, gate=gate,
                                     post=None if post is None else (post, post_bias),
-                                    pre=None if pre is None else (pre, pre_bias), **ctx.options)
-        return g.dx, g.dh, g.dgate, g.dpost, g.dpost_bias, g.dpre, g.dpre_bias, None, None
+                                    pre=None if pre is None else (pre, pre_bias), want=ctx.needs_input_grad[:7], **ctx.options)
+        return *g, None, None
 
 
 def block_norm(x, h, *, gate=None, post=None, pre=None, pack=False, **options):
@@ -115,14 +115,13 @@ class _Gelu8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, bias):
         a, z8 = ops.gelu8(z, bias)
-        ctx.has_bias = bias is not None
         return _handle(ctx, z, z8.q, z8.scale), a
 
     @staticmethod
     @_first_order
     def backward(ctx, saved, da):
         q, scale = saved
-        dz, dbias = ops.gelu8_backward(da.contiguous(), Act8(q, scale, da.shape[1]), want_bias=ctx.has_bias)
+        dz, dbias = ops.gelu8_backward(da.contiguous(), Act8(q, scale, da.shape[1]), want_bias=ctx.needs_input_grad[1])
         return dz, dbias
 
 
@@ -133,27 +132,33 @@ def gelu8(z, bias=None) -> torch.Tensor:
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, bias, q, scale):
-        x8 = ops.act8_pack(x) if q is None else Act8(q, scale, x.shape[1])
-        ctx.has_bias = bias is not None
+    def forward(ctx, x, w, bias, q, scale, keep):
+        if keep and q is None:
+            q, scale, _ = ops.act8_pack(x)
         out = x @ w.to(x.dtype)
-        return _handle(ctx, x, w, x8.q, x8.scale), out if bias is None else out + bias.to(x.dtype)
+        return _handle(ctx, x, w, *((q, scale) if keep else (None, None))), out if bias is None else out + bias.to(x.dtype)
 
     @staticmethod
     @_first_order
     def backward(ctx, saved, dy):
         w, q, scale = saved
         dy = dy.contiguous()
-        dx = dy @ w.to(dy.dtype).t() if ctx.needs_input_grad[0] else None
-        dw, db = ops.act8_wgrad(Act8(q, scale, w.shape[0]), dy, dtype=w.dtype, want_bias=ctx.has_bias)
-        return dx, dw, db, None, None
+        need_x, need_w, need_bias = ctx.needs_input_grad[:3]
+        dx = dy @ w.to(dy.dtype).t() if need_x else None
+        dw = db = None
+        if need_w:
+            dw, db = ops.act8_wgrad(Act8(q, scale, w.shape[0]), dy, dtype=w.dtype, want_bias=need_bias)
+        elif need_bias:
+            db = dy.sum(0, dtype=torch.float32)
+        return dx, dw, db, None, None, None
 
 
 def linear8(x, w, bias=None, x8: Optional[Act8] = None) -> torch.Tensor:
-    """x w + bias with w [in, out]. The input is kept in 8 bits for w's gradient: as `x8` has it (block_norm's pack, say),
-    or packed here. The product is the library's; the weight gradient is act8_wgrad's, in w's type."""
+    """x w + bias with w [in, out]. The input is kept in 8 bits for w's gradient, where that is wanted: as `x8` has it
+    (block_norm's pack, say), or packed here. The product is the library's; the weight gradient is act8_wgrad's, in w's
+    type."""
     q, scale = (None, None) if x8 is None else x8[:2]
-    return _Linear8.apply(x, w, bias, q, scale)[1]
+    return _Linear8.apply(x, w, bias, q, scale, torch.is_grad_enabled() and w.requires_grad)[1]
 
 
 __all__ = ["policy_loss", "block_norm", "gelu8", "linear8"]

@@ -59,8 +59,8 @@ class BlockNorm(NamedTuple):
 
 
 class BlockNormGrads(NamedTuple):
-    dx: torch.Tensor
-    dh: torch.Tensor
+    dx: Optional[torch.Tensor]
+    dh: Optional[torch.Tensor]
     dgate: Optional[torch.Tensor]
     dpost: Optional[torch.Tensor]
     dpost_bias: Optional[torch.Tensor]
@@ -235,9 +235,9 @@ def block_norm(x, h, *, gate=None, rows_per_gate=None, residual_scale=1.0, post=
 
 
 def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, residual_scale=1.0, post=None, pre=None,
-                        kind="layer", eps=1e-5) -> BlockNormGrads:
+                        kind="layer", eps=1e-5, want=(True,) * 7) -> BlockNormGrads:
     """Gradients of block_norm at its inputs and parameters from those at y and n (either may be None) and the
-    stats that the forward pass returned."""
+    stats that the forward pass returned. `want` says which of the seven are: the others are None and not formed."""
     me = "block_norm_backward"
     args, there = _norm_args(me, x, h, gate, rows_per_gate, residual_scale, post, pre, kind, eps)
     rows, width = x.shape
@@ -247,13 +247,14 @@ def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, r
     packed = args(0, 0, 0, 0, stats.data_ptr())
     ld_dy = _matrix(me, "dy", dy, x) if dy is not None else 0
     ld_dn = _matrix(me, "dn", dn, x) if dn is not None else 0
-    dx, dh = x.new_empty(rows, width), x.new_empty(rows, width)
-    dgate = None if gate is None else torch.empty_like(gate) if rows else torch.zeros_like(gate)
-    grads = [x.new_empty(width, dtype=torch.float32) if w else None for w in there]
+    if len(want) != 7:
+        _fail(me, "want is seven truth values, one for each gradient")
+    dx, dh = (x.new_empty(rows, width) if w else None for w in want[:2])
+    dgate = None if gate is None or not want[2] else torch.empty_like(gate) if rows else torch.zeros_like(gate)
+    grads = [x.new_empty(width, dtype=torch.float32) if w and there_is else None for there_is, w in zip(there, want[3:])]
     scratch = _scratch(lib().wc_block_norm_workspace(packed), x)
     _call(lib().wc_block_norm_backward, x.get_device(), packed, _BLOCK_NORM_GRADS.pack(
-        dy.data_ptr() if dy is not None else 0, dn.data_ptr() if dn is not None else 0, dx.data_ptr(), dh.data_ptr(),
-        dgate.data_ptr() if dgate is not None else 0, *[g.data_ptr() if g is not None else 0 for g in grads],
+        *[t.data_ptr() if t is not None else 0 for t in (dy, dn, dx, dh, dgate, *grads)],
         scratch.data_ptr(), ld_dy, ld_dn, max(1, width), max(1, width)))
     return BlockNormGrads(dx, dh, dgate, *grads)
 
