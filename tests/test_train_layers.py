@@ -149,3 +149,12 @@ def test_gelu8_sums_its_bias_only_for_a_gradient(asked, monkeypatch):
     torch.autograd.grad(layers.gelu8(z, b).sum(), (z, b))
     torch.autograd.grad(layers.gelu8(z, b.detach()).sum(), z)
     assert seen == [True, False]
+
+
+@pytest.mark.parametrize("rows,width", [(4, 4), (5, 3), (6, 4)])
+def test_linear8_refuses_the_8_bits_of_another_input(asked, rows, width):
+    """Before the forward pass, and also where the blocks are as many (a width of 3 for 4)."""
+    x, w = leaf(5, 4, seed=1), leaf(4, 3, seed=3)
+    with pytest.raises(SolveError, match="differ in shape") as e:
+        layers.linear8(x, w, x8=ops.Act8(torch.zeros(rows, 32, dtype=torch.int8), torch.zeros(rows, 1, dtype=torch.uint8), width))
+    assert e.value.code == 1

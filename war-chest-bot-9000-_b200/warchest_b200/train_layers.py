@@ -157,7 +157,11 @@ def linear8(x, w, bias=None, x8: Optional[Act8] = None) -> torch.Tensor:
     """x w + bias with w [in, out]. The input is kept in 8 bits for w's gradient, where that is wanted: as `x8` has it
     (block_norm's pack, say), or packed here. The product is the library's; the weight gradient is act8_wgrad's, in w's
     type."""
-    q, scale = (None, None) if x8 is None else x8[:2]
+    q = scale = None
+    if x8 is not None:
+        q, scale, width = x8
+        if x.dim() != 2 or (q.shape[0], width) != x.shape:
+            raise SolveError(1, "linear8: x and the 8-bit activations differ in shape")
     return _Linear8.apply(x, w, bias, q, scale, torch.is_grad_enabled() and w.requires_grad)[1]
 
 
