@@ -861,3 +861,156 @@ def test_block_norm_gradients_one_at_a_time(T, D):
         assert torch.equal(some[i], full[i]) and all(some[j] is None for j in range(7) if j != i)
     with pytest.raises(SolveError, match="seven"):
         ops.block_norm_backward(dy, dn, c["x"], c["h"], r.stats, **rest, want=(True,))
+
+
+# ---------------------------------------------- widths, strides and lengths between the others
+
+def strided(v, ld, skip, fill=math.nan):
+    """v's values in rows that are `ld` apart and start `skip` entries into theirs."""
+    room = torch.full((len(v), ld + skip), fill, dtype=v.dtype, device="cuda")
+    room[:, skip:skip + v.shape[1]] = v
+    return room[:, skip:skip + v.shape[1]]
+
+
+# rows that no cluster of CTAs can hold: from 213,000 entries of 32 bits on (170,400 with legal bytes), twice that of 16
+@pytest.mark.parametrize("T,V,dtype,legal", [(3, 220000, F32, None), (2, 180001, F32, 0.3), (2, 430001, BF16, None), (3, 350003, F16, 0.4)])
+def test_policy_loss_of_the_longest_rows(T, V, dtype, legal):
+    c = policy_case(T, V, dtype, seed=17, legal=legal)
+    check_policy(c, OPTIONS, ops.policy_loss(**c, **OPTIONS))
+    wide = c | {"logits": strided(c["logits"], V + 3, 1), "actions": c["actions"].to(torch.int32)}
+    if legal is not None:
+        wide["legal"] = strided(c["legal"].to(torch.uint8) * 4, V + 5, 2, fill=1)
+    check_policy(wide, OPTIONS | {"entropy_coef": 0.0}, ops.policy_loss(**wide, **(OPTIONS | {"entropy_coef": 0.0})))
+
+
+def test_policy_longest_rows_that_count_for_nothing():
+    V = 180000
+    c = policy_case(7, V, F32, seed=18, legal=0.5)
+    c["legal"][0] = False
+    c["legal"][1, c["actions"][1]] = False
+    c["actions"][2], c["weights"][3] = V, 0.0
+    c["logits"][3] = math.nan
+    c["logits"][4] = torch.where(torch.arange(V, device="cuda") == c["actions"][4], c["logits"][4], -math.inf)
+    c["logits"][5] = torch.finfo(F32).min
+    c["logits"][5, c["actions"][5]] = 0.5
+    c["old_logp"][5], c["ref_logp"][5] = -0.1, -0.2
+    r = ops.policy_loss(**c, **OPTIONS)
+    check_policy(c, OPTIONS, r)
+    assert (r.row_loss[:4] == 0).all() and (r.dlogits[:4] == 0).all() and (r.logp[4:6] == 0).all() and r.loss.isfinite()
+    c["logits"][6, 5], c["legal"][6, 5] = math.nan, True
+    r = ops.policy_loss(**c, **OPTIONS)
+    assert r.row_loss[6].isnan() and r.row_loss[:6].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("D", [9, 16, 20, 24, 37, 60, 130, 201, 255, 500])
+def test_block_norm_widths_between(D, kind, dtype):
+    for i, (post, pre, per) in enumerate(((True, True, 0), (True, False, 37), (False, True, None))):
+        check_norm(norm_case(75, D, dtype, kind, post, pre, per, seed=D + i))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [24, 33, 96, 97, 520, 1111, 4099])
+def test_block_norm_packs_16_bit_outputs(D, dtype):
+    """The 8 bits are those of n before it is rounded."""
+    c = norm_case(20, D, dtype, "layer", per=7)
+    r = ops.block_norm(**c, pack=True)
+    _, n = norm_plain(c, **{k: double(c[k]) for k in ("x", "h", "gate", "post", "pre")})
+    kept = ops.act8_unpack(r.n8, F32).double()
+    unit = (r.n8.scale.double() - 127).exp2().repeat_interleave(32, 1)[:, :D]
+    # half a unit and what a normalised value is off
+    assert ((kept - n.detach()).abs() <= unit * 0.5 + 64 * U * (1 + n.detach().abs().amax(1, keepdim=True))).all()
+    near(r.n, n.detach(), 64 * U * (1 + n.detach().abs().amax(1, keepdim=True)), "n")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,ld,skip", [(24, 25, 1), (96, 97, 0), (96, 104, 8), (200, 203, 3), (333, 336, 3), (1000, 1003, 1), (4097, 4100, 1)])
+def test_block_norm_strides_of_every_matrix(D, ld, skip, dtype):
+    c = norm_case(40, D, dtype, "layer", per=9, seed=4)
+    v = c | {k: strided(c[k], ld, skip) for k in ("x", "h")}
+    leaves = {k: double(c[k]) for k in ("x", "h", "gate", "post", "pre")}
+    y, n = norm_plain(c, **leaves)
+    r = ops.block_norm(**v)
+    at = lambda w: 64 * U * (1 + w.detach().abs().amax(1, keepdim=True))  # noqa: E731
+    near(r.y, y.detach(), at(y), "y")
+    near(r.n, n.detach(), at(n), "n")
+    dy, dn = randn(gen(5), 40, D, dtype=dtype), randn(gen(6), 40, D, dtype=dtype)
+    g = ops.block_norm_backward(strided(dy, ld, skip), strided(dn, ld + 1, skip), v["x"], v["h"], r.stats,
+                                **{k: w for k, w in c.items() if k not in ("x", "h")})
+    ((y * dy.double()).sum() + (n * dn.double()).sum()).backward()
+    # as check_norm has them
+    for name, t in zip(("dx", "dh", "dgate"), ("x", "h", "gate")):
+        want = leaves[t].grad
+        near(getattr(g, name), want, 128 * U * (1 + want.abs().amax(1, keepdim=True)) * (3 if name == "dgate" else 1), name)
+    for name, t in zip(("dpost", "dpost_bias", "dpre", "dpre_bias"), (*leaves["post"], *leaves["pre"])):
+        near(getattr(g, name), t.grad, 128 * U * math.sqrt(40) * 4 * (1 + t.grad.abs()), name)
+
+
+def check_gelu8(z, b, da):
+    a, z8 = ops.gelu8(z, b)
+    s = z.float() + b if b is not None else z.float()
+    near(a, gelu_plain(s.double()), 96 * U * s.double().abs() * torch.sigmoid(1.6 * s.double()), "a")
+    q, scale = packed(s)
+    assert torch.equal(z8.q.double(), q) and torch.equal(z8.scale.long(), scale)
+    v = ops.act8_unpack(z8, F32).double().requires_grad_()
+    gelu_plain(v).backward(da.double())
+    dz, db = ops.gelu8_backward(da, z8)
+    near(dz, v.grad, 128 * U * da.double().abs(), "dz")
+    near(db, v.grad.sum(0), 128 * U * da.double().abs().sum(0), "dbias")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,D", [(40, 33), (300, 63), (7, 161), (50, 31), (3, 8), (1, 4099)])
+def test_gelu8_widths_between(T, D, dtype):
+    g = gen(T + D)
+    check_gelu8(randn(g, T, D, dtype=dtype, scale=2.0), randn(g, D), randn(g, T, D, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,ld,skip", [(8, 9, 0), (40, 43, 3), (64, 65, 1), (96, 104, 8), (96, 97, 0), (161, 168, 5), (256, 257, 1), (2048, 2051, 3)])
+def test_act8_and_gelu8_strides_and_addresses(D, ld, skip, dtype):
+    g = gen(D + ld)
+    x, da = randn(g, 30, D, dtype=dtype, scale=2.0), randn(g, 30, D, dtype=dtype)
+    p = ops.act8_pack(strided(x, ld, skip))
+    q, scale = packed(x)
+    assert torch.equal(p.q.double(), q) and torch.equal(p.scale.long(), scale)
+    for bias in (None, randn(g, D), randn(g, D + 1)[1:]):
+        check_gelu8(strided(x, ld, skip), bias, strided(da, ld + 2, skip))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("ld,skip", [(104, 8), (97, 0), (99, 3)])
+def test_act8_wgrad_strides_of_every_type(ld, skip, dtype):
+    g = gen(7)
+    x8, dy = ops.act8_pack(randn(g, 500, 200, dtype=BF16)), randn(g, 500, 96, dtype=dtype)
+    for a, b in zip(ops.act8_wgrad(x8, dy), ops.act8_wgrad(x8, strided(dy, ld, skip))):
+        assert torch.equal(a, b)
+
+
+def test_backward_passes_past_32_bits():
+    """Matrices of more than 2^31 elements: the last rows' results are as they are by themselves."""
+    T, D = 140000, 16384
+    x = torch.zeros(T, D, dtype=BF16, device="cuda")
+    x[-3:] = randn(gen(1), 3, D, dtype=BF16)
+    tail, one = x[-3:].clone(), torch.ones(D, device="cuda")
+    a, z8 = ops.gelu8(x)
+    b, y8 = ops.gelu8(tail)
+    assert torch.equal(a[-3:], b) and torch.equal(z8.q[-3:], y8.q) and torch.equal(z8.scale[-3:], y8.scale)
+    del a
+    dz, db = ops.gelu8_backward(x, z8)
+    dw, dc = ops.gelu8_backward(tail, y8)
+    assert torch.equal(dz[-3:], dw)
+    near(db, dc.double(), 4 * U * dw.double().abs().sum(0), "dbias")  # (the other rows add zeros)
+    del dz, z8
+    for width in (D, 4096, 96):
+        rows = T * D // width
+        v, w = x.view(-1)[:rows * width].view(rows, width), tail.view(-1)[-3 * width:].view(3, width)
+        v[-3:] = w
+        s, t = (ops.block_norm(u, u, post=one[:width], kind="rms") for u in (v, w))
+        assert torch.equal(s.y[-3:], t.y) and torch.equal(s.stats[-3:], t.stats)
+        big = ops.block_norm_backward(v, None, v, v, s.stats, post=one[:width], kind="rms")
+        small = ops.block_norm_backward(w, None, w, w, t.stats, post=one[:width], kind="rms")
+        assert torch.equal(big.dx[-3:], small.dx) and torch.equal(big.dh[-3:], small.dh)
+        v[:-3] = 0
+        del s, big
