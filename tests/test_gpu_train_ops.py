@@ -1014,3 +1014,35 @@ def test_backward_passes_past_32_bits():
         assert torch.equal(big.dx[-3:], small.dx) and torch.equal(big.dh[-3:], small.dh)
         v[:-3] = 0
         del s, big
+
+
+@pytest.mark.parametrize("T,V,dtype", [(300, 70001, BF16), (2000, 30000, F32), (33000, 18000, F16)])
+def test_policy_loss_sums_clusters_rows_in_an_order_of_the_sizes_alone(T, V, dtype):
+    """Runs of 32768 rows, 1024 chains each, joined by halves: to the bit, where the terms cancel to their last places."""
+    g = gen(19)
+    l = lambda: -math.log(V) + randn(g, T, scale=0.3)  # noqa: E731
+    c = {"logits": randn(g, T, V, dtype=dtype, scale=0.1), "actions": torch.randint(0, V, (T,), generator=g, device="cuda"),
+         "advantages": randn(g, T), "old_logp": l(), "ref_logp": l()}
+    row = ops.policy_loss(**c, **OPTIONS, want_grad=False).row_loss.cpu()
+    w = torch.rand(T, generator=g, device="cuda").cpu()
+
+    def total(sum_of):
+        return sum_of((w * row).double())
+
+    w[T - 2:] = 0.0
+    for t in (T - 1, T - 2):  # two weights that cancel the rest: some 2^-48 of it is left
+        w[t] = -float(total(torch.sum)) / float(row[t])
+
+    def ordered(p):
+        runs = torch.zeros(-(-T // 32768) * 32768, dtype=torch.float64)
+        runs[:T] = p
+        chains = torch.zeros(len(runs) // 32768, 1024, dtype=torch.float64)
+        for part in runs.view(-1, 32, 1024).unbind(1):
+            chains = chains + part
+        tree = lambda v: v if v.shape[-1] == 1 else tree(v[..., :v.shape[-1] // 2] + v[..., v.shape[-1] // 2:])  # noqa: E731
+        runs = tree(tree(chains.view(-1, 32, 32))[..., 0].view(-1, 32))[:, 0]
+        return tree(torch.nn.functional.pad(runs, (0, 32 - len(runs))))[0] if len(runs) > 1 else runs[0]
+
+    got = ops.policy_loss(**c, weights=w.cuda(), **OPTIONS).loss
+    assert abs(float(got)) < 1e-11 * float((w * row).double().abs().sum())
+    assert float(got) == float(total(ordered).float())

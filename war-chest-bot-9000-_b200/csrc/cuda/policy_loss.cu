@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
     }
     if (CTAS > 1) cluster.sync();
     else __syncthreads();
-    double total = 0.0;
+    double total = 0.0;  // (CTAs by themselves)
     // A wait that runs out leaves NaN in the rows from here on. What a warp that gave up owes to others stays undone, so
     // that their waits run out too and none takes a place for free, or a row's parts for whole, that is not.
     bool bad = false;
@@ -536,7 +536,8 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                 const Row row(a, in, M, S, W, za);
                 if (lane == 0) {
                     if (!bad) rows[live & 1] = row, arrive(&ready[live & 1]);
-                    if (rank == 0) row.put(a, t), total += (double)(in.w * row.loss);
+                    if (rank == 0) row.put(a, t);
+                    if (CTAS == 1) total += (double)(in.w * row.loss);
                 }
                 ++live;
             } else if (rank == 0 && lane == 0) {
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
         }
     }
     __syncthreads();
-    if (rank == 0 && threadIdx.x == THREADS) part[blockIdx.x / CTAS] = total;
+    if (CTAS == 1 && threadIdx.x == THREADS) part[blockIdx.x] = total;
     if (CTAS > 1) {
         cluster.sync();  // no CTA leaves while another may still write to it
         // Where this CTA's warp has not waited for all that was sent to it, the last of that may still be on its way, for less
@@ -782,21 +783,41 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
     if (threadIdx.x == 0) part[blockIdx.x] = total;
 }
 
-// the CTAs' totals, in a fixed order
-__global__ void __launch_bounds__(1024) k_policy_total(const double* part, int n, float* loss) {
+// a sum over the CTA's threads, in a fixed order
+__device__ __forceinline__ double cta_sum(double v) {
     __shared__ double s[32];
+    const int lane = threadIdx.x & 31;
+    auto warp = [](double x) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
+        return x;
+    };
+    v = warp(v);
+    if (lane == 0) s[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return warp(lane < (int)blockDim.x / 32 ? s[lane] : 0.0);
+}
+// the CTAs' totals
+__global__ void __launch_bounds__(1024) k_policy_total(const double* part, int n, float* loss) {
     double v = 0.0;
     for (int i = threadIdx.x; i < n; i += blockDim.x) v += part[i];
-    for (int stage = 0; stage < 2; ++stage) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-        if (stage) break;
-        if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-        __syncthreads();
-        if (threadIdx.x >= 32) return;
-        v = threadIdx.x < blockDim.x / 32 ? s[threadIdx.x] : 0.0;
-    }
+    v = cta_sum(v);
     if (threadIdx.x == 0) *loss = (float)v;
+}
+// Clusters of several CTAs have no totals: how many there are is the GPU's to say, and the loss would depend on it. CTA i
+// sums up `run` rows' losses; a single one's total is the loss. (A void row's loss is 0, whatever its weight.)
+__global__ void __launch_bounds__(1024) k_policy_row_total(const float* row_loss, const float* weights, int64_t rows, int64_t run, double* part, float* loss) {
+    const int64_t first = blockIdx.x * run, last = min(first + run, rows);
+    double v = 0.0;
+#pragma unroll 8
+    for (int64_t t = first + threadIdx.x; t < last; t += 1024) {
+        const float l = row_loss[t], w = weights ? weights[t] : 1.0f;
+        if (l != 0.0f) v += (double)(w * l);
+    }
+    v = cta_sum(v);
+    if (threadIdx.x) return;
+    if (gridDim.x == 1) *loss = (float)v;
+    else part[blockIdx.x] = v;
 }
 
 constexpr int MOST_CTAS = 148 * 8;
@@ -812,7 +833,7 @@ template <class T, bool MASK>
 int64_t slice_bytes(int64_t slice) {
     return slice * sizeof(T) + (MASK ? slice + 32 : 0);
 }
-// `sm`: CTAs of one SM
+// `sm`: CTAs of one SM. (The launchers answer how many CTAs left totals; 0: the rows are still to be added.)
 template <class T, bool MASK, int WARPS, int CTAS>
 int launch_cluster(const wc_policy_loss_args& a, int sm, double* part, cudaStream_t s) {
     const int slice = (int)slice_of<T>(a, CTAS);
@@ -835,7 +856,7 @@ int launch_cluster(const wc_policy_loss_args& a, int sm, double* part, cudaStrea
     const int n = (int)std::min<int64_t>(most, a.rows);
     cfg.gridDim = n * CTAS;
     cudaLaunchKernelEx(&cfg, kernel, a, slice, slices, part, wait_limit());
-    return n;
+    return CTAS == 1 ? n : 0;
 }
 
 template <class T, bool MASK, bool ENTROPY, bool VEC>
@@ -895,6 +916,12 @@ void launch_policy_loss(const wc_policy_loss_args& a, cudaStream_t s) {
     if (a.rows) n = a.type == WC_F32   ? launch_type<float>(a, part, s)
                     : a.type == WC_F16 ? launch_type<__half>(a, part, s)
                                        : launch_type<__nv_bfloat16>(a, part, s);
+    if (!n) {
+        const int64_t run = std::max<int64_t>(32768, (a.rows + MOST_CTAS - 1) / MOST_CTAS);
+        n = (int)std::max<int64_t>(1, (a.rows + run - 1) / run);
+        k_policy_row_total<<<n, 1024, 0, s>>>(a.row_out, a.weights, a.rows, run, part, a.loss);
+        if (n == 1) return;
+    }
     k_policy_total<<<1, std::min(1024, std::max(32, (n + 31) / 32 * 32)), 0, s>>>(part, n, a.loss);
 }
 
