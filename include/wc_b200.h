@@ -517,7 +517,9 @@ int wc_gelu8_backward(const wc_act8_args* a, void* stream);
 /* The weight gradient of a linear layer whose input was kept in 8 bits:
  * dw[k, n] = sum over t of x8[t, k] dy[t, n] (weights as [in, out]), and
  * db[n] = sum over t of dy[t, n] when db is not NULL; 0 where there are no
- * rows. k is 1 to 2^20, n up to 2^20. The workspace also holds a dy in f16 or
+ * rows. k is 1 to 2^20, n up to 2^20. Of scale whole
+ * aligned words of 4 bytes are read, with the up to 3 bytes before and after the
+ * matrix that share one with it; those are not used. The workspace also holds a dy in f16 or
  * f32, or one whose rows do not start on 16 bytes, as its bf16 parts (2, 3 and
  * 1 of them). */
 typedef struct wc_act8_wgrad_args {

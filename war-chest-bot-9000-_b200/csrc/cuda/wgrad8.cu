@@ -349,7 +349,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         __syncwarp();
     } else if (warp == 2) {  // ----------------------------- x8's producer
-        // The units' rows have any alignment: the words that hold a row's are copied, and read at its first one's offset.
+        // The units' rows have any alignment: the words that hold a row's are copied, and read at its first one's offset. (So
+        // are the up to 3 bytes around the matrix that share a word with it, and not used. Copying the last word in part
+        // cost 8192 x 4096 x 4096 in bf16 291 us for 284.)
         const int64_t blocks = (a.k + 31) / 32;
         const uint32_t ring = umma::smem_u32(xs);
         int it = 0;
