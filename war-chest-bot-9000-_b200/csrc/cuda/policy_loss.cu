@@ -433,7 +433,6 @@ constexpr int MAX_SLICES = 4;
 template <class T, bool MASK, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 ? 4 : 6) k_policy_cluster(wc_policy_loss_args a, int slice, int slices, double* part, uint64_t wait_ns) {
     constexpr int N = Chunk<T>::N, THREADS = WARPS * 32;
-    constexpr int TOGETHER = 1;
     extern __shared__ __align__(128) uint8_t ring[];  // `slices` of the logits, then of the legal bytes
     __shared__ float4 parts[4][CTAS * WARPS];         // of every warp of the cluster, four (live) rows in turn
     __shared__ Row rows[2];                           // what was made of them, two in turn
@@ -619,17 +618,12 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                     if (MASK || here) {
                         for (int at = threadIdx.x * N; at < width; at += THREADS * N) some(at);
                     } else {
-                        for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
-                            Chunk<T> q[TOGETHER];
-#pragma unroll
-                            for (int k = 0; k < TOGETHER; ++k) {
-                                const int to = at + k * THREADS * N;
-                                q[k].none();
-                                if (to < width && to >= from && to <= last) q[k].read(z + to * sizeof(T));
-                                else if (to < width) some(to);
-                            }
-#pragma unroll
-                            for (int k = 0; k < TOGETHER; ++k) most.add(q[k]);
+                        for (int at = threadIdx.x * N; at < width; at += THREADS * N) {
+                            Chunk<T> q;
+                            q.none();
+                            if (at >= from && at <= last) q.read(z + at * sizeof(T));
+                            else some(at);
+                            most.add(q);
                         }
                     }
                     float m = most.get();
@@ -638,14 +632,10 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                     if (m == -INFINITY) m = 0.0f;  // nothing here counts (or is a number): its sums are 0 (or NaN)
                     const Pair f = twice(factor(m)), c = twice(-scaled(m));
                     Pair sum = 0, mean = 0;
-                    for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
-                        Chunk<T> q[TOGETHER];
-#pragma unroll
-                        for (int k = 0; k < TOGETHER; ++k)
-                            if (at + k * THREADS * N < width) q[k].read(z + (at + k * THREADS * N) * sizeof(T));
-#pragma unroll
-                        for (int k = 0; k < TOGETHER; ++k)
-                            if (at + k * THREADS * N < width) add_chunk(q[k], f, c, sum, mean);
+                    for (int at = threadIdx.x * N; at < width; at += THREADS * N) {
+                        Chunk<T> q;
+                        q.read(z + at * sizeof(T));
+                        add_chunk(q, f, c, sum, mean);
                     }
                     const float2 v = make_float2(warp_sum(both(sum)), warp_sum(both(mean)));
                     const float4 mine = make_float4(v.x == 0.0f ? -INFINITY : m, v.x, v.y, 0.0f);
@@ -672,23 +662,16 @@ __global__ void __launch_bounds__(WARPS * 32 + 32, WARPS == 16 ? 2 : WARPS == 8 
                     const int from = b - first, last = (int)a.width + from - N;  // where chunks lie in the row
                     T* const o = out - from;
                     auto chunks = [&](auto&& make) {
-                        for (int at = threadIdx.x * N; at < width; at += TOGETHER * THREADS * N) {
-                            Chunk<T> q[TOGETHER];
+                        for (int at = threadIdx.x * N; at < width; at += THREADS * N) {
+                            Chunk<T> q;
+                            q.read(z + at * sizeof(T));
+                            alignas(16) T e[N];
+                            make(q, e);
+                            if (same && at >= from && at <= last) put_chunk(o + at, e);
+                            else
 #pragma unroll
-                            for (int k = 0; k < TOGETHER; ++k)
-                                if (at + k * THREADS * N < width) q[k].read(z + (at + k * THREADS * N) * sizeof(T));
-#pragma unroll
-                            for (int k = 0; k < TOGETHER; ++k) {
-                                const int to = at + k * THREADS * N;
-                                if (to >= width) continue;
-                                alignas(16) T e[N];
-                                make(q[k], e);
-                                if (same && to >= from && to <= last) put_chunk(o + to, e);
-                                else
-#pragma unroll
-                                    for (int j = 0; j < N; ++j)
-                                        if (to + j >= from && to + j < last + N) o[to + j] = e[j];
-                            }
+                                for (int j = 0; j < N; ++j)
+                                    if (at + j >= from && at + j < last + N) o[at + j] = e[j];
                         }
                     };
                     const Row r = rows[mine & 1];
