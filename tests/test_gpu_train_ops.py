@@ -1046,3 +1046,36 @@ def test_policy_loss_sums_clusters_rows_in_an_order_of_the_sizes_alone(T, V, dty
     got = ops.policy_loss(**c, weights=w.cuda(), **OPTIONS).loss
     assert abs(float(got)) < 1e-11 * float((w * row).double().abs().sum())
     assert float(got) == float(total(ordered).float())
+
+
+def test_every_operator_inside_a_cuda_graph():
+    """Every kernel family's launch, captured once and replayed on other inputs."""
+    short, long = policy_case(64, 512, F32, seed=51, legal=0.5), policy_case(20, 40000, BF16, seed=52)
+    longest = policy_case(2, 220000, F32, seed=53)
+    narrow, wide, widest = (norm_case(40, D, BF16, "layer", per=0, seed=D) for D in (96, 1000, 5000))
+    z, da = randn(gen(1), 500, 192, dtype=BF16), randn(gen(2), 500, 96, dtype=F16)
+    inputs = [short["logits"], long["logits"], longest["logits"], narrow["x"], wide["x"], widest["x"], z, da]
+
+    def step():
+        out = []
+        for c in (short, long, longest):
+            out += ops.policy_loss(**c, **OPTIONS)
+        for c in (narrow, wide, widest):
+            r = ops.block_norm(**c, pack=True)
+            out += [r.y, r.n, r.n8.q, *ops.block_norm_backward(r.y, r.n, c["x"], c["h"], r.stats, **{k: v for k, v in c.items() if k not in ("x", "h")})]
+        a, z8 = ops.gelu8(z)
+        return out + [a, z8.q, *ops.gelu8_backward(a, z8), *ops.act8_wgrad(ops.act8_pack(z), da), ops.act8_unpack(z8)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in inputs:
+        t.copy_(t.flip(0))
+    graph.replay()
+    for a, b in zip(got, step()):
+        assert torch.equal(a, b)
