@@ -249,12 +249,15 @@ def block_norm_backward(dy, dn, x, h, stats, *, gate=None, rows_per_gate=None, r
     ld_dn = _matrix(me, "dn", dn, x) if dn is not None else 0
     if len(want) != 7:
         _fail(me, "want is seven truth values, one for each gradient")
-    dx, dh = (x.new_empty(rows, width) if w else None for w in want[:2])
+    dx = x.new_empty(rows, width) if want[0] else None
+    dh = x.new_empty(rows, width) if want[1] else None
     dgate = None if gate is None or not want[2] else torch.empty_like(gate) if rows else torch.zeros_like(gate)
     grads = [x.new_empty(width, dtype=torch.float32) if w and there_is else None for there_is, w in zip(there, want[3:])]
     scratch = _scratch(lib().wc_block_norm_workspace(packed), x)
     _call(lib().wc_block_norm_backward, x.get_device(), packed, _BLOCK_NORM_GRADS.pack(
-        *[t.data_ptr() if t is not None else 0 for t in (dy, dn, dx, dh, dgate, *grads)],
+        dy.data_ptr() if dy is not None else 0, dn.data_ptr() if dn is not None else 0,
+        dx.data_ptr() if dx is not None else 0, dh.data_ptr() if dh is not None else 0,
+        dgate.data_ptr() if dgate is not None else 0, *[g.data_ptr() if g is not None else 0 for g in grads],
         scratch.data_ptr(), ld_dy, ld_dn, max(1, width), max(1, width)))
     return BlockNormGrads(dx, dh, dgate, *grads)
 
