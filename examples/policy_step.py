@@ -26,7 +26,8 @@ WIDTH, HIDDEN, BLOCKS = 96, 192, 2
 
 
 def legal_count(root):
-    """How many actions are legal in the state that a root starts with (the shortest prefix that reads as one)."""
+    """How many actions are legal in the state that a root starts with: the one prefix that reads as a state (where a
+    state ends does not depend on what follows it, so no shorter or longer one does)."""
     for end in range(64, len(root)):
         try:
             return len(wc.legal_actions(root[:end]))

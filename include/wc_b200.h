@@ -410,7 +410,9 @@ enum { WC_F32 = 0, WC_F16 = 1, WC_BF16 = 2 };
  * A row is void when its weight is 0, its action lies outside 0 .. width - 1
  * or is not one of the entries that count (so also when none is left): its
  * results and its gradient are 0, and its logits need not be finite. Entries
- * that do not count have gradient 0. NaN and +inf elsewhere give NaN. */
+ * that do not count have gradient 0. NaN and +inf elsewhere give NaN; a row
+ * of which ratio A (where it is not clipped) or the KL term is past 32 bits has
+ * infinities and NaN in its gradient, also at entries that do not count. */
 typedef struct wc_policy_loss_args {
     const void* logits;      /* rows x width of `type` */
     const uint8_t* legal;    /* rows x width, or NULL */
@@ -517,11 +519,13 @@ int wc_gelu8_backward(const wc_act8_args* a, void* stream);
 /* The weight gradient of a linear layer whose input was kept in 8 bits:
  * dw[k, n] = sum over t of x8[t, k] dy[t, n] (weights as [in, out]), and
  * db[n] = sum over t of dy[t, n] when db is not NULL; 0 where there are no
- * rows. k is 1 to 2^20, n up to 2^20. Of scale whole
- * aligned words of 4 bytes are read, with the up to 3 bytes before and after the
- * matrix that share one with it; those are not used. The workspace also holds a dy in f16 or
- * f32, or one whose rows do not start on 16 bytes, as its bf16 parts (2, 3 and
- * 1 of them). */
+ * rows. k is 1 to 2^20, n up to 2^20. The tensor core's sums in 32 bits round
+ * towards zero; they are taken in runs of rows, so that values of one sign
+ * lose no more than about 1e-5 of the result (6e-5 where it is bf16). Of
+ * scale whole aligned words of 4 bytes are read, with the up to 3 bytes before
+ * and after the matrix that share one with it; those are not used. The
+ * workspace also holds a dy in f16 or f32, or one whose rows do not start on
+ * 16 bytes, as its bf16 parts (2, 3 and 1 of them). */
 typedef struct wc_act8_wgrad_args {
     const int8_t* q;        /* rows x 32 blocks of k values */
     const uint8_t* scale;

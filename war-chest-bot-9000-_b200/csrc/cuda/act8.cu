@@ -11,9 +11,10 @@
 // takes two shuffles. Elsewhere a warp holds 8 blocks, one value of each a
 // thread, so that its loads and stores are still next to each other.
 //
-// On a B200 131071 x 897 in f32 is packed and read back in 223 us (5.3 TB/s of the
-// 6.5 that a copy reaches), 131072 x 1024 in bf16 in 145 us (5.6 TB/s); GELU forward
-// and backward of 4095 x 16384 in bf16 takes 138 us (4.9 TB/s).
+// On a B200 131071 x 897 in f32 is packed and read back in 228 to 241 us (4.9 to 5.2
+// TB/s of the 6.5 that a copy reaches), 131072 x 1024 in bf16 in 143 us (5.7 TB/s);
+// GELU forward and backward of 4095 x 16384 in bf16 takes 139 to 143 us (4.7 to 4.9
+// TB/s).
 #include <algorithm>
 #include <type_traits>
 

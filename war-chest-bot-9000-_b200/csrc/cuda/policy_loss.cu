@@ -22,10 +22,10 @@
 // chunks do not fit have the chunks they lie in. Rows that no cluster can hold
 // are read twice by one CTA (the second time mostly from L2).
 //
-// On a B200 131072 x 512 in bf16 with legal bytes takes 93 us (3.7 TB/s of the 6.5
+// On a B200 131072 x 512 in bf16 with legal bytes takes 94 to 96 us (3.5 TB/s of the 6.5
 // that a copy reaches: the SMs issue in 65% of the cycles, 30 instructions an entry
-// with what a row costs by itself), 2048 x 131072 320 us (3.4 TB/s: 20 an entry, two
-// of them powers).
+// with what a row costs by itself), 2048 x 131072 306 to 308 us (3.5 TB/s: 20 an
+// entry, two of them powers), 512 x 300000 in f32, which no cluster holds, 632 to 642.
 #include <cooperative_groups.h>
 
 #include <algorithm>
