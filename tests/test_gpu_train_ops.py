@@ -1079,3 +1079,10 @@ def test_every_operator_inside_a_cuda_graph():
     graph.replay()
     for a, b in zip(got, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,V,dtype,legal", [(20, 290000, F32, None), (12, 430001, F16, None), (12, 430001, BF16, 0.9)])
+def test_policy_longest_rows_of_few_large_entries(T, V, dtype, legal):
+    """Most entries are small beside the sum, and many."""
+    c = policy_case(T, V, dtype, seed=20, legal=legal, scale=4.0)
+    check_policy(c, OPTIONS, ops.policy_loss(**c, **OPTIONS))

@@ -728,8 +728,15 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
             if (threadIdx.x == 0) put_void(a, t);
             continue;
         }
-        // eight entries at a time: their maximum moves the running one, then their powers are added
-        float m = -INFINITY, s = 0.0f, w = 0.0f;
+        // Eight entries at a time: their maximum moves the running one, then their powers are added up and the sum's share
+        // to what there is. A thread has hundreds of entries, most of them small beside the sum: what rounding takes off them
+        // is kept and added at the end (without it l was off by 1.3e-6 at 430000 entries with a deviation of 4).
+        float m = -INFINITY, s = 0.0f, w = 0.0f, s_rest = 0.0f, w_rest = 0.0f;
+        auto add_to = [](float& sum, float& rest, float v) {
+            const float t = sum + v, had = t - v;
+            rest += (sum - had) + (v - (t - had));
+            sum = t;
+        };
         for (int64_t j = threadIdx.x; j < V; j += 8 * 512) {
             float v[8], top = m;
 #pragma unroll
@@ -739,10 +746,13 @@ __global__ void __launch_bounds__(512) k_policy_long(wc_policy_loss_args a, doub
                 top = fmaxf(top, v[k]);
             }
             const float from = top == -INFINITY ? 0.0f : top, c = scaled(from), d = shift(m, from), f = exp2f(d);
-            w = fmaf(s, d, w) * f, s *= f, m = top;
+            w = fmaf(s, d, w) * f, w_rest = fmaf(s_rest, d, w_rest) * f, s *= f, s_rest *= f, m = top;
+            float ds = 0.0f, dw = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) add_entry(v[k], factor(from), c, s, w);
+            for (int k = 0; k < 8; ++k) add_entry(v[k], factor(from), c, ds, dw);
+            add_to(s, s_rest, ds), add_to(w, w_rest, dw);
         }
+        s += s_rest, w += w_rest;
         float top = m;
 #pragma unroll
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
