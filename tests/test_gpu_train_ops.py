@@ -1086,3 +1086,14 @@ def test_policy_longest_rows_of_few_large_entries(T, V, dtype, legal):
     """Most entries are small beside the sum, and many."""
     c = policy_case(T, V, dtype, seed=20, legal=legal, scale=4.0)
     check_policy(c, OPTIONS, ops.policy_loss(**c, **OPTIONS))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [16, 513, 1000, 3000, 40000, 350003])
+def test_policy_what_lies_under_the_mask_does_not_count(V, dtype):
+    c = policy_case(5, V, dtype, seed=23, legal=0.5)
+    want = ops.policy_loss(**c, **OPTIONS)
+    under = torch.tensor([math.nan, math.inf, -math.inf, torch.finfo(dtype).max], device="cuda").to(dtype)
+    hidden = torch.where(c["legal"], c["logits"], under[torch.arange(V, device="cuda") % 4])
+    for a, b in zip(want, ops.policy_loss(**(c | {"logits": hidden}), **OPTIONS)):
+        assert torch.equal(a, b)
