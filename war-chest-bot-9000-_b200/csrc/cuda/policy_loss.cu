@@ -25,7 +25,7 @@
 // On a B200 131072 x 512 in bf16 with legal bytes takes 94 to 96 us (3.5 TB/s of the 6.5
 // that a copy reaches: the SMs issue in 65% of the cycles, 30 instructions an entry
 // with what a row costs by itself), 2048 x 131072 306 to 308 us (3.5 TB/s: 20 an
-// entry, two of them powers), 512 x 300000 in f32, which no cluster holds, 632 to 642.
+// entry, two of them powers), 512 x 300000 in f32, which no cluster holds, 642.
 #include <cooperative_groups.h>
 
 #include <algorithm>
