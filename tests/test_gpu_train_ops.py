@@ -1097,3 +1097,24 @@ def test_policy_what_lies_under_the_mask_does_not_count(V, dtype):
     hidden = torch.where(c["legal"], c["logits"], under[torch.arange(V, device="cuda") % 4])
     for a, b in zip(want, ops.policy_loss(**(c | {"logits": hidden}), **OPTIONS)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,K,N,dtype", [(5000, 37 * 256, 4 * 128, F16), (20000, 37 * 256, 4 * 256, BF16), (17000, 37 * 256, 8 * 256, BF16)])
+def test_act8_wgrad_whole_tiles_of_several_runs(T, K, N, dtype):
+    """As many tiles as CTAs, or twice that: none is shared, and each is summed up in the workspace."""
+    from warchest_b200 import lib
+
+    g = gen(24)
+    x8, dy = ops.act8_pack(randn(g, T, K, dtype=BF16)), randn(g, T, N, dtype=dtype)
+    kind, sizes = ops._TYPES[dtype], [T, K, N, N]
+    need = lib().wc_act8_wgrad_workspace(ops._ACT8_WGRAD.pack(0, 0, 0, 0, 0, 0, *sizes, kind, kind))
+    space = torch.full((need + 64,), 99, dtype=torch.uint8, device="cuda")
+    dw = torch.empty(K, N, dtype=dtype, device="cuda")
+    ops._call(lib().wc_act8_wgrad, 0, ops._ACT8_WGRAD.pack(x8.q.data_ptr(), x8.scale.data_ptr(), dy.data_ptr(), dw.data_ptr(), 0,
+                                                           space.data_ptr(), *sizes, kind, kind))
+    assert (space[need:] == 99).all()
+    # relative to the whole: the result's rounding, and as for 32-bit results a run's bias and the runs' own sums
+    want = act8_product(x8, dy)
+    assert float((dw.double() - want).norm() / want.norm()) < EPS[dtype] / math.sqrt(3) + 1e-5
+    if dtype == F16:
+        assert torch.equal(dw, ops.act8_wgrad(x8, dy)[0].to(F16))
